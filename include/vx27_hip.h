@@ -9,6 +9,8 @@
  *   - DeltaNet recurrent decode (gate mapping, causal conv, delta rule,
  *     gated output norm), one or many tokens per call,
  *   - gated GQA decode over a bf16 KV cache (split-K flash decode),
+ *   - the same attention over a paged cache: append, ragged attention with a
+ *     sliding window and sinks, eviction by accumulated weight,
  *   - RoPE tables and KV-cache format helpers.
  * The reference's own void API (include/vx27_deltanet.h etc.) is exported by
  * the same library and routes through these entry points.
@@ -39,9 +41,9 @@ void vx27_hip_close(vx27_hip_ctx *ctx);
 /* Waits for the context stream.  Also returns -1 if a call since the last
  * sync was given a device-side index outside its range: a GQA decode
  * position outside its KV cache (pos < 0 or pos >= L: the kernels clamp it
- * so no access leaves the cache) or a vx27_hip_dn_commit index past its
- * checkpoints (nothing is copied for it).  That call's outputs are
- * undefined. */
+ * so no access leaves the cache), a vx27_hip_dn_commit index past its
+ * checkpoints (nothing is copied for it), or a length, page or token range
+ * outside its paged cache (below).  That call's outputs are undefined. */
 int vx27_hip_sync(vx27_hip_ctx *ctx);
 /* Use a caller stream (hipStream_t) for subsequent calls; NULL restores the
  * context's own stream. */
@@ -311,6 +313,135 @@ int vx27_hip_kv_write(vx27_hip_ctx *ctx, uint16_t *k_cache, uint16_t *v_cache, i
 int vx27_hip_kv_read(vx27_hip_ctx *ctx, const uint16_t *k_cache, const uint16_t *v_cache,
                      int B_total, int n_kv, int hd, int L, int b, int p0, int n,
                      float *k_rows, float *v_rows);
+
+/* ------------------------------------------------------ paged KV cache
+ * A KV cache in pages, for programs that hold many conversations of different
+ * lengths: a pool of n_pages pages of page_size rows (a multiple of 32) per KV
+ * head, and a table of each sequence's pages.  Row r of sequence b is row
+ * r % page_size of page table[b][r / page_size].  A page is stored as a
+ * sequence of the cache above is (B = n_pages, L = page_size), so
+ * vx27_hip_kv_write and vx27_hip_kv_read (page_size % 64 == 0) move rows in
+ * and out of a page:
+ *   K: [n_pages][n_kv][page_size][hd]
+ *   V: [n_pages][n_kv][page_size/32][hd][32]
+ * hd is 256.  The mixer is the reference's gated GQA (vx27_qfwd.c:172-211);
+ * its paging, windows and eviction have no counterpart there.
+ *
+ * The calls take ragged batches: n_tok new tokens, those of sequence b at
+ * q_start[b] .. q_start[b+1]-1 (device int [B+1]; at most max_T each, none
+ * for some is fine), which are the last of its len[b] rows: token t of T is
+ * row len[b] - T + t.  With q_start NULL there is one token a sequence
+ * (n_tok == B, max_T == 1).  Outputs of rows before q_start[0] and from
+ * q_start[B] on are left as they were.  Two sequences may share pages that
+ * neither call writes (a common prefix).
+ *
+ * Lengths past max_pages * page_size, pages outside the pool, token ranges
+ * outside n_tok or longer than max_T, and new tokens without a row (append)
+ * are clamped or dropped on the device, so that no access leaves the
+ * buffers, and reported by the next vx27_hip_sync; that call's outputs are
+ * undefined.  Table entries of pages without a row that the call reads or
+ * writes may hold anything. */
+
+/* Append: for every new token, q and k are normed (x*s*(1+w), or x*s*w with
+ * VX27_GQA_NORM_W) and rotated as vx27_hip_gqa_decode does, k and v are
+ * rounded to bf16 and written to their rows, and the rotated q is rounded to
+ * bf16 for vx27_hip_paged_attn.  q, k and v are fp32 or bf16 (in_dtype),
+ * element (token, head, i) at q[token*q_tok_stride + head*q_head_stride + i]
+ * and k_new[token*kv_tok_stride + head*hd + i]; 0 strides = dense.  All three
+ * 16-byte aligned (bf16: 8) with strides multiples of 4 elements; q_norm_w,
+ * k_norm_w and q_out 16-byte aligned.  With q NULL only k and v are written. */
+typedef struct {
+    int B, n_q, n_kv, hd;
+    int rope_dim;               /* even, 0 = no rotation */
+    float rope_theta, rope_yarn;
+    unsigned flags;             /* VX27_GQA_NORM_W */
+    int page_size, n_pages, max_pages;
+    const int *table;           /* [B][max_pages] */
+    const int *len;             /* [B] rows, the new tokens included */
+    const int *q_start;         /* [B+1] or NULL */
+    int n_tok, max_T;
+    const int *pos;             /* optional [n_tok] positions for the rotation; NULL = the token's row */
+    int in_dtype;               /* VX27_F32 or VX27_BF16 */
+    const void *q;
+    size_t q_tok_stride, q_head_stride;
+    const void *k_new, *v_new;
+    size_t kv_tok_stride;
+    const float *q_norm_w, *k_norm_w;
+    uint16_t *q_out;            /* bf16 [n_tok][n_q][hd] */
+    uint16_t *k_pages, *v_pages;
+} vx27_paged_append_desc;
+int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
+
+/* Attention of the new tokens over the cached rows (theirs included, so after
+ * the append): token at row i sees row j <= i if j > i - window (window 0: no
+ * limit) or j < n_sink (sinks);
+ *   out = (sum_j softmax_j(q.k_j / sqrt(hd)) v_j) * sigmoid(gate),
+ * query head h reading KV head h / (n_q/n_kv).  A token that sees nothing
+ * gets 0.  q is bf16, normed and rotated (q_out of the append).  Products on
+ * bf16 MFMA, sums and softmax statistics in fp32.  One or two tokens a
+ * sequence (at most 16 query rows a KV head) run the decode kernels: the
+ * cache's length split evenly over the device and joined, the softmax
+ * weights as three bf16 parts (fp32 accuracy; out fp32 or bf16).  More tokens
+ * run the tile kernel, whose weights are rounded to bf16 once (relative
+ * 2^-9; out may still be fp32).
+ * Optional outputs: lse [n_tok][n_q], the natural log of the softmax sum
+ * (-inf for a token that sees nothing); acc [B][n_kv][acc_stride], to which
+ * each row's weight over the call's tokens and the group's heads is added
+ * (rows nobody sees and rows from len on are left as they were).
+ * q 16-byte aligned with strides multiples of 8 elements; gate (fp32, or bf16
+ * with gate_dtype) and out 16-byte aligned, gate strides multiples of 8
+ * elements; n_q/n_kv at most 16. */
+typedef struct {
+    int B, n_q, n_kv, hd;
+    int page_size, n_pages, max_pages;
+    const int *table;           /* [B][max_pages] */
+    const int *len;             /* [B] */
+    const int *q_start;         /* [B+1] or NULL */
+    int n_tok, max_T;
+    int window, n_sink;         /* window 0: every row up to the token's own */
+    const uint16_t *q;          /* bf16; 0 strides = dense [n_tok][n_q][hd] */
+    size_t q_tok_stride, q_head_stride;
+    const uint16_t *k_pages, *v_pages;
+    const void *gate;           /* NULL: no output gate */
+    int gate_dtype;
+    size_t gate_tok_stride, gate_head_stride;
+    void *out;                  /* [n_tok][n_q][hd] */
+    int out_dtype;              /* VX27_F32 or VX27_BF16 */
+    float *lse;                 /* optional */
+    float *acc;                 /* optional; acc_stride >= max_pages*page_size */
+    size_t acc_stride;
+} vx27_paged_attn_desc;
+int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d);
+
+/* Eviction by accumulated attention weight: a sequence of more than `budget`
+ * rows keeps, per KV head, its first n_sink and last n_recent rows and the
+ * budget - n_sink - n_recent heaviest of the others by acc (ties: the lowest
+ * row; a NaN weight counts as the heaviest); shorter sequences keep every
+ * row.  The kept rows go, in row order, to rows 0 .. of the pages of
+ * dst_table, which must be pages of the pool that no sequence of the call
+ * has in `table` (fresh ones: the caller frees the old ones afterwards).
+ * Rows behind the last kept one are left as they were.  dst_len [B] receives
+ * the new lengths; acc_out [B][n_kv][acc_out_stride] (optional) the kept
+ * rows' weights; kept [B][n_kv][budget] (optional) their old rows, entries
+ * from dst_len on left as they were.  Keys keep the rotation of their
+ * original position: append later tokens with explicit positions (pos). */
+typedef struct {
+    int B, n_kv, hd;
+    int page_size, n_pages, max_pages;
+    const int *table;           /* [B][max_pages] */
+    const int *len;             /* [B] */
+    int budget, n_sink, n_recent;   /* n_sink + n_recent <= budget */
+    const float *acc;           /* [B][n_kv][acc_stride], acc_stride >= max_pages*page_size */
+    size_t acc_stride;
+    uint16_t *k_pages, *v_pages;
+    const int *dst_table;       /* [B][dst_max_pages], dst_max_pages * page_size >= min(budget, max_pages*page_size) */
+    int dst_max_pages;
+    int *dst_len;               /* [B], not len itself */
+    float *acc_out;             /* optional; acc_out_stride >= budget; must not overlap acc */
+    size_t acc_out_stride;
+    int *kept;                  /* optional */
+} vx27_paged_evict_desc;
+int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
 
 /* RoPE cos/sin tables on the device for n positions (device int array):
  * cos/sin [n][rope_dim/2].  The frequency table powf(theta, -2i/rope_dim) is

@@ -191,8 +191,8 @@ extern "C" int vx27_hip_sync(vx27_hip_ctx *ctx) {
         VX_HIP(hipMemcpyAsync(ctx->err_flag, ctx->err_host, sizeof(int), hipMemcpyHostToDevice, ctx->stream));
         VX_HIP(hipStreamSynchronize(ctx->stream));
         VX_REQUIRE(false, "vx27_hip_sync: a call since the last sync had an index outside its range (a decode "
-                          "position outside its KV cache, or a commit index past its checkpoints); that call's "
-                          "outputs are undefined");
+                          "position outside its KV cache, a commit index past its checkpoints, or a length, page or "
+                          "token range outside its paged cache); that call's outputs are undefined");
     }
     return 0;
 }

@@ -86,6 +86,37 @@ class GqaLayerPrefillDesc(C.Structure):
                 ("q_norm_w", VP), ("k_norm_w", VP), ("k_cache", VP), ("v_cache", VP), ("out", VP)]
 
 
+class PagedAppendDesc(C.Structure):
+    _fields_ = [("B", C.c_int), ("n_q", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("rope_dim", C.c_int),
+                ("rope_theta", C.c_float), ("rope_yarn", C.c_float), ("flags", C.c_uint),
+                ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int),
+                ("table", VP), ("len", VP), ("q_start", VP), ("n_tok", C.c_int), ("max_T", C.c_int), ("pos", VP),
+                ("in_dtype", C.c_int), ("q", VP), ("q_tok_stride", C.c_size_t), ("q_head_stride", C.c_size_t),
+                ("k_new", VP), ("v_new", VP), ("kv_tok_stride", C.c_size_t), ("q_norm_w", VP), ("k_norm_w", VP),
+                ("q_out", VP), ("k_pages", VP), ("v_pages", VP)]
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [("B", C.c_int), ("n_q", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int),
+                ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int),
+                ("table", VP), ("len", VP), ("q_start", VP), ("n_tok", C.c_int), ("max_T", C.c_int),
+                ("window", C.c_int), ("n_sink", C.c_int),
+                ("q", VP), ("q_tok_stride", C.c_size_t), ("q_head_stride", C.c_size_t),
+                ("k_pages", VP), ("v_pages", VP),
+                ("gate", VP), ("gate_dtype", C.c_int), ("gate_tok_stride", C.c_size_t),
+                ("gate_head_stride", C.c_size_t), ("out", VP), ("out_dtype", C.c_int),
+                ("lse", VP), ("acc", VP), ("acc_stride", C.c_size_t)]
+
+
+class PagedEvictDesc(C.Structure):
+    _fields_ = [("B", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int),
+                ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int), ("table", VP), ("len", VP),
+                ("budget", C.c_int), ("n_sink", C.c_int), ("n_recent", C.c_int),
+                ("acc", VP), ("acc_stride", C.c_size_t), ("k_pages", VP), ("v_pages", VP),
+                ("dst_table", VP), ("dst_max_pages", C.c_int), ("dst_len", VP),
+                ("acc_out", VP), ("acc_out_stride", C.c_size_t), ("kept", VP)]
+
+
 _SIGS = {
     "vx27_hip_open": (C.c_int, [C.POINTER(VP), C.c_int, C.c_char_p, C.c_size_t]),
     "vx27_hip_close": (None, [VP]),
@@ -118,6 +149,9 @@ _SIGS = {
     "vx27_hip_gqa_prefill": (C.c_int, [VP, C.POINTER(GqaPrefillDesc)]),
     "vx27_hip_gqa_decode": (C.c_int, [VP, C.POINTER(GqaDesc)]),
     "vx27_hip_gqa_decode_noalloc": (C.c_int, [VP, C.POINTER(GqaDesc)]),
+    "vx27_hip_paged_append": (C.c_int, [VP, C.POINTER(PagedAppendDesc)]),
+    "vx27_hip_paged_attn": (C.c_int, [VP, C.POINTER(PagedAttnDesc)]),
+    "vx27_hip_paged_evict": (C.c_int, [VP, C.POINTER(PagedEvictDesc)]),
     "vx27_hip_kv_write": (C.c_int, [VP, VP, VP] + [C.c_int] * 7 + [VP, VP]),
     "vx27_hip_kv_read": (C.c_int, [VP, VP, VP] + [C.c_int] * 7 + [VP, VP]),
     "vx27_hip_rope_table": (C.c_int, [VP, VP, C.c_int, C.c_int, C.c_float, C.c_float, VP, VP]),

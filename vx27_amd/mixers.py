@@ -220,3 +220,136 @@ class GatedGQALayer:
         for bb in (qb, kb, vb, pb, ob):
             bb.free()
         return out
+
+
+class PagedGQALayer:
+    """One gated GQA layer's mixer core for sequences of any length over a
+    paged bf16 KV cache (format of vx27_hip.h): a pool of n_pages pages, a
+    page list per sequence kept here on the host, and each row's accumulated
+    attention weight once a step asked for it.
+
+    step() appends the sequences' new tokens and attends from them; evict()
+    brings sequences past a budget back to it.
+    """
+
+    def __init__(self, ctx, n_seq, n_pages, page_size, q_norm_w, k_norm_w, n_q=24, n_kv=4, hd=256, rope_dim=64,
+                 theta=1e7, yarn=1.0, flags=0, window=0, n_sink=0, max_pages=None):
+        self.ctx, self.n_seq, self.n_pages, self.page = ctx, n_seq, n_pages, page_size
+        self.n_q, self.n_kv, self.hd, self.rope_dim, self.theta, self.yarn = n_q, n_kv, hd, rope_dim, theta, yarn
+        self.flags, self.window, self.n_sink = flags, window, n_sink
+        self.max_pages = max_pages or n_pages
+        n = n_pages * n_kv * page_size * hd
+        self.k_pages = ctx.buf(n * 2).zero()
+        self.v_pages = ctx.buf(n * 2).zero()
+        self.q_norm_w, self.k_norm_w = ctx.put(_f32(q_norm_w)), ctx.put(_f32(k_norm_w))
+        self.acc_stride = self.max_pages * page_size
+        self.acc = ctx.buf(n_seq * n_kv * self.acc_stride * 4).zero()
+        self.free = list(range(n_pages))[::-1]
+        self.pages = [[] for _ in range(n_seq)]
+        self.rows = [0] * n_seq          # cached rows
+        self.pos = [0] * n_seq           # positions seen (rows that were evicted included)
+
+    def _grow(self, b, rows):
+        need = -(-rows // self.page)
+        if need > self.max_pages or need - len(self.pages[b]) > len(self.free):
+            raise L.HipError(f"paged cache: sequence {b} needs {need} pages ({len(self.pages[b])} held, "
+                             f"{len(self.free)} free, {self.max_pages} at most)")
+        while len(self.pages[b]) < need:
+            self.pages[b].append(self.free.pop())
+
+    def _table(self, pages):
+        t = np.zeros((self.n_seq, self.max_pages), np.int32)
+        for b, p in enumerate(pages):
+            t[b, :len(p)] = p
+        return t
+
+    def step(self, new, qg, k_new, v_new, weigh=False, out_dtype=L.F32):
+        """new [n_seq] tokens of each sequence; qg [N][n_q][2*hd] interleaved q|gate, k_new, v_new [N][n_kv][hd],
+        the sequences' tokens one after the other.  weigh adds the rows' weights up.  Returns out [N][n_q][hd]
+        (float32)."""
+        ctx, N, hd = self.ctx, int(np.sum(new)), self.hd
+        if N == 0:
+            return np.empty((0, self.n_q, hd), np.float32)
+        for b, t in enumerate(new):
+            self._grow(b, self.rows[b] + t)
+        for b, t in enumerate(new):
+            self.rows[b] += int(t)
+        start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
+        pos = np.concatenate([np.arange(p, p + t) for p, t in zip(self.pos, new)]).astype(np.int32)
+        for b, t in enumerate(new):
+            self.pos[b] += int(t)
+        up = [ctx.put(x) for x in (_f32(qg), _f32(k_new), _f32(v_new), self._table(self.pages),
+                                   np.asarray(self.rows, np.int32), start, pos)]
+        qb, kb, vb, tb, lb, sb, pb = up
+        rot, out = ctx.buf(N * self.n_q * hd * 2), ctx.buf(N * self.n_q * hd * 4)
+        d = L.PagedAppendDesc()
+        a = L.PagedAttnDesc()
+        for x in (d, a):
+            x.B, x.n_q, x.n_kv, x.hd, x.page_size, x.n_pages = self.n_seq, self.n_q, self.n_kv, hd, self.page, self.n_pages
+            x.max_pages, x.table, x.len, x.q_start, x.n_tok, x.max_T = self.max_pages, tb.ptr, lb.ptr, sb.ptr, N, int(max(new))
+            x.k_pages, x.v_pages = self.k_pages.ptr, self.v_pages.ptr
+        d.rope_dim, d.rope_theta, d.rope_yarn, d.flags, d.pos = self.rope_dim, self.theta, self.yarn, self.flags, pb.ptr
+        d.q, d.q_tok_stride, d.q_head_stride, d.k_new, d.v_new = qb.ptr, self.n_q * 2 * hd, 2 * hd, kb.ptr, vb.ptr
+        d.q_norm_w, d.k_norm_w, d.q_out = self.q_norm_w.ptr, self.k_norm_w.ptr, rot.ptr
+        a.q, a.window, a.n_sink, a.out, a.out_dtype = rot.ptr, self.window, self.n_sink, out.ptr, out_dtype
+        if not self.flags & L.GQA_NO_GATE:
+            a.gate, a.gate_tok_stride, a.gate_head_stride = qb.ptr + hd * 4, self.n_q * 2 * hd, 2 * hd
+        if weigh:
+            a.acc, a.acc_stride = self.acc.ptr, self.acc_stride
+        check(L.lib().vx27_hip_paged_append(ctx.h, C.byref(d)), "paged_append")
+        check(L.lib().vx27_hip_paged_attn(ctx.h, C.byref(a)), "paged_attn")
+        ctx.sync()
+        if out_dtype == L.BF16:
+            res = (out.download((N, self.n_q, hd), np.uint16).astype(np.uint32) << 16).view(np.float32)
+        else:
+            res = out.download((N, self.n_q, hd), np.float32)
+        for x in up + [rot, out]:
+            x.free()
+        return res
+
+    def evict(self, budget, n_sink, n_recent):
+        """Every sequence past `budget` rows keeps that many.  Returns kept [n_seq][n_kv][budget], the old rows
+        (-1 behind a sequence's last)."""
+        ctx, n = self.ctx, [min(r, budget) for r in self.rows]
+        need = [-(-r // self.page) for r in n]
+        if sum(need) > len(self.free):
+            raise L.HipError(f"paged cache: eviction needs {sum(need)} fresh pages, {len(self.free)} are free")
+        fresh = [[self.free.pop() for _ in range(k)] for k in need]
+        width = max(1, min(self.max_pages, -(-budget // self.page)))
+        dst = self._table(fresh)[:, :width]
+        up = [ctx.put(x) for x in (self._table(self.pages), np.asarray(self.rows, np.int32), dst,
+                                   np.full((self.n_seq, self.n_kv, budget), -1, np.int32))]
+        tb, lb, db, kb = up
+        acc2, len2 = ctx.buf(self.acc.nbytes).zero(), ctx.buf(self.n_seq * 4)
+        d = L.PagedEvictDesc()
+        d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = self.n_seq, self.n_kv, self.hd, self.page, self.n_pages, self.max_pages
+        d.table, d.len, d.budget, d.n_sink, d.n_recent = tb.ptr, lb.ptr, budget, n_sink, n_recent
+        d.acc, d.acc_stride, d.k_pages, d.v_pages = self.acc.ptr, self.acc_stride, self.k_pages.ptr, self.v_pages.ptr
+        d.dst_table, d.dst_max_pages, d.dst_len, d.kept = db.ptr, width, len2.ptr, kb.ptr
+        d.acc_out, d.acc_out_stride = acc2.ptr, max(self.acc_stride, budget)
+        if budget > self.acc_stride:     # nothing can be past the budget: the weights stay where they are
+            d.acc_out = None
+        check(L.lib().vx27_hip_paged_evict(ctx.h, C.byref(d)), "paged_evict")
+        ctx.sync()
+        kept = kb.download((self.n_seq, self.n_kv, budget), np.int32)
+        self.rows = [int(x) for x in len2.download((self.n_seq,), np.int32)]
+        for p in self.pages:
+            self.free.extend(p)
+        self.pages = fresh
+        if d.acc_out:
+            self.acc.free()
+            self.acc = acc2
+        else:
+            acc2.free()
+        for x in up + [len2]:
+            x.free()
+        return kept
+
+    def read_rows(self, b):
+        """The cached rows of sequence b: K and V [rows][n_kv][hd] as float32."""
+        n, P = self.rows[b], self.page
+        k = self.k_pages.download((self.n_pages, self.n_kv, P, self.hd), np.uint16)[self.pages[b]]
+        v = self.v_pages.download((self.n_pages, self.n_kv, P // 32, self.hd, 32), np.uint16)[self.pages[b]]
+        k = k.transpose(0, 2, 1, 3).reshape(-1, self.n_kv, self.hd)[:n]
+        v = v.transpose(0, 2, 4, 1, 3).reshape(-1, self.n_kv, self.hd)[:n]
+        return tuple((x.astype(np.uint32) << 16).view(np.float32) for x in (k, v))
