@@ -19,6 +19,7 @@
 
 #include <algorithm>
 
+#include "vx_lds.h"
 #include "vx_paged.h"
 
 namespace {
@@ -174,6 +175,30 @@ __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float 
     const size_t at = (size_t)tok * a.n_q + h;
     if (a.lse) a.lse[at] = L > 0.0f || L != L ? (m + log2f(L)) * 0.6931471805599453f : -INFINITY;
     if (a.stat) a.stat[at] = make_float2(m, L > 0.0f || L != L ? 1.0f / L : 0.0f);
+}
+
+// One finished query row across a wave (lane L: dims 4L..4L+3), gated.
+__device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 r) {
+    const int lane = threadIdx.x & 63;
+    if (a.gate) {
+        const size_t at = (size_t)tok * a.g_ts + (size_t)h * a.g_hs + 4 * lane;
+        float4 x;
+        if (a.gate_bf16) {
+            const uint2 u = *(const uint2 *)((const uint16_t *)a.gate + at);
+            x = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                            __uint_as_float(u.y & 0xffff0000u));
+        } else {
+            x = *(const float4 *)((const float *)a.gate + at);
+        }
+        r.x *= 1.0f / (1.0f + expf(-x.x)); r.y *= 1.0f / (1.0f + expf(-x.y));
+        r.z *= 1.0f / (1.0f + expf(-x.z)); r.w *= 1.0f / (1.0f + expf(-x.w));
+    }
+    const size_t at = ((size_t)tok * a.n_q + h) * HDG + 4 * lane;
+    if (a.out_bf16)
+        *(uint2 *)((uint16_t *)a.out + at) = make_uint2((uint32_t)vx_f32_to_bf16(r.x) | ((uint32_t)vx_f32_to_bf16(r.y) << 16),
+                                                        (uint32_t)vx_f32_to_bf16(r.z) | ((uint32_t)vx_f32_to_bf16(r.w) << 16));
+    else
+        *(float4 *)((float *)a.out + at) = r;
 }
 
 // ---------------------------------------------------------------- decode
@@ -393,46 +418,326 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 }
 
 // ------------------------------------------------------------------ tiles
-// More than 16 query rows a KV head.  grid (64-row blocks, n_kv, B), block
-// 256: wave w takes 16 rows.
-__global__ __launch_bounds__(256) void paged_tile(Args a) {
-    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// More than 16 query rows a KV head: 128 rows (tokens x the group's heads,
+// packed) against 64 keys a step, in 4 waves, one per SIMD.  Wave (rh, ch)
+// forms S^T of rows 64 rh .. +63 and the step's key block ch (32 keys), and
+// O^T of the same rows and dims 128 ch .. +127, so K and V are each read from
+// LDS by two waves, not by four, and each operand read feeds two MFMAs
+// (v_mfma_f32_32x32x16_bf16).  The weights of the other key block come from
+// the partner wave (rh, 1 - ch) through LDS.
+//
+// Row m of a K operand holds key 16 (m/16) + 8 (m/4 % 2) + 4 (m/8 % 2) + m%4
+// of its block, so that the C layout of S^T leaves lane (g,n) with keys
+// 16 s + 8 g + 0..7 of row n in registers 8 s .. 8 s + 7: the B operand of
+// O^T += V^T P^T as it stands.  Row maxima, rescales and sums are then one
+// value a lane.
+//
+// A step's two key blocks are consecutive entries of the tile list, so a
+// sink block and the window's first block make a step without a gap.
+constexpr int TR = 128;                      // query rows of a workgroup
+constexpr int HALF = TILE * HDG * 2;         // bytes of one key block of K or of V
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+constexpr float LAZY = 8.0f;                 // a row's reference moves once its maximum is past it by 2^8
+
+struct TileSmem {
+    char k[2][2 * HALF], v[2][2 * HALF];
+    char p[4][64 * 64];                      // a wave's weights as its partner reads them
+    float mx[4][64];                         // row maxima of a wave's key block; row sums at the end
+};
+
+__device__ __forceinline__ int kswz(int r) { return (r & 3) | ((r >> 1) & 12); }
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const bf16x2_t v = (bf16x2_t){(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ bf16x8_t lds8(const char *p) { return *(const bf16x8_t *)p; }
+
+// grid (row tiles * n_split, n_kv, B), block 256.
+__global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
+    __shared__ __attribute__((aligned(16))) TileSmem sm;
+    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rh = wave >> 1, ch = wave & 1;
+    const int rt = (gridDim.x - 1 - blockIdx.x) / n_split, split = blockIdx.x % n_split;
     const vx_pseq s = vx_paged_seq(a.p, b);
-    const int R = s.T * a.qg, r0 = blockIdx.x * 64 + wave * 16;
+    const int R = s.T * a.qg, r0 = rt * TR;
     if (r0 >= R) return;
-    const vx_tiles tl = tiles_of(a, s, r0 / a.qg, min(r0 + 15, R - 1) / a.qg);
-    Rows w;
-    rows_begin(a, s, kvh, r0, w);
-    const vx_sight v = sight_of(a, s, r0 + n);
-    const int krow0 = 8 * (n >> 2) + (n & 3);
-    for (int i = 0; i < tl.nt; i++) {
-        const int key0 = tl.at(i) * TILE;
-        const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
-        const uint16_t *kr0 = a.k_pages + vx_k_index(a.p.n_kv, a.p.page_size, page, kvh, at + krow0, 8 * g);
-        const uint16_t *vt = a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, n) + 8 * g;
-        bf16x8_t ka[8], kb[8], va[16];
+    const int t0 = r0 / a.qg, t1 = min(r0 + TR - 1, R - 1) / a.qg;
+    const vx_tiles tl = tiles_of(a, s, t0, t1);
+    const int all = (tl.nt + 1) / 2, per = (all + n_split - 1) / n_split;
+    const int c0 = split * per, nt = min(per, all - c0);          // steps c0 .. c0 + nt - 1 of the list
+    // what the workgroup's rows see between them
+    const vx_sight first = vx_paged_sight(s, t0, a.window, a.n_sink), last = vx_paged_sight(s, t1, a.window, a.n_sink);
+    const int lo_min = first.i < 0 ? min(0, last.lo) : first.lo;
+
+    const int wr0 = r0 + 64 * rh;                                 // this wave's first row; rows past R repeat row R - 1
+    vx_sight v[2];
+    const uint16_t *qp[2];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            ka[k] = load8(kr0 + 32 * k);
-            kb[k] = load8(kr0 + 4 * HDG + 32 * k);
-        }
-#pragma unroll
-        for (int d = 0; d < 16; d++) va[d] = load8(vt + (size_t)d * 16 * TILE);
-        float sc[8];
-        score_tile(ka, kb, w.q, sc);
-        attend_tile<1>(w, sc, v, key0, va);
+    for (int rb = 0; rb < 2; rb++) {
+        const int r = min(wr0 + 32 * rb + n, R - 1), t = r / a.qg;
+        v[rb] = vx_paged_sight(s, t, a.window, a.n_sink);
+        qp[rb] = a.q + (size_t)(s.start + t) * a.q_ts + (size_t)(kvh * a.qg + r % a.qg) * a.q_hs + 8 * g;
     }
-    w.l += __shfl_xor(w.l, 16, 64);
-    w.l += __shfl_xor(w.l, 32, 64);
-    const int r = r0 + n;
-    if (r >= R) return;
+    const vx_sight wfirst = vx_paged_sight(s, min(wr0, R - 1) / a.qg, a.window, a.n_sink);
+    const int w_hi = wfirst.i, w_lo = vx_paged_sight(s, min(wr0 + 63, R - 1) / a.qg, a.window, a.n_sink).lo;
+
+    // key block h of step c: its first key, or none (past the list)
+    auto key_of = [&](int c, int h) -> int {
+        const int i = 2 * c + h;
+        return i < tl.nt ? tl.at(i) * TILE : -1;
+    };
+    // this wave's loads go to key block `wave / 2` of a step: 8 KiB of K (16
+    // rows) and of V (128 dims)
+    uint32_t ko[8], vo[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int r = (wave & 1) * 16 + 2 * j + (lane >> 5), d = ((wave & 1) * 8 + j) * 16 + (lane >> 2);
+        ko[j] = (uint32_t)(r * HDG * 2 + (((lane & 31) ^ kswz(r)) << 4));
+        vo[j] = (uint32_t)(d * TILE * 2 + (((lane & 3) ^ ((d >> 1) & 3)) << 4));
+    }
+    const uint32_t k_lds = vx_lds_addr(sm.k[0]) + wave * 8192, v_lds = vx_lds_addr(sm.v[0]) + wave * 8192;
+    auto page_of = [&](int c) -> size_t {   // element offset of the step's key block in the pools
+        const int key = tl.at(min(2 * c + (wave >> 1), tl.nt - 1)) * TILE;   // (past the list: its last block again)
+        const int slot = vx_page_slot(a.p, key);
+        const int page = vx_page_checked(a.p, *vx_uniform_ptr(a.p.table + (size_t)b * a.p.max_pages + slot));
+        return ((size_t)page * a.p.n_kv + kvh) * a.p.page_size * HDG + (size_t)(key - slot * a.p.page_size) * HDG;
+    };
+    auto dma_k = [&](size_t at, int buf, int j) { vx_dma16(vx_uniform_ptr((const char *)(a.k_pages + at)), ko[j], k_lds + buf * 2 * HALF + j * 1024); };
+    auto dma_v = [&](size_t at, int buf, int j) { vx_dma16(vx_uniform_ptr((const char *)(a.v_pages + at)), vo[j], v_lds + buf * 2 * HALF + j * 1024); };
+
+    floatx16_t O[2][4];
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+        for (int db = 0; db < 4; db++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) O[rb][db][i] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    if (nt > 0) {
+        size_t at1 = page_of(c0), at2 = page_of(c0 + 1);
+#pragma unroll
+        for (int j = 0; j < 8; j++) dma_k(at1, 0, j);
+#pragma unroll
+        for (int j = 0; j < 8; j++) dma_v(at1, 0, j);
+#pragma unroll
+        for (int j = 0; j < 8; j++) dma_k(at2, 1, j);
+        bf16x8_t q[2][16];
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) q[rb][k] = load8(qp[rb] + 16 * k);
+
+        // operand addresses in LDS
+        const int krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+        const int kx = g ^ kswz(krow);
+        const char *kl = sm.k[0] + ch * HALF + krow * (HDG * 2);
+        const char *vl = sm.v[0] + (128 * ch + n) * (TILE * 2);
+        const int vx = (n >> 1) & 3;
+        auto kload = [&](int buf, int k) { return lds8(kl + buf * 2 * HALF + ((k >> 3) << 8) + (((2 * (k & 7)) ^ kx) << 4)); };
+        auto vload = [&](int buf, int k, int db) { return lds8(vl + buf * 2 * HALF + (k >> 1) * HALF + db * 32 * TILE * 2 + (((2 * (k & 1) + g) ^ vx) << 4)); };
+
+        floatx16_t S[2];
+        auto s_zero = [&]() {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) S[rb][i] = 0.0f;
+        };
+        // rows' sight of a step's key block, and the row maxima for the partner
+        auto mask_max = [&](int c) {
+            const int key0 = key_of(c, ch);
+            const bool whole = key0 >= 0 && key0 + TILE - 1 <= w_hi && (key0 >= w_lo || key0 + TILE - 1 < a.n_sink);
+            if (!whole) {
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (key0 < 0 || !v[rb].sees(key0 + 16 * (i >> 3) + 8 * g + (i & 7))) S[rb][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                float x = S[rb][0];
+#pragma unroll
+                for (int i = 1; i < 16; i++) x = fmaxf(x, S[rb][i]);
+                x = fmaxf(x, __shfl_xor(x, 32, 64));
+                if (g == 0) sm.mx[wave][32 * rb + n] = x;
+            }
+        };
+
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        vx_lds_barrier();
+        s_zero();
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const bf16x8_t kf = kload(0, k);
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
+        }
+        mask_max(c0);
+
+        for (int c = 0; c < nt; c++) {
+            const int bk = c & 1;
+            // K(c+1) and V(c) have landed; every wave is done with step c-1
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            vx_lds_barrier();
+            const size_t at3 = page_of(c0 + c + 2);
+            // the rows' reference: both waves of a row see the same two maxima
+            float al[2];
+            bool moved = false;
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                const float x = fmaxf(sm.mx[wave][32 * rb + n], sm.mx[wave ^ 1][32 * rb + n]) * SC2;
+                const bool up = x > m[rb] + LAZY || (m[rb] == -INFINITY && x > m[rb]);
+                al[rb] = up ? __builtin_amdgcn_exp2f(m[rb] - x) : 1.0f;
+                m[rb] = up ? x : m[rb];
+                moved |= up;
+            }
+            if (__any(moved)) {
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++) {
+                    l[rb] *= al[rb];
+#pragma unroll
+                    for (int db = 0; db < 4; db++) O[rb][db] *= al[rb];
+                }
+            }
+            // V of keys that no row of the workgroup sees: zero, so that what
+            // stale rows hold cannot get in
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int key0 = key_of(c0 + c, h);
+                if (key0 < 0 || key0 + TILE - 1 > last.i || !(key0 >= lo_min || key0 + TILE - 1 < a.n_sink)) {
+                    uint4 *row = (uint4 *)(sm.v[bk] + h * HALF + tid * (TILE * 2));
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int key = key0 + 8 * (u ^ ((tid >> 1) & 3));
+                        uint4 x = row[u];
+                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int j = key + e;
+                            const bool seen = key0 >= 0 && j <= last.i && (j >= lo_min || j < a.n_sink);
+                            if (!seen) w[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                        }
+                        row[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            floatx16_t sc[2] = {S[0], S[1]};
+            const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+            bf16x8_t pown[2][2];
+            s_zero();
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const bf16x8_t kf = kload(bk ^ 1, k);
+                if (k < 8) {
+                    dma_k(at3, bk, k);
+                    dma_v(at2, bk ^ 1, k);
+                }
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++) {
+                    S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][k], SC2, -ms[rb]));
+                    l[rb] += p;
+                    pown[rb][k >> 3][k & 7] = (__bf16)p;
+                }
+            }
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) *(bf16x8_t *)(sm.p[wave] + ((rb * 2 + k) * 64 + lane) * 16) = pown[rb][k];
+            vx_lds_barrier();
+            bf16x8_t poth[2][2];
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) poth[rb][k] = lds8(sm.p[wave ^ 1] + ((rb * 2 + k) * 64 + lane) * 16);
+            // own key block first: the partner's weights arrive meanwhile
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) {
+                const int k = (kk & 1) + 2 * (kk < 2 ? ch : 1 - ch);
+#pragma unroll
+                for (int db = 0; db < 4; db++) {
+                    const bf16x8_t vf = vload(bk, k, db);
+#pragma unroll
+                    for (int rb = 0; rb < 2; rb++)
+                        O[rb][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, kk < 2 ? pown[rb][kk & 1] : poth[rb][kk & 1], O[rb][db], 0, 0, 0);
+                }
+            }
+            if (c + 1 < nt) mask_max(c0 + c + 1);
+            at2 = at3;
+        }
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
+    }
+    // row sums: over the lane pair and the two key blocks
+    vx_lds_barrier();
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++) {
+        l[rb] += __shfl_xor(l[rb], 32, 64);
+        if (g == 0) sm.mx[wave][32 * rb + n] = l[rb];
+    }
+    vx_lds_barrier();
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++) l[rb] += sm.mx[wave ^ 1][32 * rb + n];
+    // O through LDS (16-byte units swizzled by the row), then row by row: one
+    // row of 256 dims across a wave
+    float *so = (float *)sm.k[0];
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++) {
+        const int r = 64 * rh + 32 * rb + n;
+        const float il = n_split > 1 ? 1.0f : (l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f);
+#pragma unroll
+        for (int db = 0; db < 4; db++)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; q4++) {
+                const int u = (128 * ch + 32 * db + 8 * q4 + 4 * g) >> 2;
+                *(float4 *)(so + r * HDG + ((u ^ (r & 15)) << 2)) =
+                    make_float4(O[rb][db][4 * q4] * il, O[rb][db][4 * q4 + 1] * il, O[rb][db][4 * q4 + 2] * il, O[rb][db][4 * q4 + 3] * il);
+            }
+        if (ch == 0 && g == 0 && r0 + r < R) {
+            if (n_split > 1) {
+                const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + r) * n_split + split;
+                a.part_ml[slot] = make_float2(m[rb], l[rb]);
+            } else {
+                stat_store(a, s.start + (r0 + r) / a.qg, kvh * a.qg + (r0 + r) % a.qg, m[rb], l[rb]);
+            }
+        }
+    }
+    vx_lds_barrier();
+    for (int r = wave; r < TR && r0 + r < R; r += 4) {
+        const float4 o = *(const float4 *)(so + r * HDG + ((lane ^ (r & 15)) << 2));
+        if (n_split > 1) {
+            const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + r) * n_split + split;
+            *(float4 *)(a.part_o + slot * HDG + 4 * lane) = o;
+        } else {
+            row_store(a, s.start + (r0 + r) / a.qg, kvh * a.qg + (r0 + r) % a.qg, o);
+        }
+    }
+}
+
+// grid (max rows / 4, n_kv, B), block 256: merges a query row's n_split parts
+// in order, one row a wave.
+__global__ __launch_bounds__(256) void paged_rows_join(Args a, int n_split) {
+    const int kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+    const int r = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const vx_pseq s = vx_paged_seq(a.p, b);
+    if (r >= s.T * a.qg) return;
+    const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r) * n_split;
+    float M = -INFINITY, L = 0.0f;
+    for (int k = 0; k < n_split; k++) M = fmaxf(M, a.part_ml[slot + k].x);
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < n_split; k++) {
+        const float2 ml = a.part_ml[slot + k];
+        const float4 o = *(const float4 *)(a.part_o + (slot + k) * HDG + 4 * lane);
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        L += ml.y * w;
+        O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+    }
+    const float il = L > 0.0f || L != L ? 1.0f / L : 0.0f;
     const int tok = s.start + r / a.qg, h = kvh * a.qg + r % a.qg;
-#pragma unroll
-    for (int d = 0; d < 16; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) out_store(a, tok, h, 16 * d + 4 * g + e, w.o[d][e], w.l);
-    if (g == 0) stat_store(a, tok, h, w.m, w.l);
+    row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il));
+    if (lane == 0) stat_store(a, tok, h, M, L);
 }
 
 // grid (tile_cap / 4, n_kv, B), block 256: one wave per key tile adds the
@@ -543,10 +848,20 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         if (d->acc) VX_LAUNCH(ctx, paged_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
         return 0;
     }
+    // key splits: enough workgroups for every CU, at least 4 steps of 64 keys each
+    const int tiles = (rows + TR - 1) / TR, steps = (a.tile_cap + 1) / 2;
+    const int64_t items = (int64_t)tiles * d->n_kv * d->B;
+    const int n_split = (int)std::max<int64_t>(1, std::min<int64_t>((2 * ctx->n_cu + items - 1) / items, steps / 4));
+    a.part_rows = rows;
+    const size_t n_part = n_split > 1 ? (size_t)d->B * d->n_kv * rows * n_split : 0;
+    const size_t ml_bytes = (n_part * sizeof(float2) + 255) / 256 * 256;
     void *scr = nullptr;
-    if (d->acc && vx_ctx_scratch(ctx, stat_bytes, &scr)) return -1;
-    a.stat = (float2 *)scr;
-    VX_LAUNCH(ctx, paged_tile, dim3((rows + 63) / 64, d->n_kv, d->B), dim3(256), a);
+    if (stat_bytes + ml_bytes + n_part && vx_ctx_scratch(ctx, stat_bytes + ml_bytes + n_part * HDG * 4, &scr)) return -1;
+    a.stat = d->acc ? (float2 *)scr : nullptr;
+    a.part_ml = (float2 *)((char *)scr + stat_bytes);
+    a.part_o = (float *)((char *)scr + stat_bytes + ml_bytes);
+    VX_LAUNCH(ctx, paged_rows, dim3(tiles * n_split, d->n_kv, d->B), dim3(256), a, n_split);
+    if (n_split > 1) VX_LAUNCH(ctx, paged_rows_join, dim3((rows + 3) / 4, d->n_kv, d->B), dim3(256), a, n_split);
     if (d->acc) VX_LAUNCH(ctx, paged_tile_weigh, dim3((a.tile_cap + 3) / 4, d->n_kv, d->B), dim3(256), a);
     return 0;
 }
