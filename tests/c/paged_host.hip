@@ -30,6 +30,7 @@ int main() {
                                     const bool see = i >= 0 && j <= i && (w == 0 || j > i - w || j < s);
                                     if (see != v.sees(j)) return bad("sight", n, T, w, s, t0, t1);
                                     if (see) want.insert(j / 32);
+                                    if (((v.block(j / 32 * 32) >> (j % 32)) & 1) != (uint32_t)see) return bad("bits", n, T, w, s, t0, t1);
                                 }
                             }
                             const vx_tiles tl = vx_paged_tiles(q, t0, t1, w, s);

@@ -54,11 +54,21 @@ __host__ __device__ __forceinline__ int vx_paged_page(const vx_paged &p, int b, 
     return vx_page_checked(p, p.table[(size_t)b * p.max_pages + vx_page_slot(p, r)]);
 }
 
+// The bits of rows key0 .. key0 + 31 that lie below row n.
+__host__ __device__ __forceinline__ uint32_t vx_below(int n, int key0) {
+    if (n <= key0) return 0u;
+    return n - key0 >= 32 ? 0xffffffffu : (1u << (n - key0)) - 1u;
+}
+
 // What a token at row i sees: row j <= i if j >= lo (the window's first row)
 // or j < sink.  i = -1: nothing.
 struct vx_sight {
     int i, lo, sink;
     __host__ __device__ __forceinline__ bool sees(int j) const { return j <= i && (j >= lo || j < sink); }
+    // bits of rows key0 .. key0 + 31 (key0 >= 0)
+    __host__ __device__ __forceinline__ uint32_t block(int key0) const {
+        return vx_below(i + 1, key0) & (~vx_below(lo, key0) | vx_below(sink, key0));
+    }
 };
 __host__ __device__ __forceinline__ vx_sight vx_paged_sight(const vx_pseq &s, int t, int window, int n_sink) {
     vx_sight v;

@@ -32,6 +32,7 @@ constexpr float SC2 = 0.0625f * 1.4426950408889634f;   // 1/sqrt(256) * log2(e):
 struct Args {
     vx_paged p;
     int n_q, qg, window, n_sink;
+    uint32_t qg_magic;           // floor(2^32 / qg) + 1: row / qg as a high product (rows < 2^28), 0 for qg = 1
     const uint16_t *q;
     size_t q_ts, q_hs;
     const uint16_t *k_pages, *v_pages;
@@ -53,12 +54,16 @@ struct Args {
     float *stash;                // with acc: raw scores [B][n_kv][max rows][tile_cap * 32]
 };
 
+// The token, and the query head, of query row r of KV head kvh.
+__device__ __forceinline__ int row_tok(const Args &a, int r) { return a.qg_magic ? (int)__umulhi((uint32_t)r, a.qg_magic) : r; }
+__device__ __forceinline__ int row_head(const Args &a, int kvh, int r, int t) { return kvh * a.qg + r - t * a.qg; }
+
 __device__ __forceinline__ vx_tiles tiles_of(const Args &a, const vx_pseq &s, int t0, int t1) {
     return vx_paged_tiles(s, t0, t1, a.window, a.n_sink);
 }
 // What query row r of a sequence sees (rows past the last see nothing).
 __device__ __forceinline__ vx_sight sight_of(const Args &a, const vx_pseq &s, int r) {
-    return vx_paged_sight(s, r / a.qg, a.window, a.n_sink);
+    return vx_paged_sight(s, row_tok(a, r), a.window, a.n_sink);
 }
 
 __device__ __forceinline__ bf16x8_t load8(const uint16_t *p) { return *(const bf16x8_t *)p; }
@@ -71,9 +76,9 @@ struct Rows {
     float m, l;
 };
 __device__ __forceinline__ void rows_begin(const Args &a, const vx_pseq &s, int kvh, int r0, Rows &w) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, r = r0 + n, t = r / a.qg;
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, r = r0 + n, t = row_tok(a, r);
     const bool live = t < s.T;
-    const uint16_t *qp = a.q + (size_t)(s.start + (live ? t : 0)) * a.q_ts + (size_t)(kvh * a.qg + (live ? r % a.qg : 0)) * a.q_hs + 8 * g;
+    const uint16_t *qp = a.q + (size_t)(s.start + (live ? t : 0)) * a.q_ts + (size_t)(live ? row_head(a, kvh, r, t) : 0) * a.q_hs + 8 * g;
 #pragma unroll
     for (int k = 0; k < 8; k++) w.q[k] = load8(qp + 32 * k);
     if (!live) {
@@ -177,26 +182,30 @@ __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float 
     if (a.stat) a.stat[at] = make_float2(m, L > 0.0f || L != L ? 1.0f / L : 0.0f);
 }
 
-// One finished query row across a wave (lane L: dims 4L..4L+3), gated.
-__device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 r) {
+// hardware round-to-nearest-even pack (v_cvt_pk_bf16_f32)
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const bf16x2_t v = (bf16x2_t){(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(uint32_t, v);
+}
+// A query row's gate logits across a wave (lane L: dims 4L..4L+3).
+__device__ __forceinline__ float4 gate_row(const Args &a, int tok, int h) {
+    const size_t at = (size_t)tok * a.g_ts + (size_t)h * a.g_hs + 4 * (threadIdx.x & 63);
+    if (!a.gate_bf16) return *(const float4 *)((const float *)a.gate + at);
+    const uint2 u = *(const uint2 *)((const uint16_t *)a.gate + at);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u));
+}
+// One finished query row across a wave, gated by logits x.
+__device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 r, float4 x) {
     const int lane = threadIdx.x & 63;
-    if (a.gate) {
-        const size_t at = (size_t)tok * a.g_ts + (size_t)h * a.g_hs + 4 * lane;
-        float4 x;
-        if (a.gate_bf16) {
-            const uint2 u = *(const uint2 *)((const uint16_t *)a.gate + at);
-            x = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                            __uint_as_float(u.y & 0xffff0000u));
-        } else {
-            x = *(const float4 *)((const float *)a.gate + at);
-        }
-        r.x *= 1.0f / (1.0f + expf(-x.x)); r.y *= 1.0f / (1.0f + expf(-x.y));
-        r.z *= 1.0f / (1.0f + expf(-x.z)); r.w *= 1.0f / (1.0f + expf(-x.w));
+    if (a.gate) {   // (hardware reciprocals: one part in 2^23, below the weights' rounding)
+        auto sg = [](float y) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f)); };
+        r.x *= sg(x.x); r.y *= sg(x.y); r.z *= sg(x.z); r.w *= sg(x.w);
     }
     const size_t at = ((size_t)tok * a.n_q + h) * HDG + 4 * lane;
     if (a.out_bf16)
-        *(uint2 *)((uint16_t *)a.out + at) = make_uint2((uint32_t)vx_f32_to_bf16(r.x) | ((uint32_t)vx_f32_to_bf16(r.y) << 16),
-                                                        (uint32_t)vx_f32_to_bf16(r.z) | ((uint32_t)vx_f32_to_bf16(r.w) << 16));
+        *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack2(r.x, r.y), pack2(r.z, r.w));
     else
         *(float4 *)((float *)a.out + at) = r;
 }
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
                 O += s_o[k][r * HDG + ((((tid >> 2) ^ r) << 2) | (tid & 3))] * sc;
             }
             if (whole) {
-                const int tok = s.start + r / a.qg, h = kvh * a.qg + r % a.qg;
+                const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
                 out_store(a, tok, h, tid, O, L);
                 if (tid == 0) stat_store(a, tok, h, M, L);
             } else {
@@ -346,7 +355,7 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const vx_pseq s = vx_paged_seq(a.p, b);
     if (r >= s.T * a.qg) return;
-    const int tok = s.start + r / a.qg, h = kvh * a.qg + r % a.qg;
+    const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
     const int nt = tiles_of(a, s, 0, s.T - 1).nt;
     if (nt == 0) {
         out_store(a, tok, h, tid, 0.0f, 0.0f);
@@ -410,7 +419,8 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
     bool any = false;
     for (int r = 0; r < s.T * a.qg; r++) {
         if (!sight_of(a, s, r).sees(j)) continue;
-        const float2 ml = a.stat[(size_t)(s.start + r / a.qg) * a.n_q + kvh * a.qg + r % a.qg];
+        const int t = row_tok(a, r);
+        const float2 ml = a.stat[(size_t)(s.start + t) * a.n_q + row_head(a, kvh, r, t)];
         sum += __builtin_amdgcn_exp2f(__builtin_fmaf(st[r * stride], SC2, -ml.x)) * ml.y;
         any = true;
     }
@@ -446,41 +456,43 @@ struct TileSmem {
 };
 
 __device__ __forceinline__ int kswz(int r) { return (r & 3) | ((r >> 1) & 12); }
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-    const bf16x2_t v = (bf16x2_t){(__bf16)x, (__bf16)y};
-    return __builtin_bit_cast(uint32_t, v);
-}
 __device__ __forceinline__ bf16x8_t lds8(const char *p) { return *(const bf16x8_t *)p; }
 
-// grid (row tiles * n_split, n_kv, B), block 256.
-__global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
+// grid (items rounded up to 8), block 256; an item is (sequence, KV head, row
+// tile, key split).
+__global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_rt, int n_split) {
     __shared__ __attribute__((aligned(16))) TileSmem sm;
-    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rh = wave >> 1, ch = wave & 1;
-    const int rt = (gridDim.x - 1 - blockIdx.x) / n_split, split = blockIdx.x % n_split;
+    // The dispatcher deals workgroups round-robin over the 8 XCDs: XCD x takes
+    // a contiguous run of the items, so that the row tiles in flight on it
+    // are neighbours, whose keys its L2 then holds once.
+    const int per_xcd = (n_items + 7) / 8, item = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || item >= n_items) return;
+    const int split = item % n_split, rt = n_rt - 1 - item / n_split % n_rt, kvh = item / n_split / n_rt % a.p.n_kv, b = item / n_split / n_rt / a.p.n_kv;
     const vx_pseq s = vx_paged_seq(a.p, b);
     const int R = s.T * a.qg, r0 = rt * TR;
     if (r0 >= R) return;
-    const int t0 = r0 / a.qg, t1 = min(r0 + TR - 1, R - 1) / a.qg;
+    const int t0 = row_tok(a, r0), t1 = row_tok(a, min(r0 + TR - 1, R - 1));
     const vx_tiles tl = tiles_of(a, s, t0, t1);
     const int all = (tl.nt + 1) / 2, per = (all + n_split - 1) / n_split;
     const int c0 = split * per, nt = min(per, all - c0);          // steps c0 .. c0 + nt - 1 of the list
     // what the workgroup's rows see between them
-    const vx_sight first = vx_paged_sight(s, t0, a.window, a.n_sink), last = vx_paged_sight(s, t1, a.window, a.n_sink);
-    const int lo_min = first.i < 0 ? min(0, last.lo) : first.lo;
+    vx_sight any = vx_paged_sight(s, t0, a.window, a.n_sink);
+    if (any.i < 0) any.lo = 0;
+    any.i = vx_paged_sight(s, t1, a.window, a.n_sink).i;
 
     const int wr0 = r0 + 64 * rh;                                 // this wave's first row; rows past R repeat row R - 1
     vx_sight v[2];
     const uint16_t *qp[2];
 #pragma unroll
     for (int rb = 0; rb < 2; rb++) {
-        const int r = min(wr0 + 32 * rb + n, R - 1), t = r / a.qg;
+        const int r = min(wr0 + 32 * rb + n, R - 1), t = row_tok(a, r);
         v[rb] = vx_paged_sight(s, t, a.window, a.n_sink);
-        qp[rb] = a.q + (size_t)(s.start + t) * a.q_ts + (size_t)(kvh * a.qg + r % a.qg) * a.q_hs + 8 * g;
+        qp[rb] = a.q + (size_t)(s.start + t) * a.q_ts + (size_t)row_head(a, kvh, r, t) * a.q_hs + 8 * g;
     }
-    const vx_sight wfirst = vx_paged_sight(s, min(wr0, R - 1) / a.qg, a.window, a.n_sink);
-    const int w_hi = wfirst.i, w_lo = vx_paged_sight(s, min(wr0 + 63, R - 1) / a.qg, a.window, a.n_sink).lo;
+    const vx_sight wfirst = vx_paged_sight(s, row_tok(a, min(wr0, R - 1)), a.window, a.n_sink);
+    const int w_hi = wfirst.i, w_lo = vx_paged_sight(s, row_tok(a, min(wr0 + 63, R - 1)), a.window, a.n_sink).lo;
 
     // key block h of step c: its first key, or none (past the list)
     auto key_of = [&](int c, int h) -> int {
@@ -489,22 +501,35 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
     };
     // this wave's loads go to key block `wave / 2` of a step: 8 KiB of K (16
     // rows) and of V (128 dims)
-    uint32_t ko[8], vo[8];
+    // (of K, row r's unit u goes to slot u ^ kswz(r); over j only two bits of
+    // kswz change, so four offsets serve the eight loads, j KiB apart)
+    uint32_t ko[4];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const int r = (wave & 1) * 16 + 2 * j + (lane >> 5), d = ((wave & 1) * 8 + j) * 16 + (lane >> 2);
-        ko[j] = (uint32_t)(r * HDG * 2 + (((lane & 31) ^ kswz(r)) << 4));
-        vo[j] = (uint32_t)(d * TILE * 2 + (((lane & 3) ^ ((d >> 1) & 3)) << 4));
+    for (int j = 0; j < 4; j++) {
+        const int r = (wave & 1) * 16 + 2 * (j & 1) + 8 * (j >> 1) + (lane >> 5);
+        ko[j] = (uint32_t)((lane >> 5) * HDG * 2 + (((lane & 31) ^ kswz(r)) << 4)) + (wave & 1) * 8192;
     }
+    const uint32_t vo = (uint32_t)((lane >> 2) * TILE * 2 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4)) + (wave & 1) * 8192;
     const uint32_t k_lds = vx_lds_addr(sm.k[0]) + wave * 8192, v_lds = vx_lds_addr(sm.v[0]) + wave * 8192;
-    auto page_of = [&](int c) -> size_t {   // element offset of the step's key block in the pools
-        const int key = tl.at(min(2 * c + (wave >> 1), tl.nt - 1)) * TILE;   // (past the list: its last block again)
-        const int slot = vx_page_slot(a.p, key);
-        const int page = vx_page_checked(a.p, *vx_uniform_ptr(a.p.table + (size_t)b * a.p.max_pages + slot));
-        return ((size_t)page * a.p.n_kv + kvh) * a.p.page_size * HDG + (size_t)(key - slot * a.p.page_size) * HDG;
+    // Element offsets in the pools of this wave's key blocks: lane i holds the
+    // block of step base + i (past the list: its last block again), so a step
+    // reads a lane and not the page table.
+    int base = c0;
+    uint32_t at_lo, at_hi;
+    auto fill_at = [&]() {
+        const int key = tl.at(min(2 * (base + lane) + (wave >> 1), tl.nt - 1)) * TILE, slot = vx_page_slot(a.p, key);
+        const int page = vx_page_checked(a.p, a.p.table[(size_t)b * a.p.max_pages + slot]);
+        const uint64_t at = (((uint64_t)page * a.p.n_kv + kvh) * a.p.page_size + (key - slot * a.p.page_size)) * HDG;
+        at_lo = (uint32_t)at;
+        at_hi = (uint32_t)(at >> 32);
     };
-    auto dma_k = [&](size_t at, int buf, int j) { vx_dma16(vx_uniform_ptr((const char *)(a.k_pages + at)), ko[j], k_lds + buf * 2 * HALF + j * 1024); };
-    auto dma_v = [&](size_t at, int buf, int j) { vx_dma16(vx_uniform_ptr((const char *)(a.v_pages + at)), vo[j], v_lds + buf * 2 * HALF + j * 1024); };
+    auto at_of = [&](int c) -> size_t {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, c - base) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, c - base);
+    };
+    auto dma_k = [&](size_t at, int buf, int j) {
+        vx_dma16((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)] + j * 1024, k_lds + buf * 2 * HALF + j * 1024);
+    };
+    auto dma_v = [&](size_t at, int buf, int j) { vx_dma16((const char *)(a.v_pages + at), vo + j * 1024, v_lds + buf * 2 * HALF + j * 1024); };
 
     floatx16_t O[2][4];
 #pragma unroll
@@ -514,21 +539,39 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
 #pragma unroll
             for (int i = 0; i < 16; i++) O[rb][db][i] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    auto pin_o = [&]() {
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+            for (int db = 0; db < 4; db++) __asm__ volatile("" : "+a"(O[rb][db]));
+    };
 
     if (nt > 0) {
-        size_t at1 = page_of(c0), at2 = page_of(c0 + 1);
+        fill_at();
+        size_t at_v = at_of(c0), at_k = at_of(c0 + 1);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at1, 0, j);
+        for (int j = 0; j < 8; j++) dma_k(at_v, 0, j);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_v(at1, 0, j);
+        for (int j = 0; j < 8; j++) dma_k(at_k, 1, j);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at2, 1, j);
+        for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
+        at_v = at_k;
+        at_k = at_of(c0 + 2);
         bf16x8_t q[2][16];
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int k = 0; k < 16; k++) q[rb][k] = load8(qp[rb] + 16 * k);
 
+        auto pin_q = [&]() {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    if (k < 12) __asm__ volatile("" : "+a"(q[rb][k]));
+                    else __asm__ volatile("" : "+v"(q[rb][k]));
+                }
+        };
         // operand addresses in LDS
         const int krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
         const int kx = g ^ kswz(krow);
@@ -545,25 +588,61 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) S[rb][i] = 0.0f;
         };
-        // rows' sight of a step's key block, and the row maxima for the partner
-        auto mask_max = [&](int c) {
+        // whether some row of the wave does not see all of step c's key block
+        auto cut = [&](int c) {
             const int key0 = key_of(c, ch);
-            const bool whole = key0 >= 0 && key0 + TILE - 1 <= w_hi && (key0 >= w_lo || key0 + TILE - 1 < a.n_sink);
-            if (!whole) {
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (key0 < 0 || !v[rb].sees(key0 + 16 * (i >> 3) + 8 * g + (i & 7))) S[rb][i] = -INFINITY;
-            }
+            return key0 < 0 || key0 + TILE - 1 > w_hi || (key0 < w_lo && key0 + TILE - 1 >= a.n_sink);
+        };
+        floatx16_t sc[2];          // this step's scores
+        auto mask = [&](int c) {
+            const int key0 = key_of(c, ch);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) {
-                float x = S[rb][0];
+                const uint32_t bits = key0 < 0 ? 0u : v[rb].block(key0) >> (8 * g);
 #pragma unroll
-                for (int i = 1; i < 16; i++) x = fmaxf(x, S[rb][i]);
-                x = fmaxf(x, __shfl_xor(x, 32, 64));
-                if (g == 0) sm.mx[wave][32 * rb + n] = x;
+                for (int i = 0; i < 16; i++)
+                    if (!(bits & (1u << (16 * (i >> 3) + (i & 7))))) sc[rb][i] = -INFINITY;
             }
+        };
+        auto row_max = [&](float (&x)[2]) {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                x[rb] = sc[rb][0];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) __asm__("v_max3_f32 %0, %0, %1, %2" : "+v"(x[rb]) : "v"(sc[rb][i]), "v"(sc[rb][i + 1]));
+            }
+        };
+        // the rows' maxima for both waves (x: over a lane's keys)
+        auto publish = [&](const float (&x)[2]) {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                const float y = fmaxf(x[rb], __uint_as_float(vx_xor32_u32(__float_as_uint(x[rb]))));
+                sm.mx[wave][32 * rb + n] = y;   // (both lanes of a row write the same value)
+            }
+        };
+        // V of keys that no row of the workgroup sees: zero, so that what stale
+        // rows hold cannot get in (only sink blocks, the window's first and
+        // the last block have such keys)
+        auto bare = [&](int c) { return 2 * c <= tl.st || 2 * c + 2 >= tl.nt; };
+        auto clear_v = [&](int c, int buf) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int key0 = key_of(c, h);
+                const uint32_t seen = key0 < 0 ? 0u : any.block(key0);
+                if (seen != 0xffffffffu) {
+                    uint4 *row = (uint4 *)(sm.v[buf] + h * HALF + tid * (TILE * 2));
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const uint32_t byte = seen >> (8 * (u ^ ((tid >> 1) & 3)));
+                        uint4 x = row[u];
+                        uint32_t *w = (uint32_t *)&x;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] &= ((byte >> (2 * e)) & 1 ? 0xffffu : 0u) | ((byte >> (2 * e)) & 2 ? 0xffff0000u : 0u);
+                        row[u] = x;
+                    }
+                }
+            }
+            vx_lds_barrier();
         };
 
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -575,25 +654,85 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
         }
-        mask_max(c0);
+        sc[0] = S[0];
+        sc[1] = S[1];
+        if (cut(c0)) mask(c0);
+        {
+            float x[2];
+            row_max(x);
+            publish(x);
+        }
 
+        // A step: S of the next step on the MFMAs with this step's softmax and
+        // the loads of K(c+2) beside it, the weights' exchange, then P V with
+        // the next maxima and the loads of V(c+1) beside it.  Each wait leaves
+        // the eight newer loads in flight.
+        bool edge = bare(c0), cut1 = nt > 1 && cut(c0 + 1);
         for (int c = 0; c < nt; c++) {
             const int bk = c & 1;
-            // K(c+1) and V(c) have landed; every wave is done with step c-1
-            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            // K(c+1) has landed; every wave is done with step c-1
+            __asm__ volatile("s_waitcnt vmcnt(8)" ::: "memory");
             vx_lds_barrier();
-            const size_t at3 = page_of(c0 + c + 2);
+            float mine[2], other[2];
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                mine[rb] = sm.mx[wave][32 * rb + n];
+                other[rb] = sm.mx[wave ^ 1][32 * rb + n];
+            }
+            bf16x8_t kf[4];   // K operands, three k-steps ahead
+#pragma unroll
+            for (int k = 0; k < 3; k++) kf[k] = kload(bk ^ 1, k);
+            s_zero();
+            pin_q();
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8_t pown[2][2];
+            float ms[2];
+            // One MFMA at a time with its share of the VALU's and the loads' work
+            // behind it, in this order: what stands behind an MFMA that waits
+            // for the pipe waits too.  Element i of a row block goes through
+            // the softmax in three such shares (argument, exp2, sum and
+            // rounding), so that none waits for its own result.
+            auto s_mfma = [&](int k, int rb) {
+                if (rb == 0 && k + 3 < 16) kf[(k + 3) & 3] = kload(bk ^ 1, k + 3);
+                if (rb == 1 && k < 8) dma_k(at_k, bk, k);
+                S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k & 3], q[rb][k], S[rb], 0, 0, 0);
+            };
+            float e[2][16];
+            constexpr auto at = [](int j) { return j < 0 ? 0 : j > 13 ? 16 : j * 16 / 13; };
+            auto weigh = [&](int rb, int j) {   // share j of 0..14
+#pragma unroll
+                for (int i = at(j - 2); i < at(j - 1); i++) {
+                    l[rb] += e[rb][i];
+                    __asm__ volatile("" : "+v"(l[rb]));
+                    pown[rb][i >> 3][i & 7] = (__bf16)e[rb][i];
+                }
+#pragma unroll
+                for (int i = at(j - 1); i < at(j); i++) e[rb][i] = __builtin_amdgcn_exp2f(e[rb][i]);
+#pragma unroll
+                for (int i = at(j); i < at(j + 1); i++) e[rb][i] = __builtin_fmaf(sc[rb][i], SC2, -ms[rb]);
+            };
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++) {
+                    s_mfma(k, rb);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             // the rows' reference: both waves of a row see the same two maxima
             float al[2];
             bool moved = false;
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) {
-                const float x = fmaxf(sm.mx[wave][32 * rb + n], sm.mx[wave ^ 1][32 * rb + n]) * SC2;
-                const bool up = x > m[rb] + LAZY || (m[rb] == -INFINITY && x > m[rb]);
+                const float x = fmaxf(mine[rb], other[rb]) * SC2;
+                const bool up = x > m[rb] + LAZY;
                 al[rb] = up ? __builtin_amdgcn_exp2f(m[rb] - x) : 1.0f;
                 m[rb] = up ? x : m[rb];
+                ms[rb] = m[rb] == -INFINITY ? 0.0f : m[rb];
                 moved |= up;
             }
+            // (O stays in the MFMAs' accumulators around the rare rescale: without
+            // the pins it is copied out and back in every step)
+            pin_o();
             if (__any(moved)) {
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) {
@@ -602,73 +741,82 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
                     for (int db = 0; db < 4; db++) O[rb][db] *= al[rb];
                 }
             }
-            // V of keys that no row of the workgroup sees: zero, so that what
-            // stale rows hold cannot get in
+            pin_o();
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int key0 = key_of(c0 + c, h);
-                if (key0 < 0 || key0 + TILE - 1 > last.i || !(key0 >= lo_min || key0 + TILE - 1 < a.n_sink)) {
-                    uint4 *row = (uint4 *)(sm.v[bk] + h * HALF + tid * (TILE * 2));
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const int key = key0 + 8 * (u ^ ((tid >> 1) & 3));
-                        uint4 x = row[u];
-                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int j = key + e;
-                            const bool seen = key0 >= 0 && j <= last.i && (j >= lo_min || j < a.n_sink);
-                            if (!seen) w[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-                        }
-                        row[u] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            }
-            floatx16_t sc[2] = {S[0], S[1]};
-            const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-            bf16x8_t pown[2][2];
-            s_zero();
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const bf16x8_t kf = kload(bk ^ 1, k);
-                if (k < 8) {
-                    dma_k(at3, bk, k);
-                    dma_v(at2, bk ^ 1, k);
-                }
+            for (int k = 2; k < 16; k++)
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) {
-                    S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][k], SC2, -ms[rb]));
-                    l[rb] += p;
-                    pown[rb][k >> 3][k & 7] = (__bf16)p;
+                    s_mfma(k, rb);
+                    weigh(rb, k - 2);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) weigh(rb, 14);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++)
 #pragma unroll
                 for (int k = 0; k < 2; k++) *(bf16x8_t *)(sm.p[wave] + ((rb * 2 + k) * 64 + lane) * 16) = pown[rb][k];
+            // V(c) has landed, and every wave's weights are there
+            __asm__ volatile("s_waitcnt vmcnt(8)" ::: "memory");
             vx_lds_barrier();
-            bf16x8_t poth[2][2];
+            if (edge) clear_v(c0 + c, bk);
+            // own key block first: the partner's weights arrive meanwhile
+            bf16x8_t poth[2][2], vf[4];   // V operands three ahead
+            auto vstep = [&](int i) { return vload(bk, ((i >> 2) & 1) + 2 * (i < 8 ? ch : 1 - ch), i & 3); };
+#pragma unroll
+            for (int i = 0; i < 3; i++) vf[i] = vstep(i);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++)
 #pragma unroll
                 for (int k = 0; k < 2; k++) poth[rb][k] = lds8(sm.p[wave ^ 1] + ((rb * 2 + k) * 64 + lane) * 16);
-            // own key block first: the partner's weights arrive meanwhile
+            float x[2];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                const int k = (kk & 1) + 2 * (kk < 2 ? ch : 1 - ch);
+            for (int i = 0; i < 16; i++) {
 #pragma unroll
-                for (int db = 0; db < 4; db++) {
-                    const bf16x8_t vf = vload(bk, k, db);
-#pragma unroll
-                    for (int rb = 0; rb < 2; rb++)
-                        O[rb][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, kk < 2 ? pown[rb][kk & 1] : poth[rb][kk & 1], O[rb][db], 0, 0, 0);
+                for (int rb = 0; rb < 2; rb++) {
+                    if (rb == 0 && i + 3 < 16) vf[(i + 3) & 3] = vstep(i + 3);
+                    if (rb == 1 && i < 8) dma_v(at_v, bk ^ 1, i);
+                    O[rb][i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 3], i < 8 ? pown[rb][(i >> 2) & 1] : poth[rb][(i >> 2) & 1],
+                                                                           O[rb][i & 3], 0, 0, 0);
+                    sc[rb][i] = S[rb][i];
+                    // (in asm: here, not in a row behind the MFMAs, and without
+                    // the quieting of NaN that fmaxf puts before each)
+                    if (i == 0) x[rb] = sc[rb][0];
+                    else if (i & 1) __asm__ volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x[rb]) : "v"(sc[rb][i - 1]), "v"(sc[rb][i]));
+                    // the next step's addresses
+                    if (rb == 1 && i == 8) at_v = at_k, at_k = at_of(c0 + c + 3);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (c + 1 < nt) mask_max(c0 + c + 1);
-            at2 = at3;
+            if (cut1) {
+                mask(c0 + c + 1);
+                row_max(x);
+            }
+            publish(x);
+            edge = bare(c0 + c + 1);
+            cut1 = c + 2 < nt && cut(c0 + c + 2);
+            if (c0 + c + 5 > base + 63) {   // (one step in 60)
+                base = c0 + c + 4;
+                fill_at();
+            }
         }
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
+    }
+    // Gates of this wave's output rows (wave, wave + 4, ...: one row of 256
+    // dims across a wave), all loaded before the first is used: a load behind
+    // the rows' stores would wait for them.
+    constexpr int WR = TR / 4;
+    uint2 gt[WR];
+    const bool gated = a.gate && n_split == 1;
+    auto row_of = [&](int k) { return min(r0 + wave + 4 * k, R - 1); };
+    if (gated && a.gate_bf16) {
+#pragma unroll
+        for (int k = 0; k < WR; k++) {
+            const int r = row_of(k), t = row_tok(a, r);
+            gt[k] = *(const uint2 *)((const uint16_t *)a.gate + (size_t)(s.start + t) * a.g_ts + (size_t)row_head(a, kvh, r, t) * a.g_hs + 4 * lane);
+        }
     }
     // row sums: over the lane pair and the two key blocks
     vx_lds_barrier();
@@ -678,13 +826,11 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
         if (g == 0) sm.mx[wave][32 * rb + n] = l[rb];
     }
     vx_lds_barrier();
-#pragma unroll
-    for (int rb = 0; rb < 2; rb++) l[rb] += sm.mx[wave ^ 1][32 * rb + n];
-    // O through LDS (16-byte units swizzled by the row), then row by row: one
-    // row of 256 dims across a wave
+    // O through LDS (16-byte units swizzled by the row)
     float *so = (float *)sm.k[0];
 #pragma unroll
     for (int rb = 0; rb < 2; rb++) {
+        l[rb] += sm.mx[wave ^ 1][32 * rb + n];
         const int r = 64 * rh + 32 * rb + n;
         const float il = n_split > 1 ? 1.0f : (l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f);
 #pragma unroll
@@ -700,19 +846,37 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_split) {
                 const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + r) * n_split + split;
                 a.part_ml[slot] = make_float2(m[rb], l[rb]);
             } else {
-                stat_store(a, s.start + (r0 + r) / a.qg, kvh * a.qg + (r0 + r) % a.qg, m[rb], l[rb]);
+                const int t = row_tok(a, r0 + r);
+                stat_store(a, s.start + t, row_head(a, kvh, r0 + r, t), m[rb], l[rb]);
             }
         }
     }
     vx_lds_barrier();
-    for (int r = wave; r < TR && r0 + r < R; r += 4) {
-        const float4 o = *(const float4 *)(so + r * HDG + ((lane ^ (r & 15)) << 2));
-        if (n_split > 1) {
-            const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + r) * n_split + split;
-            *(float4 *)(a.part_o + slot * HDG + 4 * lane) = o;
-        } else {
-            row_store(a, s.start + (r0 + r) / a.qg, kvh * a.qg + (r0 + r) % a.qg, o);
+    auto orow = [&](int k) {
+        const int r = wave + 4 * k;
+        return *(const float4 *)(so + r * HDG + ((lane ^ (r & 15)) << 2));
+    };
+    if (n_split > 1) {
+#pragma unroll 4
+        for (int k = 0; k < WR; k++) {
+            const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + wave + 4 * k) * n_split + split;
+            if (r0 + wave + 4 * k < R) *(float4 *)(a.part_o + slot * HDG + 4 * lane) = orow(k);
         }
+        return;
+    }
+    float4 on = orow(0);
+#pragma unroll
+    for (int k = 0; k < WR; k++) {
+        const float4 o = on;
+        if (k + 1 < WR) on = orow(k + 1);
+        const int r = r0 + wave + 4 * k, t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
+        if (r >= R) break;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (gated)
+            x = a.gate_bf16 ? make_float4(__uint_as_float(gt[k].x << 16), __uint_as_float(gt[k].x & 0xffff0000u), __uint_as_float(gt[k].y << 16),
+                                          __uint_as_float(gt[k].y & 0xffff0000u))
+                            : gate_row(a, tok, h);
+        row_store(a, tok, h, o, x);
     }
 }
 
@@ -735,8 +899,9 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a, int n_split) {
         O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
     }
     const float il = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    const int tok = s.start + r / a.qg, h = kvh * a.qg + r % a.qg;
-    row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il));
+    const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
+    const float4 gt = a.gate ? gate_row(a, tok, h) : make_float4(0.f, 0.f, 0.f, 0.f);
+    row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il), gt);
     if (lane == 0) stat_store(a, tok, h, M, L);
 }
 
@@ -764,7 +929,8 @@ __global__ __launch_bounds__(256) void paged_tile_weigh(Args a) {
         rows_begin(a, s, kvh, r0, w);
         const vx_sight v = sight_of(a, s, r0 + n);
         const int r = min(r0 + n, s.T * a.qg - 1);
-        const float2 ml = a.stat[(size_t)(s.start + r / a.qg) * a.n_q + kvh * a.qg + r % a.qg];
+        const int t = row_tok(a, r);
+        const float2 ml = a.stat[(size_t)(s.start + t) * a.n_q + row_head(a, kvh, r, t)];
         float sc[8];
         score_tile(ka, kb, w.q, sc);
 #pragma unroll
@@ -811,8 +977,8 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     const int64_t cap = (int64_t)d->max_pages * d->page_size;
     VX_REQUIRE(!d->acc || (int64_t)d->acc_stride >= cap, "%s: acc_stride must be at least max_pages * page_size (got %zu, %lld)", who,
                d->acc_stride, (long long)cap);
-    a.n_q = d->n_q; a.qg = d->n_q / d->n_kv; a.window = d->window; a.n_sink = d->n_sink;
-    VX_REQUIRE((int64_t)d->max_T * a.qg < (1 << 30), "%s: max_T * n_q/n_kv is past 2^30 (max_T=%d)", who, d->max_T);
+    a.n_q = d->n_q; a.qg = d->n_q / d->n_kv; a.qg_magic = a.qg == 1 ? 0 : (uint32_t)((1ull << 32) / a.qg + 1); a.window = d->window; a.n_sink = d->n_sink;
+    VX_REQUIRE((int64_t)d->max_T * a.qg < (1 << 28), "%s: max_T * n_q/n_kv is past 2^28 (max_T=%d)", who, d->max_T);
     if (vx_ctx_enter(ctx)) return -1;
     if (d->n_tok == 0) return 0;
     a.p.err_flag = ctx->err_flag;
@@ -860,7 +1026,9 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     a.stat = d->acc ? (float2 *)scr : nullptr;
     a.part_ml = (float2 *)((char *)scr + stat_bytes);
     a.part_o = (float *)((char *)scr + stat_bytes + ml_bytes);
-    VX_LAUNCH(ctx, paged_rows, dim3(tiles * n_split, d->n_kv, d->B), dim3(256), a, n_split);
+    const int64_t n_items = items * n_split;
+    VX_REQUIRE(n_items < (1ll << 31) - 8, "%s: more than 2^31 workgroups (B=%d n_kv=%d max_T=%d)", who, d->B, d->n_kv, d->max_T);
+    VX_LAUNCH(ctx, paged_rows, dim3((unsigned)((n_items + 7) / 8 * 8)), dim3(256), a, (int)n_items, tiles, n_split);
     if (n_split > 1) VX_LAUNCH(ctx, paged_rows_join, dim3((rows + 3) / 4, d->n_kv, d->B), dim3(256), a, n_split);
     if (d->acc) VX_LAUNCH(ctx, paged_tile_weigh, dim3((a.tile_cap + 3) / 4, d->n_kv, d->B), dim3(256), a);
     return 0;
