@@ -29,6 +29,9 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 constexpr float SC2 = 0.0625f * 1.4426950408889634f;   // 1/sqrt(256) * log2(e): scores in the exp2 domain
 
+struct RowPlan;
+struct RowPiece;
+struct RowJoin;
 struct Args {
     vx_paged p;
     int n_q, qg, window, n_sink;
@@ -51,6 +54,10 @@ struct Args {
     float *part_o;               // [2 grid][max rows][256]
     float2 *part_ml;             // [2 grid][max rows]
     int part_rows;
+    // tiles (scratch)
+    RowPlan *plan;
+    RowPiece *pieces;
+    RowJoin *joins;
     float *stash;                // with acc: raw scores [B][n_kv][max rows][tile_cap * 32]
 };
 
@@ -458,25 +465,162 @@ struct TileSmem {
 __device__ __forceinline__ int kswz(int r) { return (r & 3) | ((r >> 1) & 12); }
 __device__ __forceinline__ bf16x8_t lds8(const char *p) { return *(const bf16x8_t *)p; }
 
-// grid (items rounded up to 8), block 256; an item is (sequence, KV head, row
-// tile, key split).
-__global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_rt, int n_split) {
+// An item is a row tile of a sequence and KV head.  One workgroup of
+// paged_plan lists the items (by KV head, sequence, last rows first), cut
+// into pieces of at most `limit` steps where there are too few items for the
+// CUs; paged_rows runs one workgroup a piece, and the parts of a cut item go
+// to slots that paged_rows_join adds up in order.
+struct RowPiece {
+    int b, kvh, r0, c0, c1, slot, pad[2];     // steps c0 .. c1 - 1 of its list; slot -1: the whole item
+};
+struct RowJoin {
+    int b, kvh, r0, slot, parts, pad[3];
+};
+struct RowPlan {
+    int pieces, joins;
+    int heads[8];                             // pieces taken of each XCD's run
+};
+__device__ __forceinline__ int row_tiles(const Args &a, const vx_pseq &s) { return (s.T * a.qg + TR - 1) / TR; }
+// Steps of entry e = b * n_rt + k of one KV head, row tile k from the end of
+// sequence b (rows that see nothing: one, for their output); 0 past its rows.
+__device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &b, int &r0) {
+    b = e / n_rt;
+    const vx_pseq s = vx_paged_seq(a.p, b);
+    const int rt = row_tiles(a, s) - 1 - (e - b * n_rt);
+    if (rt < 0) return 0;
+    r0 = rt * TR;
+    const vx_tiles tl = tiles_of(a, s, row_tok(a, r0), row_tok(a, min(r0 + TR, s.T * a.qg) - 1));
+    return max(1, (tl.nt + 1) / 2);
+}
+
+// grid 1, block 1024.
+constexpr int PLAN = 1024;
+__global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, int max_pieces) {
+    __shared__ int64_t s_steps[PLAN / 64];
+    __shared__ int s_sum[3][PLAN / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int E = a.p.B * n_rt, per = (E + PLAN - 1) / PLAN, e0 = min(tid * per, E);
+    int e1 = min(e0 + per, E);
+    int b, r0 = 0, items = 0;
+    int64_t steps = 0;
+    for (int e = e0; e < e1; e++) {
+        const int n = entry_steps(a, n_rt, e, b, r0);
+        steps += n;
+        items += n > 0;
+    }
+    for (int off = 32; off >= 1; off >>= 1) {
+        steps += __shfl_xor(steps, off, 64);
+        items += __shfl_xor(items, off, 64);
+    }
+    if (lane == 0) {
+        s_steps[wave] = steps;
+        s_sum[0][wave] = items;
+    }
+    __syncthreads();
+    steps = items = 0;
+    for (int w = 0; w < PLAN / 64; w++) {
+        steps += s_steps[w];
+        items += s_sum[0][w];
+    }
+    // As many rounds of the CUs as leave at least half a round for cuts, and
+    // pieces short enough to fill them: at most 3/2 n_cu cuts.
+    const int64_t I = (int64_t)items * a.p.n_kv, room = ((I + n_cu / 2 + n_cu - 1) / n_cu) * n_cu - I;
+    const int limit = (int)max((steps * a.p.n_kv + room - 1) / room, (int64_t)4);
+    __syncthreads();
+    // (pieces, slots, joins) of this thread's entries, then their places
+    int cnt[3] = {0, 0, 0};
+    for (int e = e0; e < e1; e++) {
+        const int n = entry_steps(a, n_rt, e, b, r0), parts = (n + limit - 1) / limit;
+        cnt[0] += parts;
+        cnt[1] += parts > 1 ? parts : 0;
+        cnt[2] += parts > 1;
+    }
+    int at[3], tot[3];
+#pragma unroll
+    for (int c = 0; c < 3; c++) {
+        int x = cnt[c];
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) s_sum[c][wave] = x;
+        at[c] = x - cnt[c];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 3; c++) {
+        tot[c] = 0;
+        for (int w = 0; w < PLAN / 64; w++) {
+            if (w < wave) at[c] += s_sum[c][w];
+            tot[c] += s_sum[c][w];
+        }
+    }
+    // (token ranges that overlap, an error that vx_paged_seq has flagged, may
+    // make more pieces than there is room for: then nothing runs)
+    if ((int64_t)tot[0] * a.p.n_kv > max_pieces) e1 = e0, tot[0] = tot[2] = 0, *a.p.err_flag = 1;
+    for (int e = e0; e < e1; e++) {
+        const int n = entry_steps(a, n_rt, e, b, r0), parts = (n + limit - 1) / limit;
+        if (parts == 0) continue;
+        for (int h = 0; h < a.p.n_kv; h++) {
+            const int slot = h * tot[1] + at[1];
+            for (int k = 0; k < parts; k++) {
+                const RowPiece pc = {b, h, r0, (int)((int64_t)n * k / parts), (int)((int64_t)n * (k + 1) / parts), parts > 1 ? slot + k : -1};
+                a.pieces[h * tot[0] + at[0] + k] = pc;
+            }
+            if (parts > 1) {
+                const RowJoin j = {b, h, r0, slot, parts};
+                a.joins[h * tot[2] + at[2]] = j;
+            }
+        }
+        at[0] += parts;
+        at[1] += parts > 1 ? parts : 0;
+        at[2] += parts > 1;
+    }
+    if (tid == 0) {
+        a.plan->pieces = tot[0] * a.p.n_kv;
+        a.plan->joins = tot[2] * a.p.n_kv;
+    }
+    if (tid < 8) a.plan->heads[tid] = 0;
+}
+
+// grid the most pieces there can be, block 256.
+__global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     __shared__ __attribute__((aligned(16))) TileSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rh = wave >> 1, ch = wave & 1;
-    // The dispatcher deals workgroups round-robin over the 8 XCDs: XCD x takes
-    // a contiguous run of the items, so that the row tiles in flight on it
-    // are neighbours, whose keys its L2 then holds once.
-    const int per_xcd = (n_items + 7) / 8, item = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per_xcd || item >= n_items) return;
-    const int split = item % n_split, rt = n_rt - 1 - item / n_split % n_rt, kvh = item / n_split / n_rt % a.p.n_kv, b = item / n_split / n_rt / a.p.n_kv;
-    const vx_pseq s = vx_paged_seq(a.p, b);
-    const int R = s.T * a.qg, r0 = rt * TR;
-    if (r0 >= R) return;
+    // The dispatcher deals workgroups round-robin over the 8 XCDs.  Each takes
+    // the next piece of its own eighth of the list, so that the row tiles in
+    // flight on an XCD are neighbours, whose keys its L2 then holds once; one
+    // whose eighth is all taken helps the next.
+    const int pieces = a.plan->pieces;
+    if ((int)blockIdx.x >= pieces) return;
+    if (tid == 0) {
+        int piece = -1;
+        for (int k = 0; k < 8 && piece < 0; k++) {
+            const int x = (blockIdx.x + k) & 7, lo = (int)((int64_t)pieces * x / 8), hi = (int)((int64_t)pieces * (x + 1) / 8);
+            const int i = lo < hi ? atomicAdd(&a.plan->heads[x], 1) : hi;
+            if (i < hi - lo) piece = lo + i;
+        }
+        *(int *)sm.mx[0] = piece;
+    }
+    __syncthreads();
+    const int piece = __builtin_amdgcn_readfirstlane(*(int *)sm.mx[0]);
+    if (piece < 0) return;
+    __syncthreads();
+    const RowPiece *pc = a.pieces + piece;
+    const int b = __builtin_amdgcn_readfirstlane(pc->b), kvh = __builtin_amdgcn_readfirstlane(pc->kvh), r0 = __builtin_amdgcn_readfirstlane(pc->r0);
+    const int c0 = __builtin_amdgcn_readfirstlane(pc->c0), c1 = __builtin_amdgcn_readfirstlane(pc->c1), slot = __builtin_amdgcn_readfirstlane(pc->slot);
+    vx_pseq s = vx_paged_seq(a.p, b);
+    s.start = __builtin_amdgcn_readfirstlane(s.start);
+    s.T = __builtin_amdgcn_readfirstlane(s.T);
+    s.len = __builtin_amdgcn_readfirstlane(s.len);
+    s.row0 = s.len - s.T;
+    const int R = s.T * a.qg;
     const int t0 = row_tok(a, r0), t1 = row_tok(a, min(r0 + TR - 1, R - 1));
     const vx_tiles tl = tiles_of(a, s, t0, t1);
-    const int all = (tl.nt + 1) / 2, per = (all + n_split - 1) / n_split;
-    const int c0 = split * per, nt = min(per, all - c0);          // steps c0 .. c0 + nt - 1 of the list
+    const int all = (tl.nt + 1) / 2, nt = min(c1, all) - c0;      // steps c0 .. c0 + nt - 1 of the list
+    const bool parted = slot >= 0;
+    const size_t slot0 = (size_t)max(slot, 0) * TR;
     // what the workgroup's rows see between them
     vx_sight any = vx_paged_sight(s, t0, a.window, a.n_sink);
     if (any.i < 0) any.lo = 0;
@@ -809,7 +953,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_
     // the rows' stores would wait for them.
     constexpr int WR = TR / 4;
     uint2 gt[WR];
-    const bool gated = a.gate && n_split == 1;
+    const bool gated = a.gate && !parted;
     auto row_of = [&](int k) { return min(r0 + wave + 4 * k, R - 1); };
     if (gated && a.gate_bf16) {
 #pragma unroll
@@ -832,7 +976,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_
     for (int rb = 0; rb < 2; rb++) {
         l[rb] += sm.mx[wave ^ 1][32 * rb + n];
         const int r = 64 * rh + 32 * rb + n;
-        const float il = n_split > 1 ? 1.0f : (l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f);
+        const float il = parted ? 1.0f : (l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f);
 #pragma unroll
         for (int db = 0; db < 4; db++)
 #pragma unroll
@@ -842,9 +986,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_
                     make_float4(O[rb][db][4 * q4] * il, O[rb][db][4 * q4 + 1] * il, O[rb][db][4 * q4 + 2] * il, O[rb][db][4 * q4 + 3] * il);
             }
         if (ch == 0 && g == 0 && r0 + r < R) {
-            if (n_split > 1) {
-                const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + r) * n_split + split;
-                a.part_ml[slot] = make_float2(m[rb], l[rb]);
+            if (parted) {
+                a.part_ml[slot0 + r] = make_float2(m[rb], l[rb]);
             } else {
                 const int t = row_tok(a, r0 + r);
                 stat_store(a, s.start + t, row_head(a, kvh, r0 + r, t), m[rb], l[rb]);
@@ -856,12 +999,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_
         const int r = wave + 4 * k;
         return *(const float4 *)(so + r * HDG + ((lane ^ (r & 15)) << 2));
     };
-    if (n_split > 1) {
+    if (parted) {
 #pragma unroll 4
-        for (int k = 0; k < WR; k++) {
-            const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r0 + wave + 4 * k) * n_split + split;
-            if (r0 + wave + 4 * k < R) *(float4 *)(a.part_o + slot * HDG + 4 * lane) = orow(k);
-        }
+        for (int k = 0; k < WR; k++)
+            if (r0 + wave + 4 * k < R) *(float4 *)(a.part_o + (slot0 + wave + 4 * k) * HDG + 4 * lane) = orow(k);
         return;
     }
     float4 on = orow(0);
@@ -880,29 +1021,35 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a, int n_items, int n_
     }
 }
 
-// grid (max rows / 4, n_kv, B), block 256: merges a query row's n_split parts
-// in order, one row a wave.
-__global__ __launch_bounds__(256) void paged_rows_join(Args a, int n_split) {
-    const int kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
-    const int r = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const vx_pseq s = vx_paged_seq(a.p, b);
-    if (r >= s.T * a.qg) return;
-    const size_t slot = (((size_t)b * a.p.n_kv + kvh) * a.part_rows + r) * n_split;
-    float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < n_split; k++) M = fmaxf(M, a.part_ml[slot + k].x);
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < n_split; k++) {
-        const float2 ml = a.part_ml[slot + k];
-        const float4 o = *(const float4 *)(a.part_o + (slot + k) * HDG + 4 * lane);
-        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        L += ml.y * w;
-        O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+// grid (the most joins there can be, TR / 16), block 256: adds up the parts
+// of a cut item, in order, four rows a wave.
+__global__ __launch_bounds__(256) void paged_rows_join(Args a) {
+    if ((int)blockIdx.x >= a.plan->joins) return;
+    const int lane = threadIdx.x & 63;
+    const RowJoin jn = a.joins[blockIdx.x];
+    const vx_pseq s = vx_paged_seq(a.p, jn.b);
+    const int q0 = blockIdx.y * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 4;
+#pragma unroll
+    for (int q = q0; q < q0 + 4; q++) {
+        const int r = jn.r0 + q;
+        if (r >= s.T * a.qg) return;
+        const size_t at = (size_t)jn.slot * TR + q;
+        float M = -INFINITY, L = 0.0f;
+        for (int k = 0; k < jn.parts; k++) M = fmaxf(M, a.part_ml[at + (size_t)k * TR].x);
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < jn.parts; k++) {
+            const float2 ml = a.part_ml[at + (size_t)k * TR];
+            const float4 o = *(const float4 *)(a.part_o + (at + (size_t)k * TR) * HDG + 4 * lane);
+            const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            L += ml.y * w;
+            O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+        }
+        const float il = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+        const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, jn.kvh, r, t);
+        const float4 gt = a.gate ? gate_row(a, tok, h) : make_float4(0.f, 0.f, 0.f, 0.f);
+        row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il), gt);
+        if (lane == 0) stat_store(a, tok, h, M, L);
     }
-    const float il = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
-    const float4 gt = a.gate ? gate_row(a, tok, h) : make_float4(0.f, 0.f, 0.f, 0.f);
-    row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il), gt);
-    if (lane == 0) stat_store(a, tok, h, M, L);
 }
 
 // grid (tile_cap / 4, n_kv, B), block 256: one wave per key tile adds the
@@ -1014,22 +1161,26 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         if (d->acc) VX_LAUNCH(ctx, paged_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
         return 0;
     }
-    // key splits: enough workgroups for every CU, at least 4 steps of 64 keys each
-    const int tiles = (rows + TR - 1) / TR, steps = (a.tile_cap + 1) / 2;
-    const int64_t items = (int64_t)tiles * d->n_kv * d->B;
-    const int n_split = (int)std::max<int64_t>(1, std::min<int64_t>((2 * ctx->n_cu + items - 1) / items, steps / 4));
-    a.part_rows = rows;
-    const size_t n_part = n_split > 1 ? (size_t)d->B * d->n_kv * rows * n_split : 0;
-    const size_t ml_bytes = (n_part * sizeof(float2) + 255) / 256 * 256;
-    void *scr = nullptr;
-    if (stat_bytes + ml_bytes + n_part && vx_ctx_scratch(ctx, stat_bytes + ml_bytes + n_part * HDG * 4, &scr)) return -1;
-    a.stat = d->acc ? (float2 *)scr : nullptr;
-    a.part_ml = (float2 *)((char *)scr + stat_bytes);
-    a.part_o = (float *)((char *)scr + stat_bytes + ml_bytes);
-    const int64_t n_items = items * n_split;
-    VX_REQUIRE(n_items < (1ll << 31) - 8, "%s: more than 2^31 workgroups (B=%d n_kv=%d max_T=%d)", who, d->B, d->n_kv, d->max_T);
-    VX_LAUNCH(ctx, paged_rows, dim3((unsigned)((n_items + 7) / 8 * 8)), dim3(256), a, (int)n_items, tiles, n_split);
-    if (n_split > 1) VX_LAUNCH(ctx, paged_rows_join, dim3((rows + 3) / 4, d->n_kv, d->B), dim3(256), a, n_split);
+    const int n_rt = (rows + TR - 1) / TR, n_cu = ctx->n_cu;
+    VX_REQUIRE((int64_t)d->B * n_rt < (1ll << 31) - PLAN, "%s: more than 2^31 row tiles (B=%d max_T=%d)", who, d->B, d->max_T);
+    // every token range ends in one tile that it need not fill; paged_plan makes at most 3/2 n_cu cuts, so twice
+    // as many parts at most
+    const int64_t cuts = (int64_t)n_cu * 3 / 2, items = ((int64_t)d->n_tok * a.qg / TR + d->B) * d->n_kv;
+    VX_REQUIRE(items + cuts < (1ll << 31), "%s: more than 2^31 workgroups (B=%d n_kv=%d n_tok=%d)", who, d->B, d->n_kv, d->n_tok);
+    const size_t ml_bytes = (size_t)2 * cuts * TR * sizeof(float2), plan_bytes = 256, piece_bytes = (size_t)(items + cuts) * sizeof(RowPiece);
+    const size_t join_bytes = ((size_t)cuts * sizeof(RowJoin) + 255) / 256 * 256;
+    void *scr;
+    if (vx_ctx_scratch(ctx, stat_bytes + ml_bytes + plan_bytes + join_bytes + (size_t)2 * cuts * TR * HDG * 4 + piece_bytes, &scr)) return -1;
+    char *at = (char *)scr;
+    a.stat = d->acc ? (float2 *)at : nullptr;
+    a.part_ml = (float2 *)(at += stat_bytes);
+    a.plan = (RowPlan *)(at += ml_bytes);
+    a.joins = (RowJoin *)(at += plan_bytes);
+    a.part_o = (float *)(at += join_bytes);
+    a.pieces = (RowPiece *)(at += (size_t)2 * cuts * TR * HDG * 4);
+    VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
+    VX_LAUNCH(ctx, paged_rows, dim3((unsigned)(items + cuts)), dim3(256), a);
+    VX_LAUNCH(ctx, paged_rows_join, dim3((unsigned)cuts, TR / 16), dim3(256), a);
     if (d->acc) VX_LAUNCH(ctx, paged_tile_weigh, dim3((a.tile_cap + 3) / 4, d->n_kv, d->B), dim3(256), a);
     return 0;
 }
