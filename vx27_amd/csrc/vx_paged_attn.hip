@@ -454,7 +454,10 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 constexpr int TR = 128;                      // query rows of a workgroup
 constexpr int HALF = TILE * HDG * 2;         // bytes of one key block of K or of V
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
-constexpr float LAZY = 8.0f;                 // a row's reference moves once its maximum is past it by 2^8
+// A row's reference is its first block's maximum and moves once a later one is
+// past it by 2^48: weights, sums and O then stay below 2^80, and a rescale of
+// O (400 instructions a wave) hardly ever runs.
+constexpr float LAZY = 48.0f;
 
 struct TileSmem {
     char k[2][2 * HALF], v[2][2 * HALF];
@@ -462,6 +465,23 @@ struct TileSmem {
     float mx[4][64];                         // row maxima of a wave's key block; row sums at the end
 };
 
+// Four direct-to-LDS loads as vx_dma16, 1 KiB apart in memory and in LDS (the
+// instruction's offset counts on both sides).
+__device__ __forceinline__ void dma16x4(const void *base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds) {
+    uint32_t saved;
+    __asm__ volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %5\n\t"
+        "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+        "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+        "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds)
+        : "memory");
+}
 __device__ __forceinline__ int kswz(int r) { return (r & 3) | ((r >> 1) & 12); }
 __device__ __forceinline__ bf16x8_t lds8(const char *p) { return *(const bf16x8_t *)p; }
 
@@ -592,16 +612,19 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     // the next piece of its own eighth of the list, so that the row tiles in
     // flight on an XCD are neighbours, whose keys its L2 then holds once; one
     // whose eighth is all taken helps the next.
-    const int pieces = a.plan->pieces;
-    if ((int)blockIdx.x >= pieces) return;
-    if (tid == 0) {
+    // (There are more workgroups than pieces, so that some are left to help.)
+    if (tid < 64) {
+        const int pieces = a.plan->pieces, x = (blockIdx.x + lane) & 7, lo = (int)((int64_t)pieces * x / 8), hi = (int)((int64_t)pieces * (x + 1) / 8);
+        const int taken = __hip_atomic_load(&a.plan->heads[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         int piece = -1;
-        for (int k = 0; k < 8 && piece < 0; k++) {
-            const int x = (blockIdx.x + k) & 7, lo = (int)((int64_t)pieces * x / 8), hi = (int)((int64_t)pieces * (x + 1) / 8);
-            const int i = lo < hi ? atomicAdd(&a.plan->heads[x], 1) : hi;
-            if (i < hi - lo) piece = lo + i;
+        for (uint32_t left = (uint32_t)__ballot(taken < hi - lo) & 255; left && piece < 0; left &= left - 1) {
+            const int k = __builtin_ctz(left);
+            int i = 0;
+            if (lane == k) i = atomicAdd(&a.plan->heads[x], 1);
+            i = __shfl(i, k, 64);
+            if (i < __shfl(hi - lo, k, 64)) piece = __shfl(lo, k, 64) + i;
         }
-        *(int *)sm.mx[0] = piece;
+        if (tid == 0) *(int *)sm.mx[0] = piece;
     }
     __syncthreads();
     const int piece = __builtin_amdgcn_readfirstlane(*(int *)sm.mx[0]);
@@ -670,10 +693,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     auto at_of = [&](int c) -> size_t {
         return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, c - base) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, c - base);
     };
-    auto dma_k = [&](size_t at, int buf, int j) {
-        vx_dma16((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)] + j * 1024, k_lds + buf * 2 * HALF + j * 1024);
+    auto dma_k = [&](size_t at, int buf, int j) {   // loads 4 j .. 4 j + 3
+        dma16x4((const char *)(a.k_pages + at) + j * 4096, ko[2 * j], ko[2 * j + 1], ko[2 * j], ko[2 * j + 1], k_lds + buf * 2 * HALF + j * 4096);
     };
-    auto dma_v = [&](size_t at, int buf, int j) { vx_dma16((const char *)(a.v_pages + at), vo + j * 1024, v_lds + buf * 2 * HALF + j * 1024); };
+    auto dma_v = [&](size_t at, int buf, int j) { dma16x4((const char *)(a.v_pages + at) + j * 4096, vo, vo, vo, vo, v_lds + buf * 2 * HALF + j * 4096); };
 
     floatx16_t O[2][4];
 #pragma unroll
@@ -694,11 +717,11 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         fill_at();
         size_t at_v = at_of(c0), at_k = at_of(c0 + 1);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at_v, 0, j);
+        for (int j = 0; j < 2; j++) dma_k(at_v, 0, j);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at_k, 1, j);
+        for (int j = 0; j < 2; j++) dma_k(at_k, 1, j);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
+        for (int j = 0; j < 2; j++) dma_v(at_v, 0, j);
         at_v = at_k;
         at_k = at_of(c0 + 2);
         bf16x8_t q[2][16];
@@ -716,14 +739,27 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                     else __asm__ volatile("" : "+v"(q[rb][k]));
                 }
         };
-        // operand addresses in LDS
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        pin_q();
+        vx_lds_barrier();
+        // Operand addresses in LDS (from an opaque copy of the lane: formed
+        // before the queries are in their registers they would be spilled)
+        int ln = lane;
+        __asm__ volatile("" : "+v"(ln));
+        const int g = ln >> 5, n = ln & 31;
         const int krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-        const int kx = g ^ kswz(krow);
-        const char *kl = sm.k[0] + ch * HALF + krow * (HDG * 2);
-        const char *vl = sm.v[0] + (128 * ch + n) * (TILE * 2);
-        const int vx = (n >> 1) & 3;
-        auto kload = [&](int buf, int k) { return lds8(kl + buf * 2 * HALF + ((k >> 3) << 8) + (((2 * (k & 7)) ^ kx) << 4)); };
-        auto vload = [&](int buf, int k, int db) { return lds8(vl + buf * 2 * HALF + (k >> 1) * HALF + db * 32 * TILE * 2 + (((2 * (k & 1) + g) ^ vx) << 4)); };
+        // (one address for each of the swizzle's values; the rest are offsets of
+        // the instructions)
+        const char *ka[8], *va[2][2];
+#pragma unroll
+        for (int k = 0; k < 8; k++) ka[k] = sm.k[0] + ch * HALF + krow * (HDG * 2) + (((2 * k + g) ^ kswz(krow)) << 4);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                va[h][k] = sm.v[0] + (h ? 1 - ch : ch) * HALF + (128 * ch + n) * (TILE * 2) + (((2 * k + g) ^ ((n >> 1) & 3)) << 4);
+        auto kload = [&](int k) { return lds8(ka[k & 7] + (k >> 3) * 256); };
+        auto vload = [&](int h, int k, int db) { return lds8(va[h][k] + db * 32 * TILE * 2); };   // h: own block, partner's
 
         floatx16_t S[2];
         auto s_zero = [&]() {
@@ -789,15 +825,15 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             vx_lds_barrier();
         };
 
-        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        vx_lds_barrier();
         s_zero();
 #pragma unroll
         for (int k = 0; k < 16; k++) {
-            const bf16x8_t kf = kload(0, k);
+            const bf16x8_t kf = kload(k);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
         }
+#pragma unroll
+        for (int k = 0; k < 8; k++) ka[k] += 2 * HALF;   // (the next step's)
         sc[0] = S[0];
         sc[1] = S[1];
         if (cut(c0)) mask(c0);
@@ -825,7 +861,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             }
             bf16x8_t kf[4];   // K operands, three k-steps ahead
 #pragma unroll
-            for (int k = 0; k < 3; k++) kf[k] = kload(bk ^ 1, k);
+            for (int k = 0; k < 3; k++) kf[k] = kload(k);
             s_zero();
             pin_q();
             __builtin_amdgcn_sched_barrier(0);
@@ -837,8 +873,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             // the softmax in three such shares (argument, exp2, sum and
             // rounding), so that none waits for its own result.
             auto s_mfma = [&](int k, int rb) {
-                if (rb == 0 && k + 3 < 16) kf[(k + 3) & 3] = kload(bk ^ 1, k + 3);
-                if (rb == 1 && k < 8) dma_k(at_k, bk, k);
+                if (rb == 0 && k + 3 < 16) kf[(k + 3) & 3] = kload(k + 3);
+                if (rb == 1 && (k & 3) == 3 && k < 8) dma_k(at_k, bk, k >> 2);
                 S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k & 3], q[rb][k], S[rb], 0, 0, 0);
             };
             float e[2][16];
@@ -877,12 +913,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             // (O stays in the MFMAs' accumulators around the rare rescale: without
             // the pins it is copied out and back in every step)
             pin_o();
-            if (__any(moved)) {
+            if (c && __any(moved)) {   // (before the first step O is 0)
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) {
                     l[rb] *= al[rb];
 #pragma unroll
-                    for (int db = 0; db < 4; db++) O[rb][db] *= al[rb];
+                    for (int db = 0; db < 4; db++) {   // (one at a time: all of O does not fit beside the rest)
+                        O[rb][db] *= al[rb];
+                        __asm__ volatile("" : "+a"(O[rb][db]));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
             pin_o();
@@ -907,7 +947,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             if (edge) clear_v(c0 + c, bk);
             // own key block first: the partner's weights arrive meanwhile
             bf16x8_t poth[2][2], vf[4];   // V operands three ahead
-            auto vstep = [&](int i) { return vload(bk, ((i >> 2) & 1) + 2 * (i < 8 ? ch : 1 - ch), i & 3); };
+            auto vstep = [&](int i) { return vload(i >> 3, (i >> 2) & 1, i & 3); };
 #pragma unroll
             for (int i = 0; i < 3; i++) vf[i] = vstep(i);
 #pragma unroll
@@ -915,13 +955,14 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
 #pragma unroll
                 for (int k = 0; k < 2; k++) poth[rb][k] = lds8(sm.p[wave ^ 1] + ((rb * 2 + k) * 64 + lane) * 16);
             float x[2];
+            bool edge2 = false, cut2 = false;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) {
                     if (rb == 0 && i + 3 < 16) vf[(i + 3) & 3] = vstep(i + 3);
-                    if (rb == 1 && i < 8) dma_v(at_v, bk ^ 1, i);
+                    if (rb == 1 && (i & 3) == 1 && i < 8) dma_v(at_v, bk ^ 1, i >> 2);
                     O[rb][i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 3], i < 8 ? pown[rb][(i >> 2) & 1] : poth[rb][(i >> 2) & 1],
                                                                            O[rb][i & 3], 0, 0, 0);
                     sc[rb][i] = S[rb][i];
@@ -931,6 +972,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                     else if (i & 1) __asm__ volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x[rb]) : "v"(sc[rb][i - 1]), "v"(sc[rb][i]));
                     // the next step's addresses
                     if (rb == 1 && i == 8) at_v = at_k, at_k = at_of(c0 + c + 3);
+                    if (rb == 1 && i == 10) edge2 = bare(c0 + c + 1);
+                    if (rb == 1 && i == 12) cut2 = c + 2 < nt && cut(c0 + c + 2);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -939,12 +982,20 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 row_max(x);
             }
             publish(x);
-            edge = bare(c0 + c + 1);
-            cut1 = c + 2 < nt && cut(c0 + c + 2);
+            edge = edge2;
+            cut1 = cut2;
             if (c0 + c + 5 > base + 63) {   // (one step in 60)
                 base = c0 + c + 4;
                 fill_at();
             }
+            // the operand addresses change buffers
+            const int flip = bk ? 2 * HALF : -2 * HALF;
+#pragma unroll
+            for (int k = 0; k < 8; k++) ka[k] += flip;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) va[h][k] -= flip;
         }
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
     }
