@@ -465,21 +465,18 @@ struct TileSmem {
     float mx[4][64];                         // row maxima of a wave's key block; row sums at the end
 };
 
-// Four direct-to-LDS loads as vx_dma16, 1 KiB apart in memory and in LDS (the
-// instruction's offset counts on both sides).
-__device__ __forceinline__ void dma16x4(const void *base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds) {
+// vx_dma16 with a constant offset, which counts in memory and in LDS.
+template <int OFF>
+__device__ __forceinline__ void dma16(const void *base, uint32_t off, uint32_t lds) {
     uint32_t saved;
     __asm__ volatile(
         "s_mov_b32 %0, m0\n\t"
-        "s_mov_b32 m0, %6\n\t"
+        "s_mov_b32 m0, %3\n\t"
         "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %5\n\t"
-        "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-        "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-        "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:%4\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
-        : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds)
+        : "v"(off), "s"(base), "s"(lds), "n"(OFF)
         : "memory");
 }
 __device__ __forceinline__ int kswz(int r) { return (r & 3) | ((r >> 1) & 12); }
@@ -693,10 +690,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     auto at_of = [&](int c) -> size_t {
         return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, c - base) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, c - base);
     };
-    auto dma_k = [&](size_t at, int buf, int j) {   // loads 4 j .. 4 j + 3
-        dma16x4((const char *)(a.k_pages + at) + j * 4096, ko[2 * j], ko[2 * j + 1], ko[2 * j], ko[2 * j + 1], k_lds + buf * 2 * HALF + j * 4096);
+    auto dma = [&](const char *p, uint32_t off, uint32_t lds, int j) {   // 1 KiB load j of 8
+        switch (j & 3) {
+            case 0: dma16<0>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
+            case 1: dma16<1024>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
+            case 2: dma16<2048>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
+            default: dma16<3072>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
+        }
     };
-    auto dma_v = [&](size_t at, int buf, int j) { dma16x4((const char *)(a.v_pages + at) + j * 4096, vo, vo, vo, vo, v_lds + buf * 2 * HALF + j * 4096); };
+    auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
+    auto dma_v = [&](size_t at, int buf, int j) { dma((const char *)(a.v_pages + at), vo, v_lds + buf * 2 * HALF, j); };
 
     floatx16_t O[2][4];
 #pragma unroll
@@ -717,11 +720,11 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         fill_at();
         size_t at_v = at_of(c0), at_k = at_of(c0 + 1);
 #pragma unroll
-        for (int j = 0; j < 2; j++) dma_k(at_v, 0, j);
+        for (int j = 0; j < 8; j++) dma_k(at_v, 0, j);
 #pragma unroll
-        for (int j = 0; j < 2; j++) dma_k(at_k, 1, j);
+        for (int j = 0; j < 8; j++) dma_k(at_k, 1, j);
 #pragma unroll
-        for (int j = 0; j < 2; j++) dma_v(at_v, 0, j);
+        for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
         at_v = at_k;
         at_k = at_of(c0 + 2);
         bf16x8_t q[2][16];
@@ -874,7 +877,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             // rounding), so that none waits for its own result.
             auto s_mfma = [&](int k, int rb) {
                 if (rb == 0 && k + 3 < 16) kf[(k + 3) & 3] = kload(k + 3);
-                if (rb == 1 && (k & 3) == 3 && k < 8) dma_k(at_k, bk, k >> 2);
+                if (rb == 1 && k < 8) dma_k(at_k, bk, k);
                 S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k & 3], q[rb][k], S[rb], 0, 0, 0);
             };
             float e[2][16];
@@ -962,7 +965,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) {
                     if (rb == 0 && i + 3 < 16) vf[(i + 3) & 3] = vstep(i + 3);
-                    if (rb == 1 && (i & 3) == 1 && i < 8) dma_v(at_v, bk ^ 1, i >> 2);
+                    if (rb == 1 && i < 8) dma_v(at_v, bk ^ 1, i);
+                    if (i >= 8 && rb == 0) ka[i - 8] += bk ? 2 * HALF : -2 * HALF;   // (the next step's buffer)
                     O[rb][i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 3], i < 8 ? pown[rb][(i >> 2) & 1] : poth[rb][(i >> 2) & 1],
                                                                            O[rb][i & 3], 0, 0, 0);
                     sc[rb][i] = S[rb][i];
@@ -988,14 +992,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 base = c0 + c + 4;
                 fill_at();
             }
-            // the operand addresses change buffers
-            const int flip = bk ? 2 * HALF : -2 * HALF;
-#pragma unroll
-            for (int k = 0; k < 8; k++) ka[k] += flip;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) va[h][k] -= flip;
+                for (int k = 0; k < 2; k++) va[h][k] += bk ? -2 * HALF : 2 * HALF;
         }
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
     }
@@ -1103,52 +1103,114 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
     }
 }
 
-// grid (tile_cap / 4, n_kv, B), block 256: one wave per key tile adds the
-// weights of every query row to it, the scores formed again.
-__global__ __launch_bounds__(256) void paged_tile_weigh(Args a) {
-    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
-    const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);
+// Every row's weights of the tile kernel's tokens, the scores formed again
+// (the tile kernel has a row's maximum and sum only at its end).  grid
+// (tile_cap / 8, n_kv, B), block 256: wave w keeps two key blocks of the tile
+// list in registers as K operands, and the 32-row tiles of queries that see
+// any of the workgroup's keys pass through LDS, one ahead.  A lane's sums are
+// over its row of each tile; at the end the 32 lanes of a key are added up.
+// One workgroup owns a key, so the order of the sums is fixed.
+constexpr int QT = 32, QBUF = QT * HDG * 2;
+__global__ __launch_bounds__(256, 2) void paged_rows_weigh(Args a) {
+    __shared__ __attribute__((aligned(16))) char sq[2][QBUF];
+    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const vx_pseq s = vx_paged_seq(a.p, b);
     const vx_tiles tl = tiles_of(a, s, 0, s.T - 1);
-    if (i >= tl.nt) return;
-    const int key0 = tl.at(i) * TILE;
-    const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
-    const uint16_t *kr0 = a.k_pages + vx_k_index(a.p.n_kv, a.p.page_size, page, kvh, at + 8 * (n >> 2) + (n & 3), 8 * g);
-    bf16x8_t ka[8], kb[8];
+    const int first = blockIdx.x * 8;
+    if (first >= tl.nt) return;
+    // the tokens that see any of the workgroup's keys lo .. hi
+    const int lo = tl.at(first) * TILE, hi = tl.at(min(first + 8, tl.nt) - 1) * TILE + TILE - 1;
+    const int t0 = max(lo - s.row0, 0);
+    const int t1 = a.window && lo >= a.n_sink ? (int)min((int64_t)s.T - 1, (int64_t)hi + a.window - 1 - s.row0) : s.T - 1;
+    const int ra = t0 * a.qg, rz = (t1 + 1) * a.qg, R = s.T * a.qg;   // query rows ra .. rz - 1
+
+    int key0[2];
+    bf16x8_t kf[2][16];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        ka[k] = load8(kr0 + 32 * k);
-        kb[k] = load8(kr0 + 4 * HDG + 32 * k);
+    for (int kb = 0; kb < 2; kb++) {
+        const int i = first + 2 * wave + kb, key = tl.at(min(i, tl.nt - 1)) * TILE;
+        key0[kb] = i < tl.nt ? key : -1;
+        const int page = vx_paged_page(a.p, b, key), krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+        const uint16_t *kp = a.k_pages + vx_k_index(a.p.n_kv, a.p.page_size, page, kvh, key - vx_page_slot(a.p, key) * a.p.page_size + krow, 8 * g);
+#pragma unroll
+        for (int k = 0; k < 16; k++) kf[kb][k] = load8(kp + 16 * k);
     }
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    int any = 0;
-    for (int r0 = 0; r0 < s.T * a.qg; r0 += 16) {
-        Rows w;
-        rows_begin(a, s, kvh, r0, w);
-        const vx_sight v = sight_of(a, s, r0 + n);
-        const int r = min(r0 + n, s.T * a.qg - 1);
-        const int t = row_tok(a, r);
-        const float2 ml = a.stat[(size_t)(s.start + t) * a.n_q + row_head(a, kvh, r, t)];
-        float sc[8];
-        score_tile(ka, kb, w.q, sc);
+    float sum[32];
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (v.sees(key0 + 8 * g + e)) {
-                sum[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], SC2, -ml.x)) * ml.y;
-                any |= 1 << e;
+    for (int i = 0; i < 32; i++) sum[i] = 0.0f;
+
+    // Queries r .. r + 31 into a buffer: 2 rows a load, 16-byte unit u of row
+    // q at slot u ^ (q & 7) (rows past the last: the last again)
+    auto stage = [&](int r, int buf) {
+        const int tb = row_tok(a, min(r, R - 1));
+        const uint16_t *base = vx_uniform_ptr(a.q + (size_t)(s.start + tb) * a.q_ts + (size_t)kvh * a.qg * a.q_hs);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int q = wave * 8 + 2 * j + (lane >> 5), row = min(r + q, R - 1), t = row_tok(a, row);
+            const uint32_t off = (uint32_t)(((size_t)(t - tb) * a.q_ts + (size_t)(row - t * a.qg) * a.q_hs) * 2) + (((lane & 31) ^ (q & 7)) << 4);
+            vx_dma16(base, off, vx_lds_addr(sq[buf]) + (wave * 8 + 2 * j) * 512);
+        }
+    };
+    auto stat_of = [&](int r) {
+        const int row = min(r + n, R - 1), t = row_tok(a, row);
+        return a.stat[(size_t)(s.start + t) * a.n_q + row_head(a, kvh, row, t)];
+    };
+    if (ra < rz) {
+        float2 st = stat_of(ra);
+        stage(ra, 0);
+        int buf = 0;
+        for (int r = ra; r < rz; r += QT, buf ^= 1) {
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            vx_lds_barrier();
+            const float2 ml = st;
+            st = stat_of(min(r + QT, rz - 1));
+            if (r + QT < rz) stage(r + QT, buf ^ 1);
+            const int row = r + n;
+            vx_sight v = vx_paged_sight(s, row_tok(a, min(row, R - 1)), a.window, a.n_sink);
+            if (row >= rz) v.i = -1;
+            floatx16_t S[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) S[kb][i] = 0.0f;
+            const char *qrow = sq[buf] + n * 512;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const bf16x8_t qf = lds8(qrow + (((2 * k + g) ^ (n & 7)) << 4));
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb][k], qf, S[kb], 0, 0, 0);
             }
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                const uint32_t bits = key0[kb] < 0 ? 0u : v.block(key0[kb]);
+                if (__all(bits == 0xffffffffu)) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[16 * kb + i] += __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], SC2, -ml.x)) * ml.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], SC2, -ml.x)) * ml.y;
+                        sum[16 * kb + i] += (bits >> (8 * g)) & (1u << (16 * (i >> 3) + (i & 7))) ? p : 0.0f;
+                    }
+                }
+            }
+        }
     }
+    // over the 32 lanes: halves of the values change sides until lane n has value n
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
+    for (int off = 16, half = 16; off >= 1; off >>= 1, half >>= 1)
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum[e] += __shfl_xor(sum[e], off, 64);
-        any |= __shfl_xor(any, off, 64);
-    }
-    float *dst = a.acc + ((size_t)b * a.p.n_kv + kvh) * a.acc_stride + key0 + 8 * g;
-    if (n == 0)
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (any >> e & 1) dst[e] += sum[e];
+        for (int i = 0; i < half; i++) {
+            const bool up = n & off;
+            const float keep = up ? sum[i + half] : sum[i], send = up ? sum[i] : sum[i + half];
+            sum[i] = keep + __shfl_xor(send, off, 64);
+        }
+    vx_sight any = vx_paged_sight(s, 0, a.window, a.n_sink);
+    if (any.i < 0) any.lo = 0;
+    any.i = s.len - 1;
+    const int kb = n >> 4, i = n & 15, key = (kb ? key0[1] : key0[0]) + 16 * (i >> 3) + 8 * g + (i & 7);
+    if ((kb ? key0[1] : key0[0]) >= 0 && any.sees(key)) a.acc[((size_t)b * a.p.n_kv + kvh) * a.acc_stride + key] += sum[0];
 }
 
 }  // namespace
@@ -1212,6 +1274,8 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         if (d->acc) VX_LAUNCH(ctx, paged_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
         return 0;
     }
+    // (a 32-row tile's queries are addressed by 32-bit offsets from its first)
+    VX_REQUIRE(!d->acc || a.q_ts < (1u << 26) && a.q_hs < (1u << 26), "%s: q strides past 2^26 elements with acc (got %zu, %zu)", who, a.q_ts, a.q_hs);
     const int n_rt = (rows + TR - 1) / TR, n_cu = ctx->n_cu;
     VX_REQUIRE((int64_t)d->B * n_rt < (1ll << 31) - PLAN, "%s: more than 2^31 row tiles (B=%d max_T=%d)", who, d->B, d->max_T);
     // every token range ends in one tile that it need not fill; paged_plan makes at most 3/2 n_cu cuts, so twice
@@ -1232,6 +1296,6 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
     VX_LAUNCH(ctx, paged_rows, dim3((unsigned)(items + cuts)), dim3(256), a);
     VX_LAUNCH(ctx, paged_rows_join, dim3((unsigned)cuts, TR / 16), dim3(256), a);
-    if (d->acc) VX_LAUNCH(ctx, paged_tile_weigh, dim3((a.tile_cap + 3) / 4, d->n_kv, d->B), dim3(256), a);
+    if (d->acc) VX_LAUNCH(ctx, paged_rows_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
     return 0;
 }
