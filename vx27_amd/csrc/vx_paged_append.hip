@@ -66,14 +66,17 @@ __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
 // grid (32-row blocks a sequence's tokens can touch, n_kv, B), block 256: one
 // workgroup per V block of one KV head, with the query heads of its group.
 // The block's cos and sin once; then wave w takes the (token, head) rows w,
-// w + 4, ... (query heads, then the key), lane l dims 4l..4l+3; v goes
-// through LDS into the dim-major block, element by element at its ends so
-// that other rows keep their contents.
+// w + 4, ... (query heads, then the key), four at a time so that their loads
+// are in flight together, lane l dims 4l..4l+3; v goes through LDS into the
+// dim-major block, element by element at its ends so that other rows keep
+// their contents.  HALFS: most angles a token has.
+template <int HALFS>
 __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
+    constexpr int NR = 4;
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    __shared__ float2 csn[VB][MAXR];
-    __shared__ float row[4][HDG];
+    __shared__ float2 csn[VB][HALFS];
+    __shared__ float row[4][NR][HDG];
     __shared__ __attribute__((aligned(16))) uint16_t vt[VB][HDG];
     const vx_pseq s = vx_paged_seq(a.p, b);
     if (s.row0 < 0 && tid == 0 && hk == 0 && blockIdx.x == 0) *a.p.err_flag = 1;
@@ -82,11 +85,28 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     const int lo = max(p0, first), hi = min(p0 + VB, s.len);
     if (lo >= hi) return;
     const int n = hi - lo, tok0 = s.start + (lo - s.row0), half = a.rope_dim / 2;
+    const int qg = a.q ? a.n_q / a.p.n_kv : 0, rows = n * (qg + 1);
     const int page = vx_paged_page(a.p, b, p0), at = p0 % a.p.page_size;
+
+    // row r of the block's (token, head) rows; past the last: the last again
+    float4 x4[NR];
+    auto load_rows = [&](int r0) {
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            const int r = min(r0 + 4 * k, rows - 1), j = r / (qg + 1), h = r % (qg + 1);   // h == qg: the key
+            const size_t src = h == qg ? (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG
+                                       : (size_t)(tok0 + j) * a.q_ts + (size_t)(hk * qg + h) * a.q_hs;
+            x4[k] = load4(h == qg ? a.k : a.q, src + 4 * lane, a.bf16);
+        }
+    };
+    load_rows(wave);
+    const float4 wk = ((const float4 *)a.k_norm_w)[lane], wq = a.q ? ((const float4 *)a.q_norm_w)[lane] : wk;
+    const float one = (a.flags & VX27_GQA_NORM_W) ? 0.0f : 1.0f;
     for (int e = tid; e < n * half; e += 256) {
         const int j = e / half, i = e % half;
         csn[j][i] = vx_rope_cs(a.rope, a.pos ? a.pos[tok0 + j] : lo + j, a.yarn, i);
     }
+#pragma unroll 4
     for (int e = tid; e < n * (HDG / 4); e += 256) {
         const int j = e / (HDG / 4), c = e % (HDG / 4);
         const float4 x = load4(a.v, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * c, a.bf16);
@@ -94,42 +114,7 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     }
     __syncthreads();
 
-    const int qg = a.q ? a.n_q / a.p.n_kv : 0;
-    for (int r = wave; r < n * (qg + 1); r += 4) {
-        const int j = r / (qg + 1), h = r % (qg + 1);   // h == qg: the key
-        const bool is_k = h == qg;
-        const size_t src = is_k ? (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG
-                                : (size_t)(tok0 + j) * a.q_ts + (size_t)(hk * qg + h) * a.q_hs;
-        const float4 x4 = load4(is_k ? a.k : a.q, src + 4 * lane, a.bf16);
-        const float4 w4 = ((const float4 *)(is_k ? a.k_norm_w : a.q_norm_w))[lane];
-        const float x[4] = {x4.x, x4.y, x4.z, x4.w}, w[4] = {w4.x, w4.y, w4.z, w4.w};
-        double ss = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) ss += (double)x[e] * (double)x[e];
-        ss = vx_wave_sum_f64_dpp(ss);
-        const float sc = 1.0f / sqrtf((float)(ss / HDG) + 1e-6f);
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = (a.flags & VX27_GQA_NORM_W) ? (x[e] * sc) * w[e] : (x[e] * sc) * (w[e] + 1.0f);
-        *(float4 *)&row[wave][4 * lane] = make_float4(y[0], y[1], y[2], y[3]);
-        __builtin_amdgcn_wave_barrier();   // (one wave's LDS operations complete in order)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int i = 4 * lane + e;
-            if (i < half) {
-                const float2 c = csn[j][i];
-                y[e] = y[e] * c.x - row[wave][i + half] * c.y;
-            } else if (i < 2 * half) {
-                const float2 c = csn[j][i - half];
-                y[e] = row[wave][i - half] * c.y + y[e] * c.x;
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        uint16_t *dst = is_k ? a.k_pages + vx_k_index(a.p.n_kv, a.p.page_size, page, hk, at + (lo - p0) + j, 4 * lane)
-                             : a.q_out + ((size_t)(tok0 + j) * a.n_q + hk * qg + h) * HDG + 4 * lane;
-        *(uint2 *)dst = pack4(y[0], y[1], y[2], y[3]);
-    }
-
+    // the V block first: its stores drain while the rows are worked on
     uint16_t *vb = a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, hk, at, 0);
     for (int e = tid; e < HDG * (VB / 8); e += 256) {
         const int d = e / (VB / 8), c = e % (VB / 8), r0 = p0 + 8 * c;
@@ -142,6 +127,52 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
             for (int k = 0; k < 8; k++)
                 if (r0 + k >= lo && r0 + k < hi) vb[(size_t)d * VB + 8 * c + k] = vt[r0 + k - lo][d];
         }
+    }
+
+    for (int r0 = wave; r0 < rows; r0 += 4 * NR) {
+        float y[NR][4];
+        double ss[NR];
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            y[k][0] = x4[k].x; y[k][1] = x4[k].y; y[k][2] = x4[k].z; y[k][3] = x4[k].w;
+            ss[k] = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) ss[k] += (double)y[k][e] * (double)y[k][e];
+        }
+        if (r0 + 4 * NR < rows) load_rows(r0 + 4 * NR);
+#pragma unroll
+        for (int k = 0; k < NR; k++) ss[k] = vx_wave_sum_f64_dpp(ss[k]);
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            const bool is_k = min(r0 + 4 * k, rows - 1) % (qg + 1) == qg;
+            const float w[4] = {is_k ? wk.x : wq.x, is_k ? wk.y : wq.y, is_k ? wk.z : wq.z, is_k ? wk.w : wq.w};
+            const float sc = 1.0f / sqrtf((float)(ss[k] / HDG) + 1e-6f);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[k][e] = (y[k][e] * sc) * (w[e] + one);
+            *(float4 *)&row[wave][k][4 * lane] = make_float4(y[k][0], y[k][1], y[k][2], y[k][3]);
+        }
+        __builtin_amdgcn_wave_barrier();   // (one wave's LDS operations complete in order)
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            const int r = r0 + 4 * k;
+            if (r >= rows) break;
+            const int j = r / (qg + 1), h = r % (qg + 1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = 4 * lane + e;
+                if (i < half) {
+                    const float2 c = csn[j][i];
+                    y[k][e] = y[k][e] * c.x - row[wave][k][i + half] * c.y;
+                } else if (i < 2 * half) {
+                    const float2 c = csn[j][i - half];
+                    y[k][e] = row[wave][k][i - half] * c.y + y[k][e] * c.x;
+                }
+            }
+            uint16_t *dst = h == qg ? a.k_pages + vx_k_index(a.p.n_kv, a.p.page_size, page, hk, at + (lo - p0) + j, 4 * lane)
+                                    : a.q_out + ((size_t)(tok0 + j) * a.n_q + hk * qg + h) * HDG + 4 * lane;
+            *(uint2 *)dst = pack4(y[k][0], y[k][1], y[k][2], y[k][3]);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -178,6 +209,9 @@ extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_
     a.pos = d->pos; a.q = d->q; a.k = d->k_new; a.v = d->v_new;
     a.q_norm_w = d->q_norm_w; a.k_norm_w = d->k_norm_w;
     a.q_out = d->q_out; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
-    VX_LAUNCH(ctx, paged_append, dim3((d->max_T + VB - 2) / VB + 1, d->n_kv, d->B), dim3(256), a);
+    const dim3 grid((d->max_T + VB - 2) / VB + 1, d->n_kv, d->B);
+    // (32 angles a token take 8 KiB of LDS, 128 take 32: two workgroups fewer a CU)
+    if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<32>), grid, dim3(256), a);
+    else VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<MAXR>), grid, dim3(256), a);
     return 0;
 }

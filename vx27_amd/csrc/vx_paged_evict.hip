@@ -6,7 +6,7 @@
 //
 //   paged_select  one workgroup per (sequence, KV head): the weight of the
 //                 last row kept is found digit by digit (a radix select over
-//                 the weights' bits, 8 at a time), then the kept rows are
+//                 the weights' bits: 12, 10 and 10), then the kept rows are
 //                 written in order by prefix sums.
 //   paged_move    copies the kept rows' K, V and weights.
 #include "vx_paged.h"
@@ -41,9 +41,13 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int SEL = 1024;
+// Wave w owns rows [w seg, (w+1) seg) and reads them 64 at a time, CH of
+// these per chunk; a sequence of up to 16 * 64 * CH rows is one chunk a wave,
+// read once and held in registers through all passes.
+constexpr int SEL = 1024, NW = SEL / 64, CH = 32, BINS = 4096;
 __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = seq_len(a, b), keep = min(n, a.budget);
     int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.budget;
     if (h == 0 && tid == 0) a.dst_len[b] = keep;
@@ -54,94 +58,180 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     const float *w = a.acc + ((size_t)b * a.p.n_kv + h) * a.acc_stride;
     const int lo = a.n_sink, hi = n - a.n_recent;     // the rows that compete
     int want = a.budget - a.n_sink - a.n_recent;      // how many of them stay
-    __shared__ int hist[256];
-    __shared__ int s_digit, s_want, wsum[SEL / 64], weq[SEL / 64];
+    __shared__ int hist[BINS];
+    __shared__ int s_sum[NW], s_eq[NW], s_found[2];
+    const int seg = ((n + NW - 1) / NW + 63) / 64 * 64, w0 = wave * seg, w1 = min(w0 + seg, n);
+    uint32_t r[CH];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < CH; k++)
+            if (base + 64 * k < w1) r[k] = rank_of(w[min(base + 64 * k + lane, n - 1)]);
+    };
+    const bool once = seg <= CH * 64;
+    load(w0);
     uint32_t prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    int shift = 32;
+    const int none = want == 0;
+    for (int pass = 0; pass < 3 && !none; pass++) {
+        const int bits = pass ? 10 : 12;
+        shift -= bits;
+        for (int i = tid; i < BINS; i += SEL) hist[i] = 0;
         __syncthreads();
-        for (int i = lo + tid; i < hi; i += SEL) {
-            const uint32_t r = rank_of(w[i]);
-            if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int left = want, dgt = 255;
-            while (hist[dgt] < left) left -= hist[dgt--];   // (at least `want` rows match the prefix)
-            s_digit = dgt;
-            s_want = left;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)s_digit << shift;
-        mask |= 0xffu << shift;
-        want = s_want;
-        __syncthreads();
-    }
-    // rows above `prefix` stay, and the first `want` equal to it; none where want started at 0
-    const bool none = a.budget == a.n_sink + a.n_recent;
-    int out = 0, eq_seen = 0;
-    for (int i0 = 0; i0 < n; i0 += SEL) {
-        const int i = i0 + tid;
-        bool forced = false, above = false, eq = false;
-        if (i < n) {
-            forced = i < lo || i >= hi;
-            if (!forced && !none) {
-                const uint32_t r = rank_of(w[i]);
-                above = r > prefix;
-                eq = r == prefix;
+        for (int base = w0; base < w1; base += CH * 64) {
+            if (!once) load(base);
+#pragma unroll
+            for (int k = 0; k < CH; k++) {
+                if (base + 64 * k >= w1) continue;   // (uniform)
+                const int i = base + 64 * k + lane;
+                const bool in = i < w1 && i >= lo && i < hi && (r[k] & mask) == prefix;
+                // rows that no token weighed are many: counted by the wave, not one by one in the same bin
+                const uint64_t zero = __ballot(in && r[k] == 0x80000000u);
+                if (in && r[k] != 0x80000000u) atomicAdd(&hist[(r[k] >> shift) & ((1 << bits) - 1)], 1);
+                if (zero && lane == 0) atomicAdd(&hist[(0x80000000u >> shift) & ((1 << bits) - 1)], __popcll(zero));
             }
         }
-        const uint64_t below = lane ? (~0ull >> (64 - lane)) : 0;
-        const uint64_t be = __ballot(eq);
-        if (lane == 0) weq[wave] = __popcll(be);
         __syncthreads();
-        int e = eq_seen + __popcll(be & below), etot = eq_seen;
-        for (int k = 0; k < SEL / 64; k++) {
-            if (k < wave) e += weq[k];
-            etot += weq[k];
+        // the bin of the want-th heaviest: thread t takes bins 4 t .. 4 t + 3 (from the top), suffix sums over the threads
+        int c[4], mine = 0;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int bin = BINS - 1 - (4 * tid + q);
+            c[q] = bin < (1 << bits) ? hist[bin] : 0;
+            mine += c[q];
         }
-        const bool stay = forced || above || (eq && e < want);
-        const uint64_t bs = __ballot(stay);
-        if (lane == 0) wsum[wave] = __popcll(bs);
-        __syncthreads();
-        int at = out + __popcll(bs & below), tot = out;
-        for (int k = 0; k < SEL / 64; k++) {
-            if (k < wave) at += wsum[k];
-            tot += wsum[k];
+        int x = mine;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
         }
-        if (stay) kept[at] = i;
-        out = tot;
-        eq_seen = etot;
+        if (lane == 63) s_sum[wave] = x;
         __syncthreads();
+        x -= mine;
+        for (int k = 0; k < wave; k++) x += s_sum[k];
+        if (x < want && x + mine >= want) {   // one thread (at least `want` rows match the prefix)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (x < want && x + c[q] >= want) {
+                    s_found[0] = BINS - 1 - (4 * tid + q);
+                    s_found[1] = want - x;
+                }
+                x += c[q];
+            }
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_found[0] << shift;
+        mask |= (uint32_t)((1 << bits) - 1) << shift;
+        want = s_found[1];
+        __syncthreads();
+    }
+    // Rows above `prefix` stay, and the first `want` equal to it: each wave
+    // counts its own of both kinds, then writes them behind those of the
+    // waves before it.
+    auto kinds = [&](int i, uint32_t u, bool &eq) {
+        const bool in = i < w1, mid = i >= lo && i < hi;
+        eq = in && mid && !none && u == prefix;
+        return in && (!mid || (!none && u > prefix));
+    };
+    int nsure = 0, neq = 0;
+    for (int base = w0; base < w1; base += CH * 64) {
+        if (!once) load(base);
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            if (base + 64 * k >= w1) continue;
+            bool eq;
+            const bool sure = kinds(base + 64 * k + lane, r[k], eq);
+            nsure += __popcll(__ballot(sure));
+            neq += __popcll(__ballot(eq));
+        }
+    }
+    if (lane == 0) {
+        s_sum[wave] = nsure;
+        s_eq[wave] = neq;
+    }
+    __syncthreads();
+    int at = 0, eqs = 0;
+    for (int k = 0; k < wave; k++) {
+        at += s_sum[k];
+        eqs += s_eq[k];
+    }
+    at += min(eqs, want);
+    const uint64_t below = lane ? (~0ull >> (64 - lane)) : 0;
+    for (int base = w0; base < w1; base += CH * 64) {
+        if (!once) load(base);
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            if (base + 64 * k >= w1) continue;
+            bool eq;
+            const int i = base + 64 * k + lane;
+            const bool sure = kinds(i, r[k], eq);
+            const uint64_t be = __ballot(eq);
+            const bool stay = sure || (eq && eqs + __popcll(be & below) < want);
+            const uint64_t bs = __ballot(stay);
+            if (stay) kept[at + __popcll(bs & below)] = i;
+            at += __popcll(bs);
+            eqs += __popcll(be);
+        }
     }
 }
 
-// grid (32-row blocks of the destination, n_kv, B), block 256: wave w moves
-// K rows w, w + 4, ...; thread d gathers dim d of the block's V rows.
+// grid (32-row blocks of the destination, n_kv, B), block 256.  K: wave w
+// moves rows w, w + 4, ..., 512 bytes each.  V: a destination block's rows
+// come from a few source blocks, each read whole (a kept row has two bytes in
+// every 64-byte line of its block) into LDS, dim by dim 68 bytes apart, so
+// that thread d's reads of dim d fall on distinct banks.
+constexpr int VROW = VB + 2;   // elements from dim to dim in LDS
 __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = seq_len(a, b), keep = min(n, a.budget), d0 = blockIdx.x * VB;
     if (d0 >= keep) return;
-    const int cnt = min(VB, keep - d0);
-    __shared__ int s_row[VB], s_page[VB];
+    const int cnt = min(VB, keep - d0), P = a.p.page_size;
+    __shared__ int s_row[VB];
+    __shared__ size_t s_blk[VB];   // element offset of the row's V block
+    __shared__ uint16_t sv[HDG * VROW];
     const int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.budget;
+    const int dpage = vx_page_checked(a.p, a.dst_table[(size_t)b * a.dst_max_pages + d0 / P]), dat = d0 % P;
     if (tid < VB) {
         const int r = kept[d0 + min(tid, cnt - 1)];
         s_row[tid] = r;
-        s_page[tid] = vx_paged_page(a.p, b, r);
+        s_blk[tid] = vx_v_index(a.p.n_kv, P, vx_paged_page(a.p, b, r), h, r % P / VB * VB, 0);
         if (a.acc_out && tid < cnt)
             a.acc_out[((size_t)b * a.p.n_kv + h) * a.acc_out_stride + d0 + tid] = a.acc[((size_t)b * a.p.n_kv + h) * a.acc_stride + r];
     }
     __syncthreads();
-    const int P = a.p.page_size;
-    const int dpage = vx_page_checked(a.p, a.dst_table[(size_t)b * a.dst_max_pages + d0 / P]), dat = d0 % P;
-    for (int j = wave; j < cnt; j += 4) {
-        const uint2 u = *(const uint2 *)(a.k_pages + vx_k_index(a.p.n_kv, P, s_page[j], h, s_row[j] % P, 4 * lane));
-        *(uint2 *)(a.k_pages + vx_k_index(a.p.n_kv, P, dpage, h, dat + j, 4 * lane)) = u;
+    // K rows: all loads, then all stores (a V block is as large as its 32 K
+    // rows, so a row's K lies at the same offset)
+    uint2 kr[VB / 4];
+#pragma unroll
+    for (int j = 0; j < VB / 4; j++) {
+        const int q = min(wave + 4 * j, cnt - 1);
+        kr[j] = *(const uint2 *)(a.k_pages + s_blk[q] + (size_t)(s_row[q] % VB) * HDG + 4 * lane);
     }
     uint16_t v[VB];
+    for (int j = 0; j < cnt;) {
+        const size_t blk = s_blk[j];
+        uint4 u[4];
 #pragma unroll
-    for (int j = 0; j < VB; j++) v[j] = a.v_pages[vx_v_index(a.p.n_kv, P, s_page[j], h, s_row[j] % P, tid)];
+        for (int i = 0; i < 4; i++) u[i] = *(const uint4 *)(a.v_pages + blk + (size_t)(tid + 256 * i) * 8);
+        if (j) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {   // unit tid + 256 i: dim unit / 4, rows 8 (unit % 4) ..
+            uint32_t *d = (uint32_t *)&sv[((tid >> 2) + 64 * i) * VROW + (tid & 3) * 8];
+            d[0] = u[i].x; d[1] = u[i].y; d[2] = u[i].z; d[3] = u[i].w;
+        }
+        __syncthreads();
+        int e = j;
+#pragma unroll
+        for (int q = 0; q < VB; q++)
+            if (q >= j && q < cnt && s_blk[q] == blk) {   // (uniform; the rows are in order, so these are j, j + 1, ...)
+                v[q] = sv[tid * VROW + s_row[q] % VB];
+                e = q + 1;
+            }
+        j = __builtin_amdgcn_readfirstlane(e);
+    }
+#pragma unroll
+    for (int j = 0; j < VB / 4; j++)
+        if (wave + 4 * j < cnt) *(uint2 *)(a.k_pages + vx_k_index(a.p.n_kv, P, dpage, h, dat + wave + 4 * j, 4 * lane)) = kr[j];
     uint16_t *dst = a.v_pages + vx_v_index(a.p.n_kv, P, dpage, h, dat, tid);
     if (cnt == VB) {
 #pragma unroll
