@@ -20,14 +20,25 @@ struct vx_pseq {
     int start, T, len, row0;
 };
 
+// A word of a table that no kernel of the call writes: through the constant
+// address space, so that it may be loaded once, early and by the scalar unit
+// (the kernels' own stores would otherwise order every use).
+__host__ __device__ __forceinline__ int vx_table_word(const int *p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return *(const __attribute__((address_space(4))) int *)(uintptr_t)p;
+#else
+    return *p;
+#endif
+}
+
 __host__ __device__ __forceinline__ vx_pseq vx_paged_seq(const vx_paged &p, int b) {
     vx_pseq s;
     const int cap = p.max_pages * p.page_size;
-    const int n = p.len[b];
+    const int n = vx_table_word(p.len + b);
     s.len = min(max(n, 0), cap);
     bool bad = s.len != n;
     if (p.q_start) {
-        const int s0 = p.q_start[b], s1 = p.q_start[b + 1];
+        const int s0 = vx_table_word(p.q_start + b), s1 = vx_table_word(p.q_start + b + 1);
         s.start = min(max(s0, 0), p.n_tok);
         s.T = min(max(s1, s.start), p.n_tok) - s.start;
         bad |= s.start != s0 || s.start + s.T != s1 || s.T > p.max_T;
@@ -51,7 +62,7 @@ __host__ __device__ __forceinline__ int vx_page_slot(const vx_paged &p, int r) {
     return p.log2_page >= 0 ? r >> p.log2_page : r / p.page_size;
 }
 __host__ __device__ __forceinline__ int vx_paged_page(const vx_paged &p, int b, int r) {
-    return vx_page_checked(p, p.table[(size_t)b * p.max_pages + vx_page_slot(p, r)]);
+    return vx_page_checked(p, vx_table_word(p.table + (size_t)b * p.max_pages + vx_page_slot(p, r)));
 }
 
 // The bits of rows key0 .. key0 + 31 that lie below row n.

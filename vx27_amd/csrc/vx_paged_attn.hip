@@ -682,7 +682,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     uint32_t at_lo, at_hi;
     auto fill_at = [&]() {
         const int key = tl.at(min(2 * (base + lane) + (wave >> 1), tl.nt - 1)) * TILE, slot = vx_page_slot(a.p, key);
-        const int page = vx_page_checked(a.p, a.p.table[(size_t)b * a.p.max_pages + slot]);
+        const int page = vx_page_checked(a.p, vx_table_word(a.p.table + (size_t)b * a.p.max_pages + slot));
         const uint64_t at = (((uint64_t)page * a.p.n_kv + kvh) * a.p.page_size + (key - slot * a.p.page_size)) * HDG;
         at_lo = (uint32_t)at;
         at_hi = (uint32_t)(at >> 32);

@@ -30,7 +30,7 @@ struct EvictArgs {
 };
 
 __device__ __forceinline__ int seq_len(const EvictArgs &a, int b) {
-    const int n = a.p.len[b], c = min(max(n, 0), a.p.max_pages * a.p.page_size);
+    const int n = vx_table_word(a.p.len + b), c = min(max(n, 0), a.p.max_pages * a.p.page_size);
     if (c != n) *a.p.err_flag = 1;
     return c;
 }
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
     __shared__ size_t s_blk[VB];   // element offset of the row's V block
     __shared__ uint16_t sv[HDG * VROW];
     const int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.budget;
-    const int dpage = vx_page_checked(a.p, a.dst_table[(size_t)b * a.dst_max_pages + d0 / P]), dat = d0 % P;
+    const int dpage = vx_page_checked(a.p, vx_table_word(a.dst_table + (size_t)b * a.dst_max_pages + d0 / P)), dat = d0 % P;
     if (tid < VB) {
         const int r = kept[d0 + min(tid, cnt - 1)];
         s_row[tid] = r;
