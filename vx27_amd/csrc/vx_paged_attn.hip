@@ -171,18 +171,6 @@ __device__ __forceinline__ void attend_tile(Rows &w, const float (&s)[8], const 
         for (int d = 0; d < 16; d++) w.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[d], p[k], w.o[d], 0, 0, 0);
 }
 
-__device__ __forceinline__ float gate_of(const Args &a, int tok, int h, int d) {
-    const size_t at = (size_t)tok * a.g_ts + (size_t)h * a.g_hs + d;
-    return a.gate_bf16 ? vx_bf16_to_f32(((const uint16_t *)a.gate)[at]) : ((const float *)a.gate)[at];
-}
-// One finished value: O / l (0 where nothing was seen), gated.
-__device__ __forceinline__ void out_store(const Args &a, int tok, int h, int d, float O, float L) {
-    float r = L > 0.0f || L != L ? O / L : 0.0f;
-    if (a.gate) r = r * (1.0f / (1.0f + expf(-gate_of(a, tok, h, d))));
-    const size_t at = ((size_t)tok * a.n_q + h) * HDG + d;
-    if (a.out_bf16) ((uint16_t *)a.out)[at] = vx_f32_to_bf16(r);
-    else ((float *)a.out)[at] = r;
-}
 __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float m, float L) {
     const size_t at = (size_t)tok * a.n_q + h;
     if (a.lse) a.lse[at] = L > 0.0f || L != L ? (m + log2f(L)) * 0.6931471805599453f : -INFINITY;
@@ -203,18 +191,34 @@ __device__ __forceinline__ float4 gate_row(const Args &a, int tok, int h) {
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                        __uint_as_float(u.y & 0xffff0000u));
 }
-// One finished query row across a wave, gated by logits x.
+__device__ __forceinline__ void row_write(const Args &a, int tok, int h, float4 r) {
+    const size_t at = ((size_t)tok * a.n_q + h) * HDG + 4 * (threadIdx.x & 63);
+    if (a.out_bf16) *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack2(r.x, r.y), pack2(r.z, r.w));
+    else *(float4 *)((float *)a.out + at) = r;
+}
+// A finished query row of the tile kernel across a wave, gated by logits x
+// (hardware exp2 and reciprocals: one part in 2^22, below its weights' rounding).
 __device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 r, float4 x) {
-    const int lane = threadIdx.x & 63;
-    if (a.gate) {   // (hardware reciprocals: one part in 2^23, below the weights' rounding)
+    if (a.gate) {
         auto sg = [](float y) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f)); };
         r.x *= sg(x.x); r.y *= sg(x.y); r.z *= sg(x.z); r.w *= sg(x.w);
     }
-    const size_t at = ((size_t)tok * a.n_q + h) * HDG + 4 * lane;
-    if (a.out_bf16)
-        *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack2(r.x, r.y), pack2(r.z, r.w));
-    else
-        *(float4 *)((float *)a.out + at) = r;
+    row_write(a, tok, h, r);
+}
+// The same from a decode row's sums (fp32 accuracy), with its statistics.
+__device__ __forceinline__ void row_finish(const Args &a, int tok, int h, float4 O, float M, float L, float4 x) {
+    const bool some = L > 0.0f || L != L;   // (0 where nothing was seen)
+    float4 r = some ? make_float4(O.x / L, O.y / L, O.z / L, O.w / L) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.gate) {
+        auto sg = [](float y) { return 1.0f / (1.0f + expf(-y)); };
+        r.x *= sg(x.x); r.y *= sg(x.y); r.z *= sg(x.z); r.w *= sg(x.w);
+    }
+    row_write(a, tok, h, r);
+    if ((threadIdx.x & 63) == 0) stat_store(a, tok, h, M, L);
+}
+__device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l, float w) {
+    L += l * w;
+    O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
 }
 
 // ---------------------------------------------------------------- decode
@@ -224,27 +228,76 @@ __device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 
 // workgroup is finished there; the first and the last piece of a
 // workgroup's range may be parts of a pair and go to its two partial slots,
 // which paged_join merges in order.
-struct Plan {
-    int total, chunk;
-};
-__device__ __forceinline__ int seq_units(const Args &a, int b, int &nt) {
-    const vx_pseq s = vx_paged_seq(a.p, b);
-    nt = tiles_of(a, s, 0, s.T - 1).nt;
-    return nt * a.p.n_kv;
-}
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_i(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xF, true); }
+// Sum over lanes 0 .. l (the VALU's DPP paths: no LDS round trips).
+__device__ __forceinline__ int wave_scan_i(int v) {
+    v += dpp_i<0x111, 0xF>(v);   // row_shr:1
+    v += dpp_i<0x112, 0xF>(v);
+    v += dpp_i<0x114, 0xF>(v);
+    v += dpp_i<0x118, 0xF>(v);
+    v += dpp_i<0x142, 0xA>(v);   // row_bcast:15 into rows 1 and 3
+    v += dpp_i<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
     return v;
 }
-__device__ __forceinline__ Plan plan_of(const Args &a, int grid) {
+// The list of a call's tiles: up to 64 sequences are held one a lane and read
+// once; more are read again where they are needed.
+struct Units {
+    vx_pseq s;          // of sequence `lane` (B <= 64)
+    vx_tiles t;
+    int upto;           // units of sequences 0 .. lane
+    int total, chunk;
+};
+__device__ __forceinline__ int seq_units(const Args &a, int b, vx_pseq &s, vx_tiles &t) {
+    s = vx_paged_seq(a.p, b);
+    t = tiles_of(a, s, 0, s.T - 1);
+    return t.nt * a.p.n_kv;
+}
+__device__ __forceinline__ Units units_of(const Args &a, int grid) {
     const int lane = threadIdx.x & 63;
-    int sum = 0, nt;
-    for (int b = lane; b < a.p.B; b += 64) sum += seq_units(a, b, nt);
-    Plan p;
-    p.total = __builtin_amdgcn_readfirstlane(wave_sum_i(sum));
-    p.chunk = max((p.total + grid - 1) / grid, a.min_tiles);
-    return p;
+    Units u;
+    if (a.p.B <= 64) {
+        const int n = seq_units(a, min(lane, a.p.B - 1), u.s, u.t);
+        u.upto = wave_scan_i(lane < a.p.B ? n : 0);
+        u.total = __builtin_amdgcn_readlane(u.upto, 63);
+    } else {
+        int sum = 0;
+        for (int b0 = 0; b0 < a.p.B; b0 += 64) {
+            const int n = seq_units(a, min(b0 + lane, a.p.B - 1), u.s, u.t);
+            sum += b0 + lane < a.p.B ? n : 0;
+        }
+        u.total = __builtin_amdgcn_readlane(wave_scan_i(sum), 63);
+    }
+    u.chunk = max((u.total + grid - 1) / grid, a.min_tiles);
+    return u;
+}
+// Sequence b: itself, its tiles, and the units before it.
+__device__ __forceinline__ int units_before(const Args &a, const Units &u, int b, vx_pseq &s, vx_tiles &t) {
+    if (a.p.B <= 64) {
+        auto get = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
+        s = {get(u.s.start), get(u.s.T), get(u.s.len), get(u.s.row0)};
+        t = {get(u.t.st), get(u.t.fm), get(u.t.nt)};
+        return get(u.upto) - t.nt * a.p.n_kv;
+    }
+    int sum = 0;
+    for (int c = threadIdx.x & 63; c < b; c += 64) sum += seq_units(a, c, s, t);
+    sum = __builtin_amdgcn_readlane(wave_scan_i(sum), 63);
+    seq_units(a, b, s, t);
+    return sum;
+}
+// The sequence of unit x < total.
+__device__ __forceinline__ int units_find(const Args &a, const Units &u, int x) {
+    const int lane = threadIdx.x & 63;
+    if (a.p.B <= 64) return __builtin_ctzll(__ballot(u.upto > x));
+    int done = 0;
+    for (int b0 = 0;; b0 += 64) {
+        vx_pseq s;
+        vx_tiles t;
+        const int n = seq_units(a, min(b0 + lane, a.p.B - 1), s, t), upto = wave_scan_i(b0 + lane < a.p.B ? n : 0);
+        const uint64_t past = __ballot(done + upto > x);
+        if (past || b0 + 64 >= a.p.B) return b0 + (past ? __builtin_ctzll(past) : 0);
+        done += __builtin_amdgcn_readlane(upto, 63);
+    }
 }
 
 __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
@@ -252,42 +305,23 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     __shared__ __attribute__((aligned(16))) float s_o[4][16 * HDG];
     __shared__ float s_m[4][16], s_l[4][16];
-    const Plan pl = plan_of(a, gridDim.x);
-    const int u0 = blockIdx.x * pl.chunk, u1 = min(u0 + pl.chunk, pl.total);
+    const Units un = units_of(a, gridDim.x);
+    const int u0 = blockIdx.x * un.chunk, u1 = min(u0 + un.chunk, un.total);
     if (u0 >= u1) return;
-    // the sequence of unit u0, and the units before it
-    int b = 0, before = 0;
-    {
-        int done = 0;
-        for (int b0 = 0; b0 < a.p.B; b0 += 64) {
-            int nt, x = b0 + lane < a.p.B ? seq_units(a, b0 + lane, nt) : 0;
-            const int own_x = x;
-            for (int off = 1; off < 64; off <<= 1) {
-                const int y = __shfl_up(x, off, 64);
-                if (lane >= off) x += y;
-            }
-            const uint64_t past = __ballot(done + x > u0);
-            if (past) {
-                const int f = __builtin_ctzll(past);
-                b = b0 + f;
-                before = done + __shfl(x - own_x, f, 64);
-                break;
-            }
-            done += __shfl(x, 63, 64);
-        }
-        b = __builtin_amdgcn_readfirstlane(b);
-        before = __builtin_amdgcn_readfirstlane(before);
-    }
+    int b = units_find(a, un, u0);
     const int krow0 = 8 * (n >> 2) + (n & 3);
+    vx_pseq s;
+    vx_tiles tl;
+    int before = units_before(a, un, b, s, tl);
     for (int u = u0; u < u1;) {
-        const vx_pseq s = vx_paged_seq(a.p, b);
-        const vx_tiles tl = tiles_of(a, s, 0, s.T - 1);
         if (u >= before + tl.nt * a.p.n_kv) {
             before += tl.nt * a.p.n_kv;
             b++;
+            if (a.p.B <= 64) units_before(a, un, b, s, tl);
+            else seq_units(a, b, s, tl);
             continue;
         }
-        const int kvh = (u - before) / tl.nt, i0 = (u - before) % tl.nt;
+        const int kvh = (u - before) / tl.nt, i0 = (u - before) - kvh * tl.nt;
         const int cnt = min(tl.nt - i0, u1 - u);
         const int R = s.T * a.qg;
         Rows w;
@@ -327,26 +361,31 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
             }
         }
         __syncthreads();
+        // wave w merges rows w, w + 4, ..., lane L dims 4L .. 4L + 3
         const bool whole = cnt == tl.nt;
         const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
-        for (int r = 0; r < R; r++) {
-            float M = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; k++) M = fmaxf(M, s_m[k][r]);
-            float L = 0.0f, O = 0.0f;
+        for (int r = wave; r < R; r += 4) {
+            const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
+            float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (whole && a.gate) gt = gate_row(a, tok, h);
+            float m[4], l[4];
+            float4 o[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float sc = s_m[k][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[k][r] - M);
-                L += s_l[k][r] * sc;
-                O += s_o[k][r * HDG + ((((tid >> 2) ^ r) << 2) | (tid & 3))] * sc;
+                m[k] = s_m[k][r];
+                l[k] = s_l[k][r];
+                o[k] = *(const float4 *)&s_o[k][r * HDG + ((lane ^ r) << 2)];
             }
+            const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            float L = 0.0f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) add_part(O, L, o[k], l[k], m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - M));
             if (whole) {
-                const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
-                out_store(a, tok, h, tid, O, L);
-                if (tid == 0) stat_store(a, tok, h, M, L);
+                row_finish(a, tok, h, O, M, L, gt);
             } else {
-                a.part_o[((size_t)slot * a.part_rows + r) * HDG + tid] = O;
-                if (tid == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
+                *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + r) * HDG + 4 * lane) = O;
+                if (lane == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
             }
         }
         __syncthreads();
@@ -355,40 +394,48 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
 }
 
 // grid (max rows, n_kv, B), block 256: merges the parts of one query row, in
-// their order: wave w takes parts w, w + 4, ...; a row of a sequence without
-// rows gets 0.
+// their order: wave w takes parts w, w + 4, ..., eight in flight; a row of a
+// sequence without rows gets 0.
 __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     const int r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const vx_pseq s = vx_paged_seq(a.p, b);
+    const Units un = units_of(a, grid);
+    vx_pseq s;
+    vx_tiles tl;
+    const int p0 = units_before(a, un, b, s, tl) + kvh * tl.nt, p1 = p0 + tl.nt;
     if (r >= s.T * a.qg) return;
     const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
-    const int nt = tiles_of(a, s, 0, s.T - 1).nt;
-    if (nt == 0) {
-        out_store(a, tok, h, tid, 0.0f, 0.0f);
-        if (tid == 0) stat_store(a, tok, h, -INFINITY, 0.0f);
-        return;
-    }
-    const Plan pl = plan_of(a, grid);
-    int sum = 0, x;
-    for (int c = lane; c < b; c += 64) sum += seq_units(a, c, x);
-    const int p0 = __builtin_amdgcn_readfirstlane(wave_sum_i(sum)) + kvh * nt, p1 = p0 + nt;
-    const int g0 = p0 / pl.chunk, g1 = (p1 - 1) / pl.chunk;
-    if (g0 == g1) return;
+    const int g0 = p0 / un.chunk, g1 = (p1 - 1) / un.chunk;
+    if (tl.nt > 0 && g0 == g1) return;
+    float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (wave == 0 && a.gate) gt = gate_row(a, tok, h);
     __shared__ float4 s_o[4][64];
     __shared__ float s_m[4], s_l[4];
     float M = -INFINITY, L = 0.0f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = g0 + wave; w <= g1; w += 4) {
-        const size_t pi = (size_t)(2 * w + (w == g0 && p0 != w * pl.chunk ? 1 : 0)) * a.part_rows + r;
-        const float2 ml = a.part_ml[pi];
-        const float4 o = ((const float4 *)(a.part_o + pi * HDG))[lane];
-        const float mn = fmaxf(M, ml.x);
+    constexpr int NP = 8;
+    for (int w0 = g0 + wave; w0 <= g1 && tl.nt > 0; w0 += 4 * NP) {
+        float2 ml[NP];
+        float4 o[NP];
+#pragma unroll
+        for (int k = 0; k < NP; k++) {   // (past the last part: the last again, weighed 0)
+            const int w = min(w0 + 4 * k, g1);
+            const size_t pi = (size_t)(2 * w + (w == g0 && p0 != w * un.chunk ? 1 : 0)) * a.part_rows + r;
+            ml[k] = a.part_ml[pi];
+            o[k] = ((const float4 *)(a.part_o + pi * HDG))[lane];
+        }
+        float mn = M;
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            if (w0 + 4 * k > g1) ml[k].x = -INFINITY;
+            mn = fmaxf(mn, ml[k].x);
+        }
         if (mn == -INFINITY) continue;
-        const float sa = __builtin_amdgcn_exp2f(M - mn), sb = __builtin_amdgcn_exp2f(ml.x - mn);
-        L = L * sa + ml.y * sb;
-        O.x = O.x * sa + o.x * sb; O.y = O.y * sa + o.y * sb;
-        O.z = O.z * sa + o.z * sb; O.w = O.w * sa + o.w * sb;
+        const float sa = __builtin_amdgcn_exp2f(M - mn);
+        L *= sa;
+        O.x *= sa; O.y *= sa; O.z *= sa; O.w *= sa;
+#pragma unroll
+        for (int k = 0; k < NP; k++) add_part(O, L, o[k], ml[k].y, __builtin_amdgcn_exp2f(ml[k].x - mn));
         M = mn;
     }
     s_o[wave][lane] = O;
@@ -397,18 +444,13 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
         s_l[wave] = L;
     }
     __syncthreads();
-    float Mt = -INFINITY;
+    if (wave) return;
+    const float Mt = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    L = 0.0f;
+    O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < 4; k++) Mt = fmaxf(Mt, s_m[k]);
-    float Lt = 0.0f, Ot = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const float sc = s_m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[k] - Mt);
-        Lt += s_l[k] * sc;
-        Ot += ((const float *)s_o[k])[tid] * sc;
-    }
-    out_store(a, tok, h, tid, Ot, Lt);
-    if (tid == 0) stat_store(a, tok, h, Mt, Lt);
+    for (int k = 0; k < 4; k++) add_part(O, L, s_o[k][lane], s_l[k], s_m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[k] - Mt));
+    row_finish(a, tok, h, O, Mt, L, gt);
 }
 
 // grid (tile_cap / 8, n_kv, B), block 256: one thread per key; the stashed
