@@ -196,12 +196,13 @@ __device__ __forceinline__ void row_write(const Args &a, int tok, int h, float4 
     if (a.out_bf16) *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack2(r.x, r.y), pack2(r.z, r.w));
     else *(float4 *)((float *)a.out + at) = r;
 }
-// A finished query row of the tile kernel across a wave, gated by logits x
-// (hardware exp2 and reciprocals: one part in 2^22, below its weights' rounding).
+// (hardware exp2 and reciprocal: one part in 2^22, below the rounding of the
+// tile kernel's weights)
+__device__ __forceinline__ float fast_sigmoid(float y) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f)); }
+// A finished query row of the tile kernel across a wave, gated by logits x.
 __device__ __forceinline__ void row_store(const Args &a, int tok, int h, float4 r, float4 x) {
     if (a.gate) {
-        auto sg = [](float y) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f)); };
-        r.x *= sg(x.x); r.y *= sg(x.y); r.z *= sg(x.z); r.w *= sg(x.w);
+        r.x *= fast_sigmoid(x.x); r.y *= fast_sigmoid(x.y); r.z *= fast_sigmoid(x.z); r.w *= fast_sigmoid(x.w);
     }
     row_write(a, tok, h, r);
 }
@@ -560,23 +561,24 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int E = a.p.B * n_rt, per = (E + PLAN - 1) / PLAN, e0 = min(tid * per, E);
     int e1 = min(e0 + per, E);
-    int b, r0 = 0, items = 0;
+    int b = 0, r0 = 0, items = 0, n0 = 0;
     int64_t steps = 0;
     for (int e = e0; e < e1; e++) {
-        const int n = entry_steps(a, n_rt, e, b, r0);
-        steps += n;
-        items += n > 0;
+        n0 = entry_steps(a, n_rt, e, b, r0);
+        steps += n0;
+        items += n0 > 0;
     }
-    for (int off = 32; off >= 1; off >>= 1) {
-        steps += __shfl_xor(steps, off, 64);
-        items += __shfl_xor(items, off, 64);
-    }
-    if (lane == 0) {
+    // (a thread's only entry is not looked up again)
+    auto steps_of = [&](int e) { return per == 1 ? n0 : entry_steps(a, n_rt, e, b, r0); };
+    items = wave_scan_i(items);
+    for (int off = 32; off >= 1; off >>= 1) steps += __shfl_xor(steps, off, 64);
+    if (lane == 63) {
         s_steps[wave] = steps;
         s_sum[0][wave] = items;
     }
     __syncthreads();
     steps = items = 0;
+#pragma unroll
     for (int w = 0; w < PLAN / 64; w++) {
         steps += s_steps[w];
         items += s_sum[0][w];
@@ -589,7 +591,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     // (pieces, slots, joins) of this thread's entries, then their places
     int cnt[3] = {0, 0, 0};
     for (int e = e0; e < e1; e++) {
-        const int n = entry_steps(a, n_rt, e, b, r0), parts = (n + limit - 1) / limit;
+        const int n = steps_of(e), parts = (n + limit - 1) / limit;
         cnt[0] += parts;
         cnt[1] += parts > 1 ? parts : 0;
         cnt[2] += parts > 1;
@@ -597,11 +599,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     int at[3], tot[3];
 #pragma unroll
     for (int c = 0; c < 3; c++) {
-        int x = cnt[c];
-        for (int off = 1; off < 64; off <<= 1) {
-            const int y = __shfl_up(x, off, 64);
-            if (lane >= off) x += y;
-        }
+        const int x = wave_scan_i(cnt[c]);
         if (lane == 63) s_sum[c][wave] = x;
         at[c] = x - cnt[c];
     }
@@ -609,16 +607,18 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
 #pragma unroll
     for (int c = 0; c < 3; c++) {
         tot[c] = 0;
+#pragma unroll
         for (int w = 0; w < PLAN / 64; w++) {
-            if (w < wave) at[c] += s_sum[c][w];
-            tot[c] += s_sum[c][w];
+            const int x = s_sum[c][w];
+            at[c] += w < wave ? x : 0;
+            tot[c] += x;
         }
     }
     // (token ranges that overlap, an error that vx_paged_seq has flagged, may
     // make more pieces than there is room for: then nothing runs)
     if ((int64_t)tot[0] * a.p.n_kv > max_pieces) e1 = e0, tot[0] = tot[2] = 0, *a.p.err_flag = 1;
     for (int e = e0; e < e1; e++) {
-        const int n = entry_steps(a, n_rt, e, b, r0), parts = (n + limit - 1) / limit;
+        const int n = steps_of(e), parts = (n + limit - 1) / limit;
         if (parts == 0) continue;
         for (int h = 0; h < a.p.n_kv; h++) {
             const int slot = h * tot[1] + at[1];
@@ -1041,18 +1041,18 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         }
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
     }
-    // Gates of this wave's output rows (wave, wave + 4, ...: one row of 256
-    // dims across a wave), all loaded before the first is used: a load behind
-    // the rows' stores would wait for them.
-    constexpr int WR = TR / 4;
-    uint2 gt[WR];
+    // Output rows of this wave: pairs (8 k + 2 wave, + 1), half a wave each,
+    // lane L dims 8 (L % 32) .. +7.  Their bf16 gates are all loaded before the
+    // first is used: a load behind the rows' stores would wait for them.
+    constexpr int WR = TR / 8;
+    uint4 gt[WR];
     const bool gated = a.gate && !parted;
-    auto row_of = [&](int k) { return min(r0 + wave + 4 * k, R - 1); };
+    auto out_row = [&](int k) { return r0 + 8 * k + 2 * wave + (lane >> 5); };
     if (gated && a.gate_bf16) {
 #pragma unroll
         for (int k = 0; k < WR; k++) {
-            const int r = row_of(k), t = row_tok(a, r);
-            gt[k] = *(const uint2 *)((const uint16_t *)a.gate + (size_t)(s.start + t) * a.g_ts + (size_t)row_head(a, kvh, r, t) * a.g_hs + 4 * lane);
+            const int r = min(out_row(k), R - 1), t = row_tok(a, r);
+            gt[k] = *(const uint4 *)((const uint16_t *)a.gate + (size_t)(s.start + t) * a.g_ts + (size_t)row_head(a, kvh, r, t) * a.g_hs + 8 * (lane & 31));
         }
     }
     // row sums: over the lane pair and the two key blocks
@@ -1088,60 +1088,110 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         }
     }
     vx_lds_barrier();
-    auto orow = [&](int k) {
-        const int r = wave + 4 * k;
-        return *(const float4 *)(so + r * HDG + ((lane ^ (r & 15)) << 2));
+    auto orow = [&](int k, float4 &x, float4 &y) {
+        const int r = out_row(k) - r0, u = 2 * (lane & 31);
+        x = *(const float4 *)(so + r * HDG + ((u ^ (r & 15)) << 2));
+        y = *(const float4 *)(so + r * HDG + (((u + 1) ^ (r & 15)) << 2));
     };
     if (parted) {
 #pragma unroll 4
-        for (int k = 0; k < WR; k++)
-            if (r0 + wave + 4 * k < R) *(float4 *)(a.part_o + (slot0 + wave + 4 * k) * HDG + 4 * lane) = orow(k);
+        for (int k = 0; k < WR; k++) {
+            float4 x, y;
+            orow(k, x, y);
+            float4 *dst = (float4 *)(a.part_o + (slot0 + out_row(k) - r0) * HDG + 8 * (lane & 31));
+            if (out_row(k) < R) {
+                dst[0] = x;
+                dst[1] = y;
+            }
+        }
         return;
     }
-    float4 on = orow(0);
+    float4 nx, ny;
+    orow(0, nx, ny);
 #pragma unroll
     for (int k = 0; k < WR; k++) {
-        const float4 o = on;
-        if (k + 1 < WR) on = orow(k + 1);
-        const int r = r0 + wave + 4 * k, t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
-        if (r >= R) break;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (gated)
-            x = a.gate_bf16 ? make_float4(__uint_as_float(gt[k].x << 16), __uint_as_float(gt[k].x & 0xffff0000u), __uint_as_float(gt[k].y << 16),
-                                          __uint_as_float(gt[k].y & 0xffff0000u))
-                            : gate_row(a, tok, h);
-        row_store(a, tok, h, o, x);
+        float x[8] = {nx.x, nx.y, nx.z, nx.w, ny.x, ny.y, ny.z, ny.w};
+        if (k + 1 < WR) orow(k + 1, nx, ny);
+        if (r0 + 8 * k + 2 * wave >= R) break;
+        const int r = out_row(k), t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
+        if (gated) {
+            float z[8];
+            if (a.gate_bf16) {
+                const uint32_t u[4] = {gt[k].x, gt[k].y, gt[k].z, gt[k].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    z[2 * e] = __uint_as_float(u[e] << 16);
+                    z[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+                }
+            } else {
+                const float4 *gp = (const float4 *)((const float *)a.gate + (size_t)min(tok, a.p.n_tok - 1) * a.g_ts + (size_t)min(h, a.n_q - 1) * a.g_hs + 8 * (lane & 31));
+                const float4 u = gp[0], w = gp[1];
+                z[0] = u.x; z[1] = u.y; z[2] = u.z; z[3] = u.w; z[4] = w.x; z[5] = w.y; z[6] = w.z; z[7] = w.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= fast_sigmoid(z[e]);
+        }
+        if (r < R) {
+            const size_t at = ((size_t)tok * a.n_q + h) * HDG + 8 * (lane & 31);
+            if (a.out_bf16) {
+                *(uint4 *)((uint16_t *)a.out + at) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+            } else {
+                float4 *dst = (float4 *)((float *)a.out + at);
+                dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        }
     }
 }
 
 // grid (the most joins there can be, TR / 16), block 256: adds up the parts
-// of a cut item, in order, four rows a wave.
+// of a cut item, in order, four rows a wave, their loads in flight together.
 __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
     if ((int)blockIdx.x >= a.plan->joins) return;
     const int lane = threadIdx.x & 63;
     const RowJoin jn = a.joins[blockIdx.x];
     const vx_pseq s = vx_paged_seq(a.p, jn.b);
-    const int q0 = blockIdx.y * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 4;
+    const int q0 = blockIdx.y * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 4, R = s.T * a.qg;
+    if (jn.r0 + q0 >= R) return;
+    constexpr int NR = 4;
+    float M[NR], L[NR];
+    float4 O[NR], gt[NR];
+    int tok[NR], h[NR];
 #pragma unroll
-    for (int q = q0; q < q0 + 4; q++) {
-        const int r = jn.r0 + q;
-        if (r >= s.T * a.qg) return;
-        const size_t at = (size_t)jn.slot * TR + q;
-        float M = -INFINITY, L = 0.0f;
-        for (int k = 0; k < jn.parts; k++) M = fmaxf(M, a.part_ml[at + (size_t)k * TR].x);
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < jn.parts; k++) {
-            const float2 ml = a.part_ml[at + (size_t)k * TR];
-            const float4 o = *(const float4 *)(a.part_o + (at + (size_t)k * TR) * HDG + 4 * lane);
-            const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-            L += ml.y * w;
-            O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+    for (int q = 0; q < NR; q++) {
+        const int r = min(jn.r0 + q0 + q, R - 1), t = row_tok(a, r);
+        tok[q] = s.start + t;
+        h[q] = row_head(a, jn.kvh, r, t);
+        gt[q] = a.gate ? gate_row(a, tok[q], h[q]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        M[q] = -INFINITY;
+        L[q] = 0.0f;
+        O[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int k = 0; k < jn.parts; k++) {
+        const size_t at = (size_t)(jn.slot + k) * TR + q0;
+        float2 ml[NR];
+        float4 o[NR];
+#pragma unroll
+        for (int q = 0; q < NR; q++) {   // (rows past the last: slots that nobody wrote, unused)
+            ml[q] = a.part_ml[at + q];
+            o[q] = *(const float4 *)(a.part_o + (at + q) * HDG + 4 * lane);
         }
-        const float il = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-        const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, jn.kvh, r, t);
-        const float4 gt = a.gate ? gate_row(a, tok, h) : make_float4(0.f, 0.f, 0.f, 0.f);
-        row_store(a, tok, h, make_float4(O.x * il, O.y * il, O.z * il, O.w * il), gt);
-        if (lane == 0) stat_store(a, tok, h, M, L);
+#pragma unroll
+        for (int q = 0; q < NR; q++) {
+            const float mn = fmaxf(M[q], ml[q].x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float w = __builtin_amdgcn_exp2f(M[q] - ref);
+            L[q] *= w;
+            O[q].x *= w; O[q].y *= w; O[q].z *= w; O[q].w *= w;
+            add_part(O[q], L[q], o[q], ml[q].y, __builtin_amdgcn_exp2f(ml[q].x - ref));
+            M[q] = mn;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < NR; q++) {
+        if (jn.r0 + q0 + q >= R) return;
+        const float il = L[q] > 0.0f || L[q] != L[q] ? 1.0f / L[q] : 0.0f;
+        row_store(a, tok[q], h[q], make_float4(O[q].x * il, O[q].y * il, O[q].z * il, O[q].w * il), gt[q]);
+        if (lane == 0) stat_store(a, tok[q], h[q], M[q], L[q]);
     }
 }
 
