@@ -479,21 +479,22 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 
 // ------------------------------------------------------------------ tiles
 // More than 16 query rows a KV head: 128 rows (tokens x the group's heads,
-// packed) against 64 keys a step, in 4 waves, one per SIMD.  Wave (rh, ch)
-// forms S^T of rows 64 rh .. +63 and the step's key block ch (32 keys), and
-// O^T of the same rows and dims 128 ch .. +127, so K and V are each read from
-// LDS by two waves, not by four, and each operand read feeds two MFMAs
-// (v_mfma_f32_32x32x16_bf16).  The weights of the other key block come from
-// the partner wave (rh, 1 - ch) through LDS.
+// packed) against 64 keys a step, in 4 waves, one per SIMD, of 32 rows each
+// (v_mfma_f32_32x32x16_bf16): S^T[key][row] = K . Q^T, O^T[dim][row] += V^T .
+// P^T.
 //
 // Row m of a K operand holds key 16 (m/16) + 8 (m/4 % 2) + 4 (m/8 % 2) + m%4
-// of its block, so that the C layout of S^T leaves lane (g,n) with keys
-// 16 s + 8 g + 0..7 of row n in registers 8 s .. 8 s + 7: the B operand of
-// O^T += V^T P^T as it stands.  Row maxima, rescales and sums are then one
+// of its 32-key block, so that the C layout of S^T leaves lane (g,n) with
+// keys 16 s + 8 g + 0..7 of row n in registers 8 s .. 8 s + 7: the B operand
+// of O^T += V^T P^T as it stands.  Row maxima, rescales and sums are then one
 // value a lane.
 //
 // A step's two key blocks are consecutive entries of the tile list, so a
 // sink block and the window's first block make a step without a gap.
+//
+// (Measured against it: waves of 64 rows x one key block, and 128 dims of O,
+// which read half as much from LDS but exchange weights and maxima through it
+// and meet twice a step: 2.1 us a step.)
 constexpr int TR = 128;                      // query rows of a workgroup
 constexpr int HALF = TILE * HDG * 2;         // bytes of one key block of K or of V
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
@@ -503,9 +504,8 @@ typedef float floatx16_t __attribute__((ext_vector_type(16)));
 constexpr float LAZY = 48.0f;
 
 struct TileSmem {
-    char k[2][2 * HALF], v[2][2 * HALF];
-    char p[4][64 * 64];                      // a wave's weights as its partner reads them
-    float mx[4][64];                         // row maxima of a wave's key block; row sums at the end
+    char k[2][2 * HALF], v[2][2 * HALF];     // [buffer][key block]
+    int piece;
 };
 
 // vx_dma16 with a constant offset, which counts in memory and in LDS.
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
 __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     __shared__ __attribute__((aligned(16))) TileSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rh = wave >> 1, ch = wave & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // The dispatcher deals workgroups round-robin over the 8 XCDs.  Each takes
     // the next piece of its own eighth of the list, so that the row tiles in
     // flight on an XCD are neighbours, whose keys its L2 then holds once; one
@@ -663,10 +663,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             i = __shfl(i, k, 64);
             if (i < __shfl(hi - lo, k, 64)) piece = __shfl(lo, k, 64) + i;
         }
-        if (tid == 0) *(int *)sm.mx[0] = piece;
+        if (tid == 0) sm.piece = piece;
     }
     __syncthreads();
-    const int piece = __builtin_amdgcn_readfirstlane(*(int *)sm.mx[0]);
+    const int piece = __builtin_amdgcn_readfirstlane(sm.piece);
     if (piece < 0) return;
     __syncthreads();
     const RowPiece *pc = a.pieces + piece;
@@ -688,17 +688,12 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     if (any.i < 0) any.lo = 0;
     any.i = vx_paged_sight(s, t1, a.window, a.n_sink).i;
 
-    const int wr0 = r0 + 64 * rh;                                 // this wave's first row; rows past R repeat row R - 1
-    vx_sight v[2];
-    const uint16_t *qp[2];
-#pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-        const int r = min(wr0 + 32 * rb + n, R - 1), t = row_tok(a, r);
-        v[rb] = vx_paged_sight(s, t, a.window, a.n_sink);
-        qp[rb] = a.q + (size_t)(s.start + t) * a.q_ts + (size_t)row_head(a, kvh, r, t) * a.q_hs + 8 * g;
-    }
-    const vx_sight wfirst = vx_paged_sight(s, row_tok(a, min(wr0, R - 1)), a.window, a.n_sink);
-    const int w_hi = wfirst.i, w_lo = vx_paged_sight(s, row_tok(a, min(wr0 + 63, R - 1)), a.window, a.n_sink).lo;
+    const int wr0 = r0 + 32 * wave;                               // this wave's first row; rows past R repeat row R - 1
+    const int qr = min(wr0 + n, R - 1), qt = row_tok(a, qr);
+    const vx_sight v = vx_paged_sight(s, qt, a.window, a.n_sink);
+    const uint16_t *qp = a.q + (size_t)(s.start + qt) * a.q_ts + (size_t)row_head(a, kvh, qr, qt) * a.q_hs + 8 * g;
+    const int w_hi = vx_paged_sight(s, row_tok(a, min(wr0, R - 1)), a.window, a.n_sink).i;
+    const int w_lo = vx_paged_sight(s, row_tok(a, min(wr0 + 31, R - 1)), a.window, a.n_sink).lo;
 
     // key block h of step c: its first key, or none (past the list)
     auto key_of = [&](int c, int h) -> int {
@@ -743,19 +738,15 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
     auto dma_v = [&](size_t at, int buf, int j) { dma((const char *)(a.v_pages + at), vo, v_lds + buf * 2 * HALF, j); };
 
-    floatx16_t O[2][4];
+    floatx16_t O[8];
 #pragma unroll
-    for (int rb = 0; rb < 2; rb++)
+    for (int db = 0; db < 8; db++)
 #pragma unroll
-        for (int db = 0; db < 4; db++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) O[rb][db][i] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int i = 0; i < 16; i++) O[db][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
     auto pin_o = [&]() {
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-            for (int db = 0; db < 4; db++) __asm__ volatile("" : "+a"(O[rb][db]));
+        for (int db = 0; db < 8; db++) __asm__ volatile("" : "+a"(O[db]));
     };
 
     if (nt > 0) {
@@ -769,81 +760,52 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
         at_v = at_k;
         at_k = at_of(c0 + 2);
-        bf16x8_t q[2][16];
+        bf16x8_t q[16];
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) q[rb][k] = load8(qp[rb] + 16 * k);
-
+        for (int k = 0; k < 16; k++) q[k] = load8(qp + 16 * k);
         auto pin_q = [&]() {
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    if (k < 12) __asm__ volatile("" : "+a"(q[rb][k]));
-                    else __asm__ volatile("" : "+v"(q[rb][k]));
-                }
+            for (int k = 0; k < 16; k++) __asm__ volatile("" : "+a"(q[k]));
         };
+        floatx16_t S[2];           // [key block]
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         pin_q();
         vx_lds_barrier();
-        // Operand addresses in LDS (from an opaque copy of the lane: formed
-        // before the queries are in their registers they would be spilled)
+        // Operand addresses in LDS, one for each of the swizzle's values; the
+        // rest are offsets of the instructions.  (From an opaque copy of the
+        // lane: formed before the queries are in their registers they would
+        // be spilled.)
         int ln = lane;
         __asm__ volatile("" : "+v"(ln));
         const int g = ln >> 5, n = ln & 31;
         const int krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
-        // (one address for each of the swizzle's values; the rest are offsets of
-        // the instructions)
-        const char *ka[8], *va[2][2];
+        const char *ka[8], *va[2];
 #pragma unroll
-        for (int k = 0; k < 8; k++) ka[k] = sm.k[0] + ch * HALF + krow * (HDG * 2) + (((2 * k + g) ^ kswz(krow)) << 4);
+        for (int k = 0; k < 8; k++) ka[k] = sm.k[0] + krow * (HDG * 2) + (((2 * k + g) ^ kswz(krow)) << 4);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-                va[h][k] = sm.v[0] + (h ? 1 - ch : ch) * HALF + (128 * ch + n) * (TILE * 2) + (((2 * k + g) ^ ((n >> 1) & 3)) << 4);
-        auto kload = [&](int k) { return lds8(ka[k & 7] + (k >> 3) * 256); };
-        auto vload = [&](int h, int k, int db) { return lds8(va[h][k] + db * 32 * TILE * 2); };   // h: own block, partner's
+        for (int k = 0; k < 2; k++) va[k] = sm.v[0] + n * (TILE * 2) + (((2 * k + g) ^ ((n >> 1) & 3)) << 4);
+        auto kload = [&](int i) { return lds8(ka[(i >> 1) & 7] + (i & 1) * HALF + (i >> 4) * 256); };                 // k-step i / 2, key block i % 2
+        auto vload = [&](int i) { return lds8(va[(i >> 3) & 1] + (i >> 4) * HALF + (i & 7) * 32 * TILE * 2); };     // 16 keys i / 8, dims 32 (i % 8)
 
-        floatx16_t S[2];
-        auto s_zero = [&]() {
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) S[rb][i] = 0.0f;
-        };
-        // whether some row of the wave does not see all of step c's key block
-        auto cut = [&](int c) {
-            const int key0 = key_of(c, ch);
-            return key0 < 0 || key0 + TILE - 1 > w_hi || (key0 < w_lo && key0 + TILE - 1 >= a.n_sink);
-        };
+        // whether some row of the wave does not see all of a key block
+        auto cut1 = [&](int key0) { return key0 < 0 || key0 + TILE - 1 > w_hi || (key0 < w_lo && key0 + TILE - 1 >= a.n_sink); };
+        auto cut = [&](int c) { return cut1(key_of(c, 0)) || cut1(key_of(c, 1)); };
         floatx16_t sc[2];          // this step's scores
         auto mask = [&](int c) {
-            const int key0 = key_of(c, ch);
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                const uint32_t bits = key0 < 0 ? 0u : v[rb].block(key0) >> (8 * g);
+            for (int kb = 0; kb < 2; kb++) {
+                const int key0 = key_of(c, kb);
+                const uint32_t bits = key0 < 0 ? 0u : v.block(key0) >> (8 * g);
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    if (!(bits & (1u << (16 * (i >> 3) + (i & 7))))) sc[rb][i] = -INFINITY;
+                    if (!(bits & (1u << (16 * (i >> 3) + (i & 7))))) sc[kb][i] = -INFINITY;
             }
         };
-        auto row_max = [&](float (&x)[2]) {
+        auto row_max = [&]() {
+            float x = sc[0][0];
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                x[rb] = sc[rb][0];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) __asm__("v_max3_f32 %0, %0, %1, %2" : "+v"(x[rb]) : "v"(sc[rb][i]), "v"(sc[rb][i + 1]));
-            }
-        };
-        // the rows' maxima for both waves (x: over a lane's keys)
-        auto publish = [&](const float (&x)[2]) {
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                const float y = fmaxf(x[rb], __uint_as_float(vx_xor32_u32(__float_as_uint(x[rb]))));
-                sm.mx[wave][32 * rb + n] = y;   // (both lanes of a row write the same value)
-            }
+            for (int i = 0; i < 32; i += 2) __asm__("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(sc[i >> 4][i & 15]), "v"(sc[i >> 4][(i & 15) + 1]));
+            return x;
         };
         // V of keys that no row of the workgroup sees: zero, so that what stale
         // rows hold cannot get in (only sink blocks, the window's first and
@@ -869,175 +831,118 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             }
             vx_lds_barrier();
         };
+        // The row's reference from its maximum x over a lane's keys; O and l
+        // follow when it moves (not before the first step, where they are 0).
+        float ms;
+        auto refer = [&](float x, bool some) {
+            x = fmaxf(x, __uint_as_float(vx_xor32_u32(__float_as_uint(x)))) * SC2;
+            const bool up = x > m + LAZY;
+            if (some && __any(up)) {
+                const float al = up ? __builtin_amdgcn_exp2f(m - x) : 1.0f;
+                l *= al;
+#pragma unroll
+                for (int db = 0; db < 8; db++) O[db] *= al;
+            }
+            m = up ? x : m;
+            ms = m == -INFINITY ? 0.0f : m;
+        };
 
-        s_zero();
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
-            const bf16x8_t kf = kload(k);
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++) S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[rb][k], S[rb], 0, 0, 0);
-        }
+            for (int i = 0; i < 16; i++) S[kb][i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i++) S[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kload(i), q[i >> 1], S[i & 1], 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < 8; k++) ka[k] += 2 * HALF;   // (the next step's)
         sc[0] = S[0];
         sc[1] = S[1];
         if (cut(c0)) mask(c0);
-        {
-            float x[2];
-            row_max(x);
-            publish(x);
-        }
+        refer(row_max(), false);
 
         // A step: S of the next step on the MFMAs with this step's softmax and
-        // the loads of K(c+2) beside it, the weights' exchange, then P V with
-        // the next maxima and the loads of V(c+1) beside it.  Each wait leaves
-        // the eight newer loads in flight.
-        bool edge = bare(c0), cut1 = nt > 1 && cut(c0 + 1);
+        // the loads of K(c+2) and V(c+1) beside it, then P V with the next
+        // step's maxima beside it.  One MFMA at a time with its share of the
+        // VALU's and the loads' work behind it, in this order: what stands
+        // behind an MFMA that waits for the pipe waits too.
+        constexpr int AHEAD = 6;   // operands read ahead of their MFMA
+        bool edge = bare(c0), cutn = nt > 1 && cut(c0 + 1);
         for (int c = 0; c < nt; c++) {
             const int bk = c & 1;
-            // K(c+1) has landed; every wave is done with step c-1
-            __asm__ volatile("s_waitcnt vmcnt(8)" ::: "memory");
-            vx_lds_barrier();
-            float mine[2], other[2];
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                mine[rb] = sm.mx[wave][32 * rb + n];
-                other[rb] = sm.mx[wave ^ 1][32 * rb + n];
-            }
-            bf16x8_t kf[4];   // K operands, three k-steps ahead
-#pragma unroll
-            for (int k = 0; k < 3; k++) kf[k] = kload(k);
-            s_zero();
-            pin_q();
-            __builtin_amdgcn_sched_barrier(0);
-            bf16x8_t pown[2][2];
-            float ms[2];
-            // One MFMA at a time with its share of the VALU's and the loads' work
-            // behind it, in this order: what stands behind an MFMA that waits
-            // for the pipe waits too.  Element i of a row block goes through
-            // the softmax in three such shares (argument, exp2, sum and
-            // rounding), so that none waits for its own result.
-            auto s_mfma = [&](int k, int rb) {
-                if (rb == 0 && k + 3 < 16) kf[(k + 3) & 3] = kload(k + 3);
-                if (rb == 1 && k < 8) dma_k(at_k, bk, k);
-                S[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k & 3], q[rb][k], S[rb], 0, 0, 0);
-            };
-            float e[2][16];
-            constexpr auto at = [](int j) { return j < 0 ? 0 : j > 13 ? 16 : j * 16 / 13; };
-            auto weigh = [&](int rb, int j) {   // share j of 0..14
-#pragma unroll
-                for (int i = at(j - 2); i < at(j - 1); i++) {
-                    l[rb] += e[rb][i];
-                    __asm__ volatile("" : "+v"(l[rb]));
-                    pown[rb][i >> 3][i & 7] = (__bf16)e[rb][i];
-                }
-#pragma unroll
-                for (int i = at(j - 1); i < at(j); i++) e[rb][i] = __builtin_amdgcn_exp2f(e[rb][i]);
-#pragma unroll
-                for (int i = at(j); i < at(j + 1); i++) e[rb][i] = __builtin_fmaf(sc[rb][i], SC2, -ms[rb]);
-            };
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++) {
-                    s_mfma(k, rb);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            // the rows' reference: both waves of a row see the same two maxima
-            float al[2];
-            bool moved = false;
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                const float x = fmaxf(mine[rb], other[rb]) * SC2;
-                const bool up = x > m[rb] + LAZY;
-                al[rb] = up ? __builtin_amdgcn_exp2f(m[rb] - x) : 1.0f;
-                m[rb] = up ? x : m[rb];
-                ms[rb] = m[rb] == -INFINITY ? 0.0f : m[rb];
-                moved |= up;
-            }
-            // (O stays in the MFMAs' accumulators around the rare rescale: without
-            // the pins it is copied out and back in every step)
-            pin_o();
-            if (c && __any(moved)) {   // (before the first step O is 0)
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++) {
-                    l[rb] *= al[rb];
-#pragma unroll
-                    for (int db = 0; db < 4; db++) {   // (one at a time: all of O does not fit beside the rest)
-                        O[rb][db] *= al[rb];
-                        __asm__ volatile("" : "+a"(O[rb][db]));
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            }
-            pin_o();
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int k = 2; k < 16; k++)
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++) {
-                    s_mfma(k, rb);
-                    weigh(rb, k - 2);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++) weigh(rb, 14);
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) *(bf16x8_t *)(sm.p[wave] + ((rb * 2 + k) * 64 + lane) * 16) = pown[rb][k];
-            // V(c) has landed, and every wave's weights are there
-            __asm__ volatile("s_waitcnt vmcnt(8)" ::: "memory");
+            // K(c+1) and V(c) have landed; every wave is done with step c-1
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
             vx_lds_barrier();
             if (edge) clear_v(c0 + c, bk);
-            // own key block first: the partner's weights arrive meanwhile
-            bf16x8_t poth[2][2], vf[4];   // V operands three ahead
-            auto vstep = [&](int i) { return vload(i >> 3, (i >> 2) & 1, i & 3); };
+            bf16x8_t f[8];
 #pragma unroll
-            for (int i = 0; i < 3; i++) vf[i] = vstep(i);
+            for (int i = 0; i < AHEAD; i++) f[i] = kload(i);
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++)
+            for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) poth[rb][k] = lds8(sm.p[wave ^ 1] + ((rb * 2 + k) * 64 + lane) * 16);
-            float x[2];
-            bool edge2 = false, cut2 = false;
+                for (int i = 0; i < 16; i++) S[kb][i] = 0.0f;
+            pin_q();
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++) {
-                    if (rb == 0 && i + 3 < 16) vf[(i + 3) & 3] = vstep(i + 3);
-                    if (rb == 1 && i < 8) dma_v(at_v, bk ^ 1, i);
-                    if (i >= 8 && rb == 0) ka[i - 8] += bk ? 2 * HALF : -2 * HALF;   // (the next step's buffer)
-                    O[rb][i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 3], i < 8 ? pown[rb][(i >> 2) & 1] : poth[rb][(i >> 2) & 1],
-                                                                           O[rb][i & 3], 0, 0, 0);
-                    sc[rb][i] = S[rb][i];
-                    // (in asm: here, not in a row behind the MFMAs, and without
-                    // the quieting of NaN that fmaxf puts before each)
-                    if (i == 0) x[rb] = sc[rb][0];
-                    else if (i & 1) __asm__ volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x[rb]) : "v"(sc[rb][i - 1]), "v"(sc[rb][i]));
-                    // the next step's addresses
-                    if (rb == 1 && i == 8) at_v = at_k, at_k = at_of(c0 + c + 3);
-                    if (rb == 1 && i == 10) edge2 = bare(c0 + c + 1);
-                    if (rb == 1 && i == 12) cut2 = c + 2 < nt && cut(c0 + c + 2);
-                    __builtin_amdgcn_sched_barrier(0);
+            // Element t of the row goes through the softmax in three shares
+            // (argument, exp2, sum and rounding), so that none waits for its
+            // own result.
+            bf16x8_t p[4];
+            float e[32];
+            auto weigh = [&](int t) {
+                if (t >= 2 && t < 34) {
+                    l += e[t - 2];
+                    __asm__ volatile("" : "+v"(l));
+                    p[(t - 2) >> 3][(t - 2) & 7] = (__bf16)e[t - 2];
                 }
+                if (t >= 1 && t < 33) e[t - 1] = __builtin_amdgcn_exp2f(e[t - 1]);
+                if (t < 32) e[t] = __builtin_fmaf(sc[t >> 4][t & 15], SC2, -ms);
+            };
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                if (i + AHEAD < 32) f[(i + AHEAD) & 7] = kload(i + AHEAD);
+                else f[(i + AHEAD) & 7] = vload(i + AHEAD - 32);
+                if (i < 16) {
+                    if (i & 1) dma_v(at_v, bk ^ 1, i >> 1);
+                    else dma_k(at_k, bk, i >> 1);
+                }
+                S[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i & 7], q[i >> 1], S[i & 1], 0, 0, 0);
+                weigh(i);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (cut1) {
+            weigh(32);
+            weigh(33);
+            pin_o();
+            float x;
+            bool edge2 = false, cut2 = false;
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                if (i + AHEAD < 32) f[(i + AHEAD) & 7] = vload(i + AHEAD);
+                O[i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i & 7], p[i >> 3], O[i & 7], 0, 0, 0);
+                sc[i >> 4][i & 15] = S[i >> 4][i & 15];
+                // (in asm: here, not in a row behind the MFMAs, and without
+                // the quieting of NaN that fmaxf puts before each)
+                if (i == 0) x = sc[0][0];
+                else if (i & 1) __asm__ volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(sc[i >> 4][(i & 15) - 1]), "v"(sc[i >> 4][i & 15]));
+                // the next step's addresses, edges and buffers
+                if (i == 1) at_v = at_k, at_k = at_of(c0 + c + 3);
+                if (i == 3) edge2 = bare(c0 + c + 1);
+                if (i == 5) cut2 = c + 2 < nt && cut(c0 + c + 2);
+                if (i >= 8 && i < 16) ka[i - 8] += bk ? 2 * HALF : -2 * HALF;
+                if (i >= 30) va[i - 30] += bk ? -2 * HALF : 2 * HALF;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            pin_o();
+            if (cutn) {
                 mask(c0 + c + 1);
-                row_max(x);
+                x = row_max();
             }
-            publish(x);
+            if (c + 1 < nt) refer(x, true);
+            pin_o();
             edge = edge2;
-            cut1 = cut2;
+            cutn = cut2;
             if (c0 + c + 5 > base + 63) {   // (one step in 60)
                 base = c0 + c + 4;
                 fill_at();
             }
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) va[h][k] += bk ? -2 * HALF : 2 * HALF;
         }
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last (unused) loads
     }
@@ -1055,35 +960,27 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             gt[k] = *(const uint4 *)((const uint16_t *)a.gate + (size_t)(s.start + t) * a.g_ts + (size_t)row_head(a, kvh, r, t) * a.g_hs + 8 * (lane & 31));
         }
     }
-    // row sums: over the lane pair and the two key blocks
-    vx_lds_barrier();
-#pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-        l[rb] += __shfl_xor(l[rb], 32, 64);
-        if (g == 0) sm.mx[wave][32 * rb + n] = l[rb];
-    }
-    vx_lds_barrier();
+    l += __uint_as_float(vx_xor32_u32(__float_as_uint(l)));
+    vx_lds_barrier();   // every wave is done with the tiles
     // O through LDS (16-byte units swizzled by the row)
     float *so = (float *)sm.k[0];
+    {
+        const int r = 32 * wave + n;
+        const float il = parted ? 1.0f : (l > 0.0f || l != l ? 1.0f / l : 0.0f);
 #pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-        l[rb] += sm.mx[wave ^ 1][32 * rb + n];
-        const int r = 64 * rh + 32 * rb + n;
-        const float il = parted ? 1.0f : (l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f);
-#pragma unroll
-        for (int db = 0; db < 4; db++)
+        for (int db = 0; db < 8; db++)
 #pragma unroll
             for (int q4 = 0; q4 < 4; q4++) {
-                const int u = (128 * ch + 32 * db + 8 * q4 + 4 * g) >> 2;
+                const int u = (32 * db + 8 * q4 + 4 * g) >> 2;
                 *(float4 *)(so + r * HDG + ((u ^ (r & 15)) << 2)) =
-                    make_float4(O[rb][db][4 * q4] * il, O[rb][db][4 * q4 + 1] * il, O[rb][db][4 * q4 + 2] * il, O[rb][db][4 * q4 + 3] * il);
+                    make_float4(O[db][4 * q4] * il, O[db][4 * q4 + 1] * il, O[db][4 * q4 + 2] * il, O[db][4 * q4 + 3] * il);
             }
-        if (ch == 0 && g == 0 && r0 + r < R) {
+        if (g == 0 && r0 + r < R) {
             if (parted) {
-                a.part_ml[slot0 + r] = make_float2(m[rb], l[rb]);
+                a.part_ml[slot0 + r] = make_float2(m, l);
             } else {
                 const int t = row_tok(a, r0 + r);
-                stat_store(a, s.start + t, row_head(a, kvh, r0 + r, t), m[rb], l[rb]);
+                stat_store(a, s.start + t, row_head(a, kvh, r0 + r, t), m, l);
             }
         }
     }
@@ -1144,16 +1041,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     }
 }
 
-// grid (the most joins there can be, TR / 16), block 256: adds up the parts
-// of a cut item, in order, four rows a wave, their loads in flight together.
+// grid any, block 256: adds up the parts of the cut items, in order, four
+// rows a wave, their loads in flight together.
 __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
-    if ((int)blockIdx.x >= a.plan->joins) return;
-    const int lane = threadIdx.x & 63;
-    const RowJoin jn = a.joins[blockIdx.x];
+    constexpr int NR = 4, PER = TR / (4 * NR);
+    const int lane = threadIdx.x & 63, todo = a.plan->joins * PER;
+    for (int it = blockIdx.x; it < todo; it += gridDim.x) {
+    const RowJoin jn = a.joins[it / PER];
     const vx_pseq s = vx_paged_seq(a.p, jn.b);
-    const int q0 = blockIdx.y * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 4, R = s.T * a.qg;
-    if (jn.r0 + q0 >= R) return;
-    constexpr int NR = 4;
+    const int q0 = it % PER * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * NR, R = s.T * a.qg;
+    if (jn.r0 + q0 >= R) continue;
     float M[NR], L[NR];
     float4 O[NR], gt[NR];
     int tok[NR], h[NR];
@@ -1188,10 +1085,11 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
     }
 #pragma unroll
     for (int q = 0; q < NR; q++) {
-        if (jn.r0 + q0 + q >= R) return;
+        if (jn.r0 + q0 + q >= R) break;
         const float il = L[q] > 0.0f || L[q] != L[q] ? 1.0f / L[q] : 0.0f;
         row_store(a, tok[q], h[q], make_float4(O[q].x * il, O[q].y * il, O[q].z * il, O[q].w * il), gt[q]);
         if (lane == 0) stat_store(a, tok[q], h[q], M[q], L[q]);
+    }
     }
 }
 
@@ -1387,7 +1285,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     a.pieces = (RowPiece *)(at += (size_t)2 * cuts * TR * HDG * 4);
     VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
     VX_LAUNCH(ctx, paged_rows, dim3((unsigned)(items + cuts)), dim3(256), a);
-    VX_LAUNCH(ctx, paged_rows_join, dim3((unsigned)cuts, TR / 16), dim3(256), a);
+    VX_LAUNCH(ctx, paged_rows_join, dim3(2 * n_cu), dim3(256), a);
     if (d->acc) VX_LAUNCH(ctx, paged_rows_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
     return 0;
 }
