@@ -199,6 +199,60 @@ def test_every_tile_counts(ctx, T, window, sink):
     at.free()
 
 
+@pytest.mark.parametrize("lens,new,window,sink", [
+    ([40, 9], [2, 2], 0, 0),                      # decode kernels, two tokens
+    ([300, 70], [2, 1], 33, 4),
+    ([90, 33], [60, 33], 0, 0),                   # tile kernel
+    ([400, 90], [130, 90], 50, 4),
+    ([3000, 10], [40, 3], 0, 0),                  # cut into parts
+])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_infinite_values_stay_with_the_rows_that_see_them(ctx, lens, new, window, sink, value):
+    """An infinite or NaN value (or a whole NaN row) reaches the tokens that see its row and no other."""
+    from vx27_amd import workloads as W
+    say(f"value {value} {lens} {new} window {window}")
+    bt = Batch(lens, new, 24, 4, 64, window, sink, seed=400 + len(lens) + new[0])
+    bits = int(W.bf16_bits(np.array([value], np.float32))[0])
+    some = {}
+    for b in range(bt.B):
+        seen = bt.seen(b)
+        part = np.nonzero(seen.any(0) & ~seen.all(0))[0]
+        picks = [part[0], part[len(part) // 2], part[-1]] if len(part) else []
+        if seen.all(0).any():
+            picks.append(np.nonzero(seen.all(0))[0][-1])
+        for q, j in enumerate(dict.fromkeys(picks)):
+            p, at = bt.table[b, j // bt.page], j % bt.page
+            if q == 1 and np.isnan(value):
+                bt.v[p, :, at // 32, :, at % 32] = bits
+                some[b, j] = slice(None)
+            else:
+                bt.v[p, q % 4, at // 32, 17 * q + 3, at % 32] = bits
+                some[b, j] = (q % 4, 17 * q + 3)
+    at = Attn(ctx, bt, out_bf16=False, gate="none", lse=False)
+    at.call()
+    ctx.sync()
+    out = at.out()
+    # where a token sees such a value its output is not finite, and everywhere else it is as without them
+    hit = np.zeros(out.shape, bool)
+    clean = bt.v.copy()
+    for (b, j), where in some.items():
+        p, a_ = bt.table[b, j // bt.page], j % bt.page
+        tokens = bt.start[b] + np.nonzero(bt.seen(b)[:, j])[0]
+        if isinstance(where, slice):
+            hit[tokens] = True
+            clean[p, :, a_ // 32, :, a_ % 32] = 0
+        else:
+            h, d = where
+            hit[np.ix_(tokens, range(6 * h, 6 * h + 6), [d])] = True
+            clean[p, h, a_ // 32, d, a_ % 32] = 0
+    bt.v = clean
+    ref = bt.result(False)
+    tol = out_tol(ref, max(lens), False, max(new) * 6 > 16)
+    assert not np.isfinite(out[hit]).any()      # (the three parts of a weight may differ in sign: an infinity can end as NaN)
+    assert np.all(np.abs(out[~hit] - ref["out"][~hit]) <= tol[~hit])
+    at.free()
+
+
 def test_matches_the_contiguous_decode(ctx):
     """Pages of a contiguous cache's size, one a sequence: vx27_hip_gqa_decode's own output within its bar, |d| <= 2e-2 +
     1e-2 |ref|, through append and attention."""

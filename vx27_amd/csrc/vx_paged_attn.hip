@@ -115,11 +115,14 @@ __device__ __forceinline__ void score_tile(const bf16x8_t (&ka)[8], const bf16x8
     }
 }
 
-// Online softmax and P V of one tile.  NP bf16 parts of each weight: three
-// hold all 24 bits of it.  V of keys no row of the wave sees is zeroed, so
-// that what stale rows hold cannot get in.
+__device__ __forceinline__ bool is_finite(float x) { return __builtin_fabsf(x) < INFINITY; }
+
+// Online softmax and P V of one tile for R rows.  NP bf16 parts of each
+// weight: three hold all 24 bits of it.  V of keys that no row sees is zeroed,
+// so that what stale rows hold cannot get in.  `one`: the rows are of one token,
+// so that all see the same keys.
 template <int NP>
-__device__ __forceinline__ void attend_tile(Rows &w, const float (&s)[8], const vx_sight &v, int key0, bf16x8_t (&va)[16]) {
+__device__ __forceinline__ void attend_tile(Rows &w, int R, bool one, const float (&s)[8], const vx_sight &v, int key0, bf16x8_t (&va)[16]) {
     const int g = (threadIdx.x & 63) >> 4;
     float x[8];
     float mt = -INFINITY;
@@ -155,14 +158,42 @@ __device__ __forceinline__ void attend_tile(Rows &w, const float (&s)[8], const 
         for (int d = 0; d < 16; d++) w.o[d] *= alpha;
     }
     if (!__all(all)) {
+        const int lane = threadIdx.x & 63;
+        const uint32_t group = (1u << R) - 1;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            // any of the 16 rows of this lane group sees key 8g + e
-            const uint64_t seen = __ballot(v.sees(key0 + 8 * g + e));
-            if (((seen >> (16 * g)) & 0xffff) == 0) {
+            // which of a lane group's rows see its key 8g + e
+            const bool see = v.sees(key0 + 8 * g + e);
+            const uint64_t seen = __ballot(see);
+            const uint32_t mine = (uint32_t)(seen >> (16 * g)) & group;
+            if (mine == 0) {
 #pragma unroll
                 for (int d = 0; d < 16; d++) va[d][e] = (__bf16)0.0f;
             }
+            if (one || !__any(mine != 0 && mine != group)) continue;
+            // A key that some rows see and others do not, with an infinite or
+            // NaN value: 0 times that would reach the others.  Its values go
+            // to the rows that see it by addition (any weight times an
+            // infinity is one) and out of the product.
+            bool odd = false;
+#pragma unroll
+            for (int d = 0; d < 16; d++) odd |= !is_finite(va[d][e]);
+            uint64_t bad = __ballot(odd && mine);
+            while (bad) {
+                const int gk = __builtin_ctzll(bad) >> 4;
+                bad &= ~(0xffffull << (16 * gk));
+                const bool own = v.sees(key0 + 8 * gk + e);
+#pragma unroll
+                for (int d = 0; d < 16; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {   // dim 16d + 4g + i is lane 4g + i's of the key's group
+                        const float x = __shfl((float)va[d][e], 16 * gk + 4 * (lane >> 4) + i, 64);
+                        if (own && !is_finite(x)) w.o[d][i] += x;
+                    }
+            }
+#pragma unroll
+            for (int d = 0; d < 16; d++)
+                if (odd && !is_finite(va[d][e])) va[d][e] = (__bf16)0.0f;
         }
     }
 #pragma unroll
@@ -348,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
                 *(float4 *)st = make_float4(sc[0], sc[1], sc[2], sc[3]);
                 *(float4 *)(st + 4) = make_float4(sc[4], sc[5], sc[6], sc[7]);
             }
-            attend_tile<3>(w, sc, v, key0, va);
+            attend_tile<3>(w, R, s.T == 1, sc, v, key0, va);
         }
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
@@ -506,6 +537,7 @@ constexpr float LAZY = 48.0f;
 struct TileSmem {
     char k[2][2 * HALF], v[2][2 * HALF];     // [buffer][key block]
     int piece;
+    int odd;                                 // some value was infinite or NaN where not every row sees it
 };
 
 // vx_dma16 with a constant offset, which counts in memory and in LDS.
@@ -663,7 +695,10 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             i = __shfl(i, k, 64);
             if (i < __shfl(hi - lo, k, 64)) piece = __shfl(lo, k, 64) + i;
         }
-        if (tid == 0) sm.piece = piece;
+        if (tid == 0) {
+            sm.piece = piece;
+            sm.odd = 0;
+        }
     }
     __syncthreads();
     const int piece = __builtin_amdgcn_readfirstlane(sm.piece);
@@ -686,14 +721,15 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     // what the workgroup's rows see between them
     vx_sight any = vx_paged_sight(s, t0, a.window, a.n_sink);
     if (any.i < 0) any.lo = 0;
+    const int i_first = any.i, lo_last = vx_paged_sight(s, t1, a.window, a.n_sink).lo;
     any.i = vx_paged_sight(s, t1, a.window, a.n_sink).i;
 
     const int wr0 = r0 + 32 * wave;                               // this wave's first row; rows past R repeat row R - 1
     const int qr = min(wr0 + n, R - 1), qt = row_tok(a, qr);
     const vx_sight v = vx_paged_sight(s, qt, a.window, a.n_sink);
     const uint16_t *qp = a.q + (size_t)(s.start + qt) * a.q_ts + (size_t)row_head(a, kvh, qr, qt) * a.q_hs + 8 * g;
-    const int w_hi = vx_paged_sight(s, row_tok(a, min(wr0, R - 1)), a.window, a.n_sink).i;
-    const int w_lo = vx_paged_sight(s, row_tok(a, min(wr0 + 31, R - 1)), a.window, a.n_sink).lo;
+    const int wi = vx_paged_sight(s, row_tok(a, min(wr0, R - 1)), a.window, a.n_sink).i;                // the least of its rows' own rows
+    const int wl = vx_paged_sight(s, row_tok(a, min(wr0 + 31, R - 1)), a.window, a.n_sink).lo;          // the highest of their windows' edges
 
     // key block h of step c: its first key, or none (past the list)
     auto key_of = [&](int c, int h) -> int {
@@ -724,6 +760,14 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         at_lo = (uint32_t)at;
         at_hi = (uint32_t)(at >> 32);
     };
+    // The blocks of the list that some row does not see all of come first
+    // (sinks, and what the window's lower edge crosses: before block lo of
+    // the list) and last (past a token's own row: from block hi on).
+    auto low = [&](int row_lo) { return tl.st + max((row_lo + TILE - 1) / TILE - tl.fm, 0); };
+    auto high = [&](int row_i) { return tl.st + (row_i + 1) / TILE - tl.fm; };
+    const int e_lo = low(lo_last), e_hi = high(i_first), w_lo = low(wl), w_hi = high(wi);
+    auto bare = [&](int c) { return 2 * c < e_lo || 2 * c + 1 >= e_hi; };    // some row of the workgroup
+    auto cut = [&](int c) { return 2 * c < w_lo || 2 * c + 1 >= w_hi; };     // some row of the wave
     auto at_of = [&](int c) -> size_t {
         return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, c - base) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, c - base);
     };
@@ -787,9 +831,6 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         auto kload = [&](int i) { return lds8(ka[(i >> 1) & 7] + (i & 1) * HALF + (i >> 4) * 256); };                 // k-step i / 2, key block i % 2
         auto vload = [&](int i) { return lds8(va[(i >> 3) & 1] + (i >> 4) * HALF + (i & 7) * 32 * TILE * 2); };     // 16 keys i / 8, dims 32 (i % 8)
 
-        // whether some row of the wave does not see all of a key block
-        auto cut1 = [&](int key0) { return key0 < 0 || key0 + TILE - 1 > w_hi || (key0 < w_lo && key0 + TILE - 1 >= a.n_sink); };
-        auto cut = [&](int c) { return cut1(key_of(c, 0)) || cut1(key_of(c, 1)); };
         floatx16_t sc[2];          // this step's scores
         auto mask = [&](int c) {
 #pragma unroll
@@ -807,17 +848,19 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             for (int i = 0; i < 32; i += 2) __asm__("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(sc[i >> 4][i & 15]), "v"(sc[i >> 4][(i & 15) + 1]));
             return x;
         };
-        // V of keys that no row of the workgroup sees: zero, so that what stale
-        // rows hold cannot get in (only sink blocks, the window's first and
-        // the last block have such keys)
-        auto bare = [&](int c) { return 2 * c <= tl.st || 2 * c + 2 >= tl.nt; };
+        // In steps with a key that some row of the workgroup does not see: V of
+        // keys that none sees becomes zero, so that what stale rows hold cannot
+        // get in; and so do infinite and NaN values (0 times these would reach
+        // the rows that do not see them), which the output adds for the rows
+        // that do.  Thread tid has dim tid.
         auto clear_v = [&](int c, int buf) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
+                if (2 * c + h >= e_lo && 2 * c + h < e_hi) continue;
                 const int key0 = key_of(c, h);
                 const uint32_t seen = key0 < 0 ? 0u : any.block(key0);
+                uint4 *row = (uint4 *)(sm.v[buf] + h * HALF + tid * (TILE * 2));
                 if (seen != 0xffffffffu) {
-                    uint4 *row = (uint4 *)(sm.v[buf] + h * HALF + tid * (TILE * 2));
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         const uint32_t byte = seen >> (8 * (u ^ ((tid >> 1) & 3)));
@@ -827,6 +870,20 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                         for (int e = 0; e < 4; e++) w[e] &= ((byte >> (2 * e)) & 1 ? 0xffffu : 0u) | ((byte >> (2 * e)) & 2 ? 0xffff0000u : 0u);
                         row[u] = x;
                     }
+                }
+                uint32_t hot = 0;   // bits 15 and 31: an exponent of all ones carries into them
+#pragma unroll
+                for (int i = 0; i < 4; i++) {   // (from a unit of each lane's own: 8 lanes then read 8 distinct slots)
+                    const uint4 x = row[(i + (tid >> 1)) & 3];
+                    const uint32_t *w = (const uint32_t *)&x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) hot |= (w[e] & 0x7f807f80u) + 0x00800080u;
+                }
+                if (hot & 0x80008000u) {
+                    uint32_t *w = (uint32_t *)row;
+                    for (int e = 0; e < TILE / 2; e++)
+                        w[e] &= ((w[e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((w[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+                    sm.odd = 1;
                 }
             }
             vx_lds_barrier();
@@ -985,6 +1042,24 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         }
     }
     vx_lds_barrier();
+    if (sm.odd) {   // (the same for every thread)
+        for (int c = c0; c < c0 + nt; c++) {
+            if (!bare(c)) continue;
+            for (int h = 0; h < 2; h++) {
+                const int key0 = key_of(c, h);
+                if (key0 < 0) continue;
+                const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
+                const uint16_t *vp = a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
+                for (int j = 0; j < TILE; j++) {
+                    const float x = vx_bf16_to_f32(vp[j]);
+                    if (is_finite(x)) continue;
+                    for (int r = 0; r < TR && r0 + r < R; r++)
+                        if (sight_of(a, s, r0 + r).sees(key0 + j)) so[r * HDG + ((((tid >> 2) ^ (r & 15)) << 2) | (tid & 3))] += x;
+                }
+            }
+        }
+        vx_lds_barrier();
+    }
     auto orow = [&](int k, float4 &x, float4 &y) {
         const int r = out_row(k) - r0, u = 2 * (lane & 31);
         x = *(const float4 *)(so + r * HDG + ((u ^ (r & 15)) << 2));
