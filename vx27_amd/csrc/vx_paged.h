@@ -65,6 +65,19 @@ __host__ __device__ __forceinline__ int vx_paged_page(const vx_paged &p, int b, 
     return vx_page_checked(p, vx_table_word(p.table + (size_t)b * p.max_pages + vx_page_slot(p, r)));
 }
 
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int vx_dpp_i(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xF, true); }
+// Sum over lanes 0 .. l (the VALU's DPP paths: no LDS round trips).
+__device__ __forceinline__ int vx_wave_scan(int v) {
+    v += vx_dpp_i<0x111, 0xF>(v);   // row_shr:1
+    v += vx_dpp_i<0x112, 0xF>(v);
+    v += vx_dpp_i<0x114, 0xF>(v);
+    v += vx_dpp_i<0x118, 0xF>(v);
+    v += vx_dpp_i<0x142, 0xA>(v);   // row_bcast:15 into rows 1 and 3
+    v += vx_dpp_i<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // The bits of rows key0 .. key0 + 31 that lie below row n.
 __host__ __device__ __forceinline__ uint32_t vx_below(int n, int key0) {
     if (n <= key0) return 0u;

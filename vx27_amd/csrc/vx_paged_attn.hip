@@ -260,18 +260,6 @@ __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l,
 // workgroup is finished there; the first and the last piece of a
 // workgroup's range may be parts of a pair and go to its two partial slots,
 // which paged_join merges in order.
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int dpp_i(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xF, true); }
-// Sum over lanes 0 .. l (the VALU's DPP paths: no LDS round trips).
-__device__ __forceinline__ int wave_scan_i(int v) {
-    v += dpp_i<0x111, 0xF>(v);   // row_shr:1
-    v += dpp_i<0x112, 0xF>(v);
-    v += dpp_i<0x114, 0xF>(v);
-    v += dpp_i<0x118, 0xF>(v);
-    v += dpp_i<0x142, 0xA>(v);   // row_bcast:15 into rows 1 and 3
-    v += dpp_i<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
-    return v;
-}
 // The list of a call's tiles: up to 64 sequences are held one a lane and read
 // once; more are read again where they are needed.
 struct Units {
@@ -290,7 +278,7 @@ __device__ __forceinline__ Units units_of(const Args &a, int grid) {
     Units u;
     if (a.p.B <= 64) {
         const int n = seq_units(a, min(lane, a.p.B - 1), u.s, u.t);
-        u.upto = wave_scan_i(lane < a.p.B ? n : 0);
+        u.upto = vx_wave_scan(lane < a.p.B ? n : 0);
         u.total = __builtin_amdgcn_readlane(u.upto, 63);
     } else {
         int sum = 0;
@@ -298,7 +286,7 @@ __device__ __forceinline__ Units units_of(const Args &a, int grid) {
             const int n = seq_units(a, min(b0 + lane, a.p.B - 1), u.s, u.t);
             sum += b0 + lane < a.p.B ? n : 0;
         }
-        u.total = __builtin_amdgcn_readlane(wave_scan_i(sum), 63);
+        u.total = __builtin_amdgcn_readlane(vx_wave_scan(sum), 63);
     }
     u.chunk = max((u.total + grid - 1) / grid, a.min_tiles);
     return u;
@@ -313,7 +301,7 @@ __device__ __forceinline__ int units_before(const Args &a, const Units &u, int b
     }
     int sum = 0;
     for (int c = threadIdx.x & 63; c < b; c += 64) sum += seq_units(a, c, s, t);
-    sum = __builtin_amdgcn_readlane(wave_scan_i(sum), 63);
+    sum = __builtin_amdgcn_readlane(vx_wave_scan(sum), 63);
     seq_units(a, b, s, t);
     return sum;
 }
@@ -325,7 +313,7 @@ __device__ __forceinline__ int units_find(const Args &a, const Units &u, int x) 
     for (int b0 = 0;; b0 += 64) {
         vx_pseq s;
         vx_tiles t;
-        const int n = seq_units(a, min(b0 + lane, a.p.B - 1), s, t), upto = wave_scan_i(b0 + lane < a.p.B ? n : 0);
+        const int n = seq_units(a, min(b0 + lane, a.p.B - 1), s, t), upto = vx_wave_scan(b0 + lane < a.p.B ? n : 0);
         const uint64_t past = __ballot(done + upto > x);
         if (past || b0 + 64 >= a.p.B) return b0 + (past ? __builtin_ctzll(past) : 0);
         done += __builtin_amdgcn_readlane(upto, 63);
@@ -602,7 +590,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     }
     // (a thread's only entry is not looked up again)
     auto steps_of = [&](int e) { return per == 1 ? n0 : entry_steps(a, n_rt, e, b, r0); };
-    items = wave_scan_i(items);
+    items = vx_wave_scan(items);
     for (int off = 32; off >= 1; off >>= 1) steps += __shfl_xor(steps, off, 64);
     if (lane == 63) {
         s_steps[wave] = steps;
@@ -631,7 +619,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     int at[3], tot[3];
 #pragma unroll
     for (int c = 0; c < 3; c++) {
-        const int x = wave_scan_i(cnt[c]);
+        const int x = vx_wave_scan(cnt[c]);
         if (lane == 63) s_sum[c][wave] = x;
         at[c] = x - cnt[c];
     }

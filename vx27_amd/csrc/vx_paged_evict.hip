@@ -6,9 +6,10 @@
 //
 //   paged_select  one workgroup per (sequence, KV head): the weight of the
 //                 last row kept is found digit by digit (a radix select over
-//                 the weights' bits: 12, 10 and 10), then the kept rows are
+//                 the weights' bits: 11, 11 and 10), then the kept rows are
 //                 written in order by prefix sums.
 //   paged_move    copies the kept rows' K, V and weights.
+#include "vx_lds.h"
 #include "vx_paged.h"
 
 namespace {
@@ -34,17 +35,26 @@ __device__ __forceinline__ int seq_len(const EvictArgs &a, int b) {
     if (c != n) *a.p.err_flag = 1;
     return c;
 }
-// Order of a weight as an unsigned number; NaN above everything, -0 as 0.
+// Order of a weight as an unsigned number; NaN above every other, -0 as 0.
+// Between OUT (no row) and KEPT (a row that stays whatever its weight).
+constexpr uint32_t OUT = 0, KEPT = 0xffffffffu;
 __device__ __forceinline__ uint32_t rank_of(float w) {
-    if (w != w) return 0xffffffffu;
+    if (w != w) return KEPT - 1;
     const uint32_t u = __float_as_uint(w + 0.0f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// how many of a ballot's lanes lie below this one
+__device__ __forceinline__ int lanes_below(uint64_t x) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, 0)); }
+
 // Wave w owns rows [w seg, (w+1) seg) and reads them 64 at a time, CH of
 // these per chunk; a sequence of up to 16 * 64 * CH rows is one chunk a wave,
-// read once and held in registers through all passes.
-constexpr int SEL = 1024, NW = SEL / 64, CH = 32, BINS = 4096;
+// read once and held in registers through all passes.  Sinks and recent rows
+// have the highest rank, so that the budget counts them like all others.
+// Attention weights are alike in their exponents: 64 lanes at one bin of a
+// histogram would be added one by one, so there are eight of it side by side,
+// each for every eighth lane.  Two buffers: a pass clears the next one's.
+constexpr int SEL = 1024, NW = SEL / 64, CH = 32, BINS = 2048, COPY = 8;
 __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -57,91 +67,82 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     }
     const float *w = a.acc + ((size_t)b * a.p.n_kv + h) * a.acc_stride;
     const int lo = a.n_sink, hi = n - a.n_recent;     // the rows that compete
-    int want = a.budget - a.n_sink - a.n_recent;      // how many of them stay
-    __shared__ int hist[BINS];
+    int want = a.budget;                              // rows of the ranks not yet decided that stay
+    __shared__ __attribute__((aligned(16))) int hist[2][BINS * COPY];
     __shared__ int s_sum[NW], s_eq[NW], s_found[2];
     const int seg = ((n + NW - 1) / NW + 63) / 64 * 64, w0 = wave * seg, w1 = min(w0 + seg, n);
     uint32_t r[CH];
     auto load = [&](int base) {
 #pragma unroll
         for (int k = 0; k < CH; k++)
-            if (base + 64 * k < w1) r[k] = rank_of(w[min(base + 64 * k + lane, n - 1)]);
+            if (base + 64 * k < w1) {   // (uniform)
+                const int i = base + 64 * k + lane;
+                r[k] = rank_of(w[min(i, n - 1)]);
+                if (i < lo || i >= hi) r[k] = KEPT;
+                if (i >= w1) r[k] = OUT;
+            }
     };
     const bool once = seg <= CH * 64;
     load(w0);
+    auto clear = [&](int buf, int bins) {
+        for (int i = tid; i < bins * COPY / 4; i += SEL) ((int4 *)hist[buf])[i] = make_int4(0, 0, 0, 0);
+    };
+    clear(0, BINS);
+    __syncthreads();
     uint32_t prefix = 0, mask = 0;
-    int shift = 32;
-    const int none = want == 0;
-    for (int pass = 0; pass < 3 && !none; pass++) {
-        const int bits = pass ? 10 : 12;
-        shift -= bits;
-        for (int i = tid; i < BINS; i += SEL) hist[i] = 0;
-        __syncthreads();
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = 1 << bits;
+        int *hp = hist[pass & 1];
+        if (pass < 2) clear(~pass & 1, BINS);
         for (int base = w0; base < w1; base += CH * 64) {
             if (!once) load(base);
 #pragma unroll
             for (int k = 0; k < CH; k++) {
-                if (base + 64 * k >= w1) continue;   // (uniform)
-                const int i = base + 64 * k + lane;
-                const bool in = i < w1 && i >= lo && i < hi && (r[k] & mask) == prefix;
-                // rows that no token weighed are many: counted by the wave, not one by one in the same bin
-                const uint64_t zero = __ballot(in && r[k] == 0x80000000u);
-                if (in && r[k] != 0x80000000u) atomicAdd(&hist[(r[k] >> shift) & ((1 << bits) - 1)], 1);
-                if (zero && lane == 0) atomicAdd(&hist[(0x80000000u >> shift) & ((1 << bits) - 1)], __popcll(zero));
+                if (base + 64 * k >= w1) continue;
+                if (((r[k] ^ prefix) & mask) == 0) atomicAdd(&hp[((r[k] >> shift) & (bins - 1)) * COPY + (lane & (COPY - 1))], 1);
             }
         }
         __syncthreads();
-        // the bin of the want-th heaviest: thread t takes bins 4 t .. 4 t + 3 (from the top), suffix sums over the threads
-        int c[4], mine = 0;
+        // the bin of the want-th heaviest: thread t takes bins 2 t and 2 t + 1
+        // (from the top), suffix sums over the threads
+        int c[2], mine = 0;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int bin = BINS - 1 - (4 * tid + q);
-            c[q] = bin < (1 << bits) ? hist[bin] : 0;
+        for (int q = 0; q < 2; q++) {
+            const int bin = BINS - 1 - (2 * tid + q);
+            c[q] = 0;
+            if (bin < bins) {
+                const int4 x = *(const int4 *)&hp[bin * COPY], y = *(const int4 *)&hp[bin * COPY + 4];
+                c[q] = (x.x + x.y + x.z + x.w) + (y.x + y.y + y.z + y.w);
+            }
             mine += c[q];
         }
-        int x = mine;
-        for (int off = 1; off < 64; off <<= 1) {
-            const int y = __shfl_up(x, off, 64);
-            if (lane >= off) x += y;
-        }
+        int x = vx_wave_scan(mine);
         if (lane == 63) s_sum[wave] = x;
         __syncthreads();
-        x -= mine;
-        for (int k = 0; k < wave; k++) x += s_sum[k];
-        if (x < want && x + mine >= want) {   // one thread (at least `want` rows match the prefix)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (x < want && x + c[q] >= want) {
-                    s_found[0] = BINS - 1 - (4 * tid + q);
-                    s_found[1] = want - x;
-                }
-                x += c[q];
-            }
+        const int waves = vx_wave_scan(lane < NW ? s_sum[lane & (NW - 1)] : 0);
+        x += (wave ? __builtin_amdgcn_readlane(waves, wave - 1) : 0) - mine;
+        if (x < want && x + mine >= want) {   // one thread (more than `want` rows match the prefix)
+            const int q = x + c[0] >= want ? 0 : 1;
+            s_found[0] = BINS - 1 - (2 * tid + q);
+            s_found[1] = want - x - (q ? c[0] : 0);
         }
         __syncthreads();
         prefix |= (uint32_t)s_found[0] << shift;
-        mask |= (uint32_t)((1 << bits) - 1) << shift;
+        mask |= (uint32_t)(bins - 1) << shift;
         want = s_found[1];
-        __syncthreads();
     }
     // Rows above `prefix` stay, and the first `want` equal to it: each wave
     // counts its own of both kinds, then writes them behind those of the
     // waves before it.
-    auto kinds = [&](int i, uint32_t u, bool &eq) {
-        const bool in = i < w1, mid = i >= lo && i < hi;
-        eq = in && mid && !none && u == prefix;
-        return in && (!mid || (!none && u > prefix));
-    };
     int nsure = 0, neq = 0;
     for (int base = w0; base < w1; base += CH * 64) {
         if (!once) load(base);
 #pragma unroll
         for (int k = 0; k < CH; k++) {
             if (base + 64 * k >= w1) continue;
-            bool eq;
-            const bool sure = kinds(base + 64 * k + lane, r[k], eq);
-            nsure += __popcll(__ballot(sure));
-            neq += __popcll(__ballot(eq));
+            nsure += __popcll(__ballot(r[k] > prefix));
+            neq += __popcll(__ballot(r[k] == prefix));
         }
     }
     if (lane == 0) {
@@ -149,25 +150,18 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
         s_eq[wave] = neq;
     }
     __syncthreads();
-    int at = 0, eqs = 0;
-    for (int k = 0; k < wave; k++) {
-        at += s_sum[k];
-        eqs += s_eq[k];
-    }
+    const int sures = vx_wave_scan(lane < NW ? s_sum[lane & (NW - 1)] : 0), equals = vx_wave_scan(lane < NW ? s_eq[lane & (NW - 1)] : 0);
+    int at = wave ? __builtin_amdgcn_readlane(sures, wave - 1) : 0, eqs = wave ? __builtin_amdgcn_readlane(equals, wave - 1) : 0;
     at += min(eqs, want);
-    const uint64_t below = lane ? (~0ull >> (64 - lane)) : 0;
     for (int base = w0; base < w1; base += CH * 64) {
         if (!once) load(base);
 #pragma unroll
         for (int k = 0; k < CH; k++) {
             if (base + 64 * k >= w1) continue;
-            bool eq;
-            const int i = base + 64 * k + lane;
-            const bool sure = kinds(i, r[k], eq);
-            const uint64_t be = __ballot(eq);
-            const bool stay = sure || (eq && eqs + __popcll(be & below) < want);
+            const uint64_t be = __ballot(r[k] == prefix);
+            const bool stay = r[k] > prefix || (r[k] == prefix && eqs + lanes_below(be) < want);
             const uint64_t bs = __ballot(stay);
-            if (stay) kept[at + __popcll(bs & below)] = i;
+            if (stay) kept[at + lanes_below(bs)] = base + 64 * k + lane;
             at += __popcll(bs);
             eqs += __popcll(be);
         }
@@ -207,27 +201,36 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
         const int q = min(wave + 4 * j, cnt - 1);
         kr[j] = *(const uint2 *)(a.k_pages + s_blk[q] + (size_t)(s_row[q] % VB) * HDG + 4 * lane);
     }
+    // the first row of each source block's (the rows are in order)
+    const int sl = lane & (VB - 1);
+    uint32_t starts = (uint32_t)__ballot(sl < cnt && (sl == 0 || s_blk[sl] != s_blk[sl - 1]));
     uint16_t v[VB];
-    for (int j = 0; j < cnt;) {
-        const size_t blk = s_blk[j];
-        uint4 u[4];
+    uint4 u[2][4];
+    auto fetch = [&](int j, uint4 (&x)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = *(const uint4 *)(a.v_pages + blk + (size_t)(tid + 256 * i) * 8);
-        if (j) __syncthreads();
+        for (int i = 0; i < 4; i++) x[i] = *(const uint4 *)(a.v_pages + s_blk[j] + (size_t)(tid + 256 * i) * 8);
+    };
+    // a source block through LDS, with the next one's loads in flight
+    auto take = [&](int buf) {
+        const int j = __builtin_ctz(starts);
+        starts &= starts - 1;
+        const int e = starts ? __builtin_ctz(starts) : cnt;
+        if (starts) fetch(e, u[buf ^ 1]);
+        if (j) vx_lds_barrier();
 #pragma unroll
         for (int i = 0; i < 4; i++) {   // unit tid + 256 i: dim unit / 4, rows 8 (unit % 4) ..
             uint32_t *d = (uint32_t *)&sv[((tid >> 2) + 64 * i) * VROW + (tid & 3) * 8];
-            d[0] = u[i].x; d[1] = u[i].y; d[2] = u[i].z; d[3] = u[i].w;
+            d[0] = u[buf][i].x; d[1] = u[buf][i].y; d[2] = u[buf][i].z; d[3] = u[buf][i].w;
         }
-        __syncthreads();
-        int e = j;
+        vx_lds_barrier();
 #pragma unroll
         for (int q = 0; q < VB; q++)
-            if (q >= j && q < cnt && s_blk[q] == blk) {   // (uniform; the rows are in order, so these are j, j + 1, ...)
-                v[q] = sv[tid * VROW + s_row[q] % VB];
-                e = q + 1;
-            }
-        j = __builtin_amdgcn_readfirstlane(e);
+            if (q >= j && q < e) v[q] = sv[tid * VROW + s_row[q] % VB];   // (uniform)
+    };
+    fetch(0, u[0]);
+    while (starts) {
+        take(0);
+        if (starts) take(1);
     }
 #pragma unroll
     for (int j = 0; j < VB / 4; j++)
