@@ -640,11 +640,13 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     for (int e = e0; e < e1; e++) {
         const int n = steps_of(e), parts = (n + limit - 1) / limit;
         if (parts == 0) continue;
+        const int len = n / parts, more = n - len * parts;   // the first `more` parts have one step more
         for (int h = 0; h < a.p.n_kv; h++) {
             const int slot = h * tot[1] + at[1];
+            RowPiece *pc = a.pieces + h * tot[0] + at[0];
             for (int k = 0; k < parts; k++) {
-                const RowPiece pc = {b, h, r0, (int)((int64_t)n * k / parts), (int)((int64_t)n * (k + 1) / parts), parts > 1 ? slot + k : -1};
-                a.pieces[h * tot[0] + at[0] + k] = pc;
+                const int c0 = k * len + min(k, more);
+                pc[k] = {b, h, r0, c0, c0 + len + (k < more), parts > 1 ? slot + k : -1};
             }
             if (parts > 1) {
                 const RowJoin j = {b, h, r0, slot, parts};
