@@ -55,6 +55,7 @@ struct Args {
     float2 *part_ml;             // [2 grid][max rows]
     int part_rows;
     // tiles (scratch)
+    int cus;
     RowPlan *plan;
     RowPiece *pieces;
     RowJoin *joins;
@@ -551,7 +552,9 @@ __device__ __forceinline__ bf16x8_t lds8(const char *p) { return *(const bf16x8_
 // CUs; paged_rows runs one workgroup a piece, and the parts of a cut item go
 // to slots that paged_rows_join adds up in order.
 struct RowPiece {
-    int b, kvh, r0, c0, c1, slot, pad[2];     // steps c0 .. c1 - 1 of its list; slot -1: the whole item
+    int b, kvh, r0, c0, c1, slot;             // steps c0 .. c1 - 1 of its list; slot -1: the whole item
+    vx_pseq s;                                // its sequence
+    int pad[2];
 };
 struct RowJoin {
     int b, kvh, r0, slot, parts, pad[3];
@@ -563,9 +566,9 @@ struct RowPlan {
 __device__ __forceinline__ int row_tiles(const Args &a, const vx_pseq &s) { return (s.T * a.qg + TR - 1) / TR; }
 // Steps of entry e = b * n_rt + k of one KV head, row tile k from the end of
 // sequence b (rows that see nothing: one, for their output); 0 past its rows.
-__device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &b, int &r0) {
+__device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &b, int &r0, vx_pseq &s) {
     b = e / n_rt;
-    const vx_pseq s = vx_paged_seq(a.p, b);
+    s = vx_paged_seq(a.p, b);
     const int rt = row_tiles(a, s) - 1 - (e - b * n_rt);
     if (rt < 0) return 0;
     r0 = rt * TR;
@@ -582,14 +585,15 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     const int E = a.p.B * n_rt, per = (E + PLAN - 1) / PLAN, e0 = min(tid * per, E);
     int e1 = min(e0 + per, E);
     int b = 0, r0 = 0, items = 0, n0 = 0;
+    vx_pseq s = {};
     int64_t steps = 0;
     for (int e = e0; e < e1; e++) {
-        n0 = entry_steps(a, n_rt, e, b, r0);
+        n0 = entry_steps(a, n_rt, e, b, r0, s);
         steps += n0;
         items += n0 > 0;
     }
     // (a thread's only entry is not looked up again)
-    auto steps_of = [&](int e) { return per == 1 ? n0 : entry_steps(a, n_rt, e, b, r0); };
+    auto steps_of = [&](int e) { return per == 1 ? n0 : entry_steps(a, n_rt, e, b, r0, s); };
     items = vx_wave_scan(items);
     for (int off = 32; off >= 1; off >>= 1) steps += __shfl_xor(steps, off, 64);
     if (lane == 63) {
@@ -646,7 +650,7 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
             RowPiece *pc = a.pieces + h * tot[0] + at[0];
             for (int k = 0; k < parts; k++) {
                 const int c0 = k * len + min(k, more);
-                pc[k] = {b, h, r0, c0, c0 + len + (k < more), parts > 1 ? slot + k : -1};
+                pc[k] = {b, h, r0, c0, c0 + len + (k < more), parts > 1 ? slot + k : -1, s};
             }
             if (parts > 1) {
                 const RowJoin j = {b, h, r0, slot, parts};
@@ -672,35 +676,43 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     // The dispatcher deals workgroups round-robin over the 8 XCDs.  Each takes
     // the next piece of its own eighth of the list, so that the row tiles in
     // flight on an XCD are neighbours, whose keys its L2 then holds once; one
-    // whose eighth is all taken helps the next.
-    // (There are more workgroups than pieces, so that some are left to help.)
-    if (tid < 64) {
-        const int pieces = a.plan->pieces, x = (blockIdx.x + lane) & 7, lo = (int)((int64_t)pieces * x / 8), hi = (int)((int64_t)pieces * (x + 1) / 8);
-        const int taken = __hip_atomic_load(&a.plan->heads[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        int piece = -1;
-        for (uint32_t left = (uint32_t)__ballot(taken < hi - lo) & 255; left && piece < 0; left &= left - 1) {
-            const int k = __builtin_ctz(left);
-            int i = 0;
-            if (lane == k) i = atomicAdd(&a.plan->heads[x], 1);
-            i = __shfl(i, k, 64);
-            if (i < __shfl(hi - lo, k, 64)) piece = __shfl(lo, k, 64) + i;
+    // whose eighth is all taken helps another, beyond the pieces that the
+    // other's CUs start with.  (The first workgroups of an XCD, as many as its
+    // eighth has pieces, see that all of it is taken.  More would only help,
+    // and only where pieces are left over: 208 more at the counters than the
+    // 240 pieces of a call took it from 73 to 77 us.)
+    const int pieces = a.plan->pieces, at_once = a.cus / 8;
+    const int helper = (int)(blockIdx.x / 8) - pieces / 8 - ((int)(blockIdx.x & 7) < pieces % 8);
+    if (helper >= 0 && (pieces / 8 < at_once || helper >= at_once)) return;
+    if (wave == 0) {
+        const int x = (blockIdx.x + lane) & 7, lo = x * (pieces / 8) + min(x, pieces % 8), n = pieces / 8 + (x < pieces % 8);
+        int i = n;
+        if (lane == 0) i = atomicAdd(&a.plan->heads[x], 1);
+        uint32_t got = (uint32_t)__ballot(lane == 0 && i < n);
+        if (!got) {   // lane k: the eighth k further on
+            const int taken = __hip_atomic_load(&a.plan->heads[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (uint32_t left = (uint32_t)__ballot(taken >= at_once && taken < n) & 255; left && !got; left &= left - 1) {
+                const int k = __builtin_ctz(left);
+                if (lane == k) i = atomicAdd(&a.plan->heads[x], 1);
+                got = (uint32_t)__ballot(lane == k && i < n);
+            }
         }
-        if (tid == 0) {
-            sm.piece = piece;
+        const int piece = __builtin_amdgcn_readlane(lo + i, __builtin_ctz(got | 1u << 31) & 7);
+        if (lane == 0) {
+            sm.piece = got ? piece : -1;
             sm.odd = 0;
         }
     }
     __syncthreads();
     const int piece = __builtin_amdgcn_readfirstlane(sm.piece);
     if (piece < 0) return;
-    __syncthreads();
     const RowPiece *pc = a.pieces + piece;
     const int b = __builtin_amdgcn_readfirstlane(pc->b), kvh = __builtin_amdgcn_readfirstlane(pc->kvh), r0 = __builtin_amdgcn_readfirstlane(pc->r0);
     const int c0 = __builtin_amdgcn_readfirstlane(pc->c0), c1 = __builtin_amdgcn_readfirstlane(pc->c1), slot = __builtin_amdgcn_readfirstlane(pc->slot);
-    vx_pseq s = vx_paged_seq(a.p, b);
-    s.start = __builtin_amdgcn_readfirstlane(s.start);
-    s.T = __builtin_amdgcn_readfirstlane(s.T);
-    s.len = __builtin_amdgcn_readfirstlane(s.len);
+    vx_pseq s;
+    s.start = __builtin_amdgcn_readfirstlane(pc->s.start);
+    s.T = __builtin_amdgcn_readfirstlane(pc->s.T);
+    s.len = __builtin_amdgcn_readfirstlane(pc->s.len);
     s.row0 = s.len - s.T;
     const int R = s.T * a.qg;
     const int t0 = row_tok(a, r0), t1 = row_tok(a, min(r0 + TR - 1, R - 1));
@@ -1331,7 +1343,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     }
     // (a 32-row tile's queries are addressed by 32-bit offsets from its first)
     VX_REQUIRE(!d->acc || a.q_ts < (1u << 26) && a.q_hs < (1u << 26), "%s: q strides past 2^26 elements with acc (got %zu, %zu)", who, a.q_ts, a.q_hs);
-    const int n_rt = (rows + TR - 1) / TR, n_cu = ctx->n_cu;
+    const int n_rt = (rows + TR - 1) / TR, n_cu = a.cus = ctx->n_cu;
     VX_REQUIRE((int64_t)d->B * n_rt < (1ll << 31) - PLAN, "%s: more than 2^31 row tiles (B=%d max_T=%d)", who, d->B, d->max_T);
     // every token range ends in one tile that it need not fill; paged_plan makes at most 3/2 n_cu cuts, so twice
     // as many parts at most
