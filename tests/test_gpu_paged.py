@@ -137,6 +137,8 @@ DECODE = [   # lens, new, n_q, n_kv, page, window, sink
     ([50] * 70, [1] * 70, 24, 4, 32, 0, 0),                          # more than 64 sequences
     ([0, 0], [1, 0], 24, 4, 64, 7, 3),
     ([5, 6], [3, 2], 4, 2, 32, 0, 0),                                # three tokens, six rows
+    ([1 + 37 * i for i in range(70)], [1] * 70, 24, 4, 64, 0, 0),    # more than 64, of many workgroups each
+    ([1 + 37 * i for i in range(131)], [i % 3 for i in range(131)], 16, 2, 32, 500, 40),
 ]
 
 
@@ -163,6 +165,9 @@ TILES = [
     ([300], [37], 10, 2, 256, 1, 0),
     ([260, 7], [260, 7], 24, 4, 64, 4096, 3),                        # a window longer than the cache
     ([2, 9], [5, 4], 24, 4, 64, 0, 0),                               # tokens without a row see nothing
+    ([400] + [3 + i for i in range(69)], [400] + [i % 4 for i in range(69)], 24, 4, 64, 0, 0),   # more than 1024 places for row tiles
+    ([1500] * 3, [700, 1, 260], 24, 4, 96, 300, 5),                  # more row tiles than CUs, pages no power of two
+    ([9000], [3], 16, 2, 64, 0, 0),                                  # one row tile a KV head, cut into many parts
 ]
 
 
@@ -380,6 +385,7 @@ def ref_evict(acc, n, budget, sink, recent):
     ([5000, 4100], 4097, 1, 64, 256, 4, "zero"),        # every weight equal: the lowest rows
     ([900, 300], 250, 2, 3, 64, 4, "odd"),              # NaN, infinities, negative numbers, -0
     ([50, 20], 4000, 1, 1, 64, 4, "heavy"),             # a budget past the capacity
+    ([40000, 33000, 32769], 9000, 4, 100, 128, 1, "ties"),   # more rows than a workgroup holds in registers
 ])
 @pytest.mark.parametrize("optional", [True, False])
 def test_evict(ctx, lens, budget, sink, recent, page, n_kv, kind, optional):
@@ -653,3 +659,103 @@ def test_no_tokens(ctx):
     ctx.sync()
     assert np.array_equal(a.bufs["out"].download(a.sentinel.shape, np.float32), a.sentinel)
     a.free()
+
+
+def test_a_step_captured_and_replayed():
+    """Append, attention with weights and eviction in one graph, replayed over fresh pages and weights: each replay's
+    bytes are the eager step's."""
+    from vx27_amd import lib as L, workloads as W
+    lens, P, n_kv, budget = [301, 90, 640], 64, 4, 128
+    bt = Batch(lens, [1] * 3, page=P, seed=31)
+    dst = 2
+    pool = bt.n_pages + 3 * dst
+    k = np.concatenate([bt.k, np.zeros((3 * dst,) + bt.k.shape[1:], np.uint16)])
+    v = np.concatenate([bt.v, np.zeros((3 * dst,) + bt.v.shape[1:], np.uint16)])
+    stride = bt.max_pages * P
+    acc = bt.r.random((3, n_kv, stride)).astype(np.float32)
+    with L.Ctx(0) as ctx:
+        up = dict(k=k, v=v, acc=acc, table=bt.table, len=np.asarray(lens, np.int32), dst=np.arange(bt.n_pages, pool, dtype=np.int32),
+                  q=W.normal(bt.r, (3, 24, HD)), kv=W.normal(bt.r, (2, 3, n_kv, HD)), w=W.normal(bt.r, HD, 0.1), rot=np.zeros((3, 24, HD), np.uint16),
+                  out=np.zeros((3, 24, HD), np.float32), dl=np.zeros(3, np.int32), ao=np.zeros((3, n_kv, budget), np.float32))
+        buf = {n: ctx.put(x) for n, x in up.items()}
+        p, a, e = L.PagedAppendDesc(), L.PagedAttnDesc(), L.PagedEvictDesc()
+        for d in (p, a, e):
+            d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = 3, n_kv, HD, P, pool, bt.max_pages
+            d.table, d.len, d.k_pages, d.v_pages = buf["table"].ptr, buf["len"].ptr, buf["k"].ptr, buf["v"].ptr
+        for d in (p, a):
+            d.n_q, d.n_tok, d.max_T = 24, 3, 1
+        p.rope_dim, p.rope_theta, p.rope_yarn, p.q, p.k_new, p.v_new = 64, 1e7, 1.0, buf["q"].ptr, buf["kv"].ptr, buf["kv"].ptr + 3 * n_kv * HD * 4
+        p.q_norm_w, p.k_norm_w, p.q_out = buf["w"].ptr, buf["w"].ptr, buf["rot"].ptr
+        a.q, a.out, a.acc, a.acc_stride = buf["rot"].ptr, buf["out"].ptr, buf["acc"].ptr, stride
+        e.budget, e.n_sink, e.n_recent, e.acc, e.acc_stride = budget, 4, 16, buf["acc"].ptr, stride
+        e.dst_table, e.dst_max_pages, e.dst_len, e.acc_out, e.acc_out_stride = buf["dst"].ptr, dst, buf["dl"].ptr, buf["ao"].ptr, budget
+        lib = L.lib()
+
+        def step():
+            L.check(lib.vx27_hip_paged_append(ctx.h, C.byref(p)))
+            L.check(lib.vx27_hip_paged_attn(ctx.h, C.byref(a)))
+            L.check(lib.vx27_hip_paged_evict(ctx.h, C.byref(e)))
+
+        def fresh():
+            for n in ("k", "v", "acc", "rot", "out", "dl", "ao"):
+                buf[n].upload(up[n])
+
+        def raw():
+            ctx.sync()
+            return [buf[n].download((buf[n].nbytes,), np.uint8) for n in ("k", "v", "acc", "rot", "out", "dl", "ao")]
+        step()
+        want = raw()
+        assert np.array_equal(buf["dl"].download((3,), np.int32), [128, 90, 128])
+        fresh()
+        ctx.graph_begin()
+        step()
+        g = ctx.graph_end()
+        try:
+            for rep in range(4):
+                fresh()
+                ctx.graph_launch(g)
+                assert all(np.array_equal(x, y) for x, y in zip(raw(), want)), rep
+                if rep % 2:
+                    fresh()
+                    step()
+                    assert all(np.array_equal(x, y) for x, y in zip(raw(), want)), rep
+        finally:
+            L.check(lib.vx27_hip_graph_destroy(g), "graph_destroy")
+
+
+def test_eviction_workspace_goes_by_the_rows(ctx):
+    """Without `kept` the call's workspace is that of the rows there can be, whatever the budget."""
+    from vx27_amd import lib as L
+    before = ctx.mem_info()["scratch_bytes"]
+    bt = Batch([70, 40], [1, 1], page=32, seed=33)
+    n = bt.max_pages
+    up = dict(k=bt.k, v=bt.v, table=np.zeros((2, n), np.int32), len=np.zeros(2, np.int32), dst=np.zeros((2, n), np.int32),
+              dl=np.full(2, -1, np.int32), acc=np.zeros((2, 4, n * 32), np.float32))
+    buf = {x: ctx.put(y) for x, y in up.items()}
+    d = L.PagedEvictDesc()
+    d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages, d.budget = 2, 4, HD, 32, bt.n_pages, n, 2 ** 31 - 1
+    d.table, d.len, d.k_pages, d.v_pages = (buf[x].ptr for x in ("table", "len", "k", "v"))
+    d.acc, d.acc_stride, d.dst_table, d.dst_max_pages, d.dst_len = buf["acc"].ptr, n * 32, buf["dst"].ptr, n, buf["dl"].ptr
+    L.check(L.lib().vx27_hip_paged_evict(ctx.h, C.byref(d)), "paged_evict")
+    ctx.sync()
+    assert np.array_equal(buf["dl"].download((2,), np.int32), [0, 0])
+    assert ctx.mem_info()["scratch_bytes"] <= max(before, 1 << 20)
+    for x in buf.values():
+        x.free()
+
+
+def test_a_refused_step_changes_nothing(ctx):
+    """A step that the pool or the library refuses leaves the layer's rows and positions, and the next one runs."""
+    from vx27_amd import lib as L, mixers as M
+    r = np.random.default_rng(34)
+    lay = M.PagedGQALayer(ctx, 2, 3, 32, np.zeros(HD), np.zeros(HD))
+    qg, k, v = (r.standard_normal((n, h, w)).astype(np.float32) for n, h, w in ((70, 24, 2 * HD), (70, 4, HD), (70, 4, HD)))
+    with pytest.raises(L.HipError, match="pages"):
+        lay.step([35, 35], qg, k, v)
+    lay.rope_dim = 3
+    with pytest.raises(L.HipError, match="rope_dim"):
+        lay.step([5, 5], qg[:10], k[:10], v[:10])
+    lay.rope_dim = 64
+    assert lay.rows == [0, 0] and lay.pos == [0, 0]
+    assert np.isfinite(lay.step([5, 5], qg[:10], k[:10], v[:10])).all()
+    assert lay.rows == [5, 5] and lay.pos == [5, 5]

@@ -1342,13 +1342,13 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         return 0;
     }
     // (a 32-row tile's queries are addressed by 32-bit offsets from its first)
-    VX_REQUIRE(!d->acc || a.q_ts < (1u << 26) && a.q_hs < (1u << 26), "%s: q strides past 2^26 elements with acc (got %zu, %zu)", who, a.q_ts, a.q_hs);
+    VX_REQUIRE(!d->acc || (a.q_ts < (1u << 26) && a.q_hs < (1u << 26)), "%s: q strides past 2^26 elements with acc (got %zu, %zu)", who, a.q_ts, a.q_hs);
     const int n_rt = (rows + TR - 1) / TR, n_cu = a.cus = ctx->n_cu;
     VX_REQUIRE((int64_t)d->B * n_rt < (1ll << 31) - PLAN, "%s: more than 2^31 row tiles (B=%d max_T=%d)", who, d->B, d->max_T);
     // every token range ends in one tile that it need not fill; paged_plan makes at most 3/2 n_cu cuts, so twice
     // as many parts at most
     const int64_t cuts = (int64_t)n_cu * 3 / 2, items = ((int64_t)d->n_tok * a.qg / TR + d->B) * d->n_kv;
-    VX_REQUIRE(items + cuts < (1ll << 31), "%s: more than 2^31 workgroups (B=%d n_kv=%d n_tok=%d)", who, d->B, d->n_kv, d->n_tok);
+    VX_REQUIRE(items + cuts < (1 << 24), "%s: more than 2^24 row tiles (B=%d n_kv=%d n_tok=%d)", who, d->B, d->n_kv, d->n_tok);
     const size_t ml_bytes = (size_t)2 * cuts * TR * sizeof(float2), plan_bytes = 256, piece_bytes = (size_t)(items + cuts) * sizeof(RowPiece);
     const size_t join_bytes = ((size_t)cuts * sizeof(RowJoin) + 255) / 256 * 256;
     void *scr;

@@ -27,7 +27,8 @@ struct EvictArgs {
     int *dst_len;
     float *acc_out;
     size_t acc_out_stride;
-    int *kept;          // [B][n_kv][budget] (the caller's or scratch)
+    int *kept;          // [B][n_kv][kept_stride] (the caller's or scratch)
+    size_t kept_stride;
 };
 
 __device__ __forceinline__ int seq_len(const EvictArgs &a, int b) {
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = seq_len(a, b), keep = min(n, a.budget);
-    int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.budget;
+    int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.kept_stride;
     if (h == 0 && tid == 0) a.dst_len[b] = keep;
     if (n <= a.budget) {
         for (int i = tid; i < n; i += SEL) kept[i] = i;
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
     __shared__ int s_row[VB];
     __shared__ size_t s_blk[VB];   // element offset of the row's V block
     __shared__ uint16_t sv[HDG * VROW];
-    const int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.budget;
+    const int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.kept_stride;
     const int dpage = vx_page_checked(a.p, vx_table_word(a.dst_table + (size_t)b * a.dst_max_pages + d0 / P)), dat = d0 % P;
     if (tid < VB) {
         const int r = kept[d0 + min(tid, cnt - 1)];
@@ -283,13 +284,15 @@ extern "C" int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_de
     a.acc = d->acc; a.acc_stride = d->acc_stride; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
     a.dst_table = d->dst_table; a.dst_max_pages = d->dst_max_pages; a.dst_len = d->dst_len;
     a.acc_out = d->acc_out; a.acc_out_stride = d->acc_out_stride;
+    const int64_t most = cap < d->budget ? cap : d->budget;   // rows a sequence keeps at most
     a.kept = d->kept;
+    a.kept_stride = d->budget;
     if (!a.kept) {
         void *scr;
-        if (vx_ctx_scratch(ctx, pairs * d->budget * sizeof(int), &scr)) return -1;
+        a.kept_stride = most;
+        if (vx_ctx_scratch(ctx, pairs * most * sizeof(int), &scr)) return -1;
         a.kept = (int *)scr;
     }
-    const int64_t most = cap < d->budget ? cap : d->budget;
     VX_LAUNCH(ctx, paged_select, dim3(d->n_kv, d->B), dim3(SEL), a);
     VX_LAUNCH(ctx, paged_move, dim3((unsigned)((most + VB - 1) / VB), d->n_kv, d->B), dim3(256), a);
     return 0;

@@ -270,16 +270,13 @@ class PagedGQALayer:
         ctx, N, hd = self.ctx, int(np.sum(new)), self.hd
         if N == 0:
             return np.empty((0, self.n_q, hd), np.float32)
-        for b, t in enumerate(new):
-            self._grow(b, self.rows[b] + t)
-        for b, t in enumerate(new):
-            self.rows[b] += int(t)
+        rows = [n + int(t) for n, t in zip(self.rows, new)]
+        for b, n in enumerate(rows):
+            self._grow(b, n)
         start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
         pos = np.concatenate([np.arange(p, p + t) for p, t in zip(self.pos, new)]).astype(np.int32)
-        for b, t in enumerate(new):
-            self.pos[b] += int(t)
         up = [ctx.put(x) for x in (_f32(qg), _f32(k_new), _f32(v_new), self._table(self.pages),
-                                   np.asarray(self.rows, np.int32), start, pos)]
+                                   np.asarray(rows, np.int32), start, pos)]
         qb, kb, vb, tb, lb, sb, pb = up
         rot, out = ctx.buf(N * self.n_q * hd * 2), ctx.buf(N * self.n_q * hd * 4)
         d = L.PagedAppendDesc()
@@ -299,6 +296,8 @@ class PagedGQALayer:
         check(L.lib().vx27_hip_paged_append(ctx.h, C.byref(d)), "paged_append")
         check(L.lib().vx27_hip_paged_attn(ctx.h, C.byref(a)), "paged_attn")
         ctx.sync()
+        self.rows = rows
+        self.pos = [p + int(t) for p, t in zip(self.pos, new)]
         if out_dtype == L.BF16:
             res = (out.download((N, self.n_q, hd), np.uint16).astype(np.uint32) << 16).view(np.float32)
         else:
