@@ -1362,7 +1362,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     a.pieces = (RowPiece *)(at += (size_t)2 * cuts * TR * HDG * 4);
     VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
     VX_LAUNCH(ctx, paged_rows, dim3((unsigned)(items + cuts)), dim3(256), a);
-    VX_LAUNCH(ctx, paged_rows_join, dim3(2 * n_cu), dim3(256), a);
+    VX_LAUNCH(ctx, paged_rows_join, dim3(8 * n_cu), dim3(256), a);
     if (d->acc) VX_LAUNCH(ctx, paged_rows_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
     return 0;
 }
