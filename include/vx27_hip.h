@@ -388,6 +388,14 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * (-inf for a token that sees nothing); acc [B][n_kv][acc_stride], to which
  * each row's weight over the call's tokens and the group's heads is added
  * (rows nobody sees and rows from len on are left as they were).
+ * An infinite or NaN value of a row reaches only the tokens that see the row,
+ * whose outputs are then not finite (an infinity may end as NaN).
+ * out must not overlap an input.  Context scratch: the parts of cut rows
+ * (at most about 100 MB), and with acc and at most 16 query rows a KV head their
+ * scores, B*n_kv*rows*4 bytes for each row that a sequence can see at most
+ * (max_pages*page_size, or sinks, window and new tokens).
+ * max_T*n_q/n_kv below 2^28; with acc and more than 16 query rows q strides
+ * below 2^26 elements.
  * q 16-byte aligned with strides multiples of 8 elements; gate (fp32, or bf16
  * with gate_dtype) and out 16-byte aligned, gate strides multiples of 8
  * elements; n_q/n_kv at most 16. */

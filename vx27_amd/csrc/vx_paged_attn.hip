@@ -261,6 +261,16 @@ __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l,
 // workgroup is finished there; the first and the last piece of a
 // workgroup's range may be parts of a pair and go to its two partial slots,
 // which paged_join merges in order.
+//
+// Bound by the stream of K and V, 1 KiB a row and KV head, which two
+// workgroups a CU (8 waves with 24 KiB of loads in flight each) take at 6.6
+// TB/s: 4 x 131072 rows, 2.15 GB, in 325 us (one workgroup a CU: 327), a
+// plain read of as much 298.  Short calls are two launches and the latencies
+// of the table, the tiles and the join: 12 us for one sequence of 1000 rows.
+//
+// 16 rows are what one MFMA tile holds, so this form ends there: a third token
+// of 6 heads goes to the tiles below (4 x 131072 rows: 328 us for two tokens
+// a sequence, 377 for three there; one of 1000 rows: 14 and 26).
 // The list of a call's tiles: up to 64 sequences are held one a lane and read
 // once; more are read again where they are needed.
 struct Units {
@@ -414,7 +424,7 @@ __global__ __launch_bounds__(256, 2) void paged_split(Args a) {
     }
 }
 
-// grid (max rows, n_kv, B), block 256: merges the parts of one query row, in
+// grid (most rows, n_kv, B), block 256 (4-7 us): merges the parts of one query row, in
 // their order: wave w takes parts w, w + 4, ..., eight in flight; a row of a
 // sequence without rows gets 0.
 __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
@@ -475,7 +485,9 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
 }
 
 // grid (tile_cap / 8, n_kv, B), block 256: one thread per key; the stashed
-// scores become weights, summed over the rows that see the key.
+// scores become weights, summed over the rows that see the key.  (The scores
+// are kept, 4 bytes a row of queries and keys against the 512 of K that a
+// second pass would read: 8 us of the 63 for 16 ragged sequences of 8190 rows.)
 __global__ __launch_bounds__(256) void paged_weigh(Args a) {
     const int kvh = blockIdx.y, b = blockIdx.z;
     const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -512,9 +524,15 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 // A step's two key blocks are consecutive entries of the tile list, so a
 // sink block and the window's first block make a step without a gap.
 //
+// Bound by the MFMAs' issue beside the softmax and by power: a step of 64 MFMAs
+// a wave takes about 2.15 us (3900 cycles at the 1.8 GHz that the chip then
+// holds; the MFMAs alone are 2050), and a piece another 13 us for its first
+// loads, its first scores and its output.  8192 tokens of 24 heads under a
+// window of 1024: 300 us, 0.65 PFLOP/s of what the rows see.
+//
 // (Measured against it: waves of 64 rows x one key block, and 128 dims of O,
 // which read half as much from LDS but exchange weights and maxima through it
-// and meet twice a step: 2.1 us a step.)
+// and meet twice a step: 315 us; a persistent loop over the pieces spilled.)
 constexpr int TR = 128;                      // query rows of a workgroup
 constexpr int HALF = TILE * HDG * 2;         // bytes of one key block of K or of V
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
@@ -576,7 +594,7 @@ __device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &
     return max(1, (tl.nt + 1) / 2);
 }
 
-// grid 1, block 1024.
+// grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).
 constexpr int PLAN = 1024;
 __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, int max_pieces) {
     __shared__ int64_t s_steps[PLAN / 64];
@@ -1119,7 +1137,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
 }
 
 // grid any, block 256: adds up the parts of the cut items, in order, four
-// rows a wave, their loads in flight together.
+// rows a wave, their loads in flight together.  (Seven chunks of 701 tokens:
+// 116 us the call with two workgroups a CU, 113 with four, 111 with eight.)
 __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
     constexpr int NR = 4, PER = TR / (4 * NR);
     const int lane = threadIdx.x & 63, todo = a.plan->joins * PER;
@@ -1177,6 +1196,9 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
 // any of the workgroup's keys pass through LDS, one ahead.  A lane's sums are
 // over its row of each tile; at the end the 32 lanes of a key are added up.
 // One workgroup owns a key, so the order of the sums is fixed.
+// 54 us for 4 x 64 tokens over 9000 rows, 28 GFLOP; 576 workgroups for 512
+// places.  (One key block a wave, four workgroups a CU: 85 us, as the queries
+// are then read from LDS twice as often.)
 constexpr int QT = 32, QBUF = QT * HDG * 2;
 __global__ __launch_bounds__(256, 2) void paged_rows_weigh(Args a) {
     __shared__ __attribute__((aligned(16))) char sq[2][QBUF];
@@ -1323,7 +1345,8 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     if (rows <= 16) {
         VX_REQUIRE((int64_t)d->B * d->n_kv * tile_cap < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %lld tiles each)", who,
                    d->B, d->n_kv, (long long)tile_cap);
-        a.min_tiles = 4;   // one a wave
+        // (one sequence of 1000 rows: 13.1 us with 4, 12.1 with 2, 11.9 with 1; of 3000: 16.4, 13.6, 15.8; of 8000: 18.8, 19.5, 19.5)
+        a.min_tiles = 2;
         const int64_t most = ((int64_t)d->B * d->n_kv * tile_cap + a.min_tiles - 1) / a.min_tiles;
         const int grid = (int)std::min<int64_t>(most, 2 * ctx->n_cu);
         a.part_rows = rows;
