@@ -139,6 +139,7 @@ DECODE = [   # lens, new, n_q, n_kv, page, window, sink
     ([5, 6], [3, 2], 4, 2, 32, 0, 0),                                # three tokens, six rows
     ([1 + 37 * i for i in range(70)], [1] * 70, 24, 4, 64, 0, 0),    # more than 64, of many workgroups each
     ([1 + 37 * i for i in range(131)], [i % 3 for i in range(131)], 16, 2, 32, 500, 40),
+    ([i % 71 for i in range(1100)], [int(i % 9 > 0) for i in range(1100)], 4, 2, 32, 0, 0),   # more than 1024
 ]
 
 

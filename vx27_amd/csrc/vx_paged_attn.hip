@@ -54,6 +54,7 @@ struct Args {
     float *part_o;               // [2 grid][max rows][256]
     float2 *part_ml;             // [2 grid][max rows]
     int part_rows;
+    int *before;                 // B > 64: [B + 1] units before each sequence
     // tiles (scratch)
     int cus;
     RowPlan *plan;
@@ -272,7 +273,8 @@ __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l,
 // of 6 heads goes to the tiles below (4 x 131072 rows: 328 us for two tokens
 // a sequence, 377 for three there; one of 1000 rows: 14 and 26).
 // The list of a call's tiles: up to 64 sequences are held one a lane and read
-// once; more are read again where they are needed.
+// once; of more, paged_units adds up the units before each first (each
+// workgroup doing so for itself took 3.2 ms for 4096 sequences of 100 rows).
 struct Units {
     vx_pseq s;          // of sequence `lane` (B <= 64)
     vx_tiles t;
@@ -292,12 +294,7 @@ __device__ __forceinline__ Units units_of(const Args &a, int grid) {
         u.upto = vx_wave_scan(lane < a.p.B ? n : 0);
         u.total = __builtin_amdgcn_readlane(u.upto, 63);
     } else {
-        int sum = 0;
-        for (int b0 = 0; b0 < a.p.B; b0 += 64) {
-            const int n = seq_units(a, min(b0 + lane, a.p.B - 1), u.s, u.t);
-            sum += b0 + lane < a.p.B ? n : 0;
-        }
-        u.total = __builtin_amdgcn_readlane(vx_wave_scan(sum), 63);
+        u.total = a.before[a.p.B];
     }
     u.chunk = max((u.total + grid - 1) / grid, a.min_tiles);
     return u;
@@ -310,24 +307,43 @@ __device__ __forceinline__ int units_before(const Args &a, const Units &u, int b
         t = {get(u.t.st), get(u.t.fm), get(u.t.nt)};
         return get(u.upto) - t.nt * a.p.n_kv;
     }
-    int sum = 0;
-    for (int c = threadIdx.x & 63; c < b; c += 64) sum += seq_units(a, c, s, t);
-    sum = __builtin_amdgcn_readlane(vx_wave_scan(sum), 63);
     seq_units(a, b, s, t);
-    return sum;
+    return a.before[b];
 }
-// The sequence of unit x < total.
+// The sequence of unit x < total: the last with at most x units before it,
+// among 64 of them at a time.
 __device__ __forceinline__ int units_find(const Args &a, const Units &u, int x) {
     const int lane = threadIdx.x & 63;
     if (a.p.B <= 64) return __builtin_ctzll(__ballot(u.upto > x));
-    int done = 0;
-    for (int b0 = 0;; b0 += 64) {
-        vx_pseq s;
-        vx_tiles t;
-        const int n = seq_units(a, min(b0 + lane, a.p.B - 1), s, t), upto = vx_wave_scan(b0 + lane < a.p.B ? n : 0);
-        const uint64_t past = __ballot(done + upto > x);
-        if (past || b0 + 64 >= a.p.B) return b0 + (past ? __builtin_ctzll(past) : 0);
-        done += __builtin_amdgcn_readlane(upto, 63);
+    int b = 0;
+    for (int n = a.p.B; n > 1;) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const uint64_t le = __ballot(at < n && a.before[b + min(at, n - 1)] <= x);
+        const int k = le ? 63 - __builtin_clzll(le) : 0;
+        b += k * step;
+        n = min(step, n - k * step);
+    }
+    return b;
+}
+
+// grid 1, block 1024: the units before each sequence, and in all.
+__global__ __launch_bounds__(1024) void paged_units(Args a) {
+    __shared__ int s_sum[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (a.p.B + 1023) / 1024, b0 = min(tid * per, a.p.B), b1 = min(b0 + per, a.p.B);
+    vx_pseq s;
+    vx_tiles t;
+    int sum = 0;
+    for (int b = b0; b < b1; b++) sum += seq_units(a, b, s, t);
+    int at = vx_wave_scan(sum);
+    if (lane == 63) s_sum[wave] = at;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) at += s_sum[w];
+    if (tid == 1023) a.before[a.p.B] = at;
+    at -= sum;
+    for (int b = b0; b < b1; b++) {
+        a.before[b] = at;
+        at += seq_units(a, b, s, t);
     }
 }
 
@@ -1353,12 +1369,15 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         const size_t n_part = (size_t)2 * grid * rows;
         const size_t o_bytes = n_part * HDG * 4, ml_bytes = (n_part * sizeof(float2) + 255) / 256 * 256;
         const size_t st_bytes = d->acc ? (size_t)d->B * d->n_kv * rows * tile_cap * TILE * 4 : 0;
+        const size_t before_bytes = d->B > 64 ? ((size_t)d->B + 1) * sizeof(int) : 0;
         void *scr;
-        if (vx_ctx_scratch(ctx, o_bytes + ml_bytes + stat_bytes + st_bytes, &scr)) return -1;
+        if (vx_ctx_scratch(ctx, o_bytes + ml_bytes + stat_bytes + st_bytes + before_bytes, &scr)) return -1;
         a.part_o = (float *)scr;
         a.part_ml = (float2 *)((char *)scr + o_bytes);
         a.stat = d->acc ? (float2 *)((char *)scr + o_bytes + ml_bytes) : nullptr;
         a.stash = d->acc ? (float *)((char *)scr + o_bytes + ml_bytes + stat_bytes) : nullptr;
+        a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes + stat_bytes + st_bytes) : nullptr;
+        if (a.before) VX_LAUNCH(ctx, paged_units, dim3(1), dim3(1024), a);
         VX_LAUNCH(ctx, paged_split, dim3(grid), dim3(256), a);
         VX_LAUNCH(ctx, paged_join, dim3(rows, d->n_kv, d->B), dim3(256), a, grid);
         if (d->acc) VX_LAUNCH(ctx, paged_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
