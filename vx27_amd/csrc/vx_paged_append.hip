@@ -95,8 +95,10 @@ __device__ __forceinline__ double wave_sums4(const double (&s)[4]) {
 // block, the others the group's query heads of 8 tokens each: a prompt's
 // workgroups are then short and many (one workgroup a block took 88 us for
 // 4364 tokens of 24 + 4 heads, its waves waiting for one another's loads).
-// The tokens' cos and sin once; then wave w takes rows w, w + 4, ..., four at
-// a time so that their loads are in flight together, lane l dims 4l..4l+3.
+// V first, then the tokens' cos and sin in its place in LDS (side by side they
+// leave room for six workgroups a CU, not eight: 50 us); then wave w takes
+// rows w, w + 4, ..., four at a time so that their loads are in flight
+// together, lane l dims 4l..4l+3.
 // Bound by bytes: 49 us for 143 MB (4096 + 268 bf16 tokens), the copy rate's
 // 27; one token for 13 sequences, a launch and its latencies, 6.5 us.  v
 // goes through LDS into the dim-major block, element by element at its ends
@@ -110,8 +112,11 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     const int blk = blockIdx.x / (1 + VB / QTOK), part = blockIdx.x % (1 + VB / QTOK);
     const bool is_k = part == 0;
     if (!is_k && !a.q) return;
-    __shared__ __attribute__((aligned(16))) float cs[VB][HALFS], sn[VB][HALFS];
-    __shared__ __attribute__((aligned(16))) uint16_t vt[VB][HDG];   // v's rows; then a row a wave
+    // v's rows; then the tokens' cos and sin, and a row a wave
+    constexpr int CS = VB * HALFS * 4;
+    __shared__ __attribute__((aligned(16))) char lds[2 * CS + 4 * HDG * 4 > VB * HDG * 2 ? 2 * CS + 4 * HDG * 4 : VB * HDG * 2];
+    float (*cs)[HALFS] = (float (*)[HALFS])lds, (*sn)[HALFS] = (float (*)[HALFS])(lds + CS);
+    uint16_t (*vt)[HDG] = (uint16_t (*)[HDG])lds;
     const vx_pseq s = vx_paged_seq(a.p, b);
     if (s.row0 < 0 && tid == 0 && hk == 0 && blockIdx.x == 0) *a.p.err_flag = 1;
     const int first = max(s.row0, 0);
@@ -144,12 +149,6 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
         page = vx_paged_page(a.p, b, p0);
         at = p0 - vx_page_slot(a.p, p0) * a.p.page_size;
     }
-    for (int e = tid; e < n * half; e += 256) {
-        const int j = e / half, i = e % half;
-        const float2 c = vx_rope_cs(a.rope, a.pos ? a.pos[tok0 + j] : lo + j, a.yarn, i);
-        cs[j][i] = c.x;
-        sn[j][i] = c.y;
-    }
     if (is_k) {
 #pragma unroll 4
         for (int e = tid; e < n * (HDG / 4); e += 256) {
@@ -157,9 +156,7 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
             const float4 x = load4(a.v, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * c, a.bf16);
             *(uint2 *)&vt[j][4 * c] = pack4(x.x, x.y, x.z, x.w);
         }
-    }
-    __syncthreads();
-    if (is_k) {
+        __syncthreads();
         uint16_t *vb = a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, hk, at, 0);
         for (int e = tid; e < HDG * (VB / 8); e += 256) {
             const int d = e / (VB / 8), c = e % (VB / 8), r0 = p0 + 8 * c;
@@ -173,15 +170,22 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
                     if (r0 + k >= lo && r0 + k < hi) vb[(size_t)d * VB + 8 * c + k] = vt[r0 + k - lo][d];
             }
         }
+        __syncthreads();
     }
+    for (int e = tid; e < n * half; e += 256) {
+        const int j = e / half, i = e % half;
+        const float2 c = vx_rope_cs(a.rope, a.pos ? a.pos[tok0 + j] : lo + j, a.yarn, i);
+        cs[j][i] = c.x;
+        sn[j][i] = c.y;
+    }
+    __syncthreads();
 
     // half a power of two from 4 on: a pair's dims i and i + half are in lanes
     // l and l ^ (half / 4), at the same element; any other half goes through LDS
     const bool pairs = half >= 4 && (half & (half - 1)) == 0;
     const bool turns = 4 * lane < 2 * half, second = 4 * lane >= half;
     const int ci = pairs ? (4 * lane) & (half - 1) : 0;
-    float *row = (float *)vt[0] + wave * HDG;
-    if (!pairs && half) __syncthreads();
+    float *row = (float *)(lds + 2 * CS) + wave * HDG;
     for (int r0 = wave; r0 < rows; r0 += 4 * NR) {
         float y[NR][4];
         double ss[NR];
@@ -264,7 +268,7 @@ extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_
     a.q_norm_w = d->q_norm_w; a.k_norm_w = d->k_norm_w;
     a.q_out = d->q_out; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
     const dim3 grid(((d->max_T + VB - 2) / VB + 1) * (1 + VB / QTOK), d->n_kv, d->B);
-    // (32 angles a token take 8 KiB of LDS, 128 take 32: the 143 MB prompt takes 49 us with the first, 71 with the second)
+    // (32 angles a token take 16 KiB of LDS, 128 take 36: the 143 MB prompt takes 49 us with the first, 62 with the second)
     if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<32>), grid, dim3(256), a);
     else VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<MAXR>), grid, dim3(256), a);
     return 0;

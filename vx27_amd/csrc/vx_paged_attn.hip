@@ -812,7 +812,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             case 0: dma16<0>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
             case 1: dma16<1024>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
             case 2: dma16<2048>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
-            default: dma16<3072>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
+            default: dma16<3 * 1024>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
         }
     };
     auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
