@@ -57,7 +57,7 @@ __device__ __forceinline__ int lanes_below(uint64_t x) { return __builtin_amdgcn
 // each for every eighth lane (8 x 32768 rows: 35 us, with one histogram 54).
 // Two buffers: a pass clears the next one's.  One workgroup a pair has the
 // whole of its weights at hand; a launch and three passes' latencies are 12 us.
-constexpr int SEL = 1024, NW = SEL / 64, CH = 32, BINS = 2048, COPY = 8;
+constexpr int SEL = 1024, NW = SEL / 64, CH = 32, BINS = 2048, COPY = 8, HROW = BINS + 4;   // (copies four banks apart)
 __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     const float *w = a.acc + ((size_t)b * a.p.n_kv + h) * a.acc_stride;
     const int lo = a.n_sink, hi = n - a.n_recent;     // the rows that compete
     int want = a.budget;                              // rows of the ranks not yet decided that stay
-    __shared__ __attribute__((aligned(16))) int hist[2][BINS * COPY];
+    __shared__ __attribute__((aligned(16))) int hist[2][COPY][HROW];
     __shared__ int s_sum[NW], s_eq[NW], s_found[2];
     const int seg = ((n + NW - 1) / NW + 63) / 64 * 64, w0 = wave * seg, w1 = min(w0 + seg, n);
     uint32_t r[CH];
@@ -87,39 +87,39 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     };
     const bool once = seg <= CH * 64;
     load(w0);
-    auto clear = [&](int buf, int bins) {
-        for (int i = tid; i < bins * COPY / 4; i += SEL) ((int4 *)hist[buf])[i] = make_int4(0, 0, 0, 0);
+    auto clear = [&](int buf) {
+        for (int i = tid; i < COPY * HROW / 4; i += SEL) ((int4 *)hist[buf])[i] = make_int4(0, 0, 0, 0);
     };
-    clear(0, BINS);
+    clear(0);
     __syncthreads();
     uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
         const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = 1 << bits;
-        int *hp = hist[pass & 1];
-        if (pass < 2) clear(~pass & 1, BINS);
+        int (*hp)[HROW] = hist[pass & 1];
+        if (pass < 2) clear(~pass & 1);
         for (int base = w0; base < w1; base += CH * 64) {
             if (!once) load(base);
 #pragma unroll
             for (int k = 0; k < CH; k++) {
                 if (base + 64 * k >= w1) continue;
-                if (((r[k] ^ prefix) & mask) == 0) atomicAdd(&hp[((r[k] >> shift) & (bins - 1)) * COPY + (lane & (COPY - 1))], 1);
+                if (((r[k] ^ prefix) & mask) == 0) atomicAdd(&hp[lane & (COPY - 1)][(r[k] >> shift) & (bins - 1)], 1);
             }
         }
         __syncthreads();
         // the bin of the want-th heaviest: thread t takes bins 2 t and 2 t + 1
         // (from the top), suffix sums over the threads
-        int c[2], mine = 0;
+        int c[2] = {0, 0};
+        const int low = BINS - 2 - 2 * tid;
+        if (low < bins) {
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const int bin = BINS - 1 - (2 * tid + q);
-            c[q] = 0;
-            if (bin < bins) {
-                const int4 x = *(const int4 *)&hp[bin * COPY], y = *(const int4 *)&hp[bin * COPY + 4];
-                c[q] = (x.x + x.y + x.z + x.w) + (y.x + y.y + y.z + y.w);
+            for (int q = 0; q < COPY; q++) {
+                const int2 x = *(const int2 *)&hp[q][low];
+                c[0] += x.y;
+                c[1] += x.x;
             }
-            mine += c[q];
         }
+        const int mine = c[0] + c[1];
         int x = vx_wave_scan(mine);
         if (lane == 63) s_sum[wave] = x;
         __syncthreads();
