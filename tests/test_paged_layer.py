@@ -1,0 +1,142 @@
+"""The bookkeeping of PagedGQALayer without a GPU: pages, rows and device
+buffers around steps and evictions that run or are refused.  "Device" memory
+is host memory and the library's calls are stubs that record their
+descriptors."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from vx27_amd import lib as L, mixers as M
+
+HD = 256
+
+
+class FakeBuf:
+    def __init__(self, ctx, nbytes):
+        self.ctx, self.nbytes = ctx, int(nbytes)
+        self.mem = np.zeros(self.nbytes, np.uint8)
+        self.ptr = self.mem.ctypes.data
+        ctx.live.append(self)
+
+    def upload(self, arr):
+        raw = np.frombuffer(np.ascontiguousarray(arr).tobytes(), np.uint8)
+        assert raw.size <= self.nbytes
+        self.mem[:raw.size] = raw
+        return self
+
+    def download(self, shape, dtype):
+        return np.frombuffer(self.mem.tobytes(), dtype)[:int(np.prod(shape))].reshape(shape).copy()
+
+    def zero(self):
+        self.mem[:] = 0
+        return self
+
+    def free(self):
+        if self.ptr:
+            self.ctx.live.remove(self)
+            self.ptr = None
+
+
+class FakeCtx:
+    h = None
+
+    def __init__(self):
+        self.live = []
+
+    def buf(self, nbytes):
+        return FakeBuf(self, nbytes)
+
+    def put(self, arr):
+        arr = np.ascontiguousarray(arr)
+        return self.buf(max(arr.nbytes, 1)).upload(arr)
+
+    def sync(self):
+        L.check(L.lib().sync_rc(), "sync")
+
+
+class FakeLib:
+    """Calls succeed unless named in `refuse`; `seen` holds (name, len, new tokens or budget) of each."""
+
+    def __init__(self):
+        self.refuse, self.seen = set(), []
+
+    def _call(self, name, d):
+        n = np.ctypeslib.as_array(C.cast(d.len, C.POINTER(C.c_int)), (d.B,)).tolist()
+        self.seen.append((name, n))
+        return -1 if name in self.refuse else 0
+
+    def vx27_hip_paged_append(self, h, d):
+        return self._call("append", d._obj)
+
+    def vx27_hip_paged_attn(self, h, d):
+        return self._call("attn", d._obj)
+
+    def vx27_hip_paged_evict(self, h, d):
+        d = d._obj
+        rc = self._call("evict", d)
+        if rc == 0 and d.n_sink + d.n_recent > d.budget:
+            return -1
+        if rc == 0:
+            n, out = (C.cast(x, C.POINTER(C.c_int)) for x in (d.len, d.dst_len))
+            kept, acc, acc_out = (C.cast(x, C.POINTER(t)) for x, t in ((d.kept, C.c_int), (d.acc, C.c_float), (d.acc_out or d.acc, C.c_float)))
+            for b in range(d.B):
+                out[b] = min(n[b], d.budget)
+                for h_ in range(d.n_kv):
+                    s = b * d.n_kv + h_
+                    for i in range(out[b]):      # (which rows stay does not matter here: the last ones)
+                        r = n[b] - out[b] + i
+                        kept[s * d.budget + i] = r
+                        if d.acc_out:
+                            acc_out[s * d.acc_out_stride + i] = acc[s * d.acc_stride + r]
+        return rc
+
+    def vx27_hip_memset(self, h, p, byte, n):
+        C.memset(p, byte, n)
+        return 0
+
+    def vx27_hip_d2d(self, h, dst, src, n):
+        C.memmove(dst, src, n)
+        return 0
+
+    def sync_rc(self):
+        return -1 if "sync" in self.refuse else 0
+
+    def vx27_hip_last_error(self):
+        return b"refused"
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    f = FakeLib()
+    monkeypatch.setattr(L, "lib", lambda: f)
+    return f
+
+
+def layer(n_seq=2, n_pages=3, page=32, **kw):
+    return M.PagedGQALayer(FakeCtx(), n_seq, n_pages, page, np.zeros(HD), np.zeros(HD), **kw)
+
+
+def tokens(n, n_q=24, n_kv=4):
+    return np.zeros((n, n_q, 2 * HD), np.float32), np.zeros((n, n_kv, HD), np.float32), np.zeros((n, n_kv, HD), np.float32)
+
+
+def held(lay):
+    return [list(p) for p in lay.pages], list(lay.free), list(lay.rows), list(lay.pos)
+
+
+@pytest.mark.parametrize("refuse", [None, "append", "attn", "sync"])
+def test_a_refused_step_takes_no_pages(fake, refuse):
+    """The pool is too small for the second sequence, or the library refuses: no sequence holds a page more, and a step
+    that needs those pages runs."""
+    lay = layer()
+    lay.step([5, 0], *tokens(5))
+    before = held(lay)
+    if refuse:
+        fake.refuse = {refuse}
+    with pytest.raises(L.HipError):
+        lay.step([40, 40] if refuse is None else [40, 1], *tokens(80 if refuse is None else 41))
+    assert held(lay) == before
+    fake.refuse = set()
+    lay.step([0, 64], *tokens(64))
+    assert lay.rows == [5, 64] and lay.free == [] and sorted(sum(lay.pages, [])) == [0, 1, 2]

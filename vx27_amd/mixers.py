@@ -11,6 +11,7 @@ Two levels, both calling libvx27_hip (no host compute):
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -249,13 +250,26 @@ class PagedGQALayer:
         self.rows = [0] * n_seq          # cached rows
         self.pos = [0] * n_seq           # positions seen (rows that were evicted included)
 
-    def _grow(self, b, rows):
-        need = -(-rows // self.page)
-        if need > self.max_pages or need - len(self.pages[b]) > len(self.free):
-            raise L.HipError(f"paged cache: sequence {b} needs {need} pages ({len(self.pages[b])} held, "
-                             f"{len(self.free)} free, {self.max_pages} at most)")
-        while len(self.pages[b]) < need:
-            self.pages[b].append(self.free.pop())
+    @contextlib.contextmanager
+    def _grown(self, rows):
+        """Pages for `rows` rows of every sequence: all of them, or none where there are too few; given back if the
+        call within fails."""
+        need = [max(-(-n // self.page), len(p)) for n, p in zip(rows, self.pages)]
+        more = sum(need) - sum(map(len, self.pages))
+        if max(need) > self.max_pages or more > len(self.free):
+            raise L.HipError(f"paged cache: {more} more pages needed ({len(self.free)} free), {max(need)} for one "
+                             f"sequence ({self.max_pages} at most)")
+        before = [len(p) for p in self.pages], list(self.free)
+        for p, n in zip(self.pages, need):
+            while len(p) < n:
+                p.append(self.free.pop())
+        try:
+            yield
+        except BaseException:
+            for p, n in zip(self.pages, before[0]):
+                del p[n:]
+            self.free = before[1]
+            raise
 
     def _table(self, pages):
         t = np.zeros((self.n_seq, self.max_pages), np.int32)
@@ -267,12 +281,17 @@ class PagedGQALayer:
         """new [n_seq] tokens of each sequence; qg [N][n_q][2*hd] interleaved q|gate, k_new, v_new [N][n_kv][hd],
         the sequences' tokens one after the other.  weigh adds the rows' weights up.  Returns out [N][n_q][hd]
         (float32)."""
-        ctx, N, hd = self.ctx, int(np.sum(new)), self.hd
-        if N == 0:
-            return np.empty((0, self.n_q, hd), np.float32)
+        if int(np.sum(new)) == 0:
+            return np.empty((0, self.n_q, self.hd), np.float32)
         rows = [n + int(t) for n, t in zip(self.rows, new)]
-        for b, n in enumerate(rows):
-            self._grow(b, n)
+        with self._grown(rows):
+            out = self._step(new, rows, qg, k_new, v_new, weigh, out_dtype)
+        self.rows = rows
+        self.pos = [p + int(t) for p, t in zip(self.pos, new)]
+        return out
+
+    def _step(self, new, rows, qg, k_new, v_new, weigh, out_dtype):
+        ctx, N, hd = self.ctx, int(np.sum(new)), self.hd
         start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
         pos = np.concatenate([np.arange(p, p + t) for p, t in zip(self.pos, new)]).astype(np.int32)
         up = [ctx.put(x) for x in (_f32(qg), _f32(k_new), _f32(v_new), self._table(self.pages),
@@ -296,8 +315,6 @@ class PagedGQALayer:
         check(L.lib().vx27_hip_paged_append(ctx.h, C.byref(d)), "paged_append")
         check(L.lib().vx27_hip_paged_attn(ctx.h, C.byref(a)), "paged_attn")
         ctx.sync()
-        self.rows = rows
-        self.pos = [p + int(t) for p, t in zip(self.pos, new)]
         if out_dtype == L.BF16:
             res = (out.download((N, self.n_q, hd), np.uint16).astype(np.uint32) << 16).view(np.float32)
         else:
