@@ -140,3 +140,24 @@ def test_a_refused_step_takes_no_pages(fake, refuse):
     fake.refuse = set()
     lay.step([0, 64], *tokens(64))
     assert lay.rows == [5, 64] and lay.free == [] and sorted(sum(lay.pages, [])) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("refuse", ["arguments", "evict", "sync"])
+def test_a_refused_eviction_keeps_every_page(fake, refuse):
+    """The library refuses the call or the sync reports one: the fresh pages are free again, the rows and their weights
+    as they were, and the same eviction runs afterwards."""
+    lay = layer(2, 8, max_pages=4)
+    lay.step([70, 3], *tokens(73))
+    lay.acc.upload(np.arange(lay.acc.nbytes // 4, dtype=np.float32))
+    before, weights = held(lay), lay.acc.download((2, 4, lay.acc_stride), np.float32)
+    if refuse != "arguments":
+        fake.refuse = {refuse}
+    with pytest.raises(L.HipError):
+        lay.evict(40, 30 if refuse == "arguments" else 4, 20)
+    assert held(lay) == before
+    assert np.array_equal(lay.acc.download(weights.shape, np.float32), weights)
+    fake.refuse = set()
+    for _ in range(3):
+        lay.evict(40, 4, 20)
+    assert lay.rows == [40, 3] and len(lay.free) + sum(map(len, lay.pages)) == 8
+    assert sorted(lay.free + sum(lay.pages, [])) == list(range(8))

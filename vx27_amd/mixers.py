@@ -330,7 +330,8 @@ class PagedGQALayer:
         need = [-(-r // self.page) for r in n]
         if sum(need) > len(self.free):
             raise L.HipError(f"paged cache: eviction needs {sum(need)} fresh pages, {len(self.free)} are free")
-        fresh = [[self.free.pop() for _ in range(k)] for k in need]
+        left = list(self.free)           # (the free pages are these only once the call has run)
+        fresh = [[left.pop() for _ in range(k)] for k in need]
         width = max(1, min(self.max_pages, -(-budget // self.page)))
         dst = self._table(fresh)[:, :width]
         up = [ctx.put(x) for x in (self._table(self.pages), np.asarray(self.rows, np.int32), dst,
@@ -349,8 +350,7 @@ class PagedGQALayer:
         ctx.sync()
         kept = kb.download((self.n_seq, self.n_kv, budget), np.int32)
         self.rows = [int(x) for x in len2.download((self.n_seq,), np.int32)]
-        for p in self.pages:
-            self.free.extend(p)
+        self.free = left + [p for pages in self.pages for p in pages]
         self.pages = fresh
         if d.acc_out:
             self.acc.free()
