@@ -161,3 +161,19 @@ def test_a_refused_eviction_keeps_every_page(fake, refuse):
         lay.evict(40, 4, 20)
     assert lay.rows == [40, 3] and len(lay.free) + sum(map(len, lay.pages)) == 8
     assert sorted(lay.free + sum(lay.pages, [])) == list(range(8))
+
+
+@pytest.mark.parametrize("refuse", ["append", "attn", "evict", "sync"])
+def test_no_buffers_stay_behind(fake, refuse):
+    """A call that runs and a call that is refused leave no device buffer of their own."""
+    lay = layer(2, 8, max_pages=4)
+    lay.step([70, 3], *tokens(73), weigh=True)
+    live = len(lay.ctx.live)
+    fake.refuse = {refuse}
+    with pytest.raises(L.HipError):
+        lay.evict(40, 4, 20) if refuse == "evict" else lay.step([1, 1], *tokens(2))
+    assert len(lay.ctx.live) == live
+    fake.refuse = set()
+    lay.step([1, 1], *tokens(2))
+    lay.evict(40, 4, 20)
+    assert len(lay.ctx.live) == live

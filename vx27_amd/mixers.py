@@ -271,6 +271,16 @@ class PagedGQALayer:
             self.free = before[1]
             raise
 
+    @contextlib.contextmanager
+    def _buffers(self):
+        """buf and put of the context for the time of one call: freed at its end, whichever it is."""
+        with contextlib.ExitStack() as stack:
+            def buf(nbytes):
+                b = self.ctx.buf(nbytes)
+                stack.callback(b.free)
+                return b
+            yield buf, lambda arr: buf(max(arr.nbytes, 1)).upload(arr)
+
     def _table(self, pages):
         t = np.zeros((self.n_seq, self.max_pages), np.int32)
         for b, p in enumerate(pages):
@@ -284,20 +294,19 @@ class PagedGQALayer:
         if int(np.sum(new)) == 0:
             return np.empty((0, self.n_q, self.hd), np.float32)
         rows = [n + int(t) for n, t in zip(self.rows, new)]
-        with self._grown(rows):
-            out = self._step(new, rows, qg, k_new, v_new, weigh, out_dtype)
+        with self._grown(rows), self._buffers() as (buf, put):
+            out = self._step(buf, put, new, rows, qg, k_new, v_new, weigh, out_dtype)
         self.rows = rows
         self.pos = [p + int(t) for p, t in zip(self.pos, new)]
         return out
 
-    def _step(self, new, rows, qg, k_new, v_new, weigh, out_dtype):
+    def _step(self, buf, put, new, rows, qg, k_new, v_new, weigh, out_dtype):
         ctx, N, hd = self.ctx, int(np.sum(new)), self.hd
         start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
         pos = np.concatenate([np.arange(p, p + t) for p, t in zip(self.pos, new)]).astype(np.int32)
-        up = [ctx.put(x) for x in (_f32(qg), _f32(k_new), _f32(v_new), self._table(self.pages),
-                                   np.asarray(rows, np.int32), start, pos)]
-        qb, kb, vb, tb, lb, sb, pb = up
-        rot, out = ctx.buf(N * self.n_q * hd * 2), ctx.buf(N * self.n_q * hd * 4)
+        qb, kb, vb, tb, lb, sb, pb = (put(x) for x in (_f32(qg), _f32(k_new), _f32(v_new), self._table(self.pages),
+                                                       np.asarray(rows, np.int32), start, pos))
+        rot, out = buf(N * self.n_q * hd * 2), buf(N * self.n_q * hd * 4)
         d = L.PagedAppendDesc()
         a = L.PagedAttnDesc()
         for x in (d, a):
@@ -316,16 +325,16 @@ class PagedGQALayer:
         check(L.lib().vx27_hip_paged_attn(ctx.h, C.byref(a)), "paged_attn")
         ctx.sync()
         if out_dtype == L.BF16:
-            res = (out.download((N, self.n_q, hd), np.uint16).astype(np.uint32) << 16).view(np.float32)
-        else:
-            res = out.download((N, self.n_q, hd), np.float32)
-        for x in up + [rot, out]:
-            x.free()
-        return res
+            return (out.download((N, self.n_q, hd), np.uint16).astype(np.uint32) << 16).view(np.float32)
+        return out.download((N, self.n_q, hd), np.float32)
 
     def evict(self, budget, n_sink, n_recent):
         """Every sequence past `budget` rows keeps that many.  Returns kept [n_seq][n_kv][budget], the old rows
         (-1 behind a sequence's last)."""
+        with self._buffers() as (buf, put):
+            return self._evict(buf, put, budget, n_sink, n_recent)
+
+    def _evict(self, buf, put, budget, n_sink, n_recent):
         ctx, n = self.ctx, [min(r, budget) for r in self.rows]
         need = [-(-r // self.page) for r in n]
         if sum(need) > len(self.free):
@@ -334,10 +343,9 @@ class PagedGQALayer:
         fresh = [[left.pop() for _ in range(k)] for k in need]
         width = max(1, min(self.max_pages, -(-budget // self.page)))
         dst = self._table(fresh)[:, :width]
-        up = [ctx.put(x) for x in (self._table(self.pages), np.asarray(self.rows, np.int32), dst,
-                                   np.full((self.n_seq, self.n_kv, budget), -1, np.int32))]
-        tb, lb, db, kb = up
-        acc2, len2 = ctx.buf(self.acc.nbytes).zero(), ctx.buf(self.n_seq * 4)
+        tb, lb, db, kb = (put(x) for x in (self._table(self.pages), np.asarray(self.rows, np.int32), dst,
+                                           np.full((self.n_seq, self.n_kv, budget), -1, np.int32)))
+        acc2, len2 = buf(self.acc.nbytes).zero(), buf(self.n_seq * 4)
         d = L.PagedEvictDesc()
         d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = self.n_seq, self.n_kv, self.hd, self.page, self.n_pages, self.max_pages
         d.table, d.len, d.budget, d.n_sink, d.n_recent = tb.ptr, lb.ptr, budget, n_sink, n_recent
@@ -349,16 +357,12 @@ class PagedGQALayer:
         check(L.lib().vx27_hip_paged_evict(ctx.h, C.byref(d)), "paged_evict")
         ctx.sync()
         kept = kb.download((self.n_seq, self.n_kv, budget), np.int32)
-        self.rows = [int(x) for x in len2.download((self.n_seq,), np.int32)]
+        n = [int(x) for x in len2.download((self.n_seq,), np.int32)]
+        if d.acc_out:
+            check(L.lib().vx27_hip_d2d(ctx.h, self.acc.ptr, acc2.ptr, self.acc.nbytes), "d2d")
+        self.rows = n
         self.free = left + [p for pages in self.pages for p in pages]
         self.pages = fresh
-        if d.acc_out:
-            self.acc.free()
-            self.acc = acc2
-        else:
-            acc2.free()
-        for x in up + [len2]:
-            x.free()
         return kept
 
     def read_rows(self, b):
