@@ -177,3 +177,32 @@ def test_no_buffers_stay_behind(fake, refuse):
     lay.step([1, 1], *tokens(2))
     lay.evict(40, 4, 20)
     assert len(lay.ctx.live) == live
+
+
+def test_eviction_touches_only_sequences_past_the_budget(fake):
+    """In a pool with two free pages one long sequence is brought back to its budget: the others keep their pages, rows
+    and weights, and where none is past the budget nothing is needed."""
+    lay = layer(3, 9, max_pages=6)
+    lay.step([64, 100, 20], *tokens(184), weigh=True)
+    assert len(lay.free) == 2
+    pages = [list(p) for p in lay.pages]
+    w = np.random.default_rng(1).random((3, 4, lay.acc_stride)).astype(np.float32)
+    lay.acc.upload(w)
+    kept = lay.evict(64, 4, 60)
+    assert fake.seen[-1] == ("evict", [0, 100, 0])
+    assert lay.rows == [64, 64, 20] and lay.pages[0] == pages[0] and lay.pages[2] == pages[2]
+    assert sorted(lay.free + sum(lay.pages, [])) == list(range(9)) and len(lay.free) == 4
+    for b, n, old in ((0, 64, range(64)), (1, 64, range(36, 100)), (2, 20, range(20))):
+        assert np.array_equal(kept[b], np.broadcast_to(list(old) + [-1] * (64 - n), (4, 64)))
+    want = w.copy()
+    want[1] = 0
+    want[1, :, :64] = w[1, :, 36:100]
+    assert np.array_equal(lay.acc.download(w.shape, np.float32), want)
+    before = held(lay)
+    lay.free = []
+    kept = lay.evict(64, 4, 60)
+    assert (lay.pages, lay.rows, lay.pos) == (before[0], before[2], before[3])
+    assert np.array_equal(kept[2, 0], list(range(20)) + [-1] * 44)
+    assert np.array_equal(lay.acc.download(w.shape, np.float32), want)
+    with pytest.raises(L.HipError):
+        lay.evict(64, 60, 60)          # refused whatever the rows

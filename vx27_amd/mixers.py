@@ -329,40 +329,44 @@ class PagedGQALayer:
         return out.download((N, self.n_q, hd), np.float32)
 
     def evict(self, budget, n_sink, n_recent):
-        """Every sequence past `budget` rows keeps that many.  Returns kept [n_seq][n_kv][budget], the old rows
-        (-1 behind a sequence's last)."""
+        """Every sequence past `budget` rows keeps that many, in fresh pages; the others stay as they are.  Returns kept
+        [n_seq][n_kv][budget], the old rows (-1 behind a sequence's last)."""
         with self._buffers() as (buf, put):
             return self._evict(buf, put, budget, n_sink, n_recent)
 
     def _evict(self, buf, put, budget, n_sink, n_recent):
-        ctx, n = self.ctx, [min(r, budget) for r in self.rows]
-        need = [-(-r // self.page) for r in n]
+        ctx, past = self.ctx, [n > budget for n in self.rows]
+        need = [-(-budget // self.page) if p else 0 for p in past]
         if sum(need) > len(self.free):
             raise L.HipError(f"paged cache: eviction needs {sum(need)} fresh pages, {len(self.free)} are free")
         left = list(self.free)           # (the free pages are these only once the call has run)
         fresh = [[left.pop() for _ in range(k)] for k in need]
         width = max(1, min(self.max_pages, -(-budget // self.page)))
         dst = self._table(fresh)[:, :width]
-        tb, lb, db, kb = (put(x) for x in (self._table(self.pages), np.asarray(self.rows, np.int32), dst,
+        # sequences within the budget take part with no rows
+        tb, lb, db, kb = (put(x) for x in (self._table(self.pages), np.where(past, self.rows, 0).astype(np.int32), dst,
                                            np.full((self.n_seq, self.n_kv, budget), -1, np.int32)))
-        acc2, len2 = buf(self.acc.nbytes).zero(), buf(self.n_seq * 4)
+        len2 = buf(self.n_seq * 4)
         d = L.PagedEvictDesc()
         d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = self.n_seq, self.n_kv, self.hd, self.page, self.n_pages, self.max_pages
         d.table, d.len, d.budget, d.n_sink, d.n_recent = tb.ptr, lb.ptr, budget, n_sink, n_recent
         d.acc, d.acc_stride, d.k_pages, d.v_pages = self.acc.ptr, self.acc_stride, self.k_pages.ptr, self.v_pages.ptr
         d.dst_table, d.dst_max_pages, d.dst_len, d.kept = db.ptr, width, len2.ptr, kb.ptr
-        d.acc_out, d.acc_out_stride = acc2.ptr, max(self.acc_stride, budget)
-        if budget > self.acc_stride:     # nothing can be past the budget: the weights stay where they are
-            d.acc_out = None
+        if any(past):                    # (then the budget is below acc_stride)
+            acc2 = buf(self.acc.nbytes).zero()
+            d.acc_out, d.acc_out_stride = acc2.ptr, self.acc_stride
         check(L.lib().vx27_hip_paged_evict(ctx.h, C.byref(d)), "paged_evict")
         ctx.sync()
         kept = kb.download((self.n_seq, self.n_kv, budget), np.int32)
-        n = [int(x) for x in len2.download((self.n_seq,), np.int32)]
-        if d.acc_out:
-            check(L.lib().vx27_hip_d2d(ctx.h, self.acc.ptr, acc2.ptr, self.acc.nbytes), "d2d")
-        self.rows = n
-        self.free = left + [p for pages in self.pages for p in pages]
-        self.pages = fresh
+        each = self.n_kv * self.acc_stride * 4
+        for b, p in enumerate(past):
+            if p:
+                check(L.lib().vx27_hip_d2d(ctx.h, self.acc.ptr + b * each, acc2.ptr + b * each, each), "d2d")
+                left += self.pages[b]
+                self.pages[b], self.rows[b] = fresh[b], budget
+            else:
+                kept[b, :, :self.rows[b]] = np.arange(self.rows[b])
+        self.free = left
         return kept
 
     def read_rows(self, b):
