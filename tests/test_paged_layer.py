@@ -206,3 +206,27 @@ def test_eviction_touches_only_sequences_past_the_budget(fake):
     assert np.array_equal(lay.acc.download(w.shape, np.float32), want)
     with pytest.raises(L.HipError):
         lay.evict(64, 60, 60)          # refused whatever the rows
+
+
+def test_an_ended_sequence_gives_everything_back(fake):
+    """end() returns a sequence's pages and clears its rows, position and weights, so that another conversation may take
+    its place."""
+    lay = layer(2, 4)
+    lay.step([70, 30], *tokens(100), weigh=True)
+    lay.acc.upload(np.ones(lay.acc.nbytes // 4, np.float32))
+    with pytest.raises(L.HipError):
+        lay.step([0, 40], *tokens(40))
+    lay.end(0)
+    assert lay.rows == [0, 30] and lay.pos == [0, 30] and lay.pages[0] == []
+    acc = lay.acc.download((2, 4 * lay.acc_stride), np.float32)
+    assert not acc[0].any() and acc[1].all()
+    lay.step([1, 90], *tokens(91))
+    assert lay.rows == [1, 120] and lay.pos == [1, 120]
+    with pytest.raises(L.HipError):
+        lay.step([40, 0], *tokens(40))     # the pool is full again
+    lay.end(0)
+    lay.end(0)
+    assert sorted(lay.free + sum(lay.pages, [])) == list(range(4))
+    for b in (-1, 2):
+        with pytest.raises(L.HipError, match="sequence"):
+            lay.end(b)

@@ -230,7 +230,8 @@ class PagedGQALayer:
     attention weight once a step asked for it.
 
     step() appends the sequences' new tokens and attends from them; evict()
-    brings sequences past a budget back to it.
+    brings sequences past a budget back to it; end() frees a sequence's place
+    for another.
     """
 
     def __init__(self, ctx, n_seq, n_pages, page_size, q_norm_w, k_norm_w, n_q=24, n_kv=4, hd=256, rope_dim=64,
@@ -368,6 +369,15 @@ class PagedGQALayer:
                 kept[b, :, :self.rows[b]] = np.arange(self.rows[b])
         self.free = left
         return kept
+
+    def end(self, b):
+        """Sequence b ends: its pages are free, and its place, rows, position and weights as at the start."""
+        if not 0 <= b < self.n_seq:
+            raise L.HipError(f"paged cache: no sequence {b} (n_seq {self.n_seq})")
+        each = self.n_kv * self.acc_stride * 4
+        check(L.lib().vx27_hip_memset(self.ctx.h, self.acc.ptr + b * each, 0, each), "memset")
+        self.free += self.pages[b]
+        self.pages[b], self.rows[b], self.pos[b] = [], 0, 0
 
     def read_rows(self, b):
         """The cached rows of sequence b: K and V [rows][n_kv][hd] as float32."""
