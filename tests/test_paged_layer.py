@@ -220,8 +220,8 @@ def test_an_ended_sequence_gives_everything_back(fake):
     assert lay.rows == [0, 30] and lay.pos == [0, 30] and lay.pages[0] == []
     acc = lay.acc.download((2, 4 * lay.acc_stride), np.float32)
     assert not acc[0].any() and acc[1].all()
-    lay.step([1, 90], *tokens(91))
-    assert lay.rows == [1, 120] and lay.pos == [1, 120]
+    lay.step([1, 60], *tokens(61))
+    assert lay.rows == [1, 90] and lay.pos == [1, 90]
     with pytest.raises(L.HipError):
         lay.step([40, 0], *tokens(40))     # the pool is full again
     lay.end(0)
