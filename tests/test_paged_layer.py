@@ -230,3 +230,26 @@ def test_an_ended_sequence_gives_everything_back(fake):
     for b in (-1, 2):
         with pytest.raises(L.HipError, match="sequence"):
             lay.end(b)
+
+
+@pytest.mark.parametrize("new,n,what", [
+    ([3], 3, "new"), ([1, 1, 1], 3, "new"), ([3, -1], 2, "new"), ([2, 1], 2, "qg"), ([2, 1], (3, 2, 3), "k_new"),
+    ([2, 1], (3, 3, 2), "v_new")])
+def test_arguments_that_hold_too_little_are_refused(fake, new, n, what):
+    """The calls read sum(new) tokens of each array: an array that holds fewer, or counts that are not one a sequence, do
+    not reach the library."""
+    lay = layer(2, 4)
+    n = (n, n, n) if isinstance(n, int) else n
+    args = [tokens(k)[i] for i, k in enumerate(n)]
+    before = held(lay)
+    with pytest.raises(L.HipError, match=what):
+        lay.step(new, *args)
+    assert fake.seen == [] and held(lay) == before
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_short_norm_weights_are_refused(fake, which):
+    w = [np.zeros(HD), np.zeros(HD)]
+    w[which] = np.zeros(HD - 1)
+    with pytest.raises(L.HipError, match="norm_w"):
+        M.PagedGQALayer(FakeCtx(), 1, 1, 32, *w)

@@ -240,6 +240,8 @@ class PagedGQALayer:
         self.n_q, self.n_kv, self.hd, self.rope_dim, self.theta, self.yarn = n_q, n_kv, hd, rope_dim, theta, yarn
         self.flags, self.window, self.n_sink = flags, window, n_sink
         self.max_pages = max_pages or n_pages
+        if np.size(q_norm_w) < hd or np.size(k_norm_w) < hd:
+            raise L.HipError(f"paged cache: q_norm_w and k_norm_w need {hd} numbers (got {np.size(q_norm_w)}, {np.size(k_norm_w)})")
         n = n_pages * n_kv * page_size * hd
         self.k_pages = ctx.buf(n * 2).zero()
         self.v_pages = ctx.buf(n * 2).zero()
@@ -292,7 +294,13 @@ class PagedGQALayer:
         """new [n_seq] tokens of each sequence; qg [N][n_q][2*hd] interleaved q|gate, k_new, v_new [N][n_kv][hd],
         the sequences' tokens one after the other.  weigh adds the rows' weights up.  Returns out [N][n_q][hd]
         (float32)."""
-        if int(np.sum(new)) == 0:
+        N = int(np.sum(new))
+        if len(new) != self.n_seq or min(new) < 0:
+            raise L.HipError(f"paged cache: new must hold a count for each of {self.n_seq} sequences (got {list(new)})")
+        for name, x, each in (("qg", qg, self.n_q * 2), ("k_new", k_new, self.n_kv), ("v_new", v_new, self.n_kv)):
+            if np.size(x) < N * each * self.hd:
+                raise L.HipError(f"paged cache: {name} holds {np.size(x)} numbers, {N} tokens need {N * each * self.hd}")
+        if N == 0:
             return np.empty((0, self.n_q, self.hd), np.float32)
         rows = [n + int(t) for n, t in zip(self.rows, new)]
         with self._grown(rows), self._buffers() as (buf, put):
