@@ -349,7 +349,8 @@ int vx27_hip_kv_read(vx27_hip_ctx *ctx, const uint16_t *k_cache, const uint16_t 
  * element (token, head, i) at q[token*q_tok_stride + head*q_head_stride + i]
  * and k_new[token*kv_tok_stride + head*hd + i]; 0 strides = dense.  All three
  * 16-byte aligned (bf16: 8) with strides multiples of 4 elements; q_norm_w,
- * k_norm_w and q_out 16-byte aligned.  With q NULL only k and v are written. */
+ * k_norm_w and q_out 16-byte aligned.  With q NULL only k and v are written.
+ * n_q/n_kv at most 4096, max_T at most 2^26. */
 typedef struct {
     int B, n_q, n_kv, hd;
     int rope_dim;               /* even, 0 = no rotation */

@@ -107,3 +107,35 @@ def test_index_arithmetic(tmp_path):
     assert r.returncode == 0, r.stderr
     out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"n_q": 4097 * 4}, "k <= 4096"), ({"n_q": 32768 * 4}, "k <= 4096"),
+    ({"n_tok": 2 ** 31 - 1, "max_T": 2 ** 26 + 1}, "2^26"), ({"n_tok": 2 ** 31 - 1, "max_T": 2 ** 31 - 1}, "2^26")])
+def test_append_limits(change, message):
+    """Row / group as a high product is exact for 8 tokens of up to 4096 heads (test_group_of_a_row), and a launch holds
+    2^32 threads a dimension."""
+    from vx27_amd import lib as L
+    d = _append()
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert L.lib().vx27_hip_paged_append(None, C.byref(d)) == -1
+    assert message in L.lib().vx27_hip_last_error().decode()
+
+
+def test_group_of_a_row():
+    """The kernels' row / group: high 32 bits of row * (floor(2^32 / group) + 1)."""
+    def div(r, g):
+        return r * (2 ** 32 // g + 1) >> 32
+    for g in [*range(2, 300), 1000, 2047, 2048, 4095, 4096]:
+        for t in (0, 1, 3, 7):                        # a workgroup of the append: 8 tokens
+            assert div(t * g, g) == t and div(t * g + g - 1, g) == t
+    for g in range(2, 17):                            # the attention: rows below 2^28
+        for t in [*range(100), *((1 << 28) // g - k for k in range(1, 100))]:
+            assert div(t * g, g) == t and div(t * g + g - 1, g) == t
+    assert div(8 * 32768 - 1, 32768) == 8             # past the limit the last row would be read as a ninth token's
+
+
+def test_launch_of_a_limit():
+    """The append's grid at its largest max_T: below 2^32 threads, 256 a workgroup."""
+    assert ((2 ** 26 + 30) // 32 + 1) * 5 * 256 < 2 ** 32

@@ -242,7 +242,11 @@ extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_
     if (vx_paged_fill(who, a.p, d->B, d->n_kv, d->hd, d->page_size, d->n_pages, d->max_pages, d->table, d->len)) return -1;
     if (vx_paged_tokens(who, a.p, d->q_start, d->n_tok, d->max_T)) return -1;
     VX_REQUIRE(d->in_dtype == VX27_F32 || d->in_dtype == VX27_BF16, "%s: in_dtype must be VX27_F32 or VX27_BF16 (got %d)", who, d->in_dtype);
-    VX_REQUIRE(!d->q || (d->n_q >= d->n_kv && d->n_q % d->n_kv == 0), "%s: need n_q = k*n_kv (n_q=%d n_kv=%d)", who, d->n_q, d->n_kv);
+    // (a row's token by a high product: exact where 8 tokens' rows times the group stay below 2^32)
+    VX_REQUIRE(!d->q || (d->n_q >= d->n_kv && d->n_q % d->n_kv == 0 && d->n_q / d->n_kv <= 4096),
+               "%s: need n_q = k*n_kv with k <= 4096 (n_q=%d n_kv=%d)", who, d->n_q, d->n_kv);
+    // (five workgroups of 256 a 32-row block: a launch holds 2^32 threads a dimension)
+    VX_REQUIRE(d->max_T <= (1 << 26), "%s: max_T is past 2^26 (got %d)", who, d->max_T);
     VX_REQUIRE(d->k_new && d->v_new && d->k_norm_w && d->k_pages && d->v_pages && (!d->q || (d->q_norm_w && d->q_out)),
                "%s: null pointer in descriptor", who);
     if (d->rope_dim != 0) {
