@@ -138,14 +138,16 @@ __device__ __forceinline__ void attend_tile(Rows &w, int R, bool one, const floa
     }
     mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
     const float m_new = fmaxf(w.m, mt * SC2);
     const bool none = m_new == -INFINITY;
+    const float ref = none ? 0.0f : m_new;
     const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(w.m - m_new);
     bf16x8_t p[NP];
     float ls = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        float pe = none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -m_new));
+        float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -ref));
         ls += pe;
 #pragma unroll
         for (int k = 0; k < NP; k++) {
@@ -477,12 +479,12 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
             if (w0 + 4 * k > g1) ml[k].x = -INFINITY;
             mn = fmaxf(mn, ml[k].x);
         }
-        if (mn == -INFINITY) continue;
-        const float sa = __builtin_amdgcn_exp2f(M - mn);
+        const float ref = mn == -INFINITY ? 0.0f : mn;   // (parts of NaN scores alone stay NaN)
+        const float sa = __builtin_amdgcn_exp2f(M - ref);
         L *= sa;
         O.x *= sa; O.y *= sa; O.z *= sa; O.w *= sa;
 #pragma unroll
-        for (int k = 0; k < NP; k++) add_part(O, L, o[k], ml[k].y, __builtin_amdgcn_exp2f(ml[k].x - mn));
+        for (int k = 0; k < NP; k++) add_part(O, L, o[k], ml[k].y, __builtin_amdgcn_exp2f(ml[k].x - ref));
         M = mn;
     }
     s_o[wave][lane] = O;
