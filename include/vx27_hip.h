@@ -377,10 +377,11 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * the append): token at row i sees row j <= i if j > i - window (window 0: no
  * limit) or j < n_sink (sinks);
  *   out = (sum_j softmax_j(q.k_j / sqrt(hd)) v_j) * sigmoid(gate),
- * query head h reading KV head h / (n_q/n_kv).  A token that sees nothing
- * gets 0.  q is bf16, normed and rotated (q_out of the append).  Products on
- * bf16 MFMA, sums and softmax statistics in fp32.  One or two tokens a
- * sequence (at most 16 query rows a KV head) run the decode kernels: the
+ * query head h reading KV head h / (n_q/n_kv).  A token that sees nothing, or
+ * only scores of -inf, gets 0 (and lse -inf, and adds no weight).  q is bf16,
+ * normed and rotated (q_out of the append).  Products on bf16 MFMA, sums and
+ * softmax statistics in fp32.  One or two tokens a sequence (at most 16 query
+ * rows a KV head) run the decode kernels: the
  * cache's length split evenly over the device and joined, the softmax
  * weights as three bf16 parts (fp32 accuracy; out fp32 or bf16).  More tokens
  * run the tile kernel, whose weights are rounded to bf16 once (relative
@@ -389,8 +390,9 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * (-inf for a token that sees nothing); acc [B][n_kv][acc_stride], to which
  * each row's weight over the call's tokens and the group's heads is added
  * (rows nobody sees and rows from len on are left as they were).
- * An infinite or NaN value of a row reaches only the tokens that see the row,
- * whose outputs are then not finite (an infinity may end as NaN).
+ * A NaN key, a score of +inf and an infinite or NaN value reach only the
+ * tokens that see the row, whose outputs are then not finite (an infinity may
+ * end as NaN); a score of -inf weighs nothing.
  * out must not overlap an input.  Context scratch: the parts of cut rows
  * (at most about 100 MB), and with acc and at most 16 query rows a KV head their
  * scores, B*n_kv*rows*4 bytes for each row that a sequence can see at most

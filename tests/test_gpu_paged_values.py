@@ -8,7 +8,7 @@ from test_gpu_paged import Attn, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
-NAN = 0x7FC1
+NAN, MINUS_INF = 0x7FC1, 0xFF80
 
 
 @pytest.mark.parametrize("lens,new,window,sink,rows", [
@@ -49,4 +49,38 @@ def test_nan_keys_reach_the_tokens_that_see_them(ctx, lens, new, window, sink, r
     assert np.isnan(out[hit]).all() and np.isnan(lse[hit]).all()
     assert np.all(np.abs(out[~hit] - ref["out"][~hit]) <= tol[~hit])
     assert not np.isnan(lse[~hit]).any()
+    at.free()
+
+
+@pytest.mark.parametrize("lens,new,rows", [
+    ([1, 40], [1, 1], 1), ([2, 40], [2, 2], 2), ([2, 40], [2, 2], 1),
+    ([300, 40], [1, 1], 300), ([3, 70], [3, 9], 3), ([60, 70], [60, 9], 40)])
+def test_scores_of_minus_infinity(ctx, lens, new, rows):  # noqa: F811
+    """Keys whose scores are -inf weigh nothing; a token that sees no others gets 0, lse -inf, and adds nothing."""
+    say(f"-inf scores {lens} {new} rows {rows}")
+    bt = Batch(lens, new, 24, 4, 64, seed=520 + rows)
+    bt.q[..., 0] = np.where(bt.q[..., 0] & 0x7FFF, bt.q[..., 0] & 0x7FFF, 0x3F80)      # q_0 > 0
+    seen = bt.seen(0)
+    none = bt.start[0] + np.nonzero(~seen[:, rows:].any(1))[0]                           # tokens without a finite score
+    assert len(none)
+    for j in range(rows):
+        p, at = bt.table[0, j // 64], j % 64
+        bt.k[p, :, at] = 0
+        bt.k[p, :, at, 0] = MINUS_INF
+    at = Attn(ctx, bt, gate="none", acc=True)
+    at.call()
+    ctx.sync()
+    out, lse = at.out(), at.bufs["lse"].download((bt.N, 24), np.float32)
+    acc = at.bufs["acc"].download((bt.B, 4, at.stride), np.float32).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        ref = bt.result(False)      # (its weights of these rows are exp(-inf - m) = 0)
+    assert not out[none].any() and np.all(lse[none] == -np.inf)
+    # (score magnitudes of the finite ones: sums of 256 products of std 2 and 1 over 16, 20.4 on average, below 64)
+    S = np.where(np.isfinite(ref["S"]), ref["S"], 0).max()
+    rel = 2 * 256 * 2.0 ** -24 * max(S, 64.0) + 2.0 ** -20 + 3 * max(lens) * 2.0 ** -24 + 2.0 ** -8
+    some = np.setdiff1d(np.arange(bt.N), none)
+    assert np.all(np.abs(out[some] - ref["out"][some]) <= 1.01 * rel * ref["W"][some] + 1e-30)
+    for b, n in enumerate(lens):
+        base, w = at.acc0[b, :, :n].astype(np.float64), ref["acc"][b]
+        assert np.all(np.abs(acc[b, :, :n] - base - w) <= 2 * rel * w + 2.0 ** -23 * (base + w)), b
     at.free()

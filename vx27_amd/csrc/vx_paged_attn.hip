@@ -209,7 +209,8 @@ __device__ __forceinline__ void attend_tile(Rows &w, int R, bool one, const floa
 __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float m, float L) {
     const size_t at = (size_t)tok * a.n_q + h;
     if (a.lse) a.lse[at] = L > 0.0f || L != L ? (m + log2f(L)) * 0.6931471805599453f : -INFINITY;
-    if (a.stat) a.stat[at] = make_float2(m, L > 0.0f || L != L ? 1.0f / L : 0.0f);
+    // (a row that weighs nothing: from 0, so that scores of -inf become weights of 0 and not NaN)
+    if (a.stat) a.stat[at] = L > 0.0f || L != L ? make_float2(m, 1.0f / L) : make_float2(0.0f, 0.0f);
 }
 
 // hardware round-to-nearest-even pack (v_cvt_pk_bf16_f32)
