@@ -392,7 +392,9 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * (rows nobody sees and rows from len on are left as they were).
  * A NaN key, a score of +inf and an infinite or NaN value reach only the
  * tokens that see the row, whose outputs are then not finite (an infinity may
- * end as NaN); a score of -inf weighs nothing.
+ * end as NaN); a score of -inf weighs nothing.  Weights are at most 1 before
+ * the division by their sum: nothing overflows while the largest |v| times the
+ * number of rows seen stays below 2^127.
  * out must not overlap an input.  Context scratch: the parts of cut rows
  * (at most about 100 MB), and with acc and at most 16 query rows a KV head their
  * scores, B*n_kv*rows*4 bytes for each row that a sequence can see at most

@@ -84,3 +84,25 @@ def test_scores_of_minus_infinity(ctx, lens, new, rows):  # noqa: F811
         base, w = at.acc0[b, :, :n].astype(np.float64), ref["acc"][b]
         assert np.all(np.abs(acc[b, :, :n] - base - w) <= 2 * rel * w + 2.0 ** -23 * (base + w)), b
     at.free()
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 60])
+@pytest.mark.parametrize("power", [60, 100])
+def test_large_values_and_rising_scores(ctx, T, power):  # noqa: F811
+    """Values of 2^60 and 2^100 where the scores rise by 30 past those of the first keys: sums stay finite."""
+    from vx27_amd import workloads as W
+    say(f"values 2^{power} T={T}")
+    bt = Batch([400, 130], [T, T], 24, 4, 64, seed=540 + T)
+    q = np.zeros((bt.N, 24, HD), np.float32)
+    q[..., 0] = 16.0
+    bt.q = W.bf16_bits(q)
+    for b, n in enumerate(bt.lens):
+        for j in range(n):
+            k = np.zeros((4, HD), np.float32)
+            k[:, 0] = 0.0 if j < 64 else 30.0 + (j % 3) / 4     # (the scores: q.k / 16)
+            v = W.normal(bt.r, (4, HD)) * np.float32(2.0 ** power)
+            bt.put_row(b, j, W.bf16_bits(k), W.bf16_bits(v))
+    at = Attn(ctx, bt, gate="none", acc=T == 60)
+    at.call()
+    at.check(f"values 2^{power} T={T}")
+    at.free()

@@ -206,11 +206,15 @@ __device__ __forceinline__ void attend_tile(Rows &w, int R, bool one, const floa
         for (int d = 0; d < 16; d++) w.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[d], p[k], w.o[d], 0, 0, 0);
 }
 
+// A row's lse, and its reference and 1 / sum for the weights' pass.  SHIFT: the
+// reference lies that far above a maximum; the weights' pass takes the maximum
+// (the difference is exact), so that its arguments are small.
+template <int SHIFT>
 __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float m, float L) {
     const size_t at = (size_t)tok * a.n_q + h;
     if (a.lse) a.lse[at] = L > 0.0f || L != L ? (m + log2f(L)) * 0.6931471805599453f : -INFINITY;
     // (a row that weighs nothing: from 0, so that scores of -inf become weights of 0 and not NaN)
-    if (a.stat) a.stat[at] = L > 0.0f || L != L ? make_float2(m, 1.0f / L) : make_float2(0.0f, 0.0f);
+    if (a.stat) a.stat[at] = L > 0.0f || L != L ? make_float2(m - SHIFT, 1.0f / (1 << SHIFT) / L) : make_float2(0.0f, 0.0f);
 }
 
 // hardware round-to-nearest-even pack (v_cvt_pk_bf16_f32)
@@ -251,7 +255,7 @@ __device__ __forceinline__ void row_finish(const Args &a, int tok, int h, float4
         r.x *= sg(x.x); r.y *= sg(x.y); r.z *= sg(x.z); r.w *= sg(x.w);
     }
     row_write(a, tok, h, r);
-    if ((threadIdx.x & 63) == 0) stat_store(a, tok, h, M, L);
+    if ((threadIdx.x & 63) == 0) stat_store<0>(a, tok, h, M, L);
 }
 __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l, float w) {
     L += l * w;
@@ -555,10 +559,13 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 constexpr int TR = 128;                      // query rows of a workgroup
 constexpr int HALF = TILE * HDG * 2;         // bytes of one key block of K or of V
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
-// A row's reference is its first block's maximum and moves once a later one is
-// past it by 2^48: weights, sums and O then stay below 2^80, and a rescale of
-// O (400 instructions a wave) hardly ever runs.
-constexpr float LAZY = 48.0f;
+// A row's reference lies 2^16 above its first block's maximum and moves once a
+// later one is past it: weights then start at 2^-16 and stay below 1, so that
+// sums and O are bounded as without a reference that stays behind (rows times
+// |v|), and a rescale of O (400 instructions a wave) hardly ever runs.  (2^8
+// takes the windowed prompt from 298 to 326 us: of a first step of sinks and
+// the window's edge a row sees few keys.)
+constexpr int LAZY = 16;
 
 struct TileSmem {
     char k[2][2 * HALF], v[2][2 * HALF];     // [buffer][key block]
@@ -932,7 +939,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
         float ms;
         auto refer = [&](float x, bool some) {
             x = fmaxf(x, __uint_as_float(vx_xor32_u32(__float_as_uint(x)))) * SC2;
-            const bool up = x > m + LAZY;
+            const bool up = x > m;
+            x += LAZY;
             if (some && __any(up)) {
                 const float al = up ? __builtin_amdgcn_exp2f(m - x) : 1.0f;
                 l *= al;
@@ -1076,7 +1084,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 a.part_ml[slot0 + r] = make_float2(m, l);
             } else {
                 const int t = row_tok(a, r0 + r);
-                stat_store(a, s.start + t, row_head(a, kvh, r0 + r, t), m, l);
+                stat_store<LAZY>(a, s.start + t, row_head(a, kvh, r0 + r, t), m, l);
             }
         }
     }
@@ -1203,7 +1211,7 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
         if (jn.r0 + q0 + q >= R) break;
         const float il = L[q] > 0.0f || L[q] != L[q] ? 1.0f / L[q] : 0.0f;
         row_store(a, tok[q], h[q], make_float4(O[q].x * il, O[q].y * il, O[q].z * il, O[q].w * il), gt[q]);
-        if (lane == 0) stat_store(a, tok[q], h[q], M[q], L[q]);
+        if (lane == 0) stat_store<LAZY>(a, tok[q], h[q], M[q], L[q]);
     }
     }
 }
