@@ -1,4 +1,6 @@
 """The paged-cache operators where values and sizes are extreme."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -106,3 +108,33 @@ def test_large_values_and_rising_scores(ctx, T, power):  # noqa: F811
     at.call()
     at.check(f"values 2^{power} T={T}")
     at.free()
+
+
+def test_eviction_of_the_largest_capacity():
+    """A capacity of 2^30 rows and a budget next to it: the short sequence is moved, whatever its capacity's launch would
+    be."""
+    from vx27_amd import lib as L
+    page, n, cap = 1 << 20, 100, 1 << 30
+    r = np.random.default_rng(560)
+    rows_k = r.integers(0, 65536, (n, HD)).astype(np.uint16)
+    block_v = r.integers(0, 65536, (4, HD, 32)).astype(np.uint16)
+    with L.Ctx(0) as c:
+        k, v, acc = c.buf(2 * page * HD * 2), c.buf(2 * page * HD * 2), c.buf(cap * 4)
+        k.upload(rows_k)
+        v.upload(block_v)
+        acc.zero()
+        table, dst = np.zeros((1, cap // page), np.int32), np.ones((1, cap // page), np.int32)
+        tb, db, ln, dl = c.put(table), c.put(dst), c.put(np.array([n], np.int32)), c.put(np.array([-1], np.int32))
+        d = L.PagedEvictDesc()
+        d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = 1, 1, HD, page, 2, cap // page
+        d.table, d.len, d.budget, d.acc, d.acc_stride = tb.ptr, ln.ptr, cap - 1, acc.ptr, cap
+        d.k_pages, d.v_pages, d.dst_table, d.dst_max_pages, d.dst_len = k.ptr, v.ptr, db.ptr, cap // page, dl.ptr
+        L.check(L.lib().vx27_hip_paged_evict(c.h, C.byref(d)), "paged_evict")
+        c.sync()
+        assert dl.download((1,), np.int32)[0] == n
+        got_k, got_v = np.empty((n, HD), np.uint16), np.empty((4, HD, 32), np.uint16)
+        half = page * HD * 2
+        L.check(L.lib().vx27_hip_d2h(c.h, got_k.ctypes.data, k.ptr + half, got_k.nbytes))
+        L.check(L.lib().vx27_hip_d2h(c.h, got_v.ctypes.data, v.ptr + half, got_v.nbytes))
+        assert np.array_equal(got_k, rows_k) and np.array_equal(got_v[:3], block_v[:3])
+        assert np.array_equal(got_v[3, :, :4], block_v[3, :, :4])

@@ -29,6 +29,7 @@ struct EvictArgs {
     size_t acc_out_stride;
     int *kept;          // [B][n_kv][kept_stride] (the caller's or scratch)
     size_t kept_stride;
+    int blk0;           // paged_move: first 32-row block of the launch
 };
 
 __device__ __forceinline__ int seq_len(const EvictArgs &a, int b) {
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
     }
 }
 
-// grid (32-row blocks of the destination, n_kv, B), block 256.  K: wave w
+// grid (32-row blocks of the destination from blk0 on, n_kv, B), block 256.  K: wave w
 // moves rows w, w + 4, ..., 512 bytes each.  V: a destination block's rows
 // come from a few source blocks, each read whole (a kept row has two bytes in
 // every 64-byte line of its block) into LDS, dim by dim 68 bytes apart, so
@@ -182,7 +183,7 @@ constexpr int VROW = VB + 2;   // elements from dim to dim in LDS
 __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = seq_len(a, b), keep = min(n, a.budget), d0 = blockIdx.x * VB;
+    const int n = seq_len(a, b), keep = min(n, a.budget), d0 = (a.blk0 + (int)blockIdx.x) * VB;
     if (d0 >= keep) return;
     const int cnt = min(VB, keep - d0), P = a.p.page_size;
     __shared__ int s_row[VB];
@@ -298,6 +299,9 @@ extern "C" int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_de
         a.kept = (int *)scr;
     }
     VX_LAUNCH(ctx, paged_select, dim3(d->n_kv, d->B), dim3(SEL), a);
-    VX_LAUNCH(ctx, paged_move, dim3((unsigned)((most + VB - 1) / VB), d->n_kv, d->B), dim3(256), a);
+    // (a launch holds 2^32 threads a dimension; kept rows past 2^28 take another)
+    constexpr int PER = 1 << 23;
+    for (int64_t left = (most + VB - 1) / VB; left > 0; left -= PER, a.blk0 += PER)
+        VX_LAUNCH(ctx, paged_move, dim3((unsigned)(left < PER ? left : PER), d->n_kv, d->B), dim3(256), a);
     return 0;
 }
