@@ -1,4 +1,6 @@
-"""The paged-cache operators where values and sizes are extreme."""
+"""The paged-cache operators where values and sizes are extreme: infinite and
+NaN keys, values near the end of bf16's range, capacities at the limits, pages
+past 2^32 elements, and work that is late on the caller's stream."""
 import ctypes as C
 
 import numpy as np
@@ -138,3 +140,119 @@ def test_eviction_of_the_largest_capacity():
         L.check(L.lib().vx27_hip_d2h(c.h, got_v.ctypes.data, v.ptr + half, got_v.nbytes))
         assert np.array_equal(got_k, rows_k) and np.array_equal(got_v[:3], block_v[:3])
         assert np.array_equal(got_v[3, :, :4], block_v[3, :, :4])
+
+
+class Step:
+    """Append, attention with weights and eviction of one batch whose pool lies `off` pages into a larger one."""
+
+    def __init__(self, ctx, lens, new, off=0):
+        from vx27_amd import lib as L, workloads as W
+        self.ctx, self.L, self.off = ctx, L, off
+        bt = self.bt = Batch(lens, new, page=64, seed=580)
+        N, n_kv, B = bt.N, 4, bt.B
+        budget, dst = 96, 2
+        pool = bt.n_pages + B * dst
+        self.k = np.concatenate([bt.k, np.zeros((B * dst,) + bt.k.shape[1:], np.uint16)])
+        self.v = np.concatenate([bt.v, np.zeros((B * dst,) + bt.v.shape[1:], np.uint16)])
+        self.lo = off * n_kv * 64 * HD * 2
+        self.up = dict(q=W.normal(bt.r, (N, 24, HD)), kv=W.normal(bt.r, (2, N, n_kv, HD)),
+                       acc=bt.r.random((B, n_kv, bt.max_pages * 64)).astype(np.float32))
+        self.outs = dict(rot=np.zeros((N, 24, HD), np.uint16), out=np.zeros((N, 24, HD), np.float32), dl=np.zeros(B, np.int32),
+                         kept=np.full((B, n_kv, budget), -1, np.int32), ao=np.zeros((B, n_kv, budget), np.float32))
+        table = np.where(bt.table >= 0, bt.table + off, bt.table)
+        const = dict(table=table, len=np.asarray(lens, np.int32), start=bt.start, w=W.normal(bt.r, HD, 0.1),
+                     dst=np.arange(bt.n_pages, pool, dtype=np.int32) + off)
+        self.buf = {n: ctx.put(x) for n, x in {**self.up, **self.outs, **const}.items()}
+        self.buf["k"], self.buf["v"] = ctx.buf(self.lo + self.k.nbytes), ctx.buf(self.lo + self.v.nbytes)
+        u = {n: x.ptr for n, x in self.buf.items()}
+        p, a, e = self.descs = L.PagedAppendDesc(), L.PagedAttnDesc(), L.PagedEvictDesc()
+        for d in self.descs:
+            d.B, d.n_kv, d.hd, d.page_size, d.n_pages, d.max_pages = B, n_kv, HD, 64, off + pool, bt.max_pages
+            d.table, d.len, d.k_pages, d.v_pages = u["table"], u["len"], u["k"], u["v"]
+        for d in (p, a):
+            d.n_q, d.q_start, d.n_tok, d.max_T = 24, u["start"], N, max(new)
+        p.rope_dim, p.rope_theta, p.rope_yarn, p.q = 64, 1e7, 1.0, u["q"]
+        p.k_new, p.v_new, p.q_norm_w, p.k_norm_w, p.q_out = u["kv"], u["kv"] + N * n_kv * HD * 4, u["w"], u["w"], u["rot"]
+        a.q, a.out, a.acc, a.acc_stride = u["rot"], u["out"], u["acc"], bt.max_pages * 64
+        e.budget, e.n_sink, e.n_recent, e.acc, e.acc_stride = budget, 4, 16, u["acc"], bt.max_pages * 64
+        e.dst_table, e.dst_max_pages, e.dst_len, e.kept = u["dst"], dst, u["dl"], u["kept"]
+        e.acc_out, e.acc_out_stride = u["ao"], budget
+
+    def h2d(self, name, host):
+        self.L.check(self.L.lib().vx27_hip_h2d(self.ctx.h, self.buf[name].ptr + self.lo, host.ctypes.data, host.nbytes))
+
+    def reset(self):
+        self.h2d("k", self.k)
+        self.h2d("v", self.v)
+        for n, x in {**self.up, **self.outs}.items():
+            self.buf[n].upload(x)
+
+    def call(self):
+        lib = self.L.lib()
+        for fn, d in zip((lib.vx27_hip_paged_append, lib.vx27_hip_paged_attn, lib.vx27_hip_paged_evict), self.descs):
+            self.L.check(fn(self.ctx.h, C.byref(d)))
+
+    def results(self):
+        self.ctx.sync()
+        got = [self.buf[n].download(x.shape, x.dtype) for n, x in {**self.outs, "acc": self.up["acc"]}.items()]
+        for n, x in (("k", self.k), ("v", self.v)):
+            h = np.empty_like(x)
+            self.L.check(self.L.lib().vx27_hip_d2h(self.ctx.h, h.ctypes.data, self.buf[n].ptr + self.lo, h.nbytes))
+            got.append(h)
+        return [x.view(np.uint8) for x in got]
+
+    def free(self):
+        for b in self.buf.values():
+            b.free()
+
+
+SHAPES = [([300, 95, 200], [1, 1, 1]), ([300, 95, 200], [2, 1, 2]), ([300, 95, 200], [130, 1, 9]), ([40 + i for i in range(70)], [1] * 70)]
+
+
+@pytest.mark.parametrize("lens,new", SHAPES)
+def test_pages_past_2_to_32_elements(ctx, lens, new):  # noqa: F811
+    """A pool whose used pages begin past 2^32 elements (8 GiB) of K and of V: every output's and page's bytes are those
+    of the same batch at the pool's start."""
+    say(f"far pages {lens[:3]} {new[:3]}")
+    got = []
+    for off in (0, (1 << 32) // (4 * 64 * HD) + 3):
+        s = Step(ctx, lens, new, off)
+        s.reset()
+        s.call()
+        got.append(s.results())
+        s.free()
+    assert all(np.array_equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.parametrize("lens,new", SHAPES)
+def test_inputs_that_are_late_on_the_callers_stream(ctx, lens, new):  # noqa: F811
+    """Copies of 64 GB are queued on the caller's stream, then one that delivers the inputs, then the calls: kernels on any
+    other stream would be done with zeros long before."""
+    from vx27_amd import lib as L
+    say(f"late inputs {lens[:3]} {new[:3]}")
+    lib, other = L.lib(), L.Ctx(0)
+    s = Step(ctx, lens, new)
+    s.reset()
+    s.call()
+    want = s.results()
+    s.reset()
+    keep = {n: ctx.put(x) for n, x in s.up.items()}
+    for n in s.up:
+        s.buf[n].zero()
+    ctx.sync()
+    big = [ctx.buf(4 << 30) for _ in range(2)]
+    try:
+        L.check(lib.vx27_hip_set_stream(ctx.h, lib.vx27_hip_get_stream(other.h)))
+        for _ in range(16):
+            L.check(lib.vx27_hip_d2d(ctx.h, big[0].ptr, big[1].ptr, 4 << 30))
+        for n, x in s.up.items():
+            L.check(lib.vx27_hip_d2d(ctx.h, s.buf[n].ptr, keep[n].ptr, x.nbytes))
+        s.call()
+        assert all(np.array_equal(x, y) for x, y in zip(s.results(), want))
+    finally:
+        ctx.sync()
+        L.check(lib.vx27_hip_set_stream(ctx.h, None))
+        other.close()
+        for b in [*big, *keep.values()]:
+            b.free()
+        s.free()
