@@ -384,12 +384,13 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * rows a KV head) run the decode kernels: the
  * cache's length split evenly over the device and joined, the softmax
  * weights as three bf16 parts (fp32 accuracy; out fp32 or bf16).  More tokens
- * run the tile kernel, whose weights are rounded to bf16 once (relative
- * 2^-9; out may still be fp32).
+ * run the tile kernel, whose weights are rounded to bf16 once (at most 2^-8
+ * relative; out may still be fp32).
  * Optional outputs: lse [n_tok][n_q], the natural log of the softmax sum
  * (-inf for a token that sees nothing); acc [B][n_kv][acc_stride], to which
  * each row's weight over the call's tokens and the group's heads is added
- * (rows nobody sees and rows from len on are left as they were).
+ * (rows nobody sees and rows from len on are left as they were: a program
+ * that gives a sequence's place to another clears its part).
  * A NaN key, a score of +inf and an infinite or NaN value reach only the
  * tokens that see the row, whose outputs are then not finite (an infinity may
  * end as NaN); a score of -inf weighs nothing.  Weights are at most 1 before

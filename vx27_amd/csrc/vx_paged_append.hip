@@ -99,8 +99,9 @@ __device__ __forceinline__ double wave_sums4(const double (&s)[4]) {
 // leave room for six workgroups a CU, not eight: 50 us); then wave w takes
 // rows w, w + 4, ..., four at a time so that their loads are in flight
 // together, lane l dims 4l..4l+3.
-// Bound by bytes: 49 us for 143 MB (4096 + 268 bf16 tokens), the copy rate's
-// 27; one token for 13 sequences, a launch and its latencies, 6.5 us.  v
+// 49 us for 143 MB (4096 + 268 bf16 tokens; 38 where the last-level cache holds
+// the inputs), the copy rate's 27: a wave's loads, norms and stores follow one
+// another; one token for 13 sequences, a launch and its latencies, 6.4 us.  v
 // goes through LDS into the dim-major block, element by element at its ends
 // so that other rows keep their contents.  HALFS: most angles a token has.
 constexpr int QTOK = 8;

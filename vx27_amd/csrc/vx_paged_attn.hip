@@ -275,6 +275,8 @@ __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l,
 // TB/s: 4 x 131072 rows, 2.15 GB, in 325 us (one workgroup a CU: 327), a
 // plain read of as much 298.  Short calls are two launches and the latencies
 // of the table, the tiles and the join: 12 us for one sequence of 1000 rows.
+// (253 VGPRs, of the 256 that two workgroups a CU leave; some 90 scalars do not
+// fit the SGPRs and are kept in lanes of them.)
 //
 // 16 rows are what one MFMA tile holds, so this form ends there: a third token
 // of 6 heads goes to the tiles below (4 x 131072 rows: 328 us for two tokens
@@ -547,11 +549,14 @@ __global__ __launch_bounds__(256) void paged_weigh(Args a) {
 // A step's two key blocks are consecutive entries of the tile list, so a
 // sink block and the window's first block make a step without a gap.
 //
-// Bound by the MFMAs' issue beside the softmax and by power: a step of 64 MFMAs
-// a wave takes about 2.15 us (3900 cycles at the 1.8 GHz that the chip then
-// holds; the MFMAs alone are 2050), and a piece another 13 us for its first
-// loads, its first scores and its output.  8192 tokens of 24 heads under a
-// window of 1024: 300 us, 0.65 PFLOP/s of what the rows see.
+// Bound by the MFMAs' issue beside the softmax: a step of 64 MFMAs a wave takes
+// about 2.15 us (3900 cycles at the 1.8 GHz that the chip then holds; the MFMAs
+// alone are 2050), and a piece another 13 us for its first loads, its first
+// scores and its output, which nothing overlaps.  8192 tokens of 24 heads under
+// a window of 1024: 300 us, 0.65 PFLOP/s of what the rows see.  (Neither is the
+// card's limit: gqp_attn_pp, of the same tile, takes 1.75 us a step.)
+// Weights are one bf16 part, as there: three would triple the second half of
+// the step's MFMAs.
 //
 // (Measured against it: waves of 64 rows x one key block, and 128 dims of O,
 // which read half as much from LDS but exchange weights and maxima through it
@@ -620,7 +625,9 @@ __device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &
     return max(1, (tl.nt + 1) / 2);
 }
 
-// grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).
+// grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).  It
+// goes by B * n_rt entries, n_rt of the longest token range: 256 decoding
+// sequences beside a chunk of 8192 tokens 105 us, 4096 beside 4096 1.8 ms.
 constexpr int PLAN = 1024;
 __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, int max_pieces) {
     __shared__ int64_t s_steps[PLAN / 64];

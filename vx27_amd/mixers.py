@@ -231,7 +231,9 @@ class PagedGQALayer:
 
     step() appends the sequences' new tokens and attends from them; evict()
     brings sequences past a budget back to it; end() frees a sequence's place
-    for another.
+    for another.  max_pages: the most pages a sequence may have (n_pages by
+    default); the weights, and the workspace of steps that add them up, go by
+    n_seq * max_pages.
     """
 
     def __init__(self, ctx, n_seq, n_pages, page_size, q_norm_w, k_norm_w, n_q=24, n_kv=4, hd=256, rope_dim=64,
