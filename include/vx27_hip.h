@@ -381,11 +381,10 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * only scores of -inf, gets 0 (and lse -inf, and adds no weight).  q is bf16,
  * normed and rotated (q_out of the append).  Products on bf16 MFMA, sums and
  * softmax statistics in fp32.  One or two tokens a sequence (at most 16 query
- * rows a KV head) run the decode kernels: the
- * cache's length split evenly over the device and joined, the softmax
- * weights as three bf16 parts (fp32 accuracy; out fp32 or bf16).  More tokens
- * run the tile kernel, whose weights are rounded to bf16 once (at most 2^-8
- * relative; out may still be fp32).
+ * rows a KV head) run the decode kernels: the cache's length split evenly over
+ * the device and joined, the softmax weights as three bf16 parts (fp32
+ * accuracy; out fp32 or bf16).  More tokens run the tile kernel, whose weights
+ * are rounded to bf16 once (at most 2^-8 relative; out may still be fp32).
  * Optional outputs: lse [n_tok][n_q], the natural log of the softmax sum
  * (-inf for a token that sees nothing); acc [B][n_kv][acc_stride], to which
  * each row's weight over the call's tokens and the group's heads is added
@@ -395,7 +394,7 @@ int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
  * tokens that see the row, whose outputs are then not finite (an infinity may
  * end as NaN); a score of -inf weighs nothing.  Weights are at most 1 before
  * the division by their sum: nothing overflows while the largest |v| times the
- * number of rows seen stays below 2^127.
+ * number of rows seen stays below 2^127, for scores below 2^24 in magnitude.
  * out must not overlap an input.  Context scratch: the parts of cut rows
  * (at most about 100 MB), and with acc and at most 16 query rows a KV head their
  * scores, B*n_kv*rows*4 bytes for each row that a sequence can see at most

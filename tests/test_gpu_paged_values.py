@@ -112,6 +112,41 @@ def test_large_values_and_rising_scores(ctx, T, power):  # noqa: F811
     at.free()
 
 
+@pytest.mark.parametrize("lens,new", [([70], [40]), ([3000, 9], [40, 3]), ([70], [1]), ([3000, 9], [2, 1])])
+@pytest.mark.parametrize("power", [10, 26, 30, 60])
+def test_weights_of_huge_scores(ctx, lens, new, power):  # noqa: F811
+    """One key whose score is 2^power, all others 0: it weighs 1 for every token, whatever a score's last place is."""
+    from vx27_amd import workloads as W
+    say(f"scores 2^{power} {lens} {new}")
+    bt = Batch(lens, new, 24, 4, 64, seed=545)
+    q = np.zeros((bt.N, 24, HD), np.float32)
+    q[..., 0] = 2.0 ** (power // 2 + 4)                       # (over 16)
+    bt.q = W.bf16_bits(q)
+    for b, n in enumerate(bt.lens):
+        for j in range(n):
+            k = np.zeros((4, HD), np.float32)
+            k[:, 0] = 2.0 ** (power - power // 2) if j == 0 else 0.0
+            bt.put_row(b, j, W.bf16_bits(k), W.bf16_bits(W.normal(bt.r, (4, HD))))
+    at = Attn(ctx, bt, gate="none", acc=True)
+    at.call()
+    ctx.sync()
+    out, lse = at.out(), at.bufs["lse"].download((bt.N, 24), np.float32)
+    acc = at.bufs["acc"].download((bt.B, 4, at.stride), np.float32).astype(np.float64)
+    for b, n in enumerate(bt.lens):
+        w = np.zeros((4, n))
+        w[:, 0] = 6 * bt.new[b]
+        base = at.acc0[b, :, :n].astype(np.float64)
+        # (the others weigh less than e^-1000; sums, the division and the last place of the accumulated weight)
+        assert np.all(np.abs(acc[b, :, :n] - base - w) <= 2.0 ** -20 * w + 2.0 ** -23 * (base + w)), b
+        _, v = bt.rows(b)
+        tok = slice(bt.start[b], bt.start[b + 1])
+        want = np.repeat(W.bf16_to_f32(v[0]).astype(np.float64), 6, axis=0)
+        assert np.all(np.abs(out[tok] - want) <= 2.0 ** -20 * np.abs(want)), b
+        # (the maximum times log2 e and back: three roundings, and those of the two constants)
+        assert np.all(np.abs(lse[tok] - 2.0 ** power) <= 2.0 ** power * 2.0 ** -22), b
+    at.free()
+
+
 def test_eviction_of_the_largest_capacity():
     """A capacity of 2^30 rows and a budget next to it: the short sequence is moved, whatever its capacity's launch would
     be."""

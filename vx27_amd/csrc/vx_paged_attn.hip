@@ -207,14 +207,16 @@ __device__ __forceinline__ void attend_tile(Rows &w, int R, bool one, const floa
 }
 
 // A row's lse, and its reference and 1 / sum for the weights' pass.  SHIFT: the
-// reference lies that far above a maximum; the weights' pass takes the maximum
-// (the difference is exact), so that its arguments are small.
+// reference lies that far above a maximum; the weights' pass takes the maximum,
+// so that its arguments are small (the difference as it was rounded: exact
+// below 2^24, and none where a last place is larger).
 template <int SHIFT>
 __device__ __forceinline__ void stat_store(const Args &a, int tok, int h, float m, float L) {
     const size_t at = (size_t)tok * a.n_q + h;
     if (a.lse) a.lse[at] = L > 0.0f || L != L ? (m + log2f(L)) * 0.6931471805599453f : -INFINITY;
     // (a row that weighs nothing: from 0, so that scores of -inf become weights of 0 and not NaN)
-    if (a.stat) a.stat[at] = L > 0.0f || L != L ? make_float2(m - SHIFT, 1.0f / (1 << SHIFT) / L) : make_float2(0.0f, 0.0f);
+    const float ref = m - SHIFT;
+    if (a.stat) a.stat[at] = L > 0.0f || L != L ? make_float2(ref, (SHIFT ? __builtin_amdgcn_exp2f(ref - m) : 1.0f) / L) : make_float2(0.0f, 0.0f);
 }
 
 // hardware round-to-nearest-even pack (v_cvt_pk_bf16_f32)
