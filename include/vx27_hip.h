@@ -436,7 +436,8 @@ int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d);
  * Rows behind the last kept one are left as they were.  dst_len [B] receives
  * the new lengths; acc_out [B][n_kv][acc_out_stride] (optional) the kept
  * rows' weights; kept [B][n_kv][budget] (optional) their old rows, entries
- * from dst_len on left as they were.  Keys keep the rotation of their
+ * from dst_len on left as they were.  The outputs must not overlap an input or
+ * one another.  Keys keep the rotation of their
  * original position: append later tokens with explicit positions (pos). */
 typedef struct {
     int B, n_kv, hd;

@@ -139,3 +139,22 @@ def test_group_of_a_row():
 def test_launch_of_a_limit():
     """The append's grid at its largest max_T: below 2^32 threads, 256 a workgroup."""
     assert ((2 ** 26 + 30) // 32 + 1) * 5 * 256 < 2 ** 32
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"acc_out": 4 * P, "kept": 4 * P + 64}, "acc_out must not overlap kept"),
+    ({"acc_out": 8 * P, "len": 8 * P + 3196}, "acc_out must not overlap len"),
+    ({"acc_out": 8 * P, "table": 8 * P + 3196}, "acc_out must not overlap table"),
+    ({"acc_out": 8 * P, "dst_table": 8 * P - 12}, "acc_out must not overlap dst_table"),
+    ({"acc_out": 2 * P}, "acc_out must not overlap dst_len"),
+    ({"dst_len": 8 * P, "dst_table": 8 * P}, "dst_len must not overlap dst_table"),
+    ({"dst_len": 8 * P, "kept": 8 * P - 3196}, "dst_len must not overlap kept"),
+    ({"dst_len": 8 * P, "acc": 8 * P - 4}, "dst_len must not overlap acc")])
+def test_eviction_outputs_that_overlap(change, message):
+    """paged_move reads lengths, tables and kept rows that another workgroup's outputs would change under it."""
+    from vx27_amd import lib as L
+    d = _evict()
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert L.lib().vx27_hip_paged_evict(None, C.byref(d)) == -1
+    assert message in L.lib().vx27_hip_last_error().decode()

@@ -257,9 +257,14 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
     }
 }
 
-bool overlap(const void *x, size_t nx, const void *y, size_t ny) {
-    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
-    return a < b + ny && b < a + nx;
+struct Span {
+    const char *name;
+    const void *p;
+    size_t bytes;
+};
+bool overlap(const Span &x, const Span &y) {
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return a < b + y.bytes && b < a + x.bytes;
 }
 
 }  // namespace
@@ -279,10 +284,15 @@ extern "C" int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_de
                "%s: dst_max_pages * page_size must hold the kept rows (got %d * %d for %d)", who, d->dst_max_pages, d->page_size, d->budget);
     VX_REQUIRE((((uintptr_t)d->k_pages | (uintptr_t)d->v_pages) & 15) == 0, "%s: the pages must be 16-byte aligned", who);
     const size_t pairs = (size_t)d->B * d->n_kv;
-    VX_REQUIRE(!d->acc_out || !overlap(d->acc, pairs * d->acc_stride * 4, d->acc_out, pairs * d->acc_out_stride * 4),
-               "%s: acc_out must not overlap acc", who);
-    VX_REQUIRE(!overlap(d->len, (size_t)d->B * 4, d->dst_len, (size_t)d->B * 4), "%s: dst_len must not overlap len", who);
-    VX_REQUIRE(!overlap(d->table, (size_t)d->B * d->max_pages * 4, d->dst_len, (size_t)d->B * 4), "%s: dst_len must not overlap table", who);
+    // what a workgroup of paged_select or paged_move writes must not be what another still reads
+    const Span acc = {"acc", d->acc, pairs * d->acc_stride * 4}, len = {"len", d->len, (size_t)d->B * 4},
+               table = {"table", d->table, (size_t)d->B * d->max_pages * 4}, dst_table = {"dst_table", d->dst_table, (size_t)d->B * d->dst_max_pages * 4},
+               dst_len = {"dst_len", d->dst_len, (size_t)d->B * 4}, kept = {"kept", d->kept, pairs * (size_t)d->budget * 4},
+               acc_out = {"acc_out", d->acc_out, pairs * d->acc_out_stride * 4};
+    const Span apart[][2] = {{acc_out, acc}, {dst_len, len}, {dst_len, table}, {acc_out, len}, {acc_out, table}, {acc_out, dst_table},
+                             {acc_out, dst_len}, {acc_out, kept}, {dst_len, dst_table}, {dst_len, kept}, {dst_len, acc}};
+    for (const auto &x : apart)
+        VX_REQUIRE(!x[0].p || !x[1].p || !overlap(x[0], x[1]), "%s: %s must not overlap %s", who, x[0].name, x[1].name);
     if (vx_ctx_enter(ctx)) return -1;
     a.p.err_flag = ctx->err_flag;
     a.budget = d->budget; a.n_sink = d->n_sink; a.n_recent = d->n_recent;
