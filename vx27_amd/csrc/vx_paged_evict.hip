@@ -165,7 +165,8 @@ __global__ __launch_bounds__(SEL) void paged_select(EvictArgs a) {
             const uint64_t be = __ballot(r[k] == prefix);
             const bool stay = r[k] > prefix || (r[k] == prefix && eqs + lanes_below(be) < want);
             const uint64_t bs = __ballot(stay);
-            if (stay) kept[at + lanes_below(bs)] = base + 64 * k + lane;
+            // (never past `keep`, whatever a changing acc would count)
+            if (stay && at + lanes_below(bs) < keep) kept[at + lanes_below(bs)] = base + 64 * k + lane;
             at += __popcll(bs);
             eqs += __popcll(be);
         }
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs a) {
     const int *kept = a.kept + ((size_t)b * a.p.n_kv + h) * a.kept_stride;
     const int dpage = vx_page_checked(a.p, vx_table_word(a.dst_table + (size_t)b * a.dst_max_pages + d0 / P)), dat = d0 % P;
     if (tid < VB) {
-        const int r = kept[d0 + min(tid, cnt - 1)];
+        const int r = min(max(kept[d0 + min(tid, cnt - 1)], 0), n - 1);   // (a row, whatever `kept` shares memory with)
         s_row[tid] = r;
         s_blk[tid] = vx_v_index(a.p.n_kv, P, vx_paged_page(a.p, b, r), h, r % P / VB * VB, 0);
         if (a.acc_out && tid < cnt)
