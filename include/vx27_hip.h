@@ -457,6 +457,103 @@ typedef struct {
 } vx27_paged_evict_desc;
 int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
 
+/* ------------------------------------------------ pages held in 4 bits
+ * The same cache at 288 bytes a row and KV head (K and V) instead of 1024:
+ * each page holds page_size/32 blocks of VX27_Q4_BLOCK_BYTES for each KV head,
+ *   K and V: [n_pages][n_kv][page_size/32][VX27_Q4_BLOCK_BYTES]
+ * A row's 256 dims are four groups of 64; the value of dim i is m + s*c with
+ * s and m of its row and group (bf16) and a 4-bit code c:
+ *   m = the largest bf16 number not above the group's values
+ *   s = the smallest bf16 number not below (the largest value - m) / 15
+ *   c = the integer nearest to (x - m) / s, ties to even (0 where s = 0)
+ * so a value is off by at most s/2.  A group that holds an infinity, a NaN or
+ * a value past the largest bf16 number is held as NaN.  Bytes of a block, from
+ * the slowest index (codes 0-3 of an 8 in the low halves of 4 bytes, 4-7 in
+ * the high ones):
+ *   K     0: c [row/4%2][dim/128][dim/8%4][row/8][row%4][dim/32%4][dim%4]; high halves: dims 4-7 of 8
+ *      4096: s [dim/64][row]    4352: m [row][dim/64]
+ *   V     0: c [dim/64][row/8][dim%16][dim/16%4][row%4]; high halves: rows 4-7 of 8
+ *      4096: s [dim/64][row]    4352: m [dim/64][row]
+ * The calls take the descriptors of their bf16 forms, whose k_pages and
+ * v_pages are then these pages, and what is said above of ragged batches, page
+ * tables and faulty tables holds for them.  Other rows of a block that an
+ * append writes to keep their values; two sequences may share only pages that
+ * neither writes. */
+#define VX27_Q4_BLOCK_BYTES 4608
+#define VX27_Q4_SPLIT_ROWS (1 << 28)
+/* vx27_hip_paged_append into 4-bit pages.  k is normed and rotated in fp64
+ * (the angle is the fp32 product of the other calls), so that rounding it to
+ * codes does not depend on the order of sums; q as there. */
+int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
+/* vx27_hip_paged_attn over 4-bit pages; acc must be NULL.  Products are exact
+ * bf16 codes on bf16 MFMA, scales and minima are applied in fp32. */
+int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d);
+
+/* The values of rows by slot (page*page_size + row of the page), as
+ * vx27_hip_paged_plan leaves them: k_out and v_out [n_rows][n_kv][hd] (either
+ * may be NULL), fp32 or rounded to bf16.  A slot of -1 leaves its output as it
+ * was; any other slot outside the pool as well, and vx27_hip_sync reports it.
+ * Pages and outputs 16-byte aligned. */
+typedef struct {
+    int n_kv, hd;
+    int page_size, n_pages;
+    int n_rows;
+    const int *slots;           /* [n_rows] */
+    const uint16_t *k_pages, *v_pages;
+    int out_dtype;              /* VX27_F32 or VX27_BF16 */
+    void *k_out, *v_out;
+} vx27_paged_read_desc;
+int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_desc *d);
+
+/* A step's rows and pages, planned on the device, for either kind of pages:
+ * gives each of B sequences the rows of its new tokens, takes pages for them
+ * from the free ones, and leaves what the other calls read.
+ *
+ * 1. A sequence with ended[b] != 0 gives its pages back: they go on top of the
+ *    free ones, in the order of the sequences and of their rows.  It has no
+ *    rows then and takes no tokens in this call.
+ * 2. A sequence whose rows and new tokens are past max_pages * page_size gets
+ *    none of the tokens.  Of the others, one that needs no further page gets
+ *    all of them, and one that needs pages does if the pages that it and the
+ *    ones before it need do not exceed the free ones.
+ * 3. A sequence gets none after all if its tokens and those that the ones
+ *    before it got in 2. exceed n_tok.
+ * 4. Pages are taken from the top of the free ones, in the order of the
+ *    sequences and their rows, and entered in the table.
+ *
+ * took [B]: the tokens that each sequence got (new_tok[b] or 0); q_start, len_out,
+ * next_pos_out and n_free_out: ranges, rows, positions and free pages after
+ * it; slot, pos and seq [n_tok] (each optional): every token's slot
+ * (page*page_size + row of the page), position and sequence, -1 from
+ * q_start[B] on.  len_out may be len, next_pos_out next_pos and n_free_out
+ * n_free (then a captured call goes on from step to step); no other output may
+ * overlap anything.  Without next_pos a token's position is its row.
+ * Table entries behind a sequence's rows, and free_pages entries from
+ * n_free_out[0] on, may hold anything; free_pages entries below n_free[0] are
+ * not written.
+ * Negative counts, lengths past the table, more free pages than n_pages and
+ * page numbers outside the pool are clamped or dropped on the device and
+ * reported by the next vx27_hip_sync; that call's outputs are undefined.
+ * n_pages * page_size below 2^31.  Context scratch: 12 bytes a sequence. */
+typedef struct {
+    int B, page_size, n_pages, max_pages;
+    int n_tok;                  /* room in slot, pos and seq */
+    const int *new_tok;         /* [B] */
+    const int *ended;           /* [B] or NULL: none */
+    const int *len;             /* [B] rows */
+    const int *next_pos;        /* [B] positions of the next tokens, or NULL */
+    int *table;                 /* [B][max_pages], in and out */
+    int *free_pages;            /* [n_pages], in and out: the free pages, the top last */
+    const int *n_free;          /* [1] */
+    int *took;                  /* [B] */
+    int *q_start;               /* [B+1] */
+    int *len_out;               /* [B] */
+    int *next_pos_out;          /* [B], NULL exactly if next_pos is */
+    int *n_free_out;            /* [1] */
+    int *slot, *pos, *seq;      /* [n_tok] each, or NULL */
+} vx27_paged_plan_desc;
+int vx27_hip_paged_plan(vx27_hip_ctx *ctx, const vx27_paged_plan_desc *d);
+
 /* RoPE cos/sin tables on the device for n positions (device int array):
  * cos/sin [n][rope_dim/2].  The frequency table powf(theta, -2i/rope_dim) is
  * evaluated on the host exactly as vx27_rope.c:11; the angle is the same

@@ -1,0 +1,188 @@
+"""The 4-bit pages in plain numpy, by the layout's definition byte by byte, and
+ragged batches over them with their float64 results."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from paged_common import HD, Batch, f64, score_err
+from vx27_amd import workloads as W
+
+BLOCK = 4608
+BF16_MAX = float(np.uint32(0x7F7F0000).view(np.float32))
+
+_r, _d = np.meshgrid(np.arange(32), np.arange(HD), indexing="ij")
+# byte and shift of the code of (row, dim); byte of its s and of its m
+K_AT = (_r // 4 % 2 * 2048 + _d // 128 * 1024 + _d // 8 % 4 * 256 + _r // 8 * 64 + _r % 4 * 16 + _d // 32 % 4 * 4 + _d % 4,
+        _d // 4 % 2 * 4, 4096 + _d // 64 * 64 + _r * 2, 4352 + _r * 8 + _d // 64 * 2)
+V_AT = (_d // 64 * 1024 + _r // 8 * 256 + _d % 16 * 16 + _d // 16 % 4 * 4 + _r % 4,
+        _r // 4 % 2 * 4, 4096 + _d // 64 * 64 + _r * 2, 4352 + _d // 64 * 64 + _r * 2)
+
+
+def bf16_bits_toward(x, up):
+    """Bits of the largest bf16 number <= x (or the smallest >= x, up), x float64 within bf16's range."""
+    b = np.asarray(x, np.float32).view(np.uint32) & np.uint32(0xFFFF0000)
+    y = b.view(np.float32).astype(np.float64)
+    wrong = y < x if up else y > x
+    neg = b >> 31 != 0
+    zero = (b << 1) == 0
+    step = np.where(neg ^ up, b + np.uint32(0x10000), b - np.uint32(0x10000))
+    step = np.where(zero, np.uint32(0x00010000 if up else 0x80010000), step)
+    return (np.where(wrong, step, b) >> 16).astype(np.uint16)
+
+
+def quantise(x):
+    """codes, s bits, m bits of rows [..., 256] in float64, by the definition."""
+    g = x.reshape(*x.shape[:-1], 4, 64)
+    ok = (np.abs(g) <= BF16_MAX).all(-1)
+    g = np.where(ok[..., None], g, 0.0)
+    m = bf16_bits_toward(g.min(-1), False)
+    mv = f64(m)
+    s = bf16_bits_toward((g.max(-1) - mv) / 15, True)
+    sv = f64(s)
+    with np.errstate(all="ignore"):
+        c = np.where(sv[..., None] > 0, np.rint((g - mv[..., None]) / sv[..., None]), 0.0)
+    s, m = np.where(ok, s, 0).astype(np.uint16), np.where(ok, m, 0x7FC0).astype(np.uint16)
+    c = np.where(ok[..., None], c, 0.0)
+    return c.astype(np.uint8).reshape(x.shape), s, m
+
+
+def values(c, s, m):
+    """float64 values of codes [..., 256] with bits s, m [..., 4]."""
+    with np.errstate(invalid="ignore"):
+        g = f64(m)[..., None] + f64(s)[..., None] * c.reshape(*c.shape[:-1], 4, 64).astype(np.float64)
+    return g.reshape(c.shape)
+
+
+def put(blk, at, row, c, s, m):
+    """Codes [256], s and m bits [4] of a row into a block's bytes."""
+    byte, shift, s_at, m_at = (t[row] for t in at)
+    for half in (0, 4):
+        i = shift == half
+        blk[byte[i]] = (blk[byte[i]] & (0xF0 if half == 0 else 0x0F)) | (c[i] << half)
+    for x, x_at in ((s, s_at[::64]), (m, m_at[::64])):
+        blk[x_at], blk[x_at + 1] = x & 255, x >> 8
+
+
+def put_rows(q, at, page, row, c, s, m):
+    """The same for rows [n] of pages [n], all KV heads: c [n][n_kv][256], s and m [n][n_kv][4]."""
+    byte, shift, s_at, m_at = (t[row % 32] for t in at)                            # [n][256]
+    for half in (0, 4):
+        i, d = np.nonzero(shift == half)
+        old = q[page[i], :, row[i] // 32, byte[i, d]]
+        q[page[i], :, row[i] // 32, byte[i, d]] = (old & (0xF0 if half == 0 else 0x0F)) | (c[i, :, d] << half)
+    i, g = np.nonzero(np.ones((len(row), 4), bool))
+    for x, x_at in ((s, s_at[:, ::64]), (m, m_at[:, ::64])):
+        q[page[i], :, row[i] // 32, x_at[i, g]] = (x[i, :, g] & 255).astype(np.uint8)
+        q[page[i], :, row[i] // 32, x_at[i, g] + 1] = (x[i, :, g] >> 8).astype(np.uint8)
+
+
+def get(blk, at, row):
+    byte, shift, s_at, m_at = (t[row] for t in at)
+    c = (blk[byte] >> shift.astype(np.uint8)) & 15
+    s, m = ((blk[x[::64]].astype(np.uint16) | (blk[x[::64] + 1].astype(np.uint16) << 8)) for x in (s_at, m_at))
+    return c, s, m
+
+
+class Batch4(Batch):
+    """A Batch whose pages are held in 4 bits: .kq and .vq [n_pages][n_kv][page/32][4608] bytes. Rows that no token
+    sees, and pages without rows, hold random codes with s and m NaN."""
+
+    def __init__(self, lens, new, *args, **kw):
+        self.where = []
+        super().__init__(lens, new, *args, **kw)
+        shape = (self.n_pages, self.n_kv, self.page // 32, BLOCK)
+        self.kq, self.vq = (self.r.integers(0, 256, shape).astype(np.uint8) for _ in range(2))
+        for q in (self.kq, self.vq):
+            q[..., 4096::2], q[..., 4097::2] = 0xC1, 0x7F
+        for b in range(self.B):
+            j = np.array([j for c, j in self.where if c == b], np.int64)
+            for q, at in ((self.kq, K_AT), (self.vq, V_AT)):
+                put_rows(q, at, self.table[b, j // self.page], j % self.page, *quantise(W.normal(self.r, (len(j), self.n_kv, HD)).astype(np.float64)))
+
+    def put_row(self, b, j, k, v):
+        self.where.append((b, j))
+
+    def set_row(self, b, j, k, v):
+        """Rows k, v [n_kv][256], quantised."""
+        p, at = self.table[b, j // self.page], j % self.page
+        for x, q, where in ((k, self.kq, K_AT), (v, self.vq, V_AT)):
+            for h, row in enumerate(zip(*quantise(np.asarray(x, np.float64)))):
+                put(q[p, h, at // 32], where, at % 32, *row)
+
+    def held(self, b):
+        """(codes [rows][n_kv][256], s, m [rows][n_kv][4]) of K and of V of sequence b."""
+        out = []
+        for q, (byte, shift, s_at, m_at) in ((self.kq, K_AT), (self.vq, V_AT)):
+            n = self.lens[b]
+            blk = q[self.table[b, :-(-n // self.page)]].transpose(0, 2, 1, 3)     # [pages][blocks][n_kv][4608]
+            blk = blk.reshape(-1, self.n_kv, BLOCK)
+            c = (blk[:, :, byte] >> shift.astype(np.uint8)) & 15                   # [blocks][n_kv][32][256]
+            s, m = (blk[:, :, x[:, ::64]].astype(np.uint16) | (blk[:, :, x[:, ::64] + 1].astype(np.uint16) << 8) for x in (s_at, m_at))
+            out.append([x.transpose(0, 2, 1, 3).reshape(-1, self.n_kv, x.shape[-1])[:n] for x in (c, s, m)])
+        return out
+
+    def result(self, gate=True, q=None):
+        """As Batch.result, over the values of the codes; W and S from the magnitudes of their terms, s c + |m|."""
+        q = f64(self.q) if q is None else q
+        out, Wt = np.zeros((self.N, self.n_q, HD)), np.zeros((self.N, self.n_q, HD))
+        lse, S = np.full((self.N, self.n_q), -np.inf), np.zeros((self.N, self.n_q))
+        for b in range(self.B):
+            if not self.lens[b] or not self.new[b]:
+                continue
+            (kc, ks, km), (vc, vs, vm) = self.held(b)
+            seen, t0 = self.seen(b), self.start[b]
+            ok = seen.any(0)
+            k, v = values(kc, ks, km), values(vc, vs, vm)
+            absm = lambda m: (m & 0x7FFF).astype(np.uint16)  # noqa: E731
+            ka, va = values(kc, ks, absm(km)), values(vc, vs, absm(vm))
+            for x in (k, v, ka, va):
+                x[~ok] = 0
+            for h in range(self.n_q):
+                g = h // self.qg
+                qq = q[t0:t0 + self.new[b], h]
+                with np.errstate(all="ignore"):
+                    s = np.where(seen, qq @ k[:, g].T / 16.0, -np.inf)
+                    m = s.max(1, keepdims=True)
+                    p = np.where(seen, np.exp(s - np.where(np.isfinite(m), m, 0)), 0.0)
+                    l = p.sum(1, keepdims=True)
+                    w = np.where(l > 0, p / l, 0.0)
+                    lse[t0:t0 + self.new[b], h] = (m + np.log(l))[:, 0]
+                out[t0:t0 + self.new[b], h] = w @ v[:, g]
+                Wt[t0:t0 + self.new[b], h] = w @ va[:, g]
+                S[t0:t0 + self.new[b], h] = (np.where(seen, np.abs(qq) @ ka[:, g].T, 0) / 16.0).max(1)
+        if gate:
+            x = 1.0 / (1.0 + np.exp(-self.gate.astype(np.float64)))
+            out *= x
+            Wt *= x
+        return {"out": out, "lse": lse, "W": Wt, "S": S}
+
+
+def out_tol(res, keys, out_bf16, part_err):
+    """Elementwise bound of the attention output's error, relative to the sum of p (s c + |m|) (W): twice the error of a
+    score (256 products and their sums in fp32: score_err of the sum of |q| (s c + |m|)), 2^-20 for exp2 and its
+    argument, 3 * keys * 2^-24 for sums over up to `keys` rows, and the rounding of the weights: `part_err`, 2^-8 for one
+    bf16 part, 2^-16 for two; and 2^-8 of the output where it is bf16."""
+    rel = 2 * score_err(res["S"])[..., None] + 2.0 ** -20 + 3 * keys * 2.0 ** -24 + part_err
+    return 1.01 * rel * res["W"] + (2.0 ** -8 * np.abs(res["out"]) if out_bf16 else 0.0) + 1e-30
+
+
+def frequencies(rope_dim, theta):
+    """The library's fp32 RoPE frequencies: the C library's powf(theta, -2 i / rope_dim)."""
+    powf = C.CDLL("libm.so.6").powf
+    powf.restype, powf.argtypes = C.c_float, [C.c_float, C.c_float]
+    return np.array([powf(theta, np.float32(-2.0 * i) / np.float32(rope_dim)) for i in range(rope_dim // 2)], np.float32)
+
+
+def norm_rope(x, w, pos, rope_dim, theta, yarn=1.0, plus_one=True):
+    """Rows x [N][heads][256] normed and rotated in float64; the angles are fp32."""
+    x = x.astype(np.float64)
+    x = x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6) * (w.astype(np.float64) + (1.0 if plus_one else 0.0))
+    h = rope_dim // 2
+    if h:
+        ang = (pos.astype(np.float32) / np.float32(yarn))[:, None] * frequencies(rope_dim, theta)
+        c, s = np.cos(ang.astype(np.float64))[:, None], np.sin(ang.astype(np.float64))[:, None]
+        a, b = x[..., :h].copy(), x[..., h:2 * h].copy()
+        x[..., :h], x[..., h:2 * h] = a * c - b * s, a * s + b * c
+    return x

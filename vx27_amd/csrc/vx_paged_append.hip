@@ -5,7 +5,7 @@
 // Per head (vx27_qfwd.c:172-186): s = 1/sqrt(mean(x^2) + 1e-6), y = x s (1+w)
 // (or x s w), the first rope_dim dims rotated as NeoX halves by the angle
 // (pos / yarn) * freq_i (fp32, as every kernel of this library forms it).
-#include "vx_paged.h"
+#include "vx_paged_q4.h"
 
 int vx_paged_fill(const char *who, vx_paged &p, int B, int n_kv, int hd, int page_size, int n_pages,
                   int max_pages, const int *table, const int *len) {
@@ -90,6 +90,174 @@ __device__ __forceinline__ double wave_sums4(const double (&s)[4]) {
     return v;
 }
 
+// ---------------------------------------------------------- 4-bit pages
+// A row's group is 16 lanes of 4 dims.  Everything is in fp64: k's values carry
+// errors of the norm's sum, the angles and the products, and in fp32 these
+// would move a code now and then (one value in 10^6) against another order of
+// the sums; in fp64 the codes are those of the exact values.
+constexpr float BF16_MAX = 3.38953139e38f;
+template <bool MAX>
+__device__ __forceinline__ double over_group(double x) {   // maximum or minimum over 16 lanes
+    auto pick = [](double u, double v) { return MAX ? fmax(u, v) : fmin(u, v); };
+    x = pick(x, vx_dpp_f64<0xB1, 0xF>(x));
+    x = pick(x, vx_dpp_f64<0x4E, 0xF>(x));
+    x = pick(x, vx_dpp_f64<0x124, 0xF>(x));
+    return pick(x, vx_dpp_f64<0x128, 0xF>(x));
+}
+// The bf16 number at or beyond x, down or up (|x| at most BF16_MAX), as the
+// bits of an fp32 number: the truncated bits, or a step on.
+__device__ __forceinline__ uint32_t bf16_below(double x) {
+    const uint32_t b = __float_as_uint((float)x) & 0xffff0000u;
+    if ((double)__uint_as_float(b) <= x) return b;
+    return (b & 0x7fffffffu) == 0 ? 0x80010000u : b & 0x80000000u ? b + 0x10000u : b - 0x10000u;
+}
+__device__ __forceinline__ uint32_t bf16_above(double x) {   // x >= 0
+    const uint32_t b = __float_as_uint((float)x) & 0xffff0000u;
+    return (double)__uint_as_float(b) >= x ? b : b + 0x10000u;
+}
+// The codes of a lane's four values as bytes, and its group's s and m (bits 16
+// to 31 of each).
+__device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_bits, uint32_t &m_bits) {
+    const int lane = threadIdx.x & 63;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 4; e++) fine &= __builtin_fabs(y[e]) <= (double)BF16_MAX;
+    const uint64_t off = __ballot(!fine);
+    if ((off >> (lane & 48)) & 0xffff) {
+        s_bits = 0;
+        m_bits = 0x7fc00000u;
+        return 0;
+    }
+    m_bits = bf16_below(over_group<false>(fmin(fmin(y[0], y[1]), fmin(y[2], y[3]))));
+    const double m = __uint_as_float(m_bits);
+    s_bits = bf16_above((over_group<true>(fmax(fmax(y[0], y[1]), fmax(y[2], y[3]))) - m) / 15.0);
+    const double s = __uint_as_float(s_bits);
+    if (s == 0.0) return 0;
+    const double rs = 1.0 / s;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        // the nearest code, and what it leaves (exact): a product with 1/s may
+        // be a last place off where the quotient is just between two
+        const double d = y[e] - m;
+        double c = __builtin_rint(d * rs);
+        const double r = 2.0 * __builtin_fma(-c, s, d);
+        if (__builtin_fabs(r) > s || (__builtin_fabs(r) == s && ((int)c & 1))) c += r > 0.0 ? 1.0 : -1.0;
+        codes |= (uint32_t)min(max((int)c, 0), 15) << (8 * e);
+    }
+    return codes;
+}
+
+// One KV head's new rows [lo, hi) of the block at row p0 of sequence b: a row a
+// wave, its codes into LDS by bytes; then thread u stores 16-byte unit u of the
+// block, or of V, where 8 rows share one, as much of it as is new.
+constexpr int CODE_ROW = HDG + 4;             // (rows 8 apart then lie in different banks)
+constexpr int Q4_CS = 512;                    // (cos, sin) of a chunk of rows
+constexpr int Q4_LDS = VB * CODE_ROW + Q4_CS * 16 + 4 * HDG * 8;
+__device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int lo, int hi, int tok0, char *lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = hi - lo, half = a.rope_dim / 2;
+    const int page = vx_paged_page(a.p, b, p0), at = p0 - vx_page_slot(a.p, p0) * a.p.page_size;
+    const size_t block = (size_t)vx_q4_block(a.p, page, hk, at) * VX_Q4_BLOCK;
+    char *codes = lds;
+    double2 *cs = (double2 *)(lds + VB * CODE_ROW);
+    double *row = (double *)(lds + VB * CODE_ROW + Q4_CS * 16) + wave * HDG;
+    auto store = [&](char *blk, int j, const double (&y)[4], bool is_v) {
+        const int r = lo - p0 + j;
+        uint32_t s, m;
+        *(uint32_t *)(codes + r * CODE_ROW + 4 * lane) = quantise(y, s, m);
+        if ((lane & 15) == 0) {
+            const int c = lane >> 4;
+            *(uint16_t *)(blk + VX_Q4_S + c * 64 + r * 2) = (uint16_t)(s >> 16);
+            *(uint16_t *)(blk + VX_Q4_M + (is_v ? c * 64 + r * 2 : r * 8 + c * 2)) = (uint16_t)(m >> 16);
+        }
+    };
+    // V
+    char *vb = (char *)a.v_pages + block;
+    for (int j = wave; j < n; j += 4) {
+        const float4 x = load4(a.v, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16);
+        const double y[4] = {x.x, x.y, x.z, x.w};
+        store(vb, j, y, true);
+    }
+    __syncthreads();
+    {
+        const int dim = 64 * (tid >> 6) + (tid & 15), r8 = 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 16 i, rows r8 .. r8 + 7
+        uint32_t fresh = 0;                                                        // its new rows
+        for (int k = 0; k < 8; k++) fresh |= p0 + r8 + k >= lo && p0 + r8 + k < hi ? 1u << k : 0u;
+        if (fresh) {
+            uint4 *dst = (uint4 *)(vb + tid * 16);
+            uint32_t u[4] = {0, 0, 0, 0}, mask = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (!((fresh >> k) & 1)) continue;
+                const int at_bit = 8 * (k & 3) + (k & 4);
+                mask |= 15u << at_bit;
+#pragma unroll
+                for (int i = 0; i < 4; i++) u[i] |= (uint32_t)codes[(r8 + k) * CODE_ROW + dim + 16 * i] << at_bit;
+            }
+            if (fresh != 255) {
+                const uint4 old = *dst;
+                u[0] |= old.x & ~mask; u[1] |= old.y & ~mask; u[2] |= old.z & ~mask; u[3] |= old.w & ~mask;
+            }
+            *dst = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+    __syncthreads();
+    // K
+    char *kb = (char *)a.k_pages + block;
+    const float4 wf = ((const float4 *)a.k_norm_w)[lane];
+    const double one = (a.flags & VX27_GQA_NORM_W) ? 0.0 : 1.0;
+    const double w[4] = {wf.x + one, wf.y + one, wf.z + one, wf.w + one};
+    const int chunk = half ? min(Q4_CS / half, VB) : VB;
+    for (int j0 = 0; j0 < n; j0 += chunk) {
+        const int j1 = min(j0 + chunk, n);
+        for (int e = tid; e < (j1 - j0) * half; e += 256) {
+            const int j = j0 + e / half, i = e % half;
+            double sn, c;
+            sincos((double)vx_rope_angle(a.rope.freq[i], a.pos ? a.pos[tok0 + j] : lo + j, a.yarn), &sn, &c);
+            cs[e] = make_double2(c, sn);
+        }
+        __syncthreads();
+        for (int j = j0 + wave; j < j1; j += 4) {
+            const float4 x = load4(a.k, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16);
+            double y[4] = {x.x, x.y, x.z, x.w};
+            double ss = y[0] * y[0];
+#pragma unroll
+            for (int e = 1; e < 4; e++) ss = __builtin_fma(y[e], y[e], ss);
+            const double sc = 1.0 / sqrt(vx_wave_sum_f64_dpp(ss) / HDG + 1e-6);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = y[e] * sc * w[e];
+            if (half) {
+                *(double2 *)(row + 4 * lane) = make_double2(y[0], y[1]);
+                *(double2 *)(row + 4 * lane + 2) = make_double2(y[2], y[3]);
+                __builtin_amdgcn_wave_barrier();   // (one wave's LDS operations complete in order)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = 4 * lane + e;
+                    if (i >= 2 * half) continue;
+                    const bool second = i >= half;
+                    const double2 c = cs[(j - j0) * half + (second ? i - half : i)];
+                    const double z = row[second ? i - half : i + half] * c.y;
+                    y[e] = y[e] * c.x + (second ? z : -z);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+            store(kb, j, y, false);
+        }
+        __syncthreads();
+    }
+    const int r = vx_q4_k_row(tid), dim = 128 * ((tid >> 6) & 1) + 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 32 i .. + 7 of row r
+    if (p0 + r >= lo && p0 + r < hi) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t *c = (const uint32_t *)(codes + r * CODE_ROW + dim + 32 * i);
+            u[i] = c[0] | (c[1] << 4);
+        }
+        *(uint4 *)(kb + tid * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
 // grid (5 a 32-row block that a sequence's tokens can touch, n_kv, B), block
 // 256.  Of a block's five workgroups the first takes one KV head's keys and V
 // block, the others the group's query heads of 8 tokens each: a prompt's
@@ -105,7 +273,7 @@ __device__ __forceinline__ double wave_sums4(const double (&s)[4]) {
 // goes through LDS into the dim-major block, element by element at its ends
 // so that other rows keep their contents.  HALFS: most angles a token has.
 constexpr int QTOK = 8;
-template <int HALFS>
+template <int HALFS, bool Q4>
 __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     constexpr int NR = 4;
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
@@ -115,7 +283,8 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     if (!is_k && !a.q) return;
     // v's rows; then the tokens' cos and sin, and a row a wave
     constexpr int CS = VB * HALFS * 4;
-    __shared__ __attribute__((aligned(16))) char lds[2 * CS + 4 * HDG * 4 > VB * HDG * 2 ? 2 * CS + 4 * HDG * 4 : VB * HDG * 2];
+    constexpr int ROTATE = 2 * CS + 4 * HDG * 4, OTHER = Q4 ? Q4_LDS : VB * HDG * 2;
+    __shared__ __attribute__((aligned(16))) char lds[ROTATE > OTHER ? ROTATE : OTHER];
     float (*cs)[HALFS] = (float (*)[HALFS])lds, (*sn)[HALFS] = (float (*)[HALFS])(lds + CS);
     uint16_t (*vt)[HDG] = (uint16_t (*)[HDG])lds;
     const vx_pseq s = vx_paged_seq(a.p, b);
@@ -126,6 +295,9 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     const int lo = max(q0, first), hi = min(q0 + (is_k ? VB : QTOK), s.len);
     if (lo >= hi) return;
     const int n = hi - lo, tok0 = s.start + (lo - s.row0), half = a.rope_dim / 2;
+    if constexpr (Q4) {
+        if (is_k) return append_q4_block(a, hk, b, p0, lo, hi, tok0, lds);
+    }
     const int per = is_k ? 1 : a.qg, rows = n * per;      // heads of a token
     const uint32_t magic = is_k ? 0 : a.qg_magic;
     const void *src = is_k ? a.k : a.q;
@@ -236,8 +408,10 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
 
 }  // namespace
 
-extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) {
-    static const char who[] = "vx27_hip_paged_append";
+namespace {
+
+template <bool Q4>
+int append(const char *who, vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) {
     VX_REQUIRE(d != nullptr, "%s: null descriptor", who);
     AppendArgs a = {};
     if (vx_paged_fill(who, a.p, d->B, d->n_kv, d->hd, d->page_size, d->n_pages, d->max_pages, d->table, d->len)) return -1;
@@ -263,6 +437,7 @@ extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_
                "%s: q, k_new and v_new must be %d-byte aligned with strides multiples of 4 elements", who, (int)al + 1);
     VX_REQUIRE((((uintptr_t)d->q_norm_w | (uintptr_t)d->k_norm_w | (uintptr_t)d->q_out | (uintptr_t)d->k_pages | (uintptr_t)d->v_pages) & 15) == 0,
                "%s: q_norm_w, k_norm_w, q_out and the pages must be 16-byte aligned", who);
+    if (Q4 && vx_q4_fits(who, d->n_pages, d->n_kv, d->page_size)) return -1;
     if (vx_ctx_enter(ctx)) return -1;
     if (d->n_tok == 0) return 0;
     a.p.err_flag = ctx->err_flag;
@@ -274,7 +449,17 @@ extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_
     a.q_out = d->q_out; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
     const dim3 grid(((d->max_T + VB - 2) / VB + 1) * (1 + VB / QTOK), d->n_kv, d->B);
     // (32 angles a token take 16 KiB of LDS, 128 take 36: the 143 MB prompt takes 49 us with the first, 62 with the second)
-    if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<32>), grid, dim3(256), a);
-    else VX_LAUNCH_NAMED(ctx, "paged_append", (paged_append<MAXR>), grid, dim3(256), a);
+    if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<32, Q4>), grid, dim3(256), a);
+    else VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<MAXR, Q4>), grid, dim3(256), a);
     return 0;
+}
+
+}  // namespace
+
+extern "C" int vx27_hip_paged_append(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) {
+    return append<false>("vx27_hip_paged_append", ctx, d);
+}
+
+extern "C" int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) {
+    return append<true>("vx27_hip_paged_append_q4", ctx, d);
 }

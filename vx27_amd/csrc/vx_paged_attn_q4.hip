@@ -1,0 +1,371 @@
+// Attention over a paged 4-bit KV cache on gfx950 (layout: vx_paged_q4.h):
+// what vx27_hip_paged_attn computes, over the values that the codes stand for.
+//
+// With a row's scales s_g and minima m_g of its four groups of 64 dims,
+//   q . k_j = sum_g s_jg (q_g . c_jg) + m_jg (sum of q_g)
+//   sum_j p_j v_j = sum_j (p_j s_jg) c_jg + p_j m_jg      for the dims of group g,
+// so no dim is ever decoded: the codes are exact bf16 operands, s multiplies
+// the scores of a group on their way out of the MFMAs and the weights on their
+// way in, and the minima's sums are MFMAs of their own (one for 16 keys' scores,
+// one for a tile's outputs).
+#include "vx_paged_q4.h"
+#include "vx_paged_rows.h"
+
+namespace {
+
+constexpr int GROUPS = HDG / VX_Q4_GROUP;
+
+// A lane's share of a tile's K and of its V.
+struct KTile {
+    uint4 c[4], s[GROUPS];
+    uint2 m[2];
+};
+struct VTile {
+    uint4 c[4], s[GROUPS], m;
+};
+__device__ __forceinline__ uint4 load16_nt(const char *p) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 x = __builtin_nontemporal_load((const u32x4 *)p);
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void load_k(const Args &a, uint32_t block, KTile &k) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const char *p = (const char *)a.k_pages + (size_t)block * VX_Q4_BLOCK;
+#pragma unroll
+    for (int j = 0; j < 4; j++) k.c[j] = load16_nt(p + (64 * j + lane) * 16);
+#pragma unroll
+    for (int j = 0; j < GROUPS; j++) k.s[j] = *(const uint4 *)(p + VX_Q4_S + j * 64 + g * 16);
+#pragma unroll
+    for (int r = 0; r < 2; r++) k.m[r] = *(const uint2 *)(p + VX_Q4_M + (8 * (n >> 2) + 4 * r + (n & 3)) * 8);
+}
+__device__ __forceinline__ void load_v(const Args &a, uint32_t block, VTile &v) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const char *p = (const char *)a.v_pages + (size_t)block * VX_Q4_BLOCK;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v.c[j] = load16_nt(p + (64 * j + lane) * 16);
+#pragma unroll
+    for (int j = 0; j < GROUPS; j++) v.s[j] = *(const uint4 *)(p + VX_Q4_S + j * 64 + g * 16);
+    v.m = *(const uint4 *)(p + VX_Q4_M + (n & 3) * 64 + g * 16);
+}
+__device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// One wave's state for ROWS query rows: 16, or 8 that take the 16 columns
+// twice, the first with the weights rounded to bf16 and the second with what
+// that left (two parts at the price of one).
+template <int ROWS>
+struct Rows {
+    bf16x8_t q[8], qs;           // qs: the groups' sums of q against the minima
+    floatx4_t o[16], om;         // om: lanes g = 0, element e: group e's sum of p m
+    float m, l;
+};
+template <int ROWS>
+__device__ __forceinline__ void rows_begin(const Args &a, const vx_pseq &s, int kvh, int r0, Rows<ROWS> &w) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, r = r0 + n % ROWS, t = row_tok(a, r);
+    const bool live = t < s.T;
+    const uint16_t *qp = a.q + (size_t)(s.start + (live ? t : 0)) * a.q_ts + (size_t)(live ? row_head(a, kvh, r, t) : 0) * a.q_hs + 8 * g;
+#pragma unroll
+    for (int k = 0; k < 8; k++) w.q[k] = load8(qp + 32 * k);
+    if (!live) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) w.q[k][e] = (__bf16)0.0f;
+    }
+    // The sums in three bf16 parts (all 24 bits): k-slots 0-3 and 4-7 of lane
+    // group 0 and 0-3 of group 1, against operands that hold the minima in
+    // each of these places.
+#pragma unroll
+    for (int e = 0; e < 8; e++) w.qs[e] = (__bf16)0.0f;
+#pragma unroll
+    for (int c = 0; c < GROUPS; c++) {
+        float x = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x += (float)w.q[2 * c][e] + (float)w.q[2 * c + 1][e];
+        x += __shfl_xor(x, 16, 64);
+        x += __shfl_xor(x, 32, 64);
+        const __bf16 hi = (__bf16)x, mid = (__bf16)(x - (float)hi), lo = (__bf16)(x - (float)hi - (float)mid);
+        w.qs[c] = g == 0 ? hi : g == 1 ? lo : (__bf16)0.0f;
+        w.qs[4 + c] = g == 0 ? mid : (__bf16)0.0f;
+    }
+#pragma unroll
+    for (int d = 0; d < 16; d++) w.o[d] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+    w.om = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+    w.m = -INFINITY;
+    w.l = 0.0f;
+}
+
+// Scores of 32 keys: lane (g,n) gets keys 8g + 0..7 of row n.
+template <int ROWS>
+__device__ __forceinline__ void score_tile(const KTile &k, const Rows<ROWS> &w, float (&s)[8]) {
+    floatx4_t acc[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const uint4 m = make_uint4(k.m[r].x, k.m[r].y, k.m[r].x, k.m[r].y);
+        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, m), w.qs, (floatx4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    }
+#pragma unroll
+    for (int c = 0; c < GROUPS; c++) {
+        float sc[8];
+        vx_q4_f32(k.s[c], sc);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            floatx4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(k.c[2 * r + c / 2], 2 * (c & 1) + i)), w.q[2 * c + i], x, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[r][e] = __builtin_fmaf(x[e], sc[4 * r + e], acc[r][e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3];
+}
+
+// Two weights in bf16; `rest`, a lane mask of all ones or zeros: what rounding
+// them leaves instead.
+template <int ROWS>
+__device__ __forceinline__ uint32_t weights2(float x, float y, uint32_t rest) {
+    const uint32_t h = pack2(x, y);
+    if (ROWS == 16) return h;
+    return pack2(x - __uint_as_float((h << 16) & rest), y - __uint_as_float(h & 0xffff0000u & rest));
+}
+template <int ROWS>
+__device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], uint32_t rest) {
+    uint4 u;
+    u.x = weights2<ROWS>(x[0], x[1], rest);
+    u.y = weights2<ROWS>(x[2], x[3], rest);
+    u.z = weights2<ROWS>(x[4], x[5], rest);
+    u.w = weights2<ROWS>(x[6], x[7], rest);
+    return __builtin_bit_cast(bf16x8_t, u);
+}
+
+// Online softmax and P V of one tile for R rows.  s and m of keys that no row
+// sees become zero, so that what stale rows hold cannot get in.  `one`: the
+// rows are of one token, so that all see the same keys.
+template <int ROWS>
+__device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, const float (&s)[8], const vx_sight &v, int key0, VTile &vt) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t rest = ROWS == 8 && (lane & 8) ? 0xffffffffu : 0u;
+    float x[8], p[8];
+    float mt = -INFINITY;
+    uint32_t sees = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const bool see = v.sees(key0 + 8 * g + e);
+        sees |= see ? 1u << e : 0u;
+        x[e] = see ? s[e] : -INFINITY;
+        mt = fmaxf(mt, x[e]);
+    }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
+    const float m_new = fmaxf(w.m, mt * SC2);
+    const bool none = m_new == -INFINITY;
+    const float ref = none ? 0.0f : m_new;
+    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(w.m - m_new);
+    float ls = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -ref));
+        ls += p[e];
+    }
+    w.l = w.l * alpha + ls;
+    w.m = m_new;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < 16; d++) w.o[d] *= alpha;
+        w.om *= alpha;
+    }
+    bf16x8_t m = __builtin_bit_cast(bf16x8_t, vt.m);
+    if (!__all(sees == 0xffu)) {
+        const uint32_t group = (1u << R) - 1;
+        uint32_t keep[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) keep[i] = ((sees >> (2 * i)) & 1 ? 0xffffu : 0u) | ((sees >> (2 * i)) & 2 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int c = 0; c < GROUPS; c++) vt.s[c] = make_uint4(vt.s[c].x & keep[0], vt.s[c].y & keep[1], vt.s[c].z & keep[2], vt.s[c].w & keep[3]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool see = (sees >> e) & 1;
+            // which of a lane group's rows see its key 8g + e
+            const uint32_t mine = (uint32_t)(__ballot(see) >> (16 * g)) & group;
+            if (mine == 0) m[e] = (__bf16)0.0f;
+            if (one || !__any(mine != 0 && mine != group)) continue;
+            // A key that some rows see and others do not, with a minimum of NaN
+            // (a group that held an infinity or a NaN): 0 times that would
+            // reach the others.  It goes to the rows that see it by addition
+            // and out of the product.
+            const bool odd = !is_finite((float)m[e]);
+            uint64_t bad = __ballot(odd && mine);
+            while (bad) {
+                const int gk = __builtin_ctzll(bad) >> 4;
+                bad &= ~(0xffffull << (16 * gk));
+                const bool own = v.sees(key0 + 8 * gk + e);
+#pragma unroll
+                for (int c = 0; c < GROUPS; c++) {
+                    const float y = __shfl((float)m[e], 16 * gk + c, 64);
+                    if (own && !is_finite(y)) w.om[c] += y;
+                }
+            }
+            if (odd) m[e] = (__bf16)0.0f;
+        }
+    }
+    w.om = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, weights8<ROWS>(p, rest), w.om, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < GROUPS; c++) {
+        float y[8];
+        vx_q4_f32(vt.s[c], y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] *= p[e];
+        const bf16x8_t pw = weights8<ROWS>(y, rest);
+#pragma unroll
+        for (int i = 0; i < 4; i++) w.o[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(vt.c[c], i)), pw, w.o[4 * c + i], 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ float add_half_row(float x) {   // the lane's value and that of lane ^ 8
+    return x + __int_as_float(vx_dpp_i<0x128, 0xF>(__float_as_int(x)));
+}
+
+// The list of tiles is cut evenly over the workgroups, as the bf16 pages' (see
+// paged_split): every (sequence, KV head, block of ROWS query rows) takes its
+// tiles, wave w of a workgroup tiles w, w + 4, ...
+template <int ROWS>
+__global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __attribute__((aligned(16))) float s_o[4][ROWS * HDG];
+    __shared__ float s_m[4][ROWS], s_l[4][ROWS];
+    const Units un = units_of<true>(a, gridDim.x);
+    const int u0 = blockIdx.x * un.chunk, u1 = min(u0 + un.chunk, un.total);
+    if (u0 >= u1) return;
+    int b = units_find(a, un, u0);
+    vx_pseq s;
+    vx_tiles tl;
+    int before = units_before<true>(a, un, b, s, tl);
+    for (int u = u0; u < u1;) {
+        const int nb = seq_blocks<true>(a, s), all = tl.nt * a.p.n_kv * nb;
+        if (u >= before + all) {
+            before += all;
+            b++;
+            if (a.p.B <= 64) units_before<true>(a, un, b, s, tl);
+            else seq_units<true>(a, b, s, tl);
+            continue;
+        }
+        const int item = (u - before) / tl.nt, i0 = (u - before) - item * tl.nt;
+        const int kvh = item / nb, r0 = (item - kvh * nb) * ROWS;
+        const int cnt = min(tl.nt - i0, u1 - u);
+        const int R = min(s.T * a.qg - r0, ROWS);
+        Rows<ROWS> w;
+        rows_begin<ROWS>(a, s, kvh, r0, w);
+        const vx_sight v = sight_of(a, s, r0 + min(n % ROWS, R - 1));   // (columns past the last row: as the last, unused)
+        const int mine = (cnt - wave + 3) / 4;      // this wave's tiles: i0 + wave + 4 j
+        // lane i holds the block of this wave's tile 64 k + i
+        uint32_t blocks = 0;
+        auto look_up = [&](int j) {
+            const int key = tl.at(i0 + wave + 4 * min(j + lane, mine - 1)) * TILE;
+            const int page = vx_paged_page(a.p, b, key);
+            blocks = vx_q4_block(a.p, page, kvh, key - vx_page_slot(a.p, key) * a.p.page_size);
+        };
+        KTile kt;
+        VTile vt;
+        if (mine > 0) {
+            look_up(0);
+            load_k(a, __builtin_amdgcn_readlane(blocks, 0), kt);
+        }
+        for (int j = 0; j < mine; j++) {
+            load_v(a, __builtin_amdgcn_readlane(blocks, j & 63), vt);
+            float sc[8];
+            score_tile<ROWS>(kt, w, sc);
+            __builtin_amdgcn_sched_barrier(0);   // (the next K's loads into the registers of this one's)
+            if (((j + 1) & 63) == 0) look_up(j + 1);
+            if (j + 1 < mine) load_k(a, __builtin_amdgcn_readlane(blocks, (j + 1) & 63), kt);
+            attend_tile<ROWS>(w, R, s.T == 1, sc, v, tl.at(i0 + wave + 4 * j) * TILE, vt);
+        }
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+#pragma unroll
+        for (int c = 0; c < GROUPS; c++) {
+            float om = w.om[c];
+            if (ROWS == 8) om = add_half_row(om);
+            om = __shfl(om, n, 64);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) w.o[4 * c + i][e] = (ROWS == 8 ? add_half_row(w.o[4 * c + i][e]) : w.o[4 * c + i][e]) + om;
+        }
+        // the four waves' results through LDS (16-byte units swizzled by the row)
+        if (n < R) {
+#pragma unroll
+            for (int d = 0; d < 16; d++) *(floatx4_t *)&s_o[wave][n * HDG + (((4 * d + g) ^ n) << 2)] = w.o[d];
+            if (g == 0) {
+                s_m[wave][n] = w.m;
+                s_l[wave][n] = w.l;
+            }
+        }
+        __syncthreads();
+        // wave w merges rows w, w + 4, ..., lane L dims 4L .. 4L + 3
+        const bool whole = cnt == tl.nt;
+        const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
+        for (int r = wave; r < R; r += 4) {
+            const int t = row_tok(a, r0 + r), tok = s.start + t, h = row_head(a, kvh, r0 + r, t);
+            float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (whole && a.gate) gt = gate_row(a, tok, h);
+            float m[4], l[4];
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                m[k] = s_m[k][r];
+                l[k] = s_l[k][r];
+                o[k] = *(const float4 *)&s_o[k][r * HDG + ((lane ^ r) << 2)];
+            }
+            const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            float L = 0.0f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) add_part(O, L, o[k], l[k], m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - M));
+            if (whole) {
+                row_finish(a, tok, h, O, M, L, gt);
+            } else {
+                *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + r) * HDG + 4 * lane) = O;
+                if (lane == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
+            }
+        }
+        __syncthreads();
+        u += cnt;
+    }
+}
+
+}  // namespace
+
+extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d) {
+    static const char who[] = "vx27_hip_paged_attn_q4";
+    VX_REQUIRE(d != nullptr, "%s: null descriptor", who);
+    VX_REQUIRE(!d->acc, "%s: acc must be NULL (the rows' weights are added up over bf16 pages only)", who);
+    if (vx_q4_fits(who, d->n_pages, d->n_kv, d->page_size)) return -1;
+    Args a = {};
+    const int todo = attn_fill(who, ctx, d, a);
+    if (todo <= 0) return todo;
+    const int rows = d->max_T * a.qg;
+    // two parts of the weights where the output is fp32, one where it is rounded to bf16 itself
+    a.block_rows = a.out_bf16 ? 16 : 8;
+    const int nb = (rows + a.block_rows - 1) / a.block_rows;
+    const int64_t units = (int64_t)d->B * d->n_kv * nb * a.tile_cap;
+    VX_REQUIRE(units < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %d tiles each)", who, d->B, d->n_kv, a.tile_cap);
+    a.min_tiles = 2;
+    const int grid = (int)std::min<int64_t>((units + a.min_tiles - 1) / a.min_tiles, 2 * ctx->n_cu);
+    a.part_rows = std::min(rows, a.block_rows);
+    const size_t n_part = (size_t)2 * grid * a.part_rows;
+    const size_t o_bytes = n_part * HDG * 4, ml_bytes = (n_part * sizeof(float2) + 255) / 256 * 256;
+    const size_t before_bytes = d->B > 64 ? ((size_t)d->B + 1) * sizeof(int) : 0;
+    void *scr;
+    if (vx_ctx_scratch(ctx, o_bytes + ml_bytes + before_bytes, &scr)) return -1;
+    a.part_o = (float *)scr;
+    a.part_ml = (float2 *)((char *)scr + o_bytes);
+    a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes) : nullptr;
+    if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true>), dim3(1), dim3(1024), a);
+    if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16>), dim3(grid), dim3(256), a);
+    else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8>), dim3(grid), dim3(256), a);
+    VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<true>), dim3(a.part_rows, d->n_kv * nb, d->B), dim3(256), a, grid);
+    return 0;
+}

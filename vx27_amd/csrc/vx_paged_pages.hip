@@ -1,0 +1,353 @@
+// The paged KV cache's pages on gfx950: rows and pages of a step planned on
+// the device, and the values of 4-bit rows read by slot.
+//
+// The plan is prefix sums over the sequences: pages given back, pages wanted
+// (which sequences can be served), tokens (which fit the call), and of those
+// that remain the pages and tokens before each.  Everything else follows from
+// these: token i's sequence is the last with at most i tokens before it, the
+// k-th page taken is entry total - 1 - k of the free pages with the released
+// ones on top.
+#include <algorithm>
+
+#include "vx_paged_q4.h"
+
+namespace {
+
+struct PlanArgs {
+    int B, page_size, n_pages, max_pages, n_tok, log2_page;
+    const int *new_tok, *ended, *len, *next_pos, *n_free;
+    int *table, *free_pages;
+    int *took, *q_start, *len_out, *next_pos_out, *n_free_out, *slot, *pos, *seq;
+    int *err_flag;
+    // scratch: pages given back and pages taken before each sequence, and in all (index B); free pages before the call
+    int *back, *grown, *was_free;
+};
+
+// What the second half of a plan reads: q_start, back and grown, global or in LDS.
+struct PlanSums {
+    const int *start, *back, *grown;
+    int was_free, released, taken;
+};
+
+__device__ __forceinline__ int plan_ceil(const PlanArgs &a, int n) {   // pages of n rows
+    return a.log2_page >= 0 ? (int)(((uint32_t)n + (uint32_t)a.page_size - 1) >> a.log2_page) : (n + a.page_size - 1) / a.page_size;
+}
+// The last b in [0, n) with at[b] <= x (at[0] = 0 <= x).
+__device__ __forceinline__ int last_le(const int *at, int n, int x) {
+    int lo = 0;
+    while (n > 1) {
+        const int h = n >> 1;
+        if (at[lo + h] <= x) lo += h, n -= h;
+        else n = h;
+    }
+    return lo;
+}
+__device__ __forceinline__ int checked_page(const PlanArgs &a, int pg) {
+    const int c = min(max(pg, 0), a.n_pages - 1);
+    if (c != pg) *a.err_flag = 1;
+    return c;
+}
+// Entry i of the free pages with the released ones on top.
+__device__ __forceinline__ int stack_page(const PlanArgs &a, const PlanSums &p, int i) {
+    if (i < p.was_free) return checked_page(a, a.free_pages[i]);
+    const int j = i - p.was_free, b = last_le(p.back, a.B, j);
+    return checked_page(a, a.table[(size_t)b * a.max_pages + (j - p.back[b])]);
+}
+// Item i of a plan's second half: a token's slot, position and sequence, a
+// page taken, or a released page that stays free.
+__device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, int64_t i, int tokens, int total) {
+    const int top = p.was_free + p.released - 1;
+    if (i < a.n_tok) {
+        const int t = (int)i;
+        int slot = -1, pos = -1, b = -1;
+        if (t < tokens) {
+            b = last_le(p.start, a.B, t);
+            const int start = p.start[b], took = p.start[b + 1] - start, row0 = a.len_out[b] - took, row = row0 + t - start;
+            const int pg = a.log2_page >= 0 ? row >> a.log2_page : row / a.page_size, held = plan_ceil(a, row0);
+            const int page = pg < held ? checked_page(a, a.table[(size_t)b * a.max_pages + pg]) : stack_page(a, p, top - (p.grown[b] + pg - held));
+            slot = page * a.page_size + (row - pg * a.page_size);
+            pos = (int)((uint32_t)(a.next_pos ? a.next_pos_out[b] - took : row0) + (uint32_t)(t - start));
+        }
+        if (a.slot) a.slot[t] = slot;
+        if (a.pos) a.pos[t] = pos;
+        if (a.seq) a.seq[t] = b;
+        return;
+    }
+    i -= a.n_tok;
+    if (i < p.taken) {
+        const int k = (int)i, b = last_le(p.grown, a.B, k);
+        const int row0 = a.len_out[b] - (p.start[b + 1] - p.start[b]);
+        a.table[(size_t)b * a.max_pages + plan_ceil(a, row0) + k - p.grown[b]] = stack_page(a, p, top - k);
+        return;
+    }
+    const int at = p.was_free + (int)(i - p.taken);   // released and not taken
+    if (at < total - p.taken) a.free_pages[at] = stack_page(a, p, at);
+}
+
+// Sums of v over the threads before this one, and in all (1024 threads).
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *sums, int64_t &all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+    }
+    __syncthreads();   // (sums may still be read from the scan before)
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    int64_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        const int64_t s = sums[w];
+        before += w < wave ? s : 0;
+        all += s;
+    }
+    return before + x - v;
+}
+
+constexpr int PLAN_THREADS = 1024;
+
+// grid 1, block 1024: the sums; ALL (at most 1024 sequences): the rest as well,
+// from LDS, in the same launch.
+template <bool ALL>
+__global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
+    __shared__ int64_t sums[16];
+    __shared__ int l_start[ALL ? PLAN_THREADS + 1 : 1], l_back[ALL ? PLAN_THREADS + 1 : 1], l_grown[ALL ? PLAN_THREADS + 1 : 1];
+    const int tid = threadIdx.x, per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS;
+    const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    const int cap = a.max_pages * a.page_size;
+    const int free_in = *a.n_free, was_free = min(max(free_in, 0), a.n_pages);
+    bool bad = was_free != free_in;
+    // a sequence as it comes: rows (0 once it ended), its pages to give back, tokens and pages wanted
+    auto look = [&](int b, int &rows, int &back, int &want, int &need) {
+        const int len = a.len[b], n = a.new_tok[b];
+        rows = min(max(len, 0), cap);
+        want = max(n, 0);
+        bad |= rows != len || want != n;
+        const bool over = a.ended && a.ended[b] != 0;
+        back = over ? plan_ceil(a, rows) : 0;
+        if (over) rows = want = 0;
+        if (want > cap - rows) want = 0;
+        need = plan_ceil(a, rows + want) - plan_ceil(a, rows);
+    };
+    int rows, back, want, need;
+    int64_t s_back = 0, s_need = 0, s_tok = 0, s_grown = 0, all;
+    for (int b = b0; b < b1; b++) {
+        look(b, rows, back, want, need);
+        s_back += back;
+        s_need += need;
+    }
+    int64_t released = 0;
+    const int64_t back0 = block_scan(s_back, sums, released), need0 = block_scan(s_need, sums, all);
+    if (was_free + released > a.n_pages) {   // (pages given back twice, or not of this pool)
+        bad = true;
+        released = a.n_pages - was_free;
+    }
+    const int64_t total = was_free + released;
+    auto served = [&](int64_t &needs, int n, int w) {
+        needs += n;
+        return n == 0 || needs <= total ? w : 0;
+    };
+    int64_t x = need0;
+    for (int b = b0; b < b1; b++) {
+        look(b, rows, back, want, need);
+        s_tok += served(x, need, want);
+    }
+    const int64_t tok0 = block_scan(s_tok, sums, all);
+    auto took_of = [&](int64_t &needs, int64_t &toks, int n, int w) {
+        const int t = served(needs, n, w);
+        toks += t;
+        return toks <= a.n_tok ? t : 0;
+    };
+    int64_t y = tok0;
+    x = need0;
+    s_tok = 0;
+    for (int b = b0; b < b1; b++) {
+        look(b, rows, back, want, need);
+        const int t = took_of(x, y, need, want);
+        s_tok += t;
+        s_grown += t ? need : 0;
+    }
+    int64_t tokens, taken;
+    int64_t start = block_scan(s_tok, sums, tokens), grown = block_scan(s_grown, sums, taken), given = back0;
+    y = tok0;
+    x = need0;
+    for (int b = b0; b < b1; b++) {
+        look(b, rows, back, want, need);
+        const int t = took_of(x, y, need, want);
+        const int at = (int)start, gr = (int)grown, bk = (int)min(given, released);
+        a.q_start[b] = at;
+        if (ALL) l_start[b] = at, l_grown[b] = gr, l_back[b] = bk;
+        else a.grown[b] = gr, a.back[b] = bk;
+        a.took[b] = t;
+        a.len_out[b] = rows + t;
+        if (a.next_pos) a.next_pos_out[b] = (int)((uint32_t)(a.ended && a.ended[b] != 0 ? 0 : a.next_pos[b]) + (uint32_t)t);
+        start += t;
+        grown += t ? need : 0;
+        given += back;
+    }
+    if (tid == 0) {
+        a.q_start[a.B] = (int)tokens;
+        if (ALL) l_start[a.B] = (int)tokens;
+        else a.was_free[0] = was_free, a.was_free[1] = (int)released, a.was_free[2] = (int)taken;
+    }
+    if (bad) *a.err_flag = 1;
+    if (!ALL) {
+        if (tid == 0) *a.n_free_out = (int)(total - taken);
+        return;
+    }
+    __syncthreads();   // (len_out and next_pos_out of all sequences are written)
+    if (tid == 0) *a.n_free_out = (int)(total - taken);
+    const PlanSums p = {l_start, l_back, l_grown, was_free, (int)released, (int)taken};
+    const int64_t items = (int64_t)a.n_tok + max(released, taken);
+    for (int64_t i = tid; i < items; i += PLAN_THREADS) plan_item(a, p, i, (int)tokens, (int)total);
+}
+
+// grid any, block 256: the second half from the sums in memory.
+__global__ __launch_bounds__(256) void pages_fill(PlanArgs a) {
+    const PlanSums p = {a.q_start, a.back, a.grown, a.was_free[0], a.was_free[1], a.was_free[2]};
+    const int tokens = a.q_start[a.B], total = p.was_free + p.released;
+    const int64_t items = (int64_t)a.n_tok + max(p.released, p.taken);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) plan_item(a, p, i, tokens, total);
+}
+
+// ------------------------------------------------------------------- read
+struct ReadArgs {
+    int n_kv, page_size, n_pages, n_rows, bf16;
+    const int *slots;
+    const char *k_pages, *v_pages;
+    void *k_out, *v_out;
+    int *err_flag;
+};
+__device__ __forceinline__ uint32_t bf16x2(float x, float y) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const bf16x2_t v = (bf16x2_t){(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float bf16_at(const char *p) { return vx_bf16_to_f32(*(const uint16_t *)p); }
+
+// grid (n_rows / 4, n_kv), block 256: a row a wave.
+__global__ __launch_bounds__(256) void paged_read_q4(ReadArgs a) {
+    const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = blockIdx.y;
+    if (i >= a.n_rows) return;
+    const int slot = __builtin_amdgcn_readfirstlane(a.slots[i]);
+    if (slot < 0 || slot >= a.n_pages * a.page_size) {
+        if (slot != -1) *a.err_flag = 1;
+        return;
+    }
+    const int page = slot / a.page_size, at = slot - page * a.page_size, row = at % VX_PG_TILE;
+    const size_t block = (((size_t)page * a.n_kv + h) * (a.page_size / VX_PG_TILE) + at / VX_PG_TILE) * VX_Q4_BLOCK;
+    const size_t out = ((size_t)i * a.n_kv + h) * VX_GQA_HD;
+    if (a.k_out) {   // lane: dims 4 lane .. + 3
+        const char *blk = a.k_pages + block;
+        const int c = lane >> 4;
+        const uint32_t w = *(const uint32_t *)(blk + vx_q4_k_unit(row, 4 * lane) * 16 + ((lane >> 3) & 3) * 4) >> (4 * (lane & 1));
+        const float s = bf16_at(blk + VX_Q4_S + c * 64 + row * 2), m = bf16_at(blk + VX_Q4_M + row * 8 + c * 2);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((w >> (8 * e)) & 15), s, m);
+        if (a.bf16) *(uint2 *)((uint16_t *)a.k_out + out + 4 * lane) = make_uint2(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]));
+        else *(float4 *)((float *)a.k_out + out + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    if (a.v_out) {   // lane (j,n): dims 64 j + 16 e + n
+        const char *blk = a.v_pages + block;
+        const int j = lane >> 4, n = lane & 15;
+        const uint4 u = *(const uint4 *)(blk + (64 * j + 16 * (row >> 3) + n) * 16);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const float s = bf16_at(blk + VX_Q4_S + j * 64 + row * 2), m = bf16_at(blk + VX_Q4_M + j * 64 + row * 2);
+        const int shift = 8 * (row & 3) + (row & 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float x = __builtin_fmaf((float)((w[e] >> shift) & 15), s, m);
+            const size_t d = out + 64 * j + 16 * e + n;
+            if (a.bf16) ((uint16_t *)a.v_out)[d] = vx_f32_to_bf16(x);
+            else ((float *)a.v_out)[d] = x;
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int vx27_hip_paged_plan(vx27_hip_ctx *ctx, const vx27_paged_plan_desc *d) {
+    static const char who[] = "vx27_hip_paged_plan";
+    VX_REQUIRE(d != nullptr, "%s: null descriptor", who);
+    VX_REQUIRE(d->B >= 1 && d->B <= 65535, "%s: need 1 <= B <= 65535 (B=%d)", who, d->B);
+    VX_REQUIRE(d->page_size >= VX_PG_TILE && d->page_size % VX_PG_TILE == 0, "%s: page_size must be a positive multiple of %d (got %d)",
+               who, VX_PG_TILE, d->page_size);
+    VX_REQUIRE(d->n_pages >= 1 && d->max_pages >= 1 && d->n_tok >= 0, "%s: need n_pages and max_pages >= 1 and n_tok >= 0 (got %d, %d, %d)", who,
+               d->n_pages, d->max_pages, d->n_tok);
+    VX_REQUIRE((int64_t)d->max_pages * d->page_size <= (1 << 30), "%s: max_pages * page_size is past 2^30 rows (%d * %d)", who,
+               d->max_pages, d->page_size);
+    VX_REQUIRE((int64_t)d->n_pages * d->page_size < (1ll << 31), "%s: n_pages * page_size is past 2^31 rows (%d * %d)", who, d->n_pages,
+               d->page_size);
+    VX_REQUIRE(d->new_tok && d->len && d->table && d->free_pages && d->n_free && d->took && d->q_start && d->len_out && d->n_free_out,
+               "%s: null pointer in descriptor", who);
+    VX_REQUIRE(!d->next_pos == !d->next_pos_out, "%s: next_pos and next_pos_out go together", who);
+    // Tokens and pages are looked up in what the call writes: an output may be
+    // its input's own array, and overlap nothing else.
+    struct Span {
+        const char *name;
+        const void *p;
+        size_t bytes;
+        int in_place;   // index of the input that it may be
+    };
+    const size_t nb = (size_t)d->B * 4, nt = (size_t)d->n_tok * 4;
+    const Span in[] = {{"new_tok", d->new_tok, nb, 0}, {"ended", d->ended, nb, 0}, {"len", d->len, nb, 0}, {"next_pos", d->next_pos, nb, 0},
+                       {"n_free", d->n_free, 4, 0}};
+    const Span out[] = {{"len_out", d->len_out, nb, 2}, {"next_pos_out", d->next_pos_out, nb, 3}, {"n_free_out", d->n_free_out, 4, 4},
+                        {"took", d->took, nb, -1}, {"q_start", d->q_start, nb + 4, -1}, {"table", d->table, nb * d->max_pages, -1},
+                        {"free_pages", d->free_pages, (size_t)d->n_pages * 4, -1}, {"slot", d->slot, nt, -1}, {"pos", d->pos, nt, -1},
+                        {"seq", d->seq, nt, -1}};
+    auto apart = [](const Span &x, const Span &y) {
+        const uintptr_t a0 = (uintptr_t)x.p, b0 = (uintptr_t)y.p;
+        return !x.p || !y.p || !x.bytes || !y.bytes || a0 + x.bytes <= b0 || b0 + y.bytes <= a0;
+    };
+    for (int i = 0; i < 10; i++) {
+        for (int j = 0; j < 5; j++)
+            VX_REQUIRE(apart(out[i], in[j]) || (out[i].in_place == j && out[i].p == in[j].p), "%s: %s must not overlap %s", who, out[i].name, in[j].name);
+        for (int j = 0; j < i; j++) VX_REQUIRE(apart(out[i], out[j]), "%s: %s must not overlap %s", who, out[i].name, out[j].name);
+    }
+    if (vx_ctx_enter(ctx)) return -1;
+    PlanArgs a = {};
+    a.B = d->B; a.page_size = d->page_size; a.n_pages = d->n_pages; a.max_pages = d->max_pages; a.n_tok = d->n_tok;
+    a.log2_page = (d->page_size & (d->page_size - 1)) == 0 ? __builtin_ctz(d->page_size) : -1;
+    a.new_tok = d->new_tok; a.ended = d->ended; a.len = d->len; a.next_pos = d->next_pos; a.n_free = d->n_free;
+    a.table = d->table; a.free_pages = d->free_pages; a.took = d->took; a.q_start = d->q_start; a.len_out = d->len_out;
+    a.next_pos_out = d->next_pos_out; a.n_free_out = d->n_free_out; a.slot = d->slot; a.pos = d->pos; a.seq = d->seq;
+    a.err_flag = ctx->err_flag;
+    if (d->B <= PLAN_THREADS && d->n_tok <= 4 * PLAN_THREADS) {
+        VX_LAUNCH_NAMED(ctx, "pages_plan", (pages_plan<true>), dim3(1), dim3(PLAN_THREADS), a);
+        return 0;
+    }
+    void *scr;
+    if (vx_ctx_scratch(ctx, ((size_t)2 * d->B + 3) * sizeof(int), &scr)) return -1;
+    a.back = (int *)scr; a.grown = a.back + d->B; a.was_free = a.grown + d->B;
+    VX_LAUNCH_NAMED(ctx, "pages_plan", (pages_plan<false>), dim3(1), dim3(PLAN_THREADS), a);
+    const int64_t most = (int64_t)d->n_tok + d->n_pages;
+    VX_LAUNCH(ctx, pages_fill, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8 * ctx->n_cu)), dim3(256), a);
+    return 0;
+}
+
+extern "C" int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_desc *d) {
+    static const char who[] = "vx27_hip_paged_read_q4";
+    VX_REQUIRE(d != nullptr, "%s: null descriptor", who);
+    VX_REQUIRE(d->hd == VX_GQA_HD, "%s: hd must be 256 (got %d)", who, d->hd);
+    VX_REQUIRE(d->n_kv >= 1 && d->n_kv <= 1024, "%s: need 1 <= n_kv <= 1024 (n_kv=%d)", who, d->n_kv);
+    VX_REQUIRE(d->page_size >= VX_PG_TILE && d->page_size % VX_PG_TILE == 0, "%s: page_size must be a positive multiple of %d (got %d)",
+               who, VX_PG_TILE, d->page_size);
+    VX_REQUIRE(d->n_pages >= 1 && (int64_t)d->n_pages * d->page_size < (1ll << 31), "%s: need n_pages >= 1 and n_pages * page_size below 2^31 (%d * %d)",
+               who, d->n_pages, d->page_size);
+    VX_REQUIRE(d->n_rows >= 0 && d->n_rows <= (1 << 25), "%s: need 0 <= n_rows <= 2^25 (got %d)", who, d->n_rows);
+    VX_REQUIRE(d->out_dtype == VX27_F32 || d->out_dtype == VX27_BF16, "%s: out_dtype must be VX27_F32 or VX27_BF16 (got %d)", who, d->out_dtype);
+    VX_REQUIRE(d->slots && (d->k_pages || !d->k_out) && (d->v_pages || !d->v_out), "%s: null pointer in descriptor", who);
+    VX_REQUIRE((((uintptr_t)d->k_pages | (uintptr_t)d->v_pages | (uintptr_t)d->k_out | (uintptr_t)d->v_out) & 15) == 0,
+               "%s: pages and outputs must be 16-byte aligned", who);
+    if (vx_ctx_enter(ctx)) return -1;
+    if (d->n_rows == 0 || (!d->k_out && !d->v_out)) return 0;
+    const ReadArgs a = {d->n_kv, d->page_size, d->n_pages, d->n_rows, d->out_dtype == VX27_BF16, d->slots,
+                        (const char *)d->k_pages, (const char *)d->v_pages, d->k_out, d->v_out, ctx->err_flag};
+    VX_LAUNCH(ctx, paged_read_q4, dim3((d->n_rows + 3) / 4, d->n_kv), dim3(256), a);
+    return 0;
+}

@@ -117,6 +117,22 @@ class PagedEvictDesc(C.Structure):
                 ("acc_out", VP), ("acc_out_stride", C.c_size_t), ("kept", VP)]
 
 
+class PagedReadDesc(C.Structure):
+    _fields_ = [("n_kv", C.c_int), ("hd", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int), ("n_rows", C.c_int),
+                ("slots", VP), ("k_pages", VP), ("v_pages", VP), ("out_dtype", C.c_int), ("k_out", VP), ("v_out", VP)]
+
+
+class PagedPlanDesc(C.Structure):
+    _fields_ = [("B", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int), ("n_tok", C.c_int),
+                ("new_tok", VP), ("ended", VP), ("len", VP), ("next_pos", VP), ("table", VP), ("free_pages", VP),
+                ("n_free", VP), ("took", VP), ("q_start", VP), ("len_out", VP), ("next_pos_out", VP),
+                ("n_free_out", VP), ("slot", VP), ("pos", VP), ("seq", VP)]
+
+
+Q4_BLOCK_BYTES = 4608           # 32 rows of K or of V of one KV head in 4-bit pages
+Q4_SPLIT_ROWS = 1 << 28         # most query rows a KV head (tokens x its group) of the 4-bit split kernel
+
+
 _SIGS = {
     "vx27_hip_open": (C.c_int, [C.POINTER(VP), C.c_int, C.c_char_p, C.c_size_t]),
     "vx27_hip_close": (None, [VP]),
@@ -152,6 +168,10 @@ _SIGS = {
     "vx27_hip_paged_append": (C.c_int, [VP, C.POINTER(PagedAppendDesc)]),
     "vx27_hip_paged_attn": (C.c_int, [VP, C.POINTER(PagedAttnDesc)]),
     "vx27_hip_paged_evict": (C.c_int, [VP, C.POINTER(PagedEvictDesc)]),
+    "vx27_hip_paged_append_q4": (C.c_int, [VP, C.POINTER(PagedAppendDesc)]),
+    "vx27_hip_paged_attn_q4": (C.c_int, [VP, C.POINTER(PagedAttnDesc)]),
+    "vx27_hip_paged_read_q4": (C.c_int, [VP, C.POINTER(PagedReadDesc)]),
+    "vx27_hip_paged_plan": (C.c_int, [VP, C.POINTER(PagedPlanDesc)]),
     "vx27_hip_kv_write": (C.c_int, [VP, VP, VP] + [C.c_int] * 7 + [VP, VP]),
     "vx27_hip_kv_read": (C.c_int, [VP, VP, VP] + [C.c_int] * 7 + [VP, VP]),
     "vx27_hip_rope_table": (C.c_int, [VP, VP, C.c_int, C.c_int, C.c_float, C.c_float, VP, VP]),
