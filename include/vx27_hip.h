@@ -480,7 +480,8 @@ int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
  * append writes to keep their values; two sequences may share only pages that
  * neither writes. */
 #define VX27_Q4_BLOCK_BYTES 4608
-#define VX27_Q4_SPLIT_ROWS (1 << 28)
+#define VX27_Q4_SPLIT_ROWS 64
+#define VX27_Q4_SPLIT_ROWS_F32 512
 /* vx27_hip_paged_append into 4-bit pages.  k is normed and rotated in fp64
  * (the angle is the fp32 product of the other calls), so that rounding it to
  * codes does not depend on the order of sums; q as there. */

@@ -159,12 +159,15 @@ class Batch4(Batch):
         return {"out": out, "lse": lse, "W": Wt, "S": S}
 
 
-def out_tol(res, keys, out_bf16, part_err):
+def out_tol(res, keys, out_bf16, part_err, rounded=False):
     """Elementwise bound of the attention output's error, relative to the sum of p (s c + |m|) (W): twice the error of a
     score (256 products and their sums in fp32: score_err of the sum of |q| (s c + |m|)), 2^-20 for exp2 and its
     argument, 3 * keys * 2^-24 for sums over up to `keys` rows, and the rounding of the weights: `part_err`, 2^-8 for one
-    bf16 part, 2^-16 for two; and 2^-8 of the output where it is bf16."""
+    bf16 part, 2^-16 for two; and 2^-8 of the output where it is bf16.  rounded: the tile kernel, whose values are
+    rounded to bf16 first, 2^-8 of a value and 2^-8 S of a score, which moves a weight and the sum by up to e to that."""
     rel = 2 * score_err(res["S"])[..., None] + 2.0 ** -20 + 3 * keys * 2.0 ** -24 + part_err
+    if rounded:
+        rel = rel + 2.0 ** -8 + np.expm1(2 * 2.0 ** -8 * res["S"])[..., None]
     return 1.01 * rel * res["W"] + (2.0 ** -8 * np.abs(res["out"]) if out_bf16 else 0.0) + 1e-30
 
 

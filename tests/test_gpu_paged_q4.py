@@ -72,10 +72,14 @@ class Attn4:
     def raw(self):
         return [self.bufs[n].download((self.bufs[n].nbytes,), np.uint8) for n in ("out", "lse")]
 
-    def part_err(self):
-        """The rounding of the weights: one bf16 part (2^-8), or two in the split kernel's fp32 outputs (2^-16)."""
-        from vx27_amd import lib as L
-        return 2.0 ** -16 if not self.out_bf16 and max(self.bt.new) * self.bt.qg <= L.Q4_SPLIT_ROWS else 2.0 ** -8
+    def tiled(self):
+        """Whether the call runs the tile kernel."""
+        rows = max(self.bt.new) * self.bt.qg
+        return rows > (self.L.Q4_SPLIT_ROWS if self.out_bf16 else self.L.Q4_SPLIT_ROWS_F32)
+
+    def tol(self, ref, keys):
+        """Weights are rounded to one bf16 part (2^-8), or two in the split kernel's fp32 outputs (2^-16)."""
+        return out_tol(ref, keys, self.out_bf16, 2.0 ** -8 if self.out_bf16 or self.tiled() else 2.0 ** -16, self.tiled())
 
     def free(self):
         for b in self.bufs.values():
@@ -86,7 +90,7 @@ class Attn4:
         bt = self.bt
         ref, out = bt.result(self.gated), self.out()
         lo, hi = bt.start[0], bt.start[-1]
-        err, tol = np.abs(out - ref["out"])[lo:hi], out_tol(ref, max(max(bt.lens), 1), self.out_bf16, self.part_err())[lo:hi]
+        err, tol = np.abs(out - ref["out"])[lo:hi], self.tol(ref, max(max(bt.lens), 1))[lo:hi]
         if err.size:
             say(f"  {tag}: max err/tol {np.nanmax(err / tol):.3f}, rel {np.linalg.norm(err) / max(np.linalg.norm(ref['out'][lo:hi]), 1e-30):.2e}")
         assert bool(np.all(err <= tol)), tag                # (a NaN fails it)
@@ -99,6 +103,8 @@ class Attn4:
         assert np.array_equal(np.isinf(lse), np.isinf(want)), tag
         f = np.isfinite(want)
         ltol = score_err(ref["S"][lo:hi]) + 2.0 ** -20 * (1 + np.abs(want)) + max(bt.lens) * 2.0 ** -24
+        if self.tiled():
+            ltol += 2.0 ** -8 * ref["S"][lo:hi]              # (keys rounded to bf16)
         assert np.all(np.abs(lse[f] - want[f]) <= ltol[f]), tag
         return ref
 
@@ -129,6 +135,8 @@ SHAPES = [   # lens, new, n_q, n_kv, page, window, sink
     ([0, 40, 5], [3, 60, 5], 24, 4, 64, 0, 0),                       # tokens before the first row see nothing
     ([2000, 1990], [300, 1], 24, 4, 64, 1, 0),
     ([1500, 40], [150, 20], 24, 4, 64, 64, 2000),
+    ([1100, 700], [1000, 33], 16, 1, 64, 500, 9),                    # rows past the fp32 outputs' limit
+    ([5000], [43], 24, 4, 256, 0, 0),                                # a short chunk over a long cache, cut into parts
 ]
 
 
@@ -187,13 +195,13 @@ def test_groups_held_as_nan_stay_with_the_rows_that_see_them(ctx, lens, new, win
     at = Attn4(ctx, bt, False, gate="none")
     at.call()
     ctx.sync()
-    out, part = at.out(), at.part_err()
+    out = at.out()
     if what == "k":
         bt.kq = clean
     else:
         bt.vq = clean
     ref = bt.result(False)
-    tol = out_tol(ref, max(lens), False, part)
+    tol = at.tol(ref, max(lens))
     assert np.isnan(out[hit]).all()
     assert np.all(np.abs(out[~hit] - ref["out"][~hit]) <= tol[~hit])
     at.free()
@@ -226,6 +234,7 @@ def test_large_scores(ctx):
         ref, out = bt.result(False), at.out()
         # a score's error is score_err(S), about 0.1 here: weights may be off by that factor, the outputs stay weighted
         # means of the values
+        assert not at.tiled()
         e = np.expm1(2 * score_err(ref["S"]))[..., None]
         assert np.all(np.abs(out - ref["out"]) <= 2 * e * ref["W"] + 2.0 ** -8 * ref["W"] + 1e-5)
         at.free()

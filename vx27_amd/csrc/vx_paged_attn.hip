@@ -432,7 +432,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     }
     // (a 32-row tile's queries are addressed by 32-bit offsets from its first)
     VX_REQUIRE(!d->acc || (a.q_ts < (1u << 26) && a.q_hs < (1u << 26)), "%s: q strides past 2^26 elements with acc (got %zu, %zu)", who, a.q_ts, a.q_hs);
-    if (rows_launch(who, ctx, d, a, rows, stat_bytes)) return -1;
+    if (rows_launch<false>(who, ctx, d, a, rows, stat_bytes)) return -1;
     if (d->acc) VX_LAUNCH(ctx, paged_rows_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);
     return 0;
 }

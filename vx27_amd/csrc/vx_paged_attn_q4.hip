@@ -347,6 +347,7 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     const int todo = attn_fill(who, ctx, d, a);
     if (todo <= 0) return todo;
     const int rows = d->max_T * a.qg;
+    if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32)) return rows_launch<true>(who, ctx, d, a, rows, 0);
     // two parts of the weights where the output is fp32, one where it is rounded to bf16 itself
     a.block_rows = a.out_bf16 ? 16 : 8;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;

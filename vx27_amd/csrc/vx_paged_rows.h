@@ -2,6 +2,7 @@
 // decode call's (vx_paged_attn.h).
 #pragma once
 #include "vx_paged_attn.h"
+#include "vx_paged_q4.h"
 
 namespace {
 
@@ -43,8 +44,10 @@ typedef float floatx16_t __attribute__((ext_vector_type(16)));
 // the window's edge a row sees few keys.)
 constexpr int LAZY = 16;
 
+template <bool Q4>
 struct TileSmem {
     char k[2][2 * HALF], v[2][2 * HALF];     // [buffer][key block]
+    char sm[Q4 ? 2 : 1][Q4 ? 4 * 512 : 16];  // 4-bit pages: s and m of a step's K blocks and V blocks, [buffer]
     int piece;
     int odd;                                 // some value was infinite or NaN where not every row sees it
 };
@@ -191,8 +194,14 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
 }
 
 // grid the most pieces there can be, block 256.
+//
+// Q4, over 4-bit pages: the same kernel over values rounded to bf16.  A wave
+// loads the codes of its quarter of a step a step earlier into registers, and
+// the two masks, fp32 FMAs and packs that make 16 bytes of LDS of a dword take
+// the places of the direct loads between the MFMAs; s and m come through LDS.
+template <bool Q4>
 __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
-    __shared__ __attribute__((aligned(16))) TileSmem sm;
+    __shared__ __attribute__((aligned(16))) TileSmem<Q4> sm;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // The dispatcher deals workgroups round-robin over the 8 XCDs.  Each takes
@@ -272,7 +281,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     }
     const uint32_t vo = (uint32_t)((lane >> 2) * TILE * 2 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4)) + (wave & 1) * 8192;
     const uint32_t k_lds = vx_lds_addr(sm.k[0]) + wave * 8192, v_lds = vx_lds_addr(sm.v[0]) + wave * 8192;
-    // Element offsets in the pools of this wave's key blocks: lane i holds the
+    // Element (4-bit pages: byte) offsets in the pools of this wave's key blocks: lane i holds the
     // block of step base + i (past the list: its last block again), so a step
     // reads a lane and not the page table.
     int base = c0;
@@ -280,7 +289,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     auto fill_at = [&]() {
         const int key = tl.at(min(2 * (base + lane) + (wave >> 1), tl.nt - 1)) * TILE, slot = vx_page_slot(a.p, key);
         const int page = vx_page_checked(a.p, vx_table_word(a.p.table + (size_t)b * a.p.max_pages + slot));
-        const uint64_t at = (((uint64_t)page * a.p.n_kv + kvh) * a.p.page_size + (key - slot * a.p.page_size)) * HDG;
+        const uint64_t at = Q4 ? (uint64_t)vx_q4_block(a.p, page, kvh, key - slot * a.p.page_size) * VX_Q4_BLOCK
+                               : (((uint64_t)page * a.p.n_kv + kvh) * a.p.page_size + (key - slot * a.p.page_size)) * HDG;
         at_lo = (uint32_t)at;
         at_hi = (uint32_t)(at >> 32);
     };
@@ -306,6 +316,64 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
     auto dma_v = [&](size_t at, int buf, int j) { dma((const char *)(a.v_pages + at), vo, v_lds + buf * 2 * HALF, j); };
 
+    // 4-bit pages: this wave's codes of a step, 16 rows of K (rows m of
+    // operand block `wave % 2`) and 128 dims of V, and the places of their
+    // 16-byte units in LDS.
+    uint4 kc[2], vc[2];
+    const int qg4 = lane >> 4, qn = lane & 15;
+    const uint32_t kd = (uint32_t)((wave >> 1) * HALF + (8 * (qn >> 2) + 4 * (wave & 1) + (qn & 3)) * (HDG * 2) + ((qg4 ^ qn) << 4));
+    const uint32_t vd = (uint32_t)((wave >> 1) * HALF + (128 * (wave & 1) + qn) * (TILE * 2) + ((qg4 ^ ((qn >> 1) & 3)) << 4));
+    auto load_codes = [&](size_t at, const uint16_t *pool, uint4 (&x)[2]) {   // quads 2 (wave % 2), + 1
+        const char *p = (const char *)pool + at + (128 * (wave & 1) + lane) * 16;
+        x[0] = *(const uint4 *)p;
+        x[1] = *(const uint4 *)(p + 1024);
+    };
+    // s and m of key block `wave / 2`: wave w % 2 = 0 takes K's, 1 V's
+    auto load_scales = [&](size_t at_k, size_t at_v, int buf) {
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(vx_lds_addr(sm.sm[buf]) + wave * 512);
+        if (lane < 32) dma16<0>((const char *)(wave & 1 ? a.v_pages : a.k_pages) + (wave & 1 ? at_v : at_k) + VX_Q4_S, lane * 16, lds);
+    };
+    float ksm[8];                              // s and m of this lane's row of K
+    auto k_scales = [&](int buf) {
+        const char *p = sm.sm[buf] + (wave & 2) * 512;
+        const int row = 8 * (qn >> 2) + 4 * (wave & 1) + (qn & 3);
+        const uint2 m = *(const uint2 *)(p + 256 + row * 8);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            ksm[c] = vx_bf16_to_f32(*(const uint16_t *)(p + c * 64 + row * 2));
+            ksm[4 + c] = __uint_as_float(c & 1 ? (c & 2 ? m.y : m.x) & 0xffff0000u : (c & 2 ? m.y : m.x) << 16);
+        }
+    };
+    auto codes8 = [&](uint32_t w, float (&x)[8]) {
+        const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] = (float)((lo >> (8 * e)) & 255);
+            x[4 + e] = (float)((hi >> (8 * e)) & 255);
+        }
+    };
+    auto put8 = [&](char *p, const float (&x)[8]) { *(uint4 *)p = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])); };
+    auto word4 = [](const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
+    // dword j of this wave's eight of K: dims 128 (j / 4) + 32 (j % 4) + 8 g .. + 7 of its row
+    auto put_k = [&](int buf, int j) {
+        float x[8];
+        codes8(word4(kc[j >> 2], j & 3), x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], ksm[j >> 1], ksm[4 + (j >> 1)]);
+        put8(sm.k[buf] + (kd ^ ((j & 3) << 6)) + (j >> 2) * 256, x);
+    };
+    // dword j of V: dim 64 (j / 4) + 16 (j % 4) + n of its 128, keys 8 g .. + 7
+    auto put_v = [&](int buf, int scales, int j) {
+        const char *p = sm.sm[scales] + ((wave & 2) + 1) * 512 + (2 * (wave & 1) + (j >> 2)) * 64 + qg4 * 16;
+        float s8[8], m8[8], x[8];
+        vx_q4_f32(*(const uint4 *)p, s8);
+        vx_q4_f32(*(const uint4 *)(p + 256), m8);
+        codes8(word4(vc[j >> 2], j & 3), x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], s8[e], m8[e]);
+        put8(sm.v[buf] + vd + j * 16 * TILE * 2, x);
+    };
+
     floatx16_t O[8];
 #pragma unroll
     for (int db = 0; db < 8; db++)
@@ -320,14 +388,40 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     if (nt > 0) {
         fill_at();
         size_t at_v = at_of(c0), at_k = at_of(c0 + 1);
+        if constexpr (Q4) {
+            // K and V of the first step, then K of the second and the codes that the loop's first step stores
+            load_codes(at_v, a.k_pages, kc);
+            load_codes(at_v, a.v_pages, vc);
+            load_scales(at_v, at_v, 0);
+            load_scales(at_k, at_k, 1);
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            vx_lds_barrier();
+            k_scales(0);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at_v, 0, j);
+            for (int j = 0; j < 8; j++) put_k(0, j);
+            load_codes(at_k, a.k_pages, kc);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_k(at_k, 1, j);
+            for (int j = 0; j < 8; j++) put_v(0, 0, j);
+            load_codes(at_k, a.v_pages, vc);
+            k_scales(1);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
-        at_v = at_k;
-        at_k = at_of(c0 + 2);
+            for (int j = 0; j < 8; j++) put_k(1, j);
+            const size_t at_2 = at_of(c0 + 2);
+            load_codes(at_2, a.k_pages, kc);
+            vx_lds_barrier();                            // (buffer 0's scales have been read)
+            load_scales(at_2, at_k, 0);                  // K's of step 2 and V's of step 1, as in the loop
+            at_v = at_2;
+            at_k = at_of(c0 + 3);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) dma_k(at_v, 0, j);
+#pragma unroll
+            for (int j = 0; j < 8; j++) dma_k(at_k, 1, j);
+#pragma unroll
+            for (int j = 0; j < 8; j++) dma_v(at_v, 0, j);
+            at_v = at_k;
+            at_k = at_of(c0 + 2);
+        }
         bf16x8_t q[16];
 #pragma unroll
         for (int k = 0; k < 16; k++) q[k] = load8(qp + 16 * k);
@@ -454,6 +548,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             // K(c+1) and V(c) have landed; every wave is done with step c-1
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
             vx_lds_barrier();
+            if constexpr (Q4) k_scales(bk);
             if (edge) clear_v(c0 + c, bk);
             bf16x8_t f[8];
 #pragma unroll
@@ -482,7 +577,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             for (int i = 0; i < 32; i++) {
                 if (i + AHEAD < 32) f[(i + AHEAD) & 7] = kload(i + AHEAD);
                 else f[(i + AHEAD) & 7] = vload(i + AHEAD - 32);
-                if (i < 16) {
+                // (4-bit pages: the codes of K(c+2) and V(c+1) are in registers, those of K(c+3) and V(c+2) follow)
+                if constexpr (Q4) {
+                    if (i < 16) {
+                        if (i & 1) put_v(bk ^ 1, bk, i >> 1);
+                        else put_k(bk, i >> 1);
+                    }
+                    if (i == 16) load_codes(at_k, a.k_pages, kc);
+                    if (i == 18) load_codes(at_v, a.v_pages, vc);
+                    if (i == 20) load_scales(at_k, at_v, bk ^ 1);
+                } else if (i < 16) {
                     if (i & 1) dma_v(at_v, bk ^ 1, i >> 1);
                     else dma_k(at_k, bk, i >> 1);
                 }
@@ -505,7 +609,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 if (i == 0) x = sc[0][0];
                 else if (i & 1) __asm__ volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(sc[i >> 4][(i & 15) - 1]), "v"(sc[i >> 4][i & 15]));
                 // the next step's addresses, edges and buffers
-                if (i == 1) at_v = at_k, at_k = at_of(c0 + c + 3);
+                if (i == 1) at_v = at_k, at_k = at_of(c0 + c + (Q4 ? 4 : 3));
                 if (i == 3) edge2 = bare(c0 + c + 1);
                 if (i == 5) cut2 = c + 2 < nt && cut(c0 + c + 2);
                 if (i >= 8 && i < 16) ka[i - 8] += bk ? 2 * HALF : -2 * HALF;
@@ -521,7 +625,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             pin_o();
             edge = edge2;
             cutn = cut2;
-            if (c0 + c + 5 > base + 63) {   // (one step in 60)
+            if (c0 + c + (Q4 ? 6 : 5) > base + 63) {   // (one step in 60)
                 base = c0 + c + 4;
                 fill_at();
             }
@@ -574,8 +678,9 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 const int key0 = key_of(c, h);
                 if (key0 < 0) continue;
                 const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
-                const uint16_t *vp = a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
-                for (int j = 0; j < TILE; j++) {
+                const uint16_t *vp = Q4 ? (const uint16_t *)((const char *)a.v_pages + (size_t)vx_q4_block(a.p, page, kvh, at) * VX_Q4_BLOCK + VX_Q4_M) + tid / VX_Q4_GROUP * TILE
+                                        : a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
+                for (int j = 0; j < TILE; j++) {   // (4-bit pages: a group that is not finite has m = NaN)
                     const float x = vx_bf16_to_f32(vp[j]);
                     if (is_finite(x)) continue;
                     for (int r = 0; r < TR && r0 + r < R; r++)
@@ -696,6 +801,7 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
 
 // Launches the tile kernel's calls, with `stat_bytes` of scratch for the rows'
 // statistics.
+template <bool Q4>
 int rows_launch(const char *who, vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d, Args &a, int rows, size_t stat_bytes) {
     const int n_rt = (rows + TR - 1) / TR, n_cu = a.cus = ctx->n_cu;
     VX_REQUIRE((int64_t)d->B * n_rt < (1ll << 31) - PLAN, "%s: more than 2^31 row tiles (B=%d max_T=%d)", who, d->B, d->max_T);
@@ -715,7 +821,7 @@ int rows_launch(const char *who, vx27_hip_ctx *ctx, const vx27_paged_attn_desc *
     a.part_o = (float *)(at += join_bytes);
     a.pieces = (RowPiece *)(at += (size_t)2 * cuts * TR * HDG * 4);
     VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
-    VX_LAUNCH(ctx, paged_rows, dim3((unsigned)(items + cuts)), dim3(256), a);
+    VX_LAUNCH_NAMED(ctx, Q4 ? "paged_rows_q4" : "paged_rows", (paged_rows<Q4>), dim3((unsigned)(items + cuts)), dim3(256), a);
     VX_LAUNCH(ctx, paged_rows_join, dim3(8 * n_cu), dim3(256), a);
     return 0;
 }
