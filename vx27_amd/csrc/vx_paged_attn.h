@@ -48,6 +48,7 @@ struct Args {
     RowPlan *plan;
     RowPiece *pieces;
     RowJoin *joins;
+    uint16_t *flat_k, *flat_v;   // 4-bit pages: values in scratch, [B][n_kv][tile_cap][32 x 256]
     float *stash;                // with acc: raw scores [B][n_kv][max rows][tile_cap * 32]
 };
 

@@ -56,6 +56,15 @@ __device__ __forceinline__ vx_bf16x8 vx_q4_codes(uint32_t w) {
     x[4] = c[0]; x[5] = c[1]; x[6] = d[0]; x[7] = d[1];
     return x;
 }
+// The same as fp32.
+__device__ __forceinline__ void vx_q4_codes_f32(uint32_t w, float (&x)[8]) {
+    typedef float floatx2 __attribute__((ext_vector_type(2)));
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    const floatx2 y[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, 512.0f, false), __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, 512.0f, true),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 512.0f, false), __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 512.0f, true)};
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = y[e >> 1][e & 1];
+}
 // Eight bf16 numbers of 16 bytes.
 __device__ __forceinline__ void vx_q4_f32(uint4 w, float (&x)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};

@@ -102,6 +102,11 @@ __device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &
 // grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).  It
 // goes by B * n_rt entries, n_rt of the longest token range: 256 decoding
 // sequences beside a chunk of 8192 tokens 105 us, 4096 beside 4096 1.8 ms.
+// 4-bit pages: row tiles of the longest token range from which the values are
+// laid out in scratch, and the most tiles there (32 KiB each, K and V: 256 MiB).
+constexpr int FLAT_ROWS = 6;
+constexpr size_t FLAT_TILES = 8192;
+
 constexpr int PLAN = 1024;
 __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, int max_pieces) {
     __shared__ int64_t s_steps[PLAN / 64];
@@ -193,15 +198,30 @@ __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, i
     if (tid < 8) a.plan->heads[tid] = 0;
 }
 
+// The values of 4-bit pages in scratch: every (sequence, KV head) has room for
+// the tiles that its tokens see, in the order of their list; a tile is a block
+// of K [32][256] and one of V [256][32], as in bf16 pages.
+__device__ __forceinline__ size_t flat_at(const Args &a, const vx_pseq &s, int b, int kvh, int key) {
+    const vx_tiles tl = tiles_of(a, s, 0, s.T - 1);
+    const int tile = key / TILE, i = tile < tl.st ? tile : tile - tl.fm + tl.st;
+    return (((size_t)b * a.p.n_kv + kvh) * a.tile_cap + i) * TILE * HDG;
+}
+
 // grid the most pieces there can be, block 256.
 //
-// Q4, over 4-bit pages: the same kernel over values rounded to bf16.  A wave
+// PG_Q4, over 4-bit pages: the same kernel over values rounded to bf16.  A wave
 // loads the codes of its quarter of a step a step earlier into registers, and
-// the two masks, fp32 FMAs and packs that make 16 bytes of LDS of a dword take
-// the places of the direct loads between the MFMAs; s and m come through LDS.
-template <bool Q4>
+// the masks, fp32 FMAs and packs that make 16 bytes of LDS of a dword take the
+// places of the direct loads between the MFMAs; s and m come through LDS.
+// That makes a step a fifth longer (8192 tokens, window of 1024: 381 us), and
+// every row tile does it again, so long token ranges have the values of what
+// they see laid out once in scratch and read them from there: PG_FLAT.
+enum { PG_BF16, PG_Q4, PG_FLAT };
+template <int PAGES>
 __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
+    constexpr bool Q4 = PAGES == PG_Q4;
     __shared__ __attribute__((aligned(16))) TileSmem<Q4> sm;
+    const uint16_t *const k_pool = PAGES == PG_FLAT ? a.flat_k : a.k_pages, *const v_pool = PAGES == PG_FLAT ? a.flat_v : a.v_pages;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // The dispatcher deals workgroups round-robin over the 8 XCDs.  Each takes
@@ -287,7 +307,14 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
     int base = c0;
     uint32_t at_lo, at_hi;
     auto fill_at = [&]() {
-        const int key = tl.at(min(2 * (base + lane) + (wave >> 1), tl.nt - 1)) * TILE, slot = vx_page_slot(a.p, key);
+        const int key = tl.at(min(2 * (base + lane) + (wave >> 1), tl.nt - 1)) * TILE;
+        if constexpr (PAGES == PG_FLAT) {
+            const uint64_t at = flat_at(a, s, b, kvh, key);
+            at_lo = (uint32_t)at;
+            at_hi = (uint32_t)(at >> 32);
+            return;
+        }
+        const int slot = vx_page_slot(a.p, key);
         const int page = vx_page_checked(a.p, vx_table_word(a.p.table + (size_t)b * a.p.max_pages + slot));
         const uint64_t at = Q4 ? (uint64_t)vx_q4_block(a.p, page, kvh, key - slot * a.p.page_size) * VX_Q4_BLOCK
                                : (((uint64_t)page * a.p.n_kv + kvh) * a.p.page_size + (key - slot * a.p.page_size)) * HDG;
@@ -313,8 +340,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             default: dma16<3 * 1024>(p + (j & 4) * 1024, off, lds + (j & 4) * 1024); break;
         }
     };
-    auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(a.k_pages + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
-    auto dma_v = [&](size_t at, int buf, int j) { dma((const char *)(a.v_pages + at), vo, v_lds + buf * 2 * HALF, j); };
+    auto dma_k = [&](size_t at, int buf, int j) { dma((const char *)(k_pool + at), ko[(j & 1) | ((j >> 2) << 1)], k_lds + buf * 2 * HALF, j); };
+    auto dma_v = [&](size_t at, int buf, int j) { dma((const char *)(v_pool + at), vo, v_lds + buf * 2 * HALF, j); };
 
     // 4-bit pages: this wave's codes of a step, 16 rows of K (rows m of
     // operand block `wave % 2`) and 128 dims of V, and the places of their
@@ -344,31 +371,33 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             ksm[4 + c] = __uint_as_float(c & 1 ? (c & 2 ? m.y : m.x) & 0xffff0000u : (c & 2 ? m.y : m.x) << 16);
         }
     };
-    auto codes8 = [&](uint32_t w, float (&x)[8]) {
-        const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[e] = (float)((lo >> (8 * e)) & 255);
-            x[4 + e] = (float)((hi >> (8 * e)) & 255);
-        }
-    };
     auto put8 = [&](char *p, const float (&x)[8]) { *(uint4 *)p = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])); };
     auto word4 = [](const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
     // dword j of this wave's eight of K: dims 128 (j / 4) + 32 (j % 4) + 8 g .. + 7 of its row
     auto put_k = [&](int buf, int j) {
         float x[8];
-        codes8(word4(kc[j >> 2], j & 3), x);
+        vx_q4_codes_f32(word4(kc[j >> 2], j & 3), x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], ksm[j >> 1], ksm[4 + (j >> 1)]);
         put8(sm.k[buf] + (kd ^ ((j & 3) << 6)) + (j >> 2) * 256, x);
     };
     // dword j of V: dim 64 (j / 4) + 16 (j % 4) + n of its 128, keys 8 g .. + 7
+    // (s and m are read from LDS two dwords ahead of their use, v_scales(0) by the caller)
+    uint4 vsm[2];
+    float s8[8], m8[8];
+    auto v_scales = [&](int scales, int half) {
+        const char *p = sm.sm[scales] + ((wave & 2) + 1) * 512 + (2 * (wave & 1) + half) * 64 + qg4 * 16;
+        vsm[0] = *(const uint4 *)p;
+        vsm[1] = *(const uint4 *)(p + 256);
+    };
     auto put_v = [&](int buf, int scales, int j) {
-        const char *p = sm.sm[scales] + ((wave & 2) + 1) * 512 + (2 * (wave & 1) + (j >> 2)) * 64 + qg4 * 16;
-        float s8[8], m8[8], x[8];
-        vx_q4_f32(*(const uint4 *)p, s8);
-        vx_q4_f32(*(const uint4 *)(p + 256), m8);
-        codes8(word4(vc[j >> 2], j & 3), x);
+        float x[8];
+        if ((j & 3) == 0) {
+            vx_q4_f32(vsm[0], s8);
+            vx_q4_f32(vsm[1], m8);
+        }
+        if (j == 2) v_scales(scales, 1);
+        vx_q4_codes_f32(word4(vc[j >> 2], j & 3), x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], s8[e], m8[e]);
         put8(sm.v[buf] + vd + j * 16 * TILE * 2, x);
@@ -400,6 +429,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
 #pragma unroll
             for (int j = 0; j < 8; j++) put_k(0, j);
             load_codes(at_k, a.k_pages, kc);
+            v_scales(0, 0);
 #pragma unroll
             for (int j = 0; j < 8; j++) put_v(0, 0, j);
             load_codes(at_k, a.v_pages, vc);
@@ -548,7 +578,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
             // K(c+1) and V(c) have landed; every wave is done with step c-1
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
             vx_lds_barrier();
-            if constexpr (Q4) k_scales(bk);
+            if constexpr (Q4) k_scales(bk), v_scales(bk, 0);
             if (edge) clear_v(c0 + c, bk);
             bf16x8_t f[8];
 #pragma unroll
@@ -679,7 +709,8 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 if (key0 < 0) continue;
                 const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
                 const uint16_t *vp = Q4 ? (const uint16_t *)((const char *)a.v_pages + (size_t)vx_q4_block(a.p, page, kvh, at) * VX_Q4_BLOCK + VX_Q4_M) + tid / VX_Q4_GROUP * TILE
-                                        : a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
+                                     : PAGES == PG_FLAT ? a.flat_v + flat_at(a, s, b, kvh, key0) + tid * TILE
+                                                        : a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
                 for (int j = 0; j < TILE; j++) {   // (4-bit pages: a group that is not finite has m = NaN)
                     const float x = vx_bf16_to_f32(vp[j]);
                     if (is_finite(x)) continue;
@@ -799,6 +830,43 @@ __global__ __launch_bounds__(256) void paged_rows_join(Args a) {
     }
 }
 
+// grid (most tiles, n_kv, B), block 256: a tile's values into scratch; thread u
+// takes 16-byte unit u of K's codes and of V's.
+template <int PAGES>   // (PG_FLAT: only where it is launched)
+__global__ __launch_bounds__(256) void paged_q4_flat(Args a) {
+    const int i = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, u = threadIdx.x, g = (u >> 4) & 3, n = u & 15;
+    const vx_pseq s = vx_paged_seq(a.p, b);
+    const vx_tiles tl = tiles_of(a, s, 0, s.T - 1);
+    if (i >= tl.nt) return;
+    const int key = tl.at(i) * TILE, page = vx_paged_page(a.p, b, key);
+    const size_t block = (size_t)vx_q4_block(a.p, page, kvh, key - vx_page_slot(a.p, key) * a.p.page_size) * VX_Q4_BLOCK;
+    const size_t out = (((size_t)b * a.p.n_kv + kvh) * a.tile_cap + i) * TILE * HDG;
+    const char *kp = (const char *)a.k_pages + block, *vp = (const char *)a.v_pages + block;
+    const uint4 kc = *(const uint4 *)(kp + u * 16), vc = *(const uint4 *)(vp + u * 16);
+    const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
+    const int row = vx_q4_k_row(u), kh = (u >> 6) & 1, j = u >> 6;
+    float ks[2], km[2], vs[8], vm[8];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        ks[c] = vx_bf16_to_f32(*(const uint16_t *)(kp + VX_Q4_S + (2 * kh + c) * 64 + row * 2));
+        km[c] = vx_bf16_to_f32(*(const uint16_t *)(kp + VX_Q4_M + row * 8 + (2 * kh + c) * 2));
+    }
+    vx_q4_f32(*(const uint4 *)(vp + VX_Q4_S + j * 64 + g * 16), vs);
+    vx_q4_f32(*(const uint4 *)(vp + VX_Q4_M + j * 64 + g * 16), vm);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        float x[8];
+        vx_q4_codes_f32(kw[q], x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], ks[q >> 1], km[q >> 1]);
+        *(uint4 *)(a.flat_k + out + row * HDG + 128 * kh + 32 * q + 8 * g) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+        vx_q4_codes_f32(vw[q], x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], vs[e], vm[e]);
+        *(uint4 *)(a.flat_v + out + (64 * j + 16 * q + n) * TILE + 8 * g) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    }
+}
+
 // Launches the tile kernel's calls, with `stat_bytes` of scratch for the rows'
 // statistics.
 template <bool Q4>
@@ -812,16 +880,26 @@ int rows_launch(const char *who, vx27_hip_ctx *ctx, const vx27_paged_attn_desc *
     const size_t ml_bytes = (size_t)2 * cuts * TR * sizeof(float2), plan_bytes = 256, piece_bytes = (size_t)(items + cuts) * sizeof(RowPiece);
     const size_t join_bytes = ((size_t)cuts * sizeof(RowJoin) + 255) / 256 * 256;
     void *scr;
-    if (vx_ctx_scratch(ctx, stat_bytes + ml_bytes + plan_bytes + join_bytes + (size_t)2 * cuts * TR * HDG * 4 + piece_bytes, &scr)) return -1;
-    char *at = (char *)scr;
+    const size_t flat_tiles = (size_t)d->B * d->n_kv * a.tile_cap;
+    const bool flat = Q4 && n_rt >= FLAT_ROWS && flat_tiles <= FLAT_TILES;
+    const size_t flat_bytes = flat ? flat_tiles * HALF : 0, parts_bytes = (size_t)2 * cuts * TR * HDG * 4;
+    if (vx_ctx_scratch(ctx, 2 * flat_bytes + stat_bytes + ml_bytes + plan_bytes + join_bytes + parts_bytes + piece_bytes, &scr)) return -1;
+    char *at = (char *)scr + 2 * flat_bytes;
     a.stat = d->acc ? (float2 *)at : nullptr;
     a.part_ml = (float2 *)(at += stat_bytes);
     a.plan = (RowPlan *)(at += ml_bytes);
     a.joins = (RowJoin *)(at += plan_bytes);
     a.part_o = (float *)(at += join_bytes);
-    a.pieces = (RowPiece *)(at += (size_t)2 * cuts * TR * HDG * 4);
+    a.pieces = (RowPiece *)(at += parts_bytes);
     VX_LAUNCH(ctx, paged_plan, dim3(1), dim3(PLAN), a, n_rt, n_cu, (int)(items + cuts));
-    VX_LAUNCH_NAMED(ctx, Q4 ? "paged_rows_q4" : "paged_rows", (paged_rows<Q4>), dim3((unsigned)(items + cuts)), dim3(256), a);
+    const dim3 grid((unsigned)(items + cuts));
+    if constexpr (Q4) if (flat) {
+        a.flat_k = (uint16_t *)scr;
+        a.flat_v = (uint16_t *)((char *)scr + flat_bytes);
+        VX_LAUNCH_NAMED(ctx, "paged_q4_flat", (paged_q4_flat<PG_FLAT>), dim3(a.tile_cap, d->n_kv, d->B), dim3(256), a);
+        VX_LAUNCH_NAMED(ctx, "paged_rows_flat", (paged_rows<PG_FLAT>), grid, dim3(256), a);
+    }
+    if (!flat) VX_LAUNCH_NAMED(ctx, Q4 ? "paged_rows_q4" : "paged_rows", (paged_rows<Q4 ? PG_Q4 : PG_BF16>), grid, dim3(256), a);
     VX_LAUNCH(ctx, paged_rows_join, dim3(8 * n_cu), dim3(256), a);
     return 0;
 }
