@@ -23,29 +23,47 @@ struct KTile {
 struct VTile {
     uint4 c[4], s[GROUPS], m;
 };
-__device__ __forceinline__ uint4 load16_nt(const char *p) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4 x = __builtin_nontemporal_load((const u32x4 *)p);
+// (Buffer loads: the block's address in scalars, a lane's part a 32-bit offset
+// that no tile changes.  As flat addresses these took enough registers to spill.)
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t *pool, uint32_t block) {
+    return __builtin_amdgcn_make_buffer_rsrc((char *)pool + (size_t)block * VX_Q4_BLOCK, 0, VX_Q4_BLOCK, 0x00020000);
+}
+constexpr int NT = 2;   // nontemporal: the codes are read once
+template <int AUX>
+__device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, AUX);
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
+// The lane, opaque: what is formed from it stays where it is used, and does not
+// take a register through the loops around.
+__device__ __forceinline__ int lane_here() {
+    int lane = threadIdx.x & 63;
+    __asm__ volatile("" : "+v"(lane));
+    return lane;
+}
 __device__ __forceinline__ void load_k(const Args &a, uint32_t block, KTile &k) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const char *p = (const char *)a.k_pages + (size_t)block * VX_Q4_BLOCK;
+    const int lane = lane_here(), g = lane >> 4, n = lane & 15;
+    const __amdgpu_buffer_rsrc_t p = block_rsrc(a.k_pages, block);
 #pragma unroll
-    for (int j = 0; j < 4; j++) k.c[j] = load16_nt(p + (64 * j + lane) * 16);
+    for (int j = 0; j < 4; j++) k.c[j] = load16<NT>(p, lane * 16 + j * 1024);
 #pragma unroll
-    for (int j = 0; j < GROUPS; j++) k.s[j] = *(const uint4 *)(p + VX_Q4_S + j * 64 + g * 16);
+    for (int j = 0; j < GROUPS; j++) k.s[j] = load16<0>(p, VX_Q4_S + g * 16 + j * 64);
 #pragma unroll
-    for (int r = 0; r < 2; r++) k.m[r] = *(const uint2 *)(p + VX_Q4_M + (8 * (n >> 2) + 4 * r + (n & 3)) * 8);
+    for (int r = 0; r < 2; r++) {
+        const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(p, VX_Q4_M + (8 * (n >> 2) + (n & 3)) * 8 + r * 32, 0, 0);
+        k.m[r] = make_uint2(x[0], x[1]);
+    }
 }
 __device__ __forceinline__ void load_v(const Args &a, uint32_t block, VTile &v) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const char *p = (const char *)a.v_pages + (size_t)block * VX_Q4_BLOCK;
+    const int lane = lane_here(), g = lane >> 4, n = lane & 15;
+    const __amdgpu_buffer_rsrc_t p = block_rsrc(a.v_pages, block);
 #pragma unroll
-    for (int j = 0; j < 4; j++) v.c[j] = load16_nt(p + (64 * j + lane) * 16);
+    for (int j = 0; j < 4; j++) v.c[j] = load16<NT>(p, lane * 16 + j * 1024);
 #pragma unroll
-    for (int j = 0; j < GROUPS; j++) v.s[j] = *(const uint4 *)(p + VX_Q4_S + j * 64 + g * 16);
-    v.m = *(const uint4 *)(p + VX_Q4_M + (n & 3) * 64 + g * 16);
+    for (int j = 0; j < GROUPS; j++) v.s[j] = load16<0>(p, VX_Q4_S + g * 16 + j * 64);
+    v.m = load16<0>(p, VX_Q4_M + (n & 3) * 64 + g * 16);
 }
 __device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
@@ -60,7 +78,7 @@ struct Rows {
 };
 template <int ROWS>
 __device__ __forceinline__ void rows_begin(const Args &a, const vx_pseq &s, int kvh, int r0, Rows<ROWS> &w) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15, r = r0 + n % ROWS, t = row_tok(a, r);
+    const int lane = lane_here(), g = lane >> 4, n = lane & 15, r = r0 + n % ROWS, t = row_tok(a, r);
     const bool live = t < s.T;
     const uint16_t *qp = a.q + (size_t)(s.start + (live ? t : 0)) * a.q_ts + (size_t)(live ? row_head(a, kvh, r, t) : 0) * a.q_hs + 8 * g;
 #pragma unroll
@@ -116,6 +134,7 @@ __device__ __forceinline__ void score_tile(const KTile &k, const Rows<ROWS> &w, 
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[r][e] = __builtin_fmaf(x[e], sc[4 * r + e], acc[r][e]);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3];
@@ -144,7 +163,7 @@ __device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], uint32_t rest)
 // rows are of one token, so that all see the same keys.
 template <int ROWS>
 __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, const float (&s)[8], const vx_sight &v, int key0, VTile &vt) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int lane = lane_here(), g = lane >> 4;
     const uint32_t rest = ROWS == 8 && (lane & 8) ? 0xffffffffu : 0u;
     float x[8], p[8];
     float mt = -INFINITY;
@@ -220,6 +239,7 @@ __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, cons
         const bf16x8_t pw = weights8<ROWS>(y, rest);
 #pragma unroll
         for (int i = 0; i < 4; i++) w.o[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(vt.c[c], i)), pw, w.o[4 * c + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -232,7 +252,7 @@ __device__ __forceinline__ float add_half_row(float x) {   // the lane's value a
 // tiles, wave w of a workgroup tiles w, w + 4, ...
 template <int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
-    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     __shared__ __attribute__((aligned(16))) float s_o[4][ROWS * HDG];
     __shared__ float s_m[4][ROWS], s_l[4][ROWS];
@@ -258,7 +278,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
         const int R = min(s.T * a.qg - r0, ROWS);
         Rows<ROWS> w;
         rows_begin<ROWS>(a, s, kvh, r0, w);
-        const vx_sight v = sight_of(a, s, r0 + min(n % ROWS, R - 1));   // (columns past the last row: as the last, unused)
+        const vx_sight v = sight_of(a, s, r0 + min(lane % ROWS, R - 1));   // (columns past the last row: as the last, unused)
         const int mine = (cnt - wave + 3) / 4;      // this wave's tiles: i0 + wave + 4 j
         // lane i holds the block of this wave's tile 64 k + i
         uint32_t blocks = 0;
@@ -282,6 +302,8 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             if (j + 1 < mine) load_k(a, __builtin_amdgcn_readlane(blocks, (j + 1) & 63), kt);
             attend_tile<ROWS>(w, R, s.T == 1, sc, v, tl.at(i0 + wave + 4 * j) * TILE, vt);
         }
+        const int ln = lane_here();
+        const int g = ln >> 4, n = ln & 15;
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
 #pragma unroll
@@ -317,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             for (int k = 0; k < 4; k++) {
                 m[k] = s_m[k][r];
                 l[k] = s_l[k][r];
-                o[k] = *(const float4 *)&s_o[k][r * HDG + ((lane ^ r) << 2)];
+                o[k] = *(const float4 *)&s_o[k][r * HDG + ((ln ^ r) << 2)];
             }
             const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
             float L = 0.0f;
@@ -327,8 +349,8 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             if (whole) {
                 row_finish(a, tok, h, O, M, L, gt);
             } else {
-                *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + r) * HDG + 4 * lane) = O;
-                if (lane == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
+                *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + r) * HDG + 4 * ln) = O;
+                if (ln == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
             }
         }
         __syncthreads();
