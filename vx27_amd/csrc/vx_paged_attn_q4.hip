@@ -140,63 +140,66 @@ __device__ __forceinline__ void score_tile(const KTile &k, const Rows<ROWS> &w, 
     for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3];
 }
 
-// Two weights in bf16; `rest`, a lane mask of all ones or zeros: what rounding
-// them leaves instead.
+// Eight weights in bf16: rounded, or of 8 rows the parts of a lane's half.
+// With h the bf16 number that a weight x is cut off to, lanes of the first half
+// (rest 0) take -h and those of the second (rest 1) x - h, which leaves 2^-16 of
+// x at most once it is rounded; the difference of the columns is the sum.
 template <int ROWS>
-__device__ __forceinline__ uint32_t weights2(float x, float y, uint32_t rest) {
-    const uint32_t h = pack2(x, y);
-    if (ROWS == 16) return h;
-    return pack2(x - __uint_as_float((h << 16) & rest), y - __uint_as_float(h & 0xffff0000u & rest));
-}
-template <int ROWS>
-__device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], uint32_t rest) {
-    uint4 u;
-    u.x = weights2<ROWS>(x[0], x[1], rest);
-    u.y = weights2<ROWS>(x[2], x[3], rest);
-    u.z = weights2<ROWS>(x[4], x[5], rest);
-    u.w = weights2<ROWS>(x[6], x[7], rest);
-    return __builtin_bit_cast(bf16x8_t, u);
+__device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], float rest) {
+    float z[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = ROWS == 16 ? x[e] : __builtin_fmaf(x[e], rest, -__uint_as_float(__float_as_uint(x[e]) & 0xffff0000u));
+    return __builtin_bit_cast(bf16x8_t, make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7])));
 }
 
-// Online softmax and P V of one tile for R rows.  s and m of keys that no row
-// sees become zero, so that what stale rows hold cannot get in.  `one`: the
-// rows are of one token, so that all see the same keys.
+// A row's reference lies 2^AHEAD above the maximum at which it last moved, and
+// moves once a score is past it: O is then hardly ever rescaled (68
+// instructions, in every second tile of a wave's 32 where it follows the
+// maximum).  Weights are at most 1; they keep fp32's exponents in bf16.
+constexpr int AHEAD = 8;
+
+// Online softmax and P V of one tile for R rows.  `whole`: every row sees every
+// key.  Else s and m of keys that no row sees become zero, so that what stale
+// rows hold cannot get in.  `one`: the rows are of one token, so that all see
+// the same keys.
 template <int ROWS>
-__device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, const float (&s)[8], const vx_sight &v, int key0, VTile &vt) {
+__device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, bool whole, float (&x)[8], const vx_sight &v, int key0, VTile &vt) {
     const int lane = lane_here(), g = lane >> 4;
-    const uint32_t rest = ROWS == 8 && (lane & 8) ? 0xffffffffu : 0u;
-    float x[8], p[8];
-    float mt = -INFINITY;
-    uint32_t sees = 0;
+    const float rest = ROWS == 8 && (lane & 8) ? 1.0f : 0.0f;
+    float p[8];
+    uint32_t sees = 0xffu;
+    if (!whole) {
+        sees = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const bool see = v.sees(key0 + 8 * g + e);
-        sees |= see ? 1u << e : 0u;
-        x[e] = see ? s[e] : -INFINITY;
-        mt = fmaxf(mt, x[e]);
+        for (int e = 0; e < 8; e++) {
+            const bool see = v.sees(key0 + 8 * g + e);
+            sees |= see ? 1u << e : 0u;
+            x[e] = see ? x[e] : -INFINITY;
+        }
     }
+    float mt = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) mt = fmaxf(mt, x[e]);
     mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
-    const float m_new = fmaxf(w.m, mt * SC2);
-    const bool none = m_new == -INFINITY;
-    const float ref = none ? 0.0f : m_new;
-    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(w.m - m_new);
-    float ls = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -ref));
-        ls += p[e];
-    }
-    w.l = w.l * alpha + ls;
-    w.m = m_new;
-    if (__any(alpha != 1.0f)) {
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * SC2;
+    if (__any(mt > w.m)) {
+        const bool up = mt > w.m;
+        const float to = mt + AHEAD, alpha = up ? __builtin_amdgcn_exp2f(w.m - to) : 1.0f;
+        w.m = up ? to : w.m;
+        w.l *= alpha;
 #pragma unroll
         for (int d = 0; d < 16; d++) w.o[d] *= alpha;
         w.om *= alpha;
     }
+    // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
+    const float ref = w.m == -INFINITY ? 0.0f : w.m;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -ref));
+        w.l += p[e];
+    }
     bf16x8_t m = __builtin_bit_cast(bf16x8_t, vt.m);
-    if (!__all(sees == 0xffu)) {
+    if (!whole) {
         const uint32_t group = (1u << R) - 1;
         uint32_t keep[4];
 #pragma unroll
@@ -243,8 +246,8 @@ __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, int R, bool one, cons
     }
 }
 
-__device__ __forceinline__ float add_half_row(float x) {   // the lane's value and that of lane ^ 8
-    return x + __int_as_float(vx_dpp_i<0x128, 0xF>(__float_as_int(x)));
+__device__ __forceinline__ float both_halves(float x) {   // what lane ^ 8 has less the lane's own (weights8)
+    return __int_as_float(vx_dpp_i<0x128, 0xF>(__float_as_int(x))) - x;
 }
 
 // The list of tiles is cut evenly over the workgroups, as the bf16 pages' (see
@@ -279,6 +282,9 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
         Rows<ROWS> w;
         rows_begin<ROWS>(a, s, kvh, r0, w);
         const vx_sight v = sight_of(a, s, r0 + min(lane % ROWS, R - 1));   // (columns past the last row: as the last, unused)
+        // tiles whose keys all rows see: from row `from` on or below the sinks' end, up to row `upto`
+        const int upto = vx_paged_sight(s, row_tok(a, r0), a.window, a.n_sink).i, from = vx_paged_sight(s, row_tok(a, r0 + R - 1), a.window, a.n_sink).lo;
+        auto whole_tile = [&](int key0) { return key0 + TILE - 1 <= upto && (key0 >= from || key0 + TILE <= a.n_sink); };
         const int mine = (cnt - wave + 3) / 4;      // this wave's tiles: i0 + wave + 4 j
         // lane i holds the block of this wave's tile 64 k + i
         uint32_t blocks = 0;
@@ -300,7 +306,8 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             __builtin_amdgcn_sched_barrier(0);   // (the next K's loads into the registers of this one's)
             if (((j + 1) & 63) == 0) look_up(j + 1);
             if (j + 1 < mine) load_k(a, __builtin_amdgcn_readlane(blocks, (j + 1) & 63), kt);
-            attend_tile<ROWS>(w, R, s.T == 1, sc, v, tl.at(i0 + wave + 4 * j) * TILE, vt);
+            const int key0 = tl.at(i0 + wave + 4 * j) * TILE;
+            attend_tile<ROWS>(w, R, s.T == 1, whole_tile(key0), sc, v, key0, vt);
         }
         const int ln = lane_here();
         const int g = ln >> 4, n = ln & 15;
@@ -309,12 +316,12 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
 #pragma unroll
         for (int c = 0; c < GROUPS; c++) {
             float om = w.om[c];
-            if (ROWS == 8) om = add_half_row(om);
+            if (ROWS == 8) om = both_halves(om);
             om = __shfl(om, n, 64);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) w.o[4 * c + i][e] = (ROWS == 8 ? add_half_row(w.o[4 * c + i][e]) : w.o[4 * c + i][e]) + om;
+                for (int e = 0; e < 4; e++) w.o[4 * c + i][e] = (ROWS == 8 ? both_halves(w.o[4 * c + i][e]) : w.o[4 * c + i][e]) + om;
         }
         // the four waves' results through LDS (16-byte units swizzled by the row)
         if (n < R) {
