@@ -52,6 +52,34 @@ __device__ __forceinline__ void wait_blocks(int blocks) {
 }
 __device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
+// A lane's share of a block's codes and scales; m as it is used.
+struct Tile {
+    uint4 c[4], s[GROUPS];
+};
+struct KTile : Tile {
+    uint2 m[2];
+};
+struct VTile : Tile {
+    bf16x8_t m;
+};
+__device__ __forceinline__ void read_tile(const char *blk, int lane, Tile &t) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) t.c[j] = *(const uint4 *)(blk + lane * 16 + j * 1024);
+#pragma unroll
+    for (int j = 0; j < GROUPS; j++) t.s[j] = *(const uint4 *)(blk + VX_Q4_S + (lane >> 4) * 16 + j * 64);
+}
+__device__ __forceinline__ void read_k(const char *blk, KTile &t) {
+    const int lane = lane_here(), n = lane & 15;
+    read_tile(blk, lane, t);
+#pragma unroll
+    for (int r = 0; r < 2; r++) t.m[r] = *(const uint2 *)(blk + VX_Q4_M + (8 * (n >> 2) + (n & 3)) * 8 + r * 32);
+}
+__device__ __forceinline__ void read_v(const char *blk, VTile &t) {
+    const int lane = lane_here();
+    read_tile(blk, lane, t);
+    t.m = *(const bf16x8_t *)(blk + VX_Q4_M + (lane & 3) * 64 + (lane >> 4) * 16);
+}
+
 // One wave's state for ROWS query rows: 16, or 8 that take the 16 columns
 // twice, the first with the weights rounded to bf16 and the second with what
 // that left (two parts at the price of one).
@@ -97,46 +125,32 @@ __device__ __forceinline__ void rows_begin(const Args &a, const vx_pseq &s, int 
     w.l = 0.0f;
 }
 
-// Scores of the 32 keys of a block in LDS: lane (g,n) gets keys 8g + 0..7 of row n.
-template <int ROWS, int NB>
-__device__ __forceinline__ void score_tile(const char *kb, const Rows<ROWS> (&w)[NB], float (&s)[NB][8]) {
-    const int lane = lane_here(), g = lane >> 4, n = lane & 15;
-    uint4 c[4], sc4[GROUPS];
-#pragma unroll
-    for (int j = 0; j < 4; j++) c[j] = *(const uint4 *)(kb + lane * 16 + j * 1024);
-#pragma unroll
-    for (int j = 0; j < GROUPS; j++) sc4[j] = *(const uint4 *)(kb + VX_Q4_S + g * 16 + j * 64);
-    floatx4_t acc[NB][2];
+// Scores of 32 keys: lane (g,n) gets keys 8g + 0..7 of row n.
+template <int ROWS>
+__device__ __forceinline__ void score_tile(const KTile &t, const Rows<ROWS> &w, float (&s)[8]) {
+    floatx4_t acc[2];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        const uint2 x = *(const uint2 *)(kb + VX_Q4_M + (8 * (n >> 2) + (n & 3)) * 8 + r * 32);
-        const uint4 m = make_uint4(x.x, x.y, x.x, x.y);
-#pragma unroll
-        for (int k = 0; k < NB; k++)
-            acc[k][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, m), w[k].qs, (floatx4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        const uint4 m = make_uint4(t.m[r].x, t.m[r].y, t.m[r].x, t.m[r].y);
+        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, m), w.qs, (floatx4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < GROUPS; i++) {
+    for (int c = 0; c < GROUPS; c++) {
         float sc[8];
-        vx_q4_f32(sc4[i], sc);
+        vx_q4_f32(t.s[c], sc);
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            const bf16x8_t lo = vx_q4_codes(word(c[2 * r + i / 2], 2 * (i & 1))), hi = vx_q4_codes(word(c[2 * r + i / 2], 2 * (i & 1) + 1));
+            floatx4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < NB; k++) {
-                floatx4_t x = {0.f, 0.f, 0.f, 0.f};
-                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, w[k].q[2 * i], x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, w[k].q[2 * i + 1], x, 0, 0, 0);
+            for (int i = 0; i < 2; i++)
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(t.c[2 * r + c / 2], 2 * (c & 1) + i)), w.q[2 * c + i], x, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[k][r][e] = __builtin_fmaf(x[e], sc[4 * r + e], acc[k][r][e]);
-            }
+            for (int e = 0; e < 4; e++) acc[r][e] = __builtin_fmaf(x[e], sc[4 * r + e], acc[r][e]);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int k = 0; k < NB; k++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) s[k][e] = acc[k][e >> 2][e & 3];
+    for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3];
 }
 
 // Eight weights in bf16: rounded, or of 8 rows the parts of a lane's half.
@@ -157,115 +171,97 @@ __device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], float rest) {
 // maximum).  Weights are at most 1; they keep fp32's exponents in bf16.
 constexpr int AHEAD = 8;
 
-// Online softmax and P V of one tile (V's block in LDS) for `rows` rows, ROWS in
-// each of NB.  `whole`: every row sees every key.  Else s and m of keys that no
-// row sees become zero, so that what stale rows hold cannot get in.  `one`: the
-// rows are of one token, so that all see the same keys.
-template <int ROWS, int NB>
-__device__ __forceinline__ void attend_tile(Rows<ROWS> (&w)[NB], int rows, bool one, bool whole, float (&x)[NB][8], const vx_sight (&v)[NB], int key0,
-                                            const char *vb) {
-    const int lane = lane_here(), g = lane >> 4, n = lane & 15;
+// x over the 16 lanes of a lane group, by OR or AND.
+template <bool AND>
+__device__ __forceinline__ uint32_t over_rows(uint32_t x) {
+    auto with = [&](int y) { x = AND ? x & (uint32_t)y : x | (uint32_t)y; };
+    with(vx_dpp_i<0xB1, 0xF>((int)x));
+    with(vx_dpp_i<0x4E, 0xF>((int)x));
+    with(vx_dpp_i<0x124, 0xF>((int)x));
+    with(vx_dpp_i<0x128, 0xF>((int)x));
+    return x;
+}
+
+// Online softmax and P V of one tile.  `whole`: every row sees every key.  Else
+// s and m of keys that no row sees become zero, so that what stale rows hold
+// cannot get in.
+template <int ROWS>
+__device__ __forceinline__ void attend_tile(Rows<ROWS> &w, bool whole, float (&x)[8], const vx_sight &v, int key0, VTile &t) {
+    const int lane = lane_here(), g = lane >> 4;
     const float rest = ROWS == 8 && (lane & 8) ? 1.0f : 0.0f;
-    uint4 c[4], s[GROUPS];
+    uint32_t any = 0xffu, all = 0xffu;           // of keys 8g + 0..7: those that some row sees, and that every row does
+    if (!whole) {
+        const uint32_t sees = (v.block(key0) >> (8 * g)) & 0xffu;
 #pragma unroll
-    for (int j = 0; j < 4; j++) c[j] = *(const uint4 *)(vb + lane * 16 + j * 1024);
+        for (int e = 0; e < 8; e++) x[e] = (sees >> e) & 1 ? x[e] : -INFINITY;
+        any = over_rows<false>(sees);
+        all = over_rows<true>(sees);
+    }
+    float mt = x[0];
 #pragma unroll
-    for (int j = 0; j < GROUPS; j++) s[j] = *(const uint4 *)(vb + VX_Q4_S + g * 16 + j * 64);
-    bf16x8_t m = *(const bf16x8_t *)(vb + VX_Q4_M + (n & 3) * 64 + g * 16);
-    uint32_t sees[NB];
+    for (int e = 1; e < 8; e++) mt = fmaxf(mt, x[e]);
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * SC2;
+    if (__any(mt > w.m)) {
+        const bool up = mt > w.m;
+        const float to = mt + AHEAD, alpha = up ? __builtin_amdgcn_exp2f(w.m - to) : 1.0f;
+        w.m = up ? to : w.m;
+        w.l *= alpha;
 #pragma unroll
-    for (int k = 0; k < NB; k++) {
-        if (!whole) {
-            sees[k] = 0;
+        for (int d = 0; d < 16; d++) w.o[d] *= alpha;
+        w.om *= alpha;
+    }
+    // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
+    const float ref = w.m == -INFINITY ? 0.0f : w.m;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool see = v[k].sees(key0 + 8 * g + e);
-                sees[k] |= see ? 1u << e : 0u;
-                x[k][e] = see ? x[k][e] : -INFINITY;
-            }
-        }
-        float mt = x[k][0];
-#pragma unroll
-        for (int e = 1; e < 8; e++) mt = fmaxf(mt, x[k][e]);
-        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * SC2;
-        if (__any(mt > w[k].m)) {
-            const bool up = mt > w[k].m;
-            const float to = mt + AHEAD, alpha = up ? __builtin_amdgcn_exp2f(w[k].m - to) : 1.0f;
-            w[k].m = up ? to : w[k].m;
-            w[k].l *= alpha;
-#pragma unroll
-            for (int d = 0; d < 16; d++) w[k].o[d] *= alpha;
-            w[k].om *= alpha;
-        }
-        // (nothing seen yet, or NaN scores alone: the reference is 0, so that those stay NaN)
-        const float ref = w[k].m == -INFINITY ? 0.0f : w[k].m;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[k][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][e], SC2, -ref));
-            w[k].l += x[k][e];
-        }
+    for (int e = 0; e < 8; e++) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], SC2, -ref));
+        w.l += x[e];
     }
     if (!whole) {
-        uint32_t group[NB];
+        uint32_t m[4], keep[4], odd = 0;         // odd: bits 15 and 31, where an exponent of all ones carries into them
 #pragma unroll
-        for (int k = 0; k < NB; k++) group[k] = (1u << max(min(rows - k * ROWS, ROWS), 0)) - 1;
+        for (int i = 0; i < 4; i++) {
+            keep[i] = ((any >> (2 * i)) & 1) * 0xffffu | ((any >> (2 * i + 1)) & 1) * 0xffff0000u;
+            m[i] = word(__builtin_bit_cast(uint4, t.m), i) & keep[i];
+            odd |= (m[i] & 0x7f807f80u) + 0x00800080u;
+        }
+        t.m = __builtin_bit_cast(bf16x8_t, make_uint4(m[0], m[1], m[2], m[3]));
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            // which of a lane group's rows see its key 8g + e
-            bool any = false, all = true;
-#pragma unroll
-            for (int k = 0; k < NB; k++) {
-                const uint32_t mine = (uint32_t)(__ballot((sees[k] >> e) & 1) >> (16 * g)) & group[k];
-                any |= mine != 0;
-                all &= mine == group[k];
-            }
-            if (!any) m[e] = (__bf16)0.0f;
-            if (one || !__any(any && !all)) continue;
+        for (int c = 0; c < GROUPS; c++) t.s[c] = make_uint4(t.s[c].x & keep[0], t.s[c].y & keep[1], t.s[c].z & keep[2], t.s[c].w & keep[3]);
+        if (__builtin_expect(__any((odd & 0x80008000u) && any != all), 0)) {
             // A key that some rows see and others do not, with a minimum of NaN
             // (a group that held an infinity or a NaN): 0 times that would
             // reach the others.  It goes to the rows that see it by addition
             // and out of the product.
-            const bool odd = !is_finite((float)m[e]);
-            uint64_t bad = __ballot(odd && any);
-            while (bad) {
-                const int gk = __builtin_ctzll(bad) >> 4;
-                bad &= ~(0xffffull << (16 * gk));
 #pragma unroll
-                for (int i = 0; i < GROUPS; i++) {
-                    const float y = __shfl((float)m[e], 16 * gk + i, 64);
+            for (int e = 0; e < 8; e++) {
+                const bool bad_here = ((any & ~all) >> e) & 1 && !is_finite((float)t.m[e]);
+                uint64_t bad = __ballot(bad_here);
+                while (bad) {
+                    const int gk = __builtin_ctzll(bad) >> 4;
+                    bad &= ~(0xffffull << (16 * gk));
+                    const bool own = v.sees(key0 + 8 * gk + e);
 #pragma unroll
-                    for (int k = 0; k < NB; k++)
-                        if (v[k].sees(key0 + 8 * gk + e) && !is_finite(y)) w[k].om[i] += y;
+                    for (int c = 0; c < GROUPS; c++) {
+                        const float y = __shfl((float)t.m[e], 16 * gk + c, 64);
+                        if (own && !is_finite(y)) w.om[c] += y;
+                    }
                 }
+                if (bad_here) t.m[e] = (__bf16)0.0f;
             }
-            if (odd) m[e] = (__bf16)0.0f;
         }
     }
+    w.om = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.m, weights8<ROWS>(x, rest), w.om, 0, 0, 0);
 #pragma unroll
-    for (int k = 0; k < NB; k++) w[k].om = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, weights8<ROWS>(x[k], rest), w[k].om, 0, 0, 0);
+    for (int c = 0; c < GROUPS; c++) {
+        float y[8];
+        vx_q4_f32(t.s[c], y);
 #pragma unroll
-    for (int i = 0; i < GROUPS; i++) {
-        float sc[8];
-        vx_q4_f32(s[i], sc);
-        bf16x8_t pw[NB];
+        for (int e = 0; e < 8; e++) y[e] *= x[e];
+        const bf16x8_t pw = weights8<ROWS>(y, rest);
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = x[k][e] * sc[e];
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = (sees[k] >> e) & 1 ? y[e] : 0.0f;
-            }
-            pw[k] = weights8<ROWS>(y, rest);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bf16x8_t codes = vx_q4_codes(word(c[i], j));
-#pragma unroll
-            for (int k = 0; k < NB; k++) w[k].o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes, pw[k], w[k].o[4 * i + j], 0, 0, 0);
-        }
+        for (int i = 0; i < 4; i++) w.o[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(t.c[c], i)), pw, w.o[4 * c + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -275,16 +271,16 @@ __device__ __forceinline__ float both_halves(float x) {   // what lane ^ 8 has l
 }
 
 // The list of tiles is cut evenly over the workgroups, as the bf16 pages' (see
-// paged_split): every (sequence, KV head, block of ROWS * NB query rows) takes
-// its tiles, wave w of a workgroup tiles w, w + 4, ...  A wave has rings of
-// DEPTH blocks of K and of V in LDS, filled by direct loads that many tiles
+// paged_split): every (sequence, KV head, block of ROWS query rows) takes its
+// tiles, wave w of a workgroup tiles w, w + 4, ...  A wave has a ring of DEPTH
+// tiles in LDS (K's block, V's block), filled by direct loads that many tiles
 // ahead.
-template <int ROWS, int NB, int DEPTH, int PER_SIMD>
-__global__ __launch_bounds__(256, PER_SIMD) void paged_q4_split(Args a) {
+constexpr int DEPTH = 2, RING = DEPTH * 2 * VX_Q4_BLOCK;
+template <int ROWS>
+__global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    constexpr int RING = DEPTH * 2 * VX_Q4_BLOCK;
-    static_assert(RING >= ROWS * HDG * 4 && DEPTH == 2, "the waves' results take the rings' place; wait_blocks counts two tiles");
+    static_assert(RING >= ROWS * HDG * 4 && DEPTH == 2, "the waves' results take the rings' place; the waits count two tiles");
     __shared__ __attribute__((aligned(16))) char ring[4][RING];
     __shared__ float s_m[4][ROWS], s_l[4][ROWS];
     float (*s_o)[ROWS * HDG] = (float (*)[ROWS * HDG])ring;
@@ -305,9 +301,9 @@ __global__ __launch_bounds__(256, PER_SIMD) void paged_q4_split(Args a) {
             continue;
         }
         const int item = (u - before) / tl.nt, i0 = (u - before) - item * tl.nt;
-        const int kvh = item / nb, r0 = (item - kvh * nb) * (ROWS * NB);
+        const int kvh = item / nb, r0 = (item - kvh * nb) * ROWS;
         const int cnt = min(tl.nt - i0, u1 - u);
-        const int R = min(s.T * a.qg - r0, ROWS * NB);
+        const int R = min(s.T * a.qg - r0, ROWS);
         const int mine = (cnt - wave + 3) / 4;      // this wave's tiles: i0 + wave + 4 j
         // lane i holds the block of this wave's tile 64 k + i
         uint32_t blocks = 0;
@@ -328,88 +324,85 @@ __global__ __launch_bounds__(256, PER_SIMD) void paged_q4_split(Args a) {
                 load_block(a.v_pages, __builtin_amdgcn_readlane(blocks, j), ring_lds + slot_of(j) + VX_Q4_BLOCK);
             }
         }
-        Rows<ROWS> w[NB];
-        vx_sight v[NB];
-#pragma unroll
-        for (int k = 0; k < NB; k++) {
-            rows_begin<ROWS>(a, s, kvh, r0 + k * ROWS, w[k]);
-            v[k] = sight_of(a, s, min(r0 + k * ROWS + lane % ROWS, r0 + R - 1));   // (columns past the last row: as the last, unused)
-        }
+        Rows<ROWS> w;
+        rows_begin<ROWS>(a, s, kvh, r0, w);
+        const vx_sight v = sight_of(a, s, r0 + min(lane % ROWS, R - 1));   // (columns past the last row: as the last, unused)
         // tiles whose keys all rows see: from row `from` on or below the sinks' end, up to row `upto`
         const int upto = vx_paged_sight(s, row_tok(a, r0), a.window, a.n_sink).i, from = vx_paged_sight(s, row_tok(a, r0 + R - 1), a.window, a.n_sink).lo;
         auto whole_tile = [&](int key0) { return key0 + TILE - 1 <= upto && (key0 >= from || key0 + TILE <= a.n_sink); };
         for (int j = 0; j < mine; j++) {
-            const char *kb = ring[wave] + slot_of(j), *vb = kb + VX_Q4_BLOCK;
+            const char *blk = ring[wave] + slot_of(j);
             const int left = mine - 1 - j;
-            const bool more = left >= DEPTH;
-            float sc[NB][8];
-            wait_blocks(left ? 3 : 1);           // K of this tile is there: V, and K and V of the next, may be in flight
-            score_tile<ROWS, NB>(kb, w, sc);
+            const bool more = left >= DEPTH;     // the places of this tile's blocks then take the tile's DEPTH on
+            float sc[8];
+            {
+                KTile kt;
+                wait_blocks(left ? 3 : 1);       // (V, and K and V of the next tile, may be in flight)
+                read_k(blk, kt);
+                score_tile<ROWS>(kt, w, sc);
+            }
             __asm__ volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
             if (more) {
                 if (((j + DEPTH) & 63) == 0) look_up(j + DEPTH);
                 load_block(a.k_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j));
             }
+            VTile vt;
             wait_blocks(more ? 3 : left ? 2 : 0);
+            read_v(blk + VX_Q4_BLOCK, vt);
             const int key0 = tl.at(i0 + wave + 4 * j) * TILE;
-            attend_tile<ROWS, NB>(w, R, s.T == 1, whole_tile(key0), sc, v, key0, vb);
+            attend_tile<ROWS>(w, whole_tile(key0), sc, v, key0, vt);
             __asm__ volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
             if (more) load_block(a.v_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j) + VX_Q4_BLOCK);
         }
+        const int ln = lane_here(), g = ln >> 4, n = ln & 15;
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+#pragma unroll
+        for (int c = 0; c < GROUPS; c++) {
+            float om = w.om[c];
+            if (ROWS == 8) om = both_halves(om);
+            om = __shfl(om, n, 64);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) w.o[4 * c + i][e] = (ROWS == 8 ? both_halves(w.o[4 * c + i][e]) : w.o[4 * c + i][e]) + om;
+        }
+        // the four waves' results through LDS (16-byte units swizzled by the row)
+        vx_lds_barrier();                        // (every wave is done with its ring)
+        if (n < R) {
+#pragma unroll
+            for (int d = 0; d < 16; d++) *(floatx4_t *)&s_o[wave][n * HDG + (((4 * d + g) ^ n) << 2)] = w.o[d];
+            if (g == 0) {
+                s_m[wave][n] = w.m;
+                s_l[wave][n] = w.l;
+            }
+        }
+        vx_lds_barrier();
+        // wave w merges rows w, w + 4, ..., lane L dims 4L .. 4L + 3
         const bool whole = cnt == tl.nt;
         const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
+        for (int r = wave; r < R; r += 4) {
+            const int t = row_tok(a, r0 + r), tok = s.start + t, h = row_head(a, kvh, r0 + r, t);
+            float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (whole && a.gate) gt = gate_row(a, tok, h);
+            float m[4], l[4];
+            float4 o[4];
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
-            const int ln = lane_here(), g = ln >> 4, n = ln & 15, Rk = min(R - k * ROWS, ROWS), rk = r0 + k * ROWS;
-            if (Rk <= 0) break;
-            Rows<ROWS> &x = w[k];
-            x.l += __shfl_xor(x.l, 16, 64);
-            x.l += __shfl_xor(x.l, 32, 64);
-#pragma unroll
-            for (int c = 0; c < GROUPS; c++) {
-                float om = x.om[c];
-                if (ROWS == 8) om = both_halves(om);
-                om = __shfl(om, n, 64);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x.o[4 * c + i][e] = (ROWS == 8 ? both_halves(x.o[4 * c + i][e]) : x.o[4 * c + i][e]) + om;
+            for (int k = 0; k < 4; k++) {
+                m[k] = s_m[k][r];
+                l[k] = s_l[k][r];
+                o[k] = *(const float4 *)&s_o[k][r * HDG + ((ln ^ r) << 2)];
             }
-            // the four waves' results through LDS (16-byte units swizzled by the row)
-            vx_lds_barrier();                    // (every wave is done with its ring, and with the rows before)
-            if (n < Rk) {
+            const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            float L = 0.0f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int d = 0; d < 16; d++) *(floatx4_t *)&s_o[wave][n * HDG + (((4 * d + g) ^ n) << 2)] = x.o[d];
-                if (g == 0) {
-                    s_m[wave][n] = x.m;
-                    s_l[wave][n] = x.l;
-                }
-            }
-            vx_lds_barrier();
-            // wave w merges rows w, w + 4, ..., lane L dims 4L .. 4L + 3
-            for (int r = wave; r < Rk; r += 4) {
-                const int t = row_tok(a, rk + r), tok = s.start + t, h = row_head(a, kvh, rk + r, t);
-                float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (whole && a.gate) gt = gate_row(a, tok, h);
-                float m[4], l[4];
-                float4 o[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    m[i] = s_m[i][r];
-                    l[i] = s_l[i][r];
-                    o[i] = *(const float4 *)&s_o[i][r * HDG + ((ln ^ r) << 2)];
-                }
-                const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                float L = 0.0f;
-                float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int i = 0; i < 4; i++) add_part(O, L, o[i], l[i], m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - M));
-                if (whole) {
-                    row_finish(a, tok, h, O, M, L, gt);
-                } else {
-                    *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + k * ROWS + r) * HDG + 4 * ln) = O;
-                    if (ln == 0) a.part_ml[(size_t)slot * a.part_rows + k * ROWS + r] = make_float2(M, L);
-                }
+            for (int k = 0; k < 4; k++) add_part(O, L, o[k], l[k], m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - M));
+            if (whole) {
+                row_finish(a, tok, h, O, M, L, gt);
+            } else {
+                *(float4 *)(a.part_o + ((size_t)slot * a.part_rows + r) * HDG + 4 * ln) = O;
+                if (ln == 0) a.part_ml[(size_t)slot * a.part_rows + r] = make_float2(M, L);
             }
         }
         vx_lds_barrier();
@@ -430,13 +423,12 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     const int rows = d->max_T * a.qg;
     if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32)) return rows_launch<true>(who, ctx, d, a, rows, 0);
     // two parts of the weights where the output is fp32, one where it is rounded to bf16 itself
-    const int one = a.out_bf16 ? 16 : 8, n_b = std::min((rows + one - 1) / one, 1);
-    a.block_rows = one * n_b;
+    a.block_rows = a.out_bf16 ? 16 : 8;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;
     const int64_t units = (int64_t)d->B * d->n_kv * nb * a.tile_cap;
     VX_REQUIRE(units < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %d tiles each)", who, d->B, d->n_kv, a.tile_cap);
     a.min_tiles = 2;
-    const int grid = (int)std::min<int64_t>((units + a.min_tiles - 1) / a.min_tiles, (n_b == 1 ? 2 : 1) * ctx->n_cu);
+    const int grid = (int)std::min<int64_t>((units + a.min_tiles - 1) / a.min_tiles, 2 * ctx->n_cu);
     a.part_rows = std::min(rows, a.block_rows);
     const size_t n_part = (size_t)2 * grid * a.part_rows;
     const size_t o_bytes = n_part * HDG * 4, ml_bytes = (n_part * sizeof(float2) + 255) / 256 * 256;
@@ -447,17 +439,8 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     a.part_ml = (float2 *)((char *)scr + o_bytes);
     a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes) : nullptr;
     if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true>), dim3(1), dim3(1024), a);
-#define SPLIT(ROWS, NB, PER) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<ROWS, NB, 2, PER>), dim3(grid), dim3(256), a)
-    if (one == 16) {
-        if (n_b == 1) SPLIT(16, 1, 2);
-        else if (n_b == 2) SPLIT(16, 2, 1);
-        else SPLIT(16, 3, 1);
-    } else {
-        if (n_b == 1) SPLIT(8, 1, 2);
-        else if (n_b == 2) SPLIT(8, 2, 1);
-        else SPLIT(8, 3, 1);
-    }
-#undef SPLIT
+    if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16>), dim3(grid), dim3(256), a);
+    else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8>), dim3(grid), dim3(256), a);
     VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<true>), dim3(a.part_rows, d->n_kv * nb, d->B), dim3(256), a, grid);
     return 0;
 }
