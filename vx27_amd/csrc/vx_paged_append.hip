@@ -104,16 +104,12 @@ __device__ __forceinline__ double over_group(double x) {   // maximum or minimum
     x = pick(x, vx_dpp_f64<0x124, 0xF>(x));
     return pick(x, vx_dpp_f64<0x128, 0xF>(x));
 }
-// The bf16 number at or beyond x, down or up (|x| at most BF16_MAX), as the
-// bits of an fp32 number: the truncated bits, or a step on.
+// The largest bf16 number not above x (|x| at most BF16_MAX), as the bits of an
+// fp32 number: the truncated bits, or a step on.
 __device__ __forceinline__ uint32_t bf16_below(double x) {
     const uint32_t b = __float_as_uint((float)x) & 0xffff0000u;
     if ((double)__uint_as_float(b) <= x) return b;
     return (b & 0x7fffffffu) == 0 ? 0x80010000u : b & 0x80000000u ? b + 0x10000u : b - 0x10000u;
-}
-__device__ __forceinline__ uint32_t bf16_above(double x) {   // x >= 0
-    const uint32_t b = __float_as_uint((float)x) & 0xffff0000u;
-    return (double)__uint_as_float(b) >= x ? b : b + 0x10000u;
 }
 // The codes of a lane's four values as bytes, and its group's s and m (bits 16
 // to 31 of each).
@@ -130,19 +126,40 @@ __device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_b
     }
     m_bits = bf16_below(over_group<false>(fmin(fmin(y[0], y[1]), fmin(y[2], y[3]))));
     const double m = __uint_as_float(m_bits);
-    s_bits = bf16_above((over_group<true>(fmax(fmax(y[0], y[1]), fmax(y[2], y[3]))) - m) / 15.0);
-    const double s = __uint_as_float(s_bits);
-    if (s == 0.0) return 0;
-    const double rs = 1.0 / s;
+    // s: the bf16 number just below range / 15 (a last place of the product may
+    // be off), and up while 15 s (exact) is below the range
+    const double range = over_group<true>(fmax(fmax(y[0], y[1]), fmax(y[2], y[3]))) - m;
+    uint32_t b = __float_as_uint((float)(range * (1.0 / 15.0))) & 0xffff0000u;
+    if (b) b -= 0x10000u;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if ((double)__uint_as_float(b) * 15.0 < range) b += 0x10000u;
+    s_bits = b;
+    const float s = __uint_as_float(s_bits), rs = __builtin_amdgcn_rcpf(s);
+    if (s_bits == 0) return 0;
+    // The nearest code.  In fp32 the quotient is 2^-17 off at most (three
+    // roundings of 2^-23 and less of it, 15 and less); where that could decide,
+    // by what the code leaves in fp64, where it is exact.
     uint32_t codes = 0;
+    float far = 0.0f, q[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        // the nearest code, and what it leaves (exact): a product with 1/s may
-        // be a last place off where the quotient is just between two
+        q[e] = (float)(y[e] - m) * rs;
+        const float c = __builtin_rintf(q[e]);
+        far = fmaxf(far, __builtin_fabsf(q[e] - c));
+        codes |= (uint32_t)c << (8 * e);
+    }
+    // (a tiny s: fp32 has no reciprocal of it; a range past fp32: the quotient is infinite)
+    const bool sure = far < 0.5f - 0x1p-16f && s > 0x1p-100f && range < 0x1p127;
+    if (__all(sure)) return codes;
+    codes = 0;
+    const double rd = 1.0 / (double)s;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
         const double d = y[e] - m;
-        double c = __builtin_rint(d * rs);
-        const double r = 2.0 * __builtin_fma(-c, s, d);
-        if (__builtin_fabs(r) > s || (__builtin_fabs(r) == s && ((int)c & 1))) c += r > 0.0 ? 1.0 : -1.0;
+        double c = __builtin_rint(d * rd);
+        const double r = 2.0 * __builtin_fma(-c, (double)s, d);
+        if (__builtin_fabs(r) > (double)s || (__builtin_fabs(r) == (double)s && ((int)c & 1))) c += r > 0.0 ? 1.0 : -1.0;
         codes |= (uint32_t)min(max((int)c, 0), 15) << (8 * e);
     }
     return codes;
@@ -172,13 +189,19 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
             *(uint16_t *)(blk + VX_Q4_M + (is_v ? c * 64 + r * 2 : r * 8 + c * 2)) = (uint16_t)(m >> 16);
         }
     };
+    // (a wave's next row is loaded while it works on one; rows unrolled or four at a time take the registers of the
+    // other workgroups' waves)
+    auto load_row = [&](const void *src, int j) { return load4(src, (size_t)(tok0 + min(j, n - 1)) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16); };
     // V
     char *vb = (char *)a.v_pages + block;
+    float4 x = load_row(a.v, wave);
+#pragma unroll 1
     for (int j = wave; j < n; j += 4) {
-        const float4 x = load4(a.v, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16);
         const double y[4] = {x.x, x.y, x.z, x.w};
+        x = load_row(a.v, j + 4);
         store(vb, j, y, true);
     }
+    x = load_row(a.k, wave);
     __syncthreads();
     {
         const int dim = 64 * (tid >> 6) + (tid & 15), r8 = 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 16 i, rows r8 .. r8 + 7
@@ -208,7 +231,7 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
     const float4 wf = ((const float4 *)a.k_norm_w)[lane];
     const double one = (a.flags & VX27_GQA_NORM_W) ? 0.0 : 1.0;
     const double w[4] = {wf.x + one, wf.y + one, wf.z + one, wf.w + one};
-    const int chunk = half ? min(Q4_CS / half, VB) : VB;
+    const int chunk = half ? min(Q4_CS / half & ~3, VB) : VB;   // (4 rows at least: half is 128 at most)
     for (int j0 = 0; j0 < n; j0 += chunk) {
         const int j1 = min(j0 + chunk, n);
         for (int e = tid; e < (j1 - j0) * half; e += 256) {
@@ -218,9 +241,11 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
             cs[e] = make_double2(c, sn);
         }
         __syncthreads();
+        // (a chunk is a multiple of 4 rows, or all: a wave's rows go on from one to the next)
+#pragma unroll 1
         for (int j = j0 + wave; j < j1; j += 4) {
-            const float4 x = load4(a.k, (size_t)(tok0 + j) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16);
             double y[4] = {x.x, x.y, x.z, x.w};
+            x = load_row(a.k, j + 4);
             double ss = y[0] * y[0];
 #pragma unroll
             for (int e = 1; e < 4; e++) ss = __builtin_fma(y[e], y[e], ss);

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256) void pages_fill(PlanArgs a) {
 
 // ------------------------------------------------------------------- read
 struct ReadArgs {
-    int n_kv, page_size, n_pages, n_rows, bf16;
+    int n_kv, page_size, n_pages, n_rows, bf16, log2_page;
     const int *slots;
     const char *k_pages, *v_pages;
     void *k_out, *v_out;
@@ -226,45 +226,151 @@ __device__ __forceinline__ uint32_t bf16x2(float x, float y) {
     const bf16x2_t v = (bf16x2_t){(__bf16)x, (__bf16)y};
     return __builtin_bit_cast(uint32_t, v);
 }
-__device__ __forceinline__ float bf16_at(const char *p) { return vx_bf16_to_f32(*(const uint16_t *)p); }
 
-// grid (n_rows / 4, n_kv), block 256: a row a wave.
-__global__ __launch_bounds__(256) void paged_read_q4(ReadArgs a) {
-    const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = blockIdx.y;
-    if (i >= a.n_rows) return;
-    const int slot = __builtin_amdgcn_readfirstlane(a.slots[i]);
-    if (slot < 0 || slot >= a.n_pages * a.page_size) {
-        if (slot != -1) *a.err_flag = 1;
+// Of 4 lanes that have 4 words each, lane t gets the words t of all, in order.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const uint32_t t = threadIdx.x & 3;
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t y = (uint32_t)vx_dpp_i<0xB1, 0xF>((int)w[i ^ 1]);   // of lane ^ 1 (all lanes take part)
+        x[i] = (t ^ i) & 1 ? y : w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t y = (uint32_t)vx_dpp_i<0x4E, 0xF>((int)x[i ^ 2]);   // of lane ^ 2
+        w[i] = (t ^ i) & 2 ? y : x[i];
+    }
+}
+__device__ __forceinline__ void put_values(const ReadArgs &a, void *out, size_t at, const float (&x)[4]) {
+    if (a.bf16) *(uint2 *)((uint16_t *)out + at) = make_uint2(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]));
+    else *(float4 *)((float *)out + at) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// 8 rows of K or of V a wave, whose loads are in flight together (the slots'
+// checks and the conversions come behind them: between the loads they made each
+// row wait for its own).  Eight rows of a block that share V's units, as a
+// sequence read in order has them, are one load of codes and up to three of s
+// and m; any other rows three loads each.  (Loads and stores, 16 cycles each,
+// bound the second form.)  32768 rows of 4 heads in order 37 us in bf16 (the
+// copy rate: 33) and 79 in fp32, in random order 56; 77 rows 3.2.
+constexpr int READ_ROWS = 8;
+template <bool V>
+__device__ __forceinline__ void read_rows(const ReadArgs &a, int i0, int h, const char *pages, void *out) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int mine = a.slots[min(i0 + min(lane, READ_ROWS - 1), a.n_rows - 1)];
+    const bool in = mine >= 0 && mine < a.n_pages * a.page_size;
+    const int place = in ? mine : 0;
+    const int page = a.log2_page >= 0 ? place >> a.log2_page : place / a.page_size, at = place - page * a.page_size;
+    const int block = (int)(((uint32_t)page * (uint32_t)a.n_kv + (uint32_t)h) * (uint32_t)(a.page_size / VX_PG_TILE) + (uint32_t)(at / VX_PG_TILE));
+    auto block_of = [&](int k) { return pages + (size_t)(uint32_t)__builtin_amdgcn_readlane(block, k) * VX_Q4_BLOCK; };
+    auto row_of = [&](int k) { return __builtin_amdgcn_readlane(at, k) % VX_PG_TILE; };
+    auto out_at = [&](int k) { return ((size_t)(i0 + k) * a.n_kv + h) * VX_GQA_HD; };
+    const int first = __builtin_amdgcn_readfirstlane(mine);
+    if (first >= 0 && first % READ_ROWS == 0 && i0 + READ_ROWS <= a.n_rows && __all(in && mine == first + min(lane, READ_ROWS - 1))) {
+        const char *blk = block_of(0);
+        const int r0 = row_of(0);
+        if constexpr (V) {   // lane (j,n): a unit, dims 64 j + 16 i + n of the 8 rows; then dims 64 j + 16 (n % 4) + 4 (n / 4) + e
+            const int n = lane & 15;
+            const uint4 c = *(const uint4 *)(blk + (64 * g + 2 * r0 + n) * 16);
+            const uint4 s4 = *(const uint4 *)(blk + VX_Q4_S + g * 64 + r0 * 2), m4 = *(const uint4 *)(blk + VX_Q4_M + g * 64 + r0 * 2);
+            float s[8], m[8];
+            vx_q4_f32(s4, s);
+            vx_q4_f32(m4, m);
+            uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            transpose4(w);
+#pragma unroll
+            for (int k = 0; k < READ_ROWS; k++) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((w[e] >> (8 * (k & 3) + (k & 4))) & 15), s[k], m[k]);
+                put_values(a, out, out_at(k) + 64 * g + 16 * (n & 3) + 4 * (n >> 2), x);
+            }
+        } else {             // lane (half, k, g, r): a unit, dims 128 k + 32 i + 8 g .. + 7 of row 4 half + r
+            const int kh = (lane >> 4) & 1, gd = (lane >> 2) & 3, r = 4 * (lane >> 5) + (lane & 3);
+            const uint4 c = *(const uint4 *)(blk + vx_q4_k_unit(r0 + r, 128 * kh + 8 * gd) * 16);
+            const uint32_t m2 = *(const uint32_t *)(blk + VX_Q4_M + (r0 + r) * 8 + kh * 4);
+            uint16_t s2[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) s2[e] = *(const uint16_t *)(blk + VX_Q4_S + (2 * kh + e) * 64 + (r0 + r) * 2);
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float s = vx_bf16_to_f32(s2[i >> 1]), m = __uint_as_float(i >> 1 ? m2 & 0xffff0000u : m2 << 16);
+                const size_t o = out_at(r) + 128 * kh + 32 * i;
+                if (a.bf16) {
+                    float x[8];
+                    vx_q4_codes_f32(w[i], x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(x[e], s, m);
+                    *(uint4 *)((uint16_t *)out + o + 8 * gd) = make_uint4(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]), bf16x2(x[4], x[5]), bf16x2(x[6], x[7]));
+                    continue;
+                }
+                // fp32: four lanes' 16 bytes side by side, dims 4 gd .. + 3 of 16 (32 bytes a lane: 8192 rows 19.9 us, so 17.7)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint32_t y = (uint32_t)__shfl((int)w[i], (lane & ~12) + 8 * t + 4 * (gd >> 1), 64), z = (gd & 1 ? y >> 4 : y) & 0x0f0f0f0fu;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((z >> (8 * e)) & 255), s, m);
+                    put_values(a, out, o + 16 * t + 4 * gd, x);
+                }
+            }
+        }
         return;
     }
-    const int page = slot / a.page_size, at = slot - page * a.page_size, row = at % VX_PG_TILE;
-    const size_t block = (((size_t)page * a.n_kv + h) * (a.page_size / VX_PG_TILE) + at / VX_PG_TILE) * VX_Q4_BLOCK;
-    const size_t out = ((size_t)i * a.n_kv + h) * VX_GQA_HD;
-    if (a.k_out) {   // lane: dims 4 lane .. + 3
-        const char *blk = a.k_pages + block;
-        const int c = lane >> 4;
-        const uint32_t w = *(const uint32_t *)(blk + vx_q4_k_unit(row, 4 * lane) * 16 + ((lane >> 3) & 3) * 4) >> (4 * (lane & 1));
-        const float s = bf16_at(blk + VX_Q4_S + c * 64 + row * 2), m = bf16_at(blk + VX_Q4_M + row * 8 + c * 2);
-        float x[4];
+    // row by row: lane L has dims 4L .. 4L + 3 of K, and of V as above
+    const uint32_t c_at = V ? g * 1024 + (lane & 15) * 16 : vx_q4_k_unit(0, 4 * lane) * 16 + ((lane >> 3) & 3) * 4;
+    const uint32_t s_at = VX_Q4_S + g * 64, m_at = VX_Q4_M + g * (V ? 64 : 2);
+    uint32_t c[READ_ROWS][V ? 4 : 1];
+    uint16_t s[READ_ROWS], m[READ_ROWS];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((w >> (8 * e)) & 15), s, m);
-        if (a.bf16) *(uint2 *)((uint16_t *)a.k_out + out + 4 * lane) = make_uint2(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]));
-        else *(float4 *)((float *)a.k_out + out + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
-    }
-    if (a.v_out) {   // lane (j,n): dims 64 j + 16 e + n
-        const char *blk = a.v_pages + block;
-        const int j = lane >> 4, n = lane & 15;
-        const uint4 u = *(const uint4 *)(blk + (64 * j + 16 * (row >> 3) + n) * 16);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        const float s = bf16_at(blk + VX_Q4_S + j * 64 + row * 2), m = bf16_at(blk + VX_Q4_M + j * 64 + row * 2);
-        const int shift = 8 * (row & 3) + (row & 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float x = __builtin_fmaf((float)((w[e] >> shift) & 15), s, m);
-            const size_t d = out + 64 * j + 16 * e + n;
-            if (a.bf16) ((uint16_t *)a.v_out)[d] = vx_f32_to_bf16(x);
-            else ((float *)a.v_out)[d] = x;
+    for (int k = 0; k < READ_ROWS; k++) {
+        const int r = row_of(k);
+        const char *blk = block_of(k), *codes = blk + (V ? (r >> 3) * 256 : vx_q4_k_unit(r, 0) * 16);
+        if constexpr (V) {
+            const uint4 x = *(const uint4 *)(codes + c_at);
+            c[k][0] = x.x; c[k][1] = x.y; c[k][2] = x.z; c[k][3] = x.w;
+        } else {
+            c[k][0] = *(const uint32_t *)(codes + c_at);
         }
+        s[k] = *(const uint16_t *)(blk + r * 2 + s_at);
+        m[k] = *(const uint16_t *)(blk + r * (V ? 2 : 8) + m_at);
+    }
+    if (!in && mine != -1) *a.err_flag = 1;
+    const uint64_t live = __ballot(in);
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; k++) {
+        if (i0 + k >= a.n_rows) return;
+        if (!((live >> k) & 1)) continue;
+        const int r = row_of(k);
+        const float sc = vx_bf16_to_f32(s[k]), mn = vx_bf16_to_f32(m[k]);
+        float x[4];
+        size_t o = out_at(k);
+        if constexpr (V) {
+            const int shift = 8 * (r & 3) + (r & 4);
+            transpose4(c[k]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((c[k][e] >> shift) & 15), sc, mn);
+            o += 64 * g + 16 * (lane & 3) + 4 * ((lane >> 2) & 3);
+        } else {
+            const uint32_t w = (lane & 1 ? c[k][0] >> 4 : c[k][0]) & 0x0f0f0f0fu;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf((float)((w >> (8 * e)) & 255), sc, mn);
+            o += 4 * lane;
+        }
+        put_values(a, out, o, x);
+    }
+}
+
+// grid (n_rows / (4 READ_ROWS), n_kv, 2), block 256: z 0 reads K, 1 V.
+__global__ __launch_bounds__(256) void paged_read_q4(ReadArgs a) {
+    const int i0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * READ_ROWS;
+    if (i0 >= a.n_rows) return;
+    if (blockIdx.z == 0) {
+        if (a.k_out) read_rows<false>(a, i0, blockIdx.y, a.k_pages, a.k_out);
+    } else {
+        if (a.v_out) read_rows<true>(a, i0, blockIdx.y, a.v_pages, a.v_out);
     }
 }
 
@@ -339,6 +445,7 @@ extern "C" int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_d
                who, VX_PG_TILE, d->page_size);
     VX_REQUIRE(d->n_pages >= 1 && (int64_t)d->n_pages * d->page_size < (1ll << 31), "%s: need n_pages >= 1 and n_pages * page_size below 2^31 (%d * %d)",
                who, d->n_pages, d->page_size);
+    if (vx_q4_fits(who, d->n_pages, d->n_kv, d->page_size)) return -1;
     VX_REQUIRE(d->n_rows >= 0 && d->n_rows <= (1 << 25), "%s: need 0 <= n_rows <= 2^25 (got %d)", who, d->n_rows);
     VX_REQUIRE(d->out_dtype == VX27_F32 || d->out_dtype == VX27_BF16, "%s: out_dtype must be VX27_F32 or VX27_BF16 (got %d)", who, d->out_dtype);
     VX_REQUIRE(d->slots && (d->k_pages || !d->k_out) && (d->v_pages || !d->v_out), "%s: null pointer in descriptor", who);
@@ -346,8 +453,9 @@ extern "C" int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_d
                "%s: pages and outputs must be 16-byte aligned", who);
     if (vx_ctx_enter(ctx)) return -1;
     if (d->n_rows == 0 || (!d->k_out && !d->v_out)) return 0;
-    const ReadArgs a = {d->n_kv, d->page_size, d->n_pages, d->n_rows, d->out_dtype == VX27_BF16, d->slots,
+    const ReadArgs a = {d->n_kv, d->page_size, d->n_pages, d->n_rows, d->out_dtype == VX27_BF16,
+                        (d->page_size & (d->page_size - 1)) == 0 ? __builtin_ctz(d->page_size) : -1, d->slots,
                         (const char *)d->k_pages, (const char *)d->v_pages, d->k_out, d->v_out, ctx->err_flag};
-    VX_LAUNCH(ctx, paged_read_q4, dim3((d->n_rows + 3) / 4, d->n_kv), dim3(256), a);
+    VX_LAUNCH(ctx, paged_read_q4, dim3((d->n_rows + 4 * READ_ROWS - 1) / (4 * READ_ROWS), d->n_kv, 2), dim3(256), a);
     return 0;
 }
