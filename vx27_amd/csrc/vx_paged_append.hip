@@ -91,18 +91,23 @@ __device__ __forceinline__ double wave_sums4(const double (&s)[4]) {
 }
 
 // ---------------------------------------------------------- 4-bit pages
-// A row's group is 16 lanes of 4 dims.  Everything is in fp64: k's values carry
-// errors of the norm's sum, the angles and the products, and in fp32 these
-// would move a code now and then (one value in 10^6) against another order of
-// the sums; in fp64 the codes are those of the exact values.
+// A row's group is 16 lanes of 4 dims.  Values are taken as they are: v's in
+// fp32 (REAL float), k's in fp64.  (k carries errors of the norm's sum, the
+// angles and the products, and in fp32 these would move a code now and then,
+// one value in 10^6, against another order of the sums; in fp64 the codes are
+// those of the exact values.)
 constexpr float BF16_MAX = 3.38953139e38f;
-template <bool MAX>
-__device__ __forceinline__ double over_group(double x) {   // maximum or minimum over 16 lanes
-    auto pick = [](double u, double v) { return MAX ? fmax(u, v) : fmin(u, v); };
-    x = pick(x, vx_dpp_f64<0xB1, 0xF>(x));
-    x = pick(x, vx_dpp_f64<0x4E, 0xF>(x));
-    x = pick(x, vx_dpp_f64<0x124, 0xF>(x));
-    return pick(x, vx_dpp_f64<0x128, 0xF>(x));
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false)); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_f(double x) { return vx_dpp_f64<CTRL, 0xF>(x); }
+template <bool MAX, typename REAL>
+__device__ __forceinline__ REAL over_group(REAL x) {   // maximum or minimum over 16 lanes
+    auto pick = [](REAL u, REAL v) { return MAX ? __builtin_elementwise_max(u, v) : __builtin_elementwise_min(u, v); };
+    x = pick(x, dpp_f<0xB1>(x));
+    x = pick(x, dpp_f<0x4E>(x));
+    x = pick(x, dpp_f<0x124>(x));
+    return pick(x, dpp_f<0x128>(x));
 }
 // The largest bf16 number not above x (|x| at most BF16_MAX), as the bits of an
 // fp32 number: the truncated bits, or a step on.
@@ -113,22 +118,26 @@ __device__ __forceinline__ uint32_t bf16_below(double x) {
 }
 // The codes of a lane's four values as bytes, and its group's s and m (bits 16
 // to 31 of each).
-__device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_bits, uint32_t &m_bits) {
+template <typename REAL>
+__device__ __forceinline__ uint32_t quantise(const REAL (&y)[4], uint32_t &s_bits, uint32_t &m_bits) {
     const int lane = threadIdx.x & 63;
     bool fine = true;
 #pragma unroll
-    for (int e = 0; e < 4; e++) fine &= __builtin_fabs(y[e]) <= (double)BF16_MAX;
+    for (int e = 0; e < 4; e++) fine &= __builtin_elementwise_abs(y[e]) <= (REAL)BF16_MAX;
     const uint64_t off = __ballot(!fine);
     if ((off >> (lane & 48)) & 0xffff) {
         s_bits = 0;
         m_bits = 0x7fc00000u;
         return 0;
     }
-    m_bits = bf16_below(over_group<false>(fmin(fmin(y[0], y[1]), fmin(y[2], y[3]))));
+    REAL lo = y[0], hi = y[0];
+#pragma unroll
+    for (int e = 1; e < 4; e++) lo = __builtin_elementwise_min(lo, y[e]), hi = __builtin_elementwise_max(hi, y[e]);
+    m_bits = bf16_below(over_group<false>(lo));
     const double m = __uint_as_float(m_bits);
     // s: the bf16 number just below range / 15 (a last place of the product may
     // be off), and up while 15 s (exact) is below the range
-    const double range = over_group<true>(fmax(fmax(y[0], y[1]), fmax(y[2], y[3]))) - m;
+    const double range = (double)over_group<true>(hi) - m;
     uint32_t b = __float_as_uint((float)(range * (1.0 / 15.0))) & 0xffff0000u;
     if (b) b -= 0x10000u;
 #pragma unroll
@@ -141,12 +150,11 @@ __device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_b
     // roundings of 2^-23 and less of it, 15 and less); where that could decide,
     // by what the code leaves in fp64, where it is exact.
     uint32_t codes = 0;
-    float far = 0.0f, q[4];
+    float far = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        q[e] = (float)(y[e] - m) * rs;
-        const float c = __builtin_rintf(q[e]);
-        far = fmaxf(far, __builtin_fabsf(q[e] - c));
+        const float q = (float)(y[e] - (REAL)m) * rs, c = __builtin_rintf(q);
+        far = fmaxf(far, __builtin_fabsf(q - c));
         codes |= (uint32_t)c << (8 * e);
     }
     // (a tiny s: fp32 has no reciprocal of it; a range past fp32: the quotient is infinite)
@@ -156,7 +164,7 @@ __device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_b
     const double rd = 1.0 / (double)s;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const double d = y[e] - m;
+        const double d = (double)y[e] - m;
         double c = __builtin_rint(d * rd);
         const double r = 2.0 * __builtin_fma(-c, (double)s, d);
         if (__builtin_fabs(r) > (double)s || (__builtin_fabs(r) == (double)s && ((int)c & 1))) c += r > 0.0 ? 1.0 : -1.0;
@@ -165,12 +173,23 @@ __device__ __forceinline__ uint32_t quantise(const double (&y)[4], uint32_t &s_b
     return codes;
 }
 
+// 1 / sqrt(x) of a normal x within 2^-50: two of Newton's steps from the
+// hardware's 2^-22 (at the ends of fp32's range by the library).
+__device__ __forceinline__ double inv_sqrt(double x) {
+    if (!(x < 1e30)) return 1.0 / sqrt(x);      // (x is 1e-6 at least, or NaN)
+    double r = __builtin_amdgcn_rsqf((float)x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) r = __builtin_fma(r * 0.5, __builtin_fma(-x * r, r, 1.0), r);
+    return r;
+}
+
 // One KV head's new rows [lo, hi) of the block at row p0 of sequence b: a row a
 // wave, its codes into LDS by bytes; then thread u stores 16-byte unit u of the
 // block, or of V, where 8 rows share one, as much of it as is new.
 constexpr int CODE_ROW = HDG + 4;             // (rows 8 apart then lie in different banks)
 constexpr int Q4_CS = 512;                    // (cos, sin) of a chunk of rows
 constexpr int Q4_LDS = VB * CODE_ROW + Q4_CS * 16 + 4 * HDG * 8;
+template <bool V>
 __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int lo, int hi, int tok0, char *lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = hi - lo, half = a.rope_dim / 2;
@@ -179,36 +198,34 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
     char *codes = lds;
     double2 *cs = (double2 *)(lds + VB * CODE_ROW);
     double *row = (double *)(lds + VB * CODE_ROW + Q4_CS * 16) + wave * HDG;
-    auto store = [&](char *blk, int j, const double (&y)[4], bool is_v) {
+    char *blk = (char *)(V ? a.v_pages : a.k_pages) + block;
+    auto store = [&](int j, const auto &y) {
         const int r = lo - p0 + j;
         uint32_t s, m;
         *(uint32_t *)(codes + r * CODE_ROW + 4 * lane) = quantise(y, s, m);
         if ((lane & 15) == 0) {
             const int c = lane >> 4;
             *(uint16_t *)(blk + VX_Q4_S + c * 64 + r * 2) = (uint16_t)(s >> 16);
-            *(uint16_t *)(blk + VX_Q4_M + (is_v ? c * 64 + r * 2 : r * 8 + c * 2)) = (uint16_t)(m >> 16);
+            *(uint16_t *)(blk + VX_Q4_M + (V ? c * 64 + r * 2 : r * 8 + c * 2)) = (uint16_t)(m >> 16);
         }
     };
     // (a wave's next row is loaded while it works on one; rows unrolled or four at a time take the registers of the
     // other workgroups' waves)
-    auto load_row = [&](const void *src, int j) { return load4(src, (size_t)(tok0 + min(j, n - 1)) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16); };
-    // V
-    char *vb = (char *)a.v_pages + block;
-    float4 x = load_row(a.v, wave);
+    auto load_row = [&](int j) { return load4(V ? a.v : a.k, (size_t)(tok0 + min(j, n - 1)) * a.kv_ts + (size_t)hk * HDG + 4 * lane, a.bf16); };
+    float4 x = load_row(wave);
+    if constexpr (V) {
 #pragma unroll 1
-    for (int j = wave; j < n; j += 4) {
-        const double y[4] = {x.x, x.y, x.z, x.w};
-        x = load_row(a.v, j + 4);
-        store(vb, j, y, true);
-    }
-    x = load_row(a.k, wave);
-    __syncthreads();
-    {
+        for (int j = wave; j < n; j += 4) {
+            const float y[4] = {x.x, x.y, x.z, x.w};
+            x = load_row(j + 4);
+            store(j, y);
+        }
+        __syncthreads();
         const int dim = 64 * (tid >> 6) + (tid & 15), r8 = 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 16 i, rows r8 .. r8 + 7
         uint32_t fresh = 0;                                                        // its new rows
         for (int k = 0; k < 8; k++) fresh |= p0 + r8 + k >= lo && p0 + r8 + k < hi ? 1u << k : 0u;
         if (fresh) {
-            uint4 *dst = (uint4 *)(vb + tid * 16);
+            uint4 *dst = (uint4 *)(blk + tid * 16);
             uint32_t u[4] = {0, 0, 0, 0}, mask = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -224,10 +241,8 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
             }
             *dst = make_uint4(u[0], u[1], u[2], u[3]);
         }
+        return;
     }
-    __syncthreads();
-    // K
-    char *kb = (char *)a.k_pages + block;
     const float4 wf = ((const float4 *)a.k_norm_w)[lane];
     const double one = (a.flags & VX27_GQA_NORM_W) ? 0.0 : 1.0;
     const double w[4] = {wf.x + one, wf.y + one, wf.z + one, wf.w + one};
@@ -245,11 +260,11 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
 #pragma unroll 1
         for (int j = j0 + wave; j < j1; j += 4) {
             double y[4] = {x.x, x.y, x.z, x.w};
-            x = load_row(a.k, j + 4);
+            x = load_row(j + 4);
             double ss = y[0] * y[0];
 #pragma unroll
             for (int e = 1; e < 4; e++) ss = __builtin_fma(y[e], y[e], ss);
-            const double sc = 1.0 / sqrt(vx_wave_sum_f64_dpp(ss) / HDG + 1e-6);
+            const double sc = inv_sqrt(vx_wave_sum_f64_dpp(ss) * (1.0 / HDG) + 1e-6);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = y[e] * sc * w[e];
             if (half) {
@@ -267,7 +282,7 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
                 }
                 __builtin_amdgcn_wave_barrier();
             }
-            store(kb, j, y, false);
+            store(j, y);
         }
         __syncthreads();
     }
@@ -279,7 +294,7 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
             const uint32_t *c = (const uint32_t *)(codes + r * CODE_ROW + dim + 32 * i);
             u[i] = c[0] | (c[1] << 4);
         }
-        *(uint4 *)(kb + tid * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+        *(uint4 *)(blk + tid * 16) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
@@ -303,8 +318,9 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     constexpr int NR = 4;
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int blk = blockIdx.x / (1 + VB / QTOK), part = blockIdx.x % (1 + VB / QTOK);
-    const bool is_k = part == 0;
+    constexpr int KV = Q4 ? 2 : 1;                        // workgroups of a block's keys and values
+    const int blk = blockIdx.x / (KV + VB / QTOK), part = blockIdx.x % (KV + VB / QTOK);
+    const bool is_k = part < KV;
     if (!is_k && !a.q) return;
     // v's rows; then the tokens' cos and sin, and a row a wave
     constexpr int CS = VB * HALFS * 4;
@@ -316,12 +332,13 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     if (s.row0 < 0 && tid == 0 && hk == 0 && blockIdx.x == 0) *a.p.err_flag = 1;
     const int first = max(s.row0, 0);
     const int p0 = (first / VB + blk) * VB;               // first row of the block
-    const int q0 = is_k ? p0 : p0 + QTOK * (part - 1);    // this workgroup's rows [lo, hi)
+    const int q0 = is_k ? p0 : p0 + QTOK * (part - KV);    // this workgroup's rows [lo, hi)
     const int lo = max(q0, first), hi = min(q0 + (is_k ? VB : QTOK), s.len);
     if (lo >= hi) return;
     const int n = hi - lo, tok0 = s.start + (lo - s.row0), half = a.rope_dim / 2;
     if constexpr (Q4) {
-        if (is_k) return append_q4_block(a, hk, b, p0, lo, hi, tok0, lds);
+        if (part == 0) return append_q4_block<false>(a, hk, b, p0, lo, hi, tok0, lds);
+        if (part == 1) return append_q4_block<true>(a, hk, b, p0, lo, hi, tok0, lds);
     }
     const int per = is_k ? 1 : a.qg, rows = n * per;      // heads of a token
     const uint32_t magic = is_k ? 0 : a.qg_magic;
@@ -472,7 +489,7 @@ int append(const char *who, vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) 
     a.pos = d->pos; a.q = d->q; a.k = d->k_new; a.v = d->v_new;
     a.q_norm_w = d->q_norm_w; a.k_norm_w = d->k_norm_w;
     a.q_out = d->q_out; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
-    const dim3 grid(((d->max_T + VB - 2) / VB + 1) * (1 + VB / QTOK), d->n_kv, d->B);
+    const dim3 grid(((d->max_T + VB - 2) / VB + 1) * ((Q4 ? 2 : 1) + VB / QTOK), d->n_kv, d->B);
     // (32 angles a token take 16 KiB of LDS, 128 take 36: the 143 MB prompt takes 49 us with the first, 62 with the second)
     if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<32, Q4>), grid, dim3(256), a);
     else VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<MAXR, Q4>), grid, dim3(256), a);
