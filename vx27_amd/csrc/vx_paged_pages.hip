@@ -55,18 +55,21 @@ __device__ __forceinline__ int stack_page(const PlanArgs &a, const PlanSums &p, 
 }
 // Item i of a plan's second half: a token's slot, position and sequence, a
 // page taken, or a released page that stays free.
-__device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, int64_t i, int tokens, int total) {
+template <typename FROM>   // from(b, row0, pos0): row and position of the first token that sequence b got
+__device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, int64_t i, int tokens, int total, FROM from) {
     const int top = p.was_free + p.released - 1;
     if (i < a.n_tok) {
         const int t = (int)i;
         int slot = -1, pos = -1, b = -1;
         if (t < tokens) {
             b = last_le(p.start, a.B, t);
-            const int start = p.start[b], took = p.start[b + 1] - start, row0 = a.len_out[b] - took, row = row0 + t - start;
+            int row0, pos0;
+            from(b, row0, pos0);
+            const int start = p.start[b], row = row0 + t - start;
             const int pg = a.log2_page >= 0 ? row >> a.log2_page : row / a.page_size, held = plan_ceil(a, row0);
             const int page = pg < held ? checked_page(a, a.table[(size_t)b * a.max_pages + pg]) : stack_page(a, p, top - (p.grown[b] + pg - held));
             slot = page * a.page_size + (row - pg * a.page_size);
-            pos = (int)((uint32_t)(a.next_pos ? a.next_pos_out[b] - took : row0) + (uint32_t)(t - start));
+            pos = (int)((uint32_t)pos0 + (uint32_t)(t - start));
         }
         if (a.slot) a.slot[t] = slot;
         if (a.pos) a.pos[t] = pos;
@@ -76,7 +79,8 @@ __device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, 
     i -= a.n_tok;
     if (i < p.taken) {
         const int k = (int)i, b = last_le(p.grown, a.B, k);
-        const int row0 = a.len_out[b] - (p.start[b + 1] - p.start[b]);
+        int row0, pos0;
+        from(b, row0, pos0);
         a.table[(size_t)b * a.max_pages + plan_ceil(a, row0) + k - p.grown[b]] = stack_page(a, p, top - k);
         return;
     }
@@ -84,125 +88,144 @@ __device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, 
     if (at < total - p.taken) a.free_pages[at] = stack_page(a, p, at);
 }
 
-// Sums of v over the threads before this one, and in all (1024 threads).
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *sums, int64_t &all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t x = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t y = __shfl_up(x, off, 64);
-        if (lane >= off) x += y;
-    }
-    __syncthreads();   // (sums may still be read from the scan before)
-    if (lane == 63) sums[wave] = x;
-    __syncthreads();
-    int64_t before = 0;
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; w++) {
-        const int64_t s = sums[w];
-        before += w < wave ? s : 0;
-        all += s;
-    }
-    return before + x - v;
+constexpr int PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int64_t add_dpp(int64_t x) {
+    const uint64_t u = (uint64_t)x;
+    return x + (int64_t)((uint64_t)(uint32_t)vx_dpp_i<CTRL, ROW_MASK>((int)(u >> 32)) << 32 | (uint32_t)vx_dpp_i<CTRL, ROW_MASK>((int)(uint32_t)u));
 }
-
-constexpr int PLAN_THREADS = 1024;
+// Sums over lanes 0 .. l.
+__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
+    x = add_dpp<0x111, 0xF>(x);   // row_shr:1
+    x = add_dpp<0x112, 0xF>(x);
+    x = add_dpp<0x114, 0xF>(x);
+    x = add_dpp<0x118, 0xF>(x);
+    x = add_dpp<0x142, 0xA>(x);   // row_bcast:15 into rows 1 and 3
+    return add_dpp<0x143, 0xC>(x);   // row_bcast:31 into rows 2 and 3
+}
+// Sums of v[i] over the threads before this one (into v), and in all.  waves:
+// those that have any; sums: [N][PLAN_WAVES], of this call alone.
+template <int N>
+__device__ __forceinline__ void block_scan(int64_t (&v)[N], int64_t (&all)[N], int64_t *sums, int waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] = wave_scan64(v[i]);
+        if (lane == 63) sums[i * PLAN_WAVES + wave] = x[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        int64_t before = 0;
+        all[i] = 0;
+        for (int w = 0; w < waves; w++) {
+            const int64_t s = sums[i * PLAN_WAVES + w];
+            before += w < wave ? s : 0;
+            all[i] += s;
+        }
+        v[i] = before + x[i] - v[i];
+    }
+}
 
 // grid 1, block 1024: the sums; ALL (at most 1024 sequences): the rest as well,
 // from LDS, in the same launch.
 template <bool ALL>
 __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
-    __shared__ int64_t sums[16];
-    __shared__ int l_start[ALL ? PLAN_THREADS + 1 : 1], l_back[ALL ? PLAN_THREADS + 1 : 1], l_grown[ALL ? PLAN_THREADS + 1 : 1];
-    const int tid = threadIdx.x, per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS;
+    __shared__ int64_t sums[5 * PLAN_WAVES];
+    constexpr int L = ALL ? PLAN_THREADS + 1 : 1;
+    __shared__ int l_start[L], l_back[L], l_grown[L], l_row0[L], l_pos0[L];
+    const int tid = threadIdx.x, per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS, waves = min((a.B + per - 1) / per + 63, PLAN_THREADS) / 64;
     const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     const int cap = a.max_pages * a.page_size;
     const int free_in = *a.n_free, was_free = min(max(free_in, 0), a.n_pages);
     bool bad = was_free != free_in;
     // a sequence as it comes: rows (0 once it ended), its pages to give back, tokens and pages wanted
-    auto look = [&](int b, int &rows, int &back, int &want, int &need) {
-        const int len = a.len[b], n = a.new_tok[b];
-        rows = min(max(len, 0), cap);
-        want = max(n, 0);
-        bad |= rows != len || want != n;
-        const bool over = a.ended && a.ended[b] != 0;
-        back = over ? plan_ceil(a, rows) : 0;
-        if (over) rows = want = 0;
-        if (want > cap - rows) want = 0;
-        need = plan_ceil(a, rows + want) - plan_ceil(a, rows);
+    struct Seq {
+        int rows, back, want, need;
+        bool over;
     };
-    int rows, back, want, need;
-    int64_t s_back = 0, s_need = 0, s_tok = 0, s_grown = 0, all;
+    auto read = [&](int b) {
+        Seq s;
+        const int len = a.len[b], n = a.new_tok[b];
+        s.over = a.ended && a.ended[b] != 0;
+        s.rows = min(max(len, 0), cap);
+        s.want = max(n, 0);
+        bad |= s.rows != len || s.want != n;
+        s.back = s.over ? plan_ceil(a, s.rows) : 0;
+        if (s.over) s.rows = s.want = 0;
+        if (s.want > cap - s.rows) s.want = 0;
+        s.need = plan_ceil(a, s.rows + s.want) - plan_ceil(a, s.rows);
+        return s;
+    };
+    Seq one = {};
+    if (per == 1 && b0 < b1) one = read(b0);
+    auto look = [&](int b) { return per == 1 ? one : read(b); };   // (a thread's only sequence is read once)
+    int64_t first[2] = {0, 0}, all2[2], tok[1] = {0}, all1[1], last[2] = {0, 0}, given[2];
     for (int b = b0; b < b1; b++) {
-        look(b, rows, back, want, need);
-        s_back += back;
-        s_need += need;
+        const Seq s = look(b);
+        first[0] += s.back;
+        first[1] += s.need;
     }
-    int64_t released = 0;
-    const int64_t back0 = block_scan(s_back, sums, released), need0 = block_scan(s_need, sums, all);
+    block_scan<2>(first, all2, sums, waves);
+    int64_t released = all2[0];
     if (was_free + released > a.n_pages) {   // (pages given back twice, or not of this pool)
         bad = true;
         released = a.n_pages - was_free;
     }
     const int64_t total = was_free + released;
-    auto served = [&](int64_t &needs, int n, int w) {
-        needs += n;
-        return n == 0 || needs <= total ? w : 0;
+    auto served = [&](int64_t &needs, const Seq &s) {
+        needs += s.need;
+        return s.need == 0 || needs <= total ? s.want : 0;
     };
-    int64_t x = need0;
-    for (int b = b0; b < b1; b++) {
-        look(b, rows, back, want, need);
-        s_tok += served(x, need, want);
-    }
-    const int64_t tok0 = block_scan(s_tok, sums, all);
-    auto took_of = [&](int64_t &needs, int64_t &toks, int n, int w) {
-        const int t = served(needs, n, w);
+    int64_t x = first[1];
+    for (int b = b0; b < b1; b++) tok[0] += served(x, look(b));
+    block_scan<1>(tok, all1, sums + 2 * PLAN_WAVES, waves);
+    auto took_of = [&](int64_t &needs, int64_t &toks, const Seq &s) {
+        const int t = served(needs, s);
         toks += t;
         return toks <= a.n_tok ? t : 0;
     };
-    int64_t y = tok0;
-    x = need0;
-    s_tok = 0;
+    int64_t y = tok[0];
+    x = first[1];
     for (int b = b0; b < b1; b++) {
-        look(b, rows, back, want, need);
-        const int t = took_of(x, y, need, want);
-        s_tok += t;
-        s_grown += t ? need : 0;
+        const Seq s = look(b);
+        const int t = took_of(x, y, s);
+        last[0] += t;
+        last[1] += t ? s.need : 0;
     }
-    int64_t tokens, taken;
-    int64_t start = block_scan(s_tok, sums, tokens), grown = block_scan(s_grown, sums, taken), given = back0;
-    y = tok0;
-    x = need0;
+    block_scan<2>(last, given, sums + 3 * PLAN_WAVES, waves);
+    const int64_t tokens = given[0], taken = given[1];
+    y = tok[0];
+    x = first[1];
     for (int b = b0; b < b1; b++) {
-        look(b, rows, back, want, need);
-        const int t = took_of(x, y, need, want);
-        const int at = (int)start, gr = (int)grown, bk = (int)min(given, released);
-        a.q_start[b] = at;
-        if (ALL) l_start[b] = at, l_grown[b] = gr, l_back[b] = bk;
+        const Seq s = look(b);
+        const int t = took_of(x, y, s);
+        const int at = (int)last[0], gr = (int)last[1], bk = (int)min(first[0], released);
+        const int pos = a.next_pos && !s.over ? a.next_pos[b] : 0;
+        if (ALL) l_start[b] = at, l_grown[b] = gr, l_back[b] = bk, l_row0[b] = s.rows, l_pos0[b] = a.next_pos ? pos : s.rows;
         else a.grown[b] = gr, a.back[b] = bk;
+        a.q_start[b] = at;
         a.took[b] = t;
-        a.len_out[b] = rows + t;
-        if (a.next_pos) a.next_pos_out[b] = (int)((uint32_t)(a.ended && a.ended[b] != 0 ? 0 : a.next_pos[b]) + (uint32_t)t);
-        start += t;
-        grown += t ? need : 0;
-        given += back;
+        a.len_out[b] = s.rows + t;
+        if (a.next_pos) a.next_pos_out[b] = (int)((uint32_t)pos + (uint32_t)t);
+        last[0] += t;
+        last[1] += t ? s.need : 0;
+        first[0] += s.back;
     }
     if (tid == 0) {
         a.q_start[a.B] = (int)tokens;
-        if (ALL) l_start[a.B] = (int)tokens;
-        else a.was_free[0] = was_free, a.was_free[1] = (int)released, a.was_free[2] = (int)taken;
+        if (!ALL) a.was_free[0] = was_free, a.was_free[1] = (int)released, a.was_free[2] = (int)taken;
     }
     if (bad) *a.err_flag = 1;
-    if (!ALL) {
-        if (tid == 0) *a.n_free_out = (int)(total - taken);
-        return;
-    }
-    __syncthreads();   // (len_out and next_pos_out of all sequences are written)
+    __syncthreads();                         // (every thread has read n_free, which n_free_out may be)
     if (tid == 0) *a.n_free_out = (int)(total - taken);
-    const PlanSums p = {l_start, l_back, l_grown, was_free, (int)released, (int)taken};
-    const int64_t items = (int64_t)a.n_tok + max(released, taken);
-    for (int64_t i = tid; i < items; i += PLAN_THREADS) plan_item(a, p, i, (int)tokens, (int)total);
+    if constexpr (ALL) {
+        const PlanSums p = {l_start, l_back, l_grown, was_free, (int)released, (int)taken};
+        const int64_t items = (int64_t)a.n_tok + max(released, taken);
+        for (int64_t i = tid; i < items; i += PLAN_THREADS)
+            plan_item(a, p, i, (int)tokens, (int)total, [&](int b, int &row0, int &pos0) { row0 = l_row0[b], pos0 = l_pos0[b]; });
+    }
 }
 
 // grid any, block 256: the second half from the sums in memory.
@@ -210,7 +233,13 @@ __global__ __launch_bounds__(256) void pages_fill(PlanArgs a) {
     const PlanSums p = {a.q_start, a.back, a.grown, a.was_free[0], a.was_free[1], a.was_free[2]};
     const int tokens = a.q_start[a.B], total = p.was_free + p.released;
     const int64_t items = (int64_t)a.n_tok + max(p.released, p.taken);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) plan_item(a, p, i, tokens, total);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        plan_item(a, p, i, tokens, total, [&](int b, int &row0, int &pos0) {
+            const int took = a.q_start[b + 1] - a.q_start[b];
+            row0 = a.len_out[b] - took;
+            pos0 = a.next_pos ? (int)((uint32_t)a.next_pos_out[b] - (uint32_t)took) : row0;
+        });
+    }
 }
 
 // ------------------------------------------------------------------- read
