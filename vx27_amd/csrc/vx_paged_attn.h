@@ -212,7 +212,8 @@ __global__ __launch_bounds__(1024) void paged_units(Args a) {
     }
 }
 
-// grid (most rows of a block, n_kv x most blocks, B), block 256 (4-7 us): merges the parts of one query row, in
+// grid (most rows of a block, n_kv, B), or BL (n_kv x most blocks, most rows of
+// a block, B), block 256 (4-7 us): merges the parts of one query row, in
 // their order: wave w takes parts w, w + 4, ..., eight in flight; a row of a
 // sequence without rows gets 0.
 template <bool BL>
@@ -223,8 +224,8 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     vx_pseq s;
     vx_tiles tl;
     const int before = units_before<BL>(a, un, b, s, tl), nb = seq_blocks<BL>(a, s);
-    const int kvh = BL ? (int)blockIdx.y % a.p.n_kv : (int)blockIdx.y, blk = BL ? (int)blockIdx.y / a.p.n_kv : 0;
-    const int pr = blockIdx.x, r = BL ? blk * a.block_rows + pr : pr;   // the row, in its block and in all
+    const int kvh = BL ? (int)blockIdx.x % a.p.n_kv : (int)blockIdx.y, blk = BL ? (int)blockIdx.x / a.p.n_kv : 0;
+    const int pr = BL ? blockIdx.y : blockIdx.x, r = BL ? blk * a.block_rows + pr : pr;   // the row, in its block and in all
     if (r >= s.T * a.qg) return;
     const int p0 = before + (kvh * nb + blk) * tl.nt, p1 = p0 + tl.nt;
     const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);

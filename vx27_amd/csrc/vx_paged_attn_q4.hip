@@ -441,6 +441,6 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true>), dim3(1), dim3(1024), a);
     if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16>), dim3(grid), dim3(256), a);
     else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8>), dim3(grid), dim3(256), a);
-    VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<true>), dim3(a.part_rows, d->n_kv * nb, d->B), dim3(256), a, grid);
+    VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<true>), dim3(d->n_kv * nb, a.part_rows, d->B), dim3(256), a, grid);
     return 0;
 }
