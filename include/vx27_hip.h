@@ -480,14 +480,25 @@ int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
  * append writes to keep their values; two sequences may share only pages that
  * neither writes. */
 #define VX27_Q4_BLOCK_BYTES 4608
-#define VX27_Q4_SPLIT_ROWS 64
+#define VX27_Q4_SPLIT_ROWS 96
 #define VX27_Q4_SPLIT_ROWS_F32 512
 /* vx27_hip_paged_append into 4-bit pages.  k is normed and rotated in fp64
  * (the angle is the fp32 product of the other calls), so that rounding it to
  * codes does not depend on the order of sums; q as there. */
 int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
-/* vx27_hip_paged_attn over 4-bit pages; acc must be NULL.  Products are exact
- * bf16 codes on bf16 MFMA, scales and minima are applied in fp32. */
+/* vx27_hip_paged_attn over 4-bit pages; acc must be NULL.  Up to
+ * VX27_Q4_SPLIT_ROWS query rows a KV head (max_T * n_q/n_kv; fp32 outputs:
+ * VX27_Q4_SPLIT_ROWS_F32) run the decode kernels: codes and q are exact
+ * operands of bf16 MFMAs, s and m are applied in fp32, and the softmax weights
+ * are two bf16 parts (at most 2^-16 off).  More rows run the tile kernel: the
+ * rows' values, and the weights, are rounded to bf16 once.  A group held as NaN
+ * reaches only the tokens that see its row, whose outputs are then NaN (of a
+ * value row: the group's dims).
+ * Nothing overflows while the largest |s*15| + |m| of V times the number of
+ * rows seen stays below 2^127; of K, while a score's 256 products do.
+ * Context scratch: that of vx27_hip_paged_attn, and where more than 640 query
+ * rows read the same tiles, their values in bf16 (32 KiB for each 32 rows that a
+ * sequence can see and KV head, 256 MB at most). */
 int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d);
 
 /* The values of rows by slot (page*page_size + row of the page), as

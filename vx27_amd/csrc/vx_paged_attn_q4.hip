@@ -8,6 +8,13 @@
 // the scores of a group on their way out of the MFMAs and the weights on their
 // way in, and the minima's sums are MFMAs of their own (one for 16 keys' scores,
 // one for a tile's outputs).
+//
+// The split kernel on 4 x 131072 rows of 4 KV heads (604 MB): 106 us, 5.7 TB/s
+// of 7.2; a wave's 32 tiles take 2100 cycles of the VALU each (half of them the
+// codes' masks and conversions and the weights' parts), which keeps it busy for
+// about two thirds of the time at the two waves a SIMD that 235 registers allow.
+// Ragged windows of 32 sequences: 41 us for 141 MB, of which some 10 are the
+// first loads' chain (lengths, table, blocks) and the waves' merge.
 #include "vx_paged_q4.h"
 #include "vx_paged_rows.h"
 
@@ -153,23 +160,50 @@ __device__ __forceinline__ void score_tile(const KTile &t, const Rows<ROWS> &w, 
     for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3];
 }
 
-// Eight weights in bf16: rounded, or of 8 rows the parts of a lane's half.
-// With h the bf16 number that a weight x is cut off to, lanes of the first half
-// (rest 0) take -h and those of the second (rest 1) x - h, which leaves 2^-16 of
-// x at most once it is rounded; the difference of the columns is the sum.
-template <int ROWS>
-__device__ __forceinline__ bf16x8_t weights8(const float (&x)[8], float rest) {
-    float z[8];
+// Eight weights as two bf16 parts, h and x - h.  (One part is not enough for
+// bf16 outputs either: the codes' and the minima's sums are each some 2.5 times
+// a value and cancel, so that its rounding of 2^-9 became 0.005 of the output.)
+// Of 16 rows they are operands of two MFMAs; of 8 the two halves of the 16
+// columns, -h (rest 0) and x - h (rest 1), and the difference of the columns is
+// the sum.  h is x rounded, which leaves 2^-18 of x; CUT: cut off, which leaves
+// 2^-16 and is less work (the windows of 32 sequences 46.5 us against 48.5):
+// enough below an output in bf16.
+struct Weights {
+    bf16x8_t hi, lo;
+};
+template <int ROWS, bool CUT>
+__device__ __forceinline__ Weights weights8(const float (&x)[8], float rest) {
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = ROWS == 16 ? x[e] : __builtin_fmaf(x[e], rest, -__uint_as_float(__float_as_uint(x[e]) & 0xffff0000u));
-    return __builtin_bit_cast(bf16x8_t, make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7])));
+    for (int i = 0; i < 4; i++) {
+        float u = __uint_as_float(__float_as_uint(x[2 * i]) & 0xffff0000u), v = __uint_as_float(__float_as_uint(x[2 * i + 1]) & 0xffff0000u);
+        if (!CUT) {
+            h[i] = pack2(x[2 * i], x[2 * i + 1]);
+            u = __uint_as_float(h[i] << 16);
+            v = __uint_as_float(h[i] & 0xffff0000u);
+        }
+        if (ROWS == 16) l[i] = pack2(x[2 * i] - u, x[2 * i + 1] - v);
+        else h[i] = pack2(__builtin_fmaf(x[2 * i], rest, -u), __builtin_fmaf(x[2 * i + 1], rest, -v));
+    }
+    Weights w;
+    w.hi = __builtin_bit_cast(bf16x8_t, make_uint4(h[0], h[1], h[2], h[3]));
+    if (ROWS == 16) w.lo = __builtin_bit_cast(bf16x8_t, make_uint4(l[0], l[1], l[2], l[3]));
+    return w;
+}
+template <int ROWS>
+__device__ __forceinline__ floatx4_t weigh(bf16x8_t x, const Weights &w, floatx4_t o) {
+    o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w.hi, o, 0, 0, 0);
+    if (ROWS == 16) o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w.lo, o, 0, 0, 0);
+    return o;
 }
 
 // A row's reference lies 2^AHEAD above the maximum at which it last moved, and
-// moves once a score is past it: O is then hardly ever rescaled (68
-// instructions, in every second tile of a wave's 32 where it follows the
-// maximum).  Weights are at most 1; they keep fp32's exponents in bf16.
-constexpr int AHEAD = 8;
+// moves once a score is past it, so that O (68 instructions) is rescaled in fewer
+// tiles than every second, as where it follows the maximum.  Weights are at most 1.
+// (The further ahead, the more rows' heaviest weights are no powers of two, whose
+// parts are exact: with 2^8 the error of fp32 outputs over 131072 rows grows from
+// 4e-6 to 8e-6, for 1% of the time.)
+constexpr int AHEAD = 1;
 
 // x over the 16 lanes of a lane group, by OR or AND.
 template <bool AND>
@@ -185,7 +219,7 @@ __device__ __forceinline__ uint32_t over_rows(uint32_t x) {
 // Online softmax and P V of one tile.  `whole`: every row sees every key.  Else
 // s and m of keys that no row sees become zero, so that what stale rows hold
 // cannot get in.
-template <int ROWS>
+template <int ROWS, bool CUT>
 __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, bool whole, float (&x)[8], const vx_sight &v, int key0, VTile &t) {
     const int lane = lane_here(), g = lane >> 4;
     const float rest = ROWS == 8 && (lane & 8) ? 1.0f : 0.0f;
@@ -252,16 +286,16 @@ __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, bool whole, float (&x
             }
         }
     }
-    w.om = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.m, weights8<ROWS>(x, rest), w.om, 0, 0, 0);
+    w.om = weigh<ROWS>(t.m, weights8<ROWS, CUT>(x, rest), w.om);
 #pragma unroll
     for (int c = 0; c < GROUPS; c++) {
         float y[8];
         vx_q4_f32(t.s[c], y);
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] *= x[e];
-        const bf16x8_t pw = weights8<ROWS>(y, rest);
+        const Weights pw = weights8<ROWS, CUT>(y, rest);
 #pragma unroll
-        for (int i = 0; i < 4; i++) w.o[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx_q4_codes(word(t.c[c], i)), pw, w.o[4 * c + i], 0, 0, 0);
+        for (int i = 0; i < 4; i++) w.o[4 * c + i] = weigh<ROWS>(vx_q4_codes(word(t.c[c], i)), pw, w.o[4 * c + i]);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -276,7 +310,7 @@ __device__ __forceinline__ float both_halves(float x) {   // what lane ^ 8 has l
 // tiles in LDS (K's block, V's block), filled by direct loads that many tiles
 // ahead.
 constexpr int DEPTH = 2, RING = DEPTH * 2 * VX_Q4_BLOCK;
-template <int ROWS>
+template <int ROWS, bool CUT>
 __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -350,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             wait_blocks(more ? 3 : left ? 2 : 0);
             read_v(blk + VX_Q4_BLOCK, vt);
             const int key0 = tl.at(i0 + wave + 4 * j) * TILE;
-            attend_tile<ROWS>(w, whole_tile(key0), sc, v, key0, vt);
+            attend_tile<ROWS, CUT>(w, whole_tile(key0), sc, v, key0, vt);
             __asm__ volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
             if (more) load_block(a.v_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j) + VX_Q4_BLOCK);
         }
@@ -421,9 +455,15 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     const int todo = attn_fill(who, ctx, d, a);
     if (todo <= 0) return todo;
     const int rows = d->max_T * a.qg;
+    // The split kernel reads and decodes a tile for every 16 rows, the tile kernel
+    // once for 128.  Tokens of 6 heads, us by the split and by the tile kernel,
+    // 4 x 6000 | 1 x 30000 | 32 x 8000 rows: 8 tokens 41, 53 | 44, 95 | 187, 320;
+    // 16 tokens 55, 56 | 59, 99 | 349, 323; 24 tokens 73, 66 | 78, 93 | 524, 331.
+    // fp32 outputs stay with the split kernel, which rounds neither keys nor
+    // values and has two parts of the weights, to where a call is a prompt.
     if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32)) return rows_launch<true>(who, ctx, d, a, rows, 0);
-    // two parts of the weights where the output is fp32, one where it is rounded to bf16 itself
-    a.block_rows = a.out_bf16 ? 16 : 8;
+    // (decoding tokens of 6 heads: 8 rows a block)
+    a.block_rows = rows <= 8 ? 8 : 16;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;
     const int64_t units = (int64_t)d->B * d->n_kv * nb * a.tile_cap;
     VX_REQUIRE(units < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %d tiles each)", who, d->B, d->n_kv, a.tile_cap);
@@ -439,8 +479,9 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     a.part_ml = (float2 *)((char *)scr + o_bytes);
     a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes) : nullptr;
     if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true>), dim3(1), dim3(1024), a);
-    if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16>), dim3(grid), dim3(256), a);
-    else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8>), dim3(grid), dim3(256), a);
+    if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16, false>), dim3(grid), dim3(256), a);
+    else if (a.out_bf16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8, true>), dim3(grid), dim3(256), a);
+    else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8, false>), dim3(grid), dim3(256), a);
     VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<true>), dim3(d->n_kv * nb, a.part_rows, d->B), dim3(256), a, grid);
     return 0;
 }
