@@ -30,24 +30,42 @@ __device__ __forceinline__ int lane_here() {
     return lane;
 }
 // Block `block` of a pool into LDS, a wave's five loads (in flight: the caller
-// counts them).  The codes are read once: nontemporal.
+// counts them).  ONCE: codes that no other workgroup reads, nontemporal (4 x
+// 131072 rows 111 us against 122; tiles that three blocks of rows read 55 against
+// 53).
 constexpr int LOADS = 5;
+template <bool ONCE>
 __device__ __forceinline__ void load_block(const uint16_t *pool, uint32_t block, uint32_t lds) {
     const int lane = lane_here();
     const char *base = (const char *)pool + (size_t)block * VX_Q4_BLOCK;
     uint32_t saved;
-    __asm__ volatile(
-        "s_mov_b32 %0, m0\n\t"
-        "s_mov_b32 m0, %3\n\t"
-        "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %2 nt\n\t"
-        "global_load_lds_dwordx4 %1, %2 offset:1024 nt\n\t"
-        "global_load_lds_dwordx4 %1, %2 offset:2048 nt\n\t"
-        "global_load_lds_dwordx4 %1, %2 offset:3072 nt\n\t"
-        "s_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(lane * 16), "s"(base), "s"(lds)
-        : "memory");
+    if (ONCE) {
+        __asm__ volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %3\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %1, %2 nt\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:1024 nt\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:2048 nt\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:3072 nt\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "v"(lane * 16), "s"(base), "s"(lds)
+            : "memory");
+    } else {
+        __asm__ volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %3\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %1, %2\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:2048\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:3072\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "v"(lane * 16), "s"(base), "s"(lds)
+            : "memory");
+    }
     if (lane < 32) vx_dma16(base + VX_Q4_S, lane * 16, lds + VX_Q4_S);
 }
 // Waits until at most `blocks` of this wave's blocks are in flight.
@@ -354,8 +372,8 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
 #pragma unroll
             for (int j = 0; j < DEPTH; j++) {
                 if (j >= mine) break;
-                load_block(a.k_pages, __builtin_amdgcn_readlane(blocks, j), ring_lds + slot_of(j));
-                load_block(a.v_pages, __builtin_amdgcn_readlane(blocks, j), ring_lds + slot_of(j) + VX_Q4_BLOCK);
+                load_block<ROWS == 8>(a.k_pages, __builtin_amdgcn_readlane(blocks, j), ring_lds + slot_of(j));
+                load_block<ROWS == 8>(a.v_pages, __builtin_amdgcn_readlane(blocks, j), ring_lds + slot_of(j) + VX_Q4_BLOCK);
             }
         }
         Rows<ROWS> w;
@@ -378,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             __asm__ volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
             if (more) {
                 if (((j + DEPTH) & 63) == 0) look_up(j + DEPTH);
-                load_block(a.k_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j));
+                load_block<ROWS == 8>(a.k_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j));
             }
             VTile vt;
             wait_blocks(more ? 3 : left ? 2 : 0);
@@ -386,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             const int key0 = tl.at(i0 + wave + 4 * j) * TILE;
             attend_tile<ROWS, CUT>(w, whole_tile(key0), sc, v, key0, vt);
             __asm__ volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-            if (more) load_block(a.v_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j) + VX_Q4_BLOCK);
+            if (more) load_block<ROWS == 8>(a.v_pages, __builtin_amdgcn_readlane(blocks, (j + DEPTH) & 63), ring_lds + slot_of(j) + VX_Q4_BLOCK);
         }
         const int ln = lane_here(), g = ln >> 4, n = ln & 15;
         w.l += __shfl_xor(w.l, 16, 64);
