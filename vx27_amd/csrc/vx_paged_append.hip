@@ -1,6 +1,6 @@
 // Append to a paged KV cache on gfx950: the new tokens' q and k are normed
-// and rotated, k and v rounded to bf16 into their pages, q to bf16 for the
-// attention.
+// and rotated, k and v rounded to bf16 or to 4 bits into their pages, q to bf16
+// for the attention.
 //
 // Per head (vx27_qfwd.c:172-186): s = 1/sqrt(mean(x^2) + 1e-6), y = x s (1+w)
 // (or x s w), the first rope_dim dims rotated as NeoX halves by the angle
@@ -183,9 +183,12 @@ __device__ __forceinline__ double inv_sqrt(double x) {
     return r;
 }
 
-// One KV head's new rows [lo, hi) of the block at row p0 of sequence b: a row a
-// wave, its codes into LDS by bytes; then thread u stores 16-byte unit u of the
-// block, or of V, where 8 rows share one, as much of it as is new.
+// One KV head's new keys or values, rows [lo, hi) of the block at row p0 of
+// sequence b: a row a wave, its codes into LDS by bytes; then thread u stores
+// 16-byte unit u of the block, or of V, where 8 rows share one, as much of it as
+// is new.  8192 tokens of 24 + 4 heads take 65 us, 27 of these for keys and
+// values alone (41 with both in one workgroup, its waves' rows one after the
+// other, and quotients in fp64).
 constexpr int CODE_ROW = HDG + 4;             // (rows 8 apart then lie in different banks)
 constexpr int Q4_CS = 512;                    // (cos, sin) of a chunk of rows
 constexpr int Q4_LDS = VB * CODE_ROW + Q4_CS * 16 + 4 * HDG * 8;
@@ -298,9 +301,10 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
     }
 }
 
-// grid (5 a 32-row block that a sequence's tokens can touch, n_kv, B), block
-// 256.  Of a block's five workgroups the first takes one KV head's keys and V
-// block, the others the group's query heads of 8 tokens each: a prompt's
+// grid (5, or Q4 6, a 32-row block that a sequence's tokens can touch, n_kv, B),
+// block 256.  Of a block's workgroups the first takes one KV head's keys and V
+// block (Q4: two, the keys and the V block), the others the group's query heads
+// of 8 tokens each: a prompt's
 // workgroups are then short and many (one workgroup a block took 88 us for
 // 4364 tokens of 24 + 4 heads, its waves waiting for one another's loads).
 // V first, then the tokens' cos and sin in its place in LDS (side by side they
@@ -462,7 +466,7 @@ int append(const char *who, vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) 
     // (a row's token by a high product: exact where 8 tokens' rows times the group stay below 2^32)
     VX_REQUIRE(!d->q || (d->n_q >= d->n_kv && d->n_q % d->n_kv == 0 && d->n_q / d->n_kv <= 4096),
                "%s: need n_q = k*n_kv with k <= 4096 (n_q=%d n_kv=%d)", who, d->n_q, d->n_kv);
-    // (five workgroups of 256 a 32-row block: a launch holds 2^32 threads a dimension)
+    // (five or six workgroups of 256 a 32-row block: a launch holds 2^32 threads a dimension)
     VX_REQUIRE(d->max_T <= (1 << 26), "%s: max_T is past 2^26 (got %d)", who, d->max_T);
     VX_REQUIRE(d->k_new && d->v_new && d->k_norm_w && d->k_pages && d->v_pages && (!d->q || (d->q_norm_w && d->q_out)),
                "%s: null pointer in descriptor", who);

@@ -6,7 +6,9 @@
 // that remain the pages and tokens before each.  Everything else follows from
 // these: token i's sequence is the last with at most i tokens before it, the
 // k-th page taken is entry total - 1 - k of the free pages with the released
-// ones on top.
+// ones on top.  Latencies bound it: 13 sequences 4.5 us, a launch and two
+// dependent loads (8.7 with a scan each by shuffles, and lengths read again in
+// each pass); 2000 sequences with 330000 tokens 20.7, 11 of them the sums.
 #include <algorithm>
 
 #include "vx_paged_q4.h"
