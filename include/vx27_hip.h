@@ -466,10 +466,10 @@ int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
  *   m = the largest bf16 number not above the group's values
  *   s = the smallest bf16 number not below (the largest value - m) / 15
  *   c = the integer nearest to (x - m) / s, ties to even (0 where s = 0)
- * so a value is off by at most s/2.  A group that holds an infinity, a NaN or
- * a value past the largest bf16 number is held as NaN.  Bytes of a block, from
- * the slowest index (codes 0-3 of an 8 in the low halves of 4 bytes, 4-7 in
- * the high ones):
+ * so a value is off by at most s/2 (a value of 2^127 and more may come back as
+ * an infinity).  A group that holds an infinity, a NaN or a value past the
+ * largest bf16 number is held as NaN.  Bytes of a block, from the slowest index
+ * (codes 0-3 of an 8 in the low halves of 4 bytes, 4-7 in the high ones):
  *   K     0: c [row/4%2][dim/128][dim/8%4][row/8][row%4][dim/32%4][dim%4]; high halves: dims 4-7 of 8
  *      4096: s [dim/64][row]    4352: m [row][dim/64]
  *   V     0: c [dim/64][row/8][dim%16][dim/16%4][row%4]; high halves: rows 4-7 of 8
@@ -484,7 +484,7 @@ int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
 #define VX27_Q4_SPLIT_ROWS_F32 512
 /* vx27_hip_paged_append into 4-bit pages.  k is normed and rotated in fp64
  * (the angle is the fp32 product of the other calls), so that rounding it to
- * codes does not depend on the order of sums; q as there. */
+ * codes does not depend on the order of sums; q as there.  max_T at most 2^25. */
 int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
 /* vx27_hip_paged_attn over 4-bit pages; acc must be NULL.  Up to
  * VX27_Q4_SPLIT_ROWS query rows a KV head (max_T * n_q/n_kv; fp32 outputs:
@@ -505,7 +505,7 @@ int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_desc *d);
  * vx27_hip_paged_plan leaves them: k_out and v_out [n_rows][n_kv][hd] (either
  * may be NULL), fp32 or rounded to bf16.  A slot of -1 leaves its output as it
  * was; any other slot outside the pool as well, and vx27_hip_sync reports it.
- * Pages and outputs 16-byte aligned. */
+ * Pages and outputs 16-byte aligned; outputs must not overlap an input. */
 typedef struct {
     int n_kv, hd;
     int page_size, n_pages;

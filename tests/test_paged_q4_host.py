@@ -32,7 +32,7 @@ MAKE = {"append_q4": _append, "attn_q4": _attn, "read_q4": _read, "plan": _plan}
 BIG = {"page_size": 1 << 20, "n_pages": 1 << 19, "max_pages": 1, "n_kv": 1, "n_q": 6}      # 2^34 blocks
 CASES = [(k, *c) for k in ("append_q4", "attn_q4") for c in COMMON + TOKENS] + [
     ("append_q4", {"rope_dim": 7}, "rope_dim"), ("append_q4", {"in_dtype": 2}, "in_dtype"), ("append_q4", {"k_new": None}, "null pointer"),
-    ("append_q4", {"q_head_stride": 258}, "multiples of 4"), ("append_q4", BIG, "2^32 blocks"),
+    ("append_q4", {"n_tok": 2 ** 31 - 1, "max_T": 2 ** 25 + 1}, "2^25"), ("append_q4", {"q_head_stride": 258}, "multiples of 4"), ("append_q4", BIG, "2^32 blocks"),
     ("attn_q4", {"n_q": 68}, "k <= 16"), ("attn_q4", {"window": -1}, "negative"), ("attn_q4", {"out_dtype": 3}, "out_dtype"),
     ("attn_q4", {"gate": P + 8}, "aligned"), ("attn_q4", {"acc": P, "acc_stride": 256}, "acc must be NULL"), ("attn_q4", BIG, "2^32 blocks"),
     ("read_q4", {"hd": 128}, "hd must be 256"), ("read_q4", {"n_kv": 0}, "n_kv"), ("read_q4", {"n_kv": 1025}, "n_kv"),
@@ -133,3 +133,8 @@ def test_quantise_is_the_definition():
                 assert int(c[64 * g + i]) == round(t)       # (Fraction rounds ties to even)
         assert np.all(np.abs(values(c, s, m) - x).reshape(4, 64) <= f64(s)[:, None] / 2 * (1 + 2.0 ** -40))
     assert f64(bf16_bits_toward(np.array([1.001, -1.001, 0.0]), True)).tolist() == [1.0078125, -1.0, 0.0]
+
+
+def test_launch_of_a_limit():
+    """The append's grid at its largest max_T: below 2^32 threads, 256 a workgroup, 12 of them a 32-row block."""
+    assert ((2 ** 25 + 30) // 32 + 1) * 12 * 256 < 2 ** 32

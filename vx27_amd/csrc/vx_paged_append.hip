@@ -186,26 +186,29 @@ __device__ __forceinline__ double inv_sqrt(double x) {
 // One KV head's new keys or values, rows [lo, hi) of the block at row p0 of
 // sequence b: a row a wave, its codes into LDS by bytes; then thread u stores
 // 16-byte unit u of the block, or of V, where 8 rows share one, as much of it as
-// is new.  8192 tokens of 24 + 4 heads take 65 us, 27 of these for keys and
-// values alone (41 with both in one workgroup, its waves' rows one after the
-// other, and quotients in fp64).
+// is new.  8192 tokens of 24 + 4 heads take 59 us (the copy rate's 47), keys and
+// values alone 25; with a block's 32 rows in one workgroup, whose waves' rows
+// follow one another, 65, and 4 us more for 64 tokens.
+constexpr int Q4_ROWS = 8;                    // rows of a workgroup: those that share V's units
 constexpr int CODE_ROW = HDG + 4;             // (rows 8 apart then lie in different banks)
-constexpr int Q4_CS = 512;                    // (cos, sin) of a chunk of rows
-constexpr int Q4_LDS = VB * CODE_ROW + Q4_CS * 16 + 4 * HDG * 8;
-template <bool V>
-__device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int lo, int hi, int tok0, char *lds) {
+template <bool Q4>
+constexpr int KV_GROUPS = Q4 ? 2 * VB / Q4_ROWS : 1;
+template <int HALFS>                          // codes, the rows' (cos, sin), a row a wave
+constexpr int Q4_LDS = Q4_ROWS * CODE_ROW + Q4_ROWS * HALFS * 16 + 4 * HDG * 8;
+template <bool V, int HALFS>
+__device__ void append_q4_rows(const AppendArgs &a, int hk, int b, int p0, int q0, int lo, int hi, int tok0, char *lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = hi - lo, half = a.rope_dim / 2;
     const int page = vx_paged_page(a.p, b, p0), at = p0 - vx_page_slot(a.p, p0) * a.p.page_size;
     const size_t block = (size_t)vx_q4_block(a.p, page, hk, at) * VX_Q4_BLOCK;
     char *codes = lds;
-    double2 *cs = (double2 *)(lds + VB * CODE_ROW);
-    double *row = (double *)(lds + VB * CODE_ROW + Q4_CS * 16) + wave * HDG;
+    double2 *cs = (double2 *)(lds + Q4_ROWS * CODE_ROW);
+    double *row = (double *)(lds + Q4_ROWS * CODE_ROW + Q4_ROWS * HALFS * 16) + wave * HDG;
     char *blk = (char *)(V ? a.v_pages : a.k_pages) + block;
     auto store = [&](int j, const auto &y) {
         const int r = lo - p0 + j;
         uint32_t s, m;
-        *(uint32_t *)(codes + r * CODE_ROW + 4 * lane) = quantise(y, s, m);
+        *(uint32_t *)(codes + r % Q4_ROWS * CODE_ROW + 4 * lane) = quantise(y, s, m);
         if ((lane & 15) == 0) {
             const int c = lane >> 4;
             *(uint16_t *)(blk + VX_Q4_S + c * 64 + r * 2) = (uint16_t)(s >> 16);
@@ -224,19 +227,19 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
             store(j, y);
         }
         __syncthreads();
-        const int dim = 64 * (tid >> 6) + (tid & 15), r8 = 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 16 i, rows r8 .. r8 + 7
-        uint32_t fresh = 0;                                                        // its new rows
-        for (int k = 0; k < 8; k++) fresh |= p0 + r8 + k >= lo && p0 + r8 + k < hi ? 1u << k : 0u;
-        if (fresh) {
-            uint4 *dst = (uint4 *)(blk + tid * 16);
+        if (tid < 64) {      // unit (j, rows' eighth, n): dims 64 j + n + 16 i
+            const int dim = 64 * (tid >> 4) + (tid & 15);
+            uint32_t fresh = 0;                                  // the new rows of the eight
+            for (int k = 0; k < Q4_ROWS; k++) fresh |= q0 + k >= lo && q0 + k < hi ? 1u << k : 0u;
+            uint4 *dst = (uint4 *)(blk + (64 * (tid >> 4) + 2 * (q0 - p0) + (tid & 15)) * 16);
             uint32_t u[4] = {0, 0, 0, 0}, mask = 0;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
+            for (int k = 0; k < Q4_ROWS; k++) {
                 if (!((fresh >> k) & 1)) continue;
                 const int at_bit = 8 * (k & 3) + (k & 4);
                 mask |= 15u << at_bit;
 #pragma unroll
-                for (int i = 0; i < 4; i++) u[i] |= (uint32_t)codes[(r8 + k) * CODE_ROW + dim + 16 * i] << at_bit;
+                for (int i = 0; i < 4; i++) u[i] |= (uint32_t)codes[k * CODE_ROW + dim + 16 * i] << at_bit;
             }
             if (fresh != 255) {
                 const uint4 old = *dst;
@@ -249,62 +252,58 @@ __device__ void append_q4_block(const AppendArgs &a, int hk, int b, int p0, int 
     const float4 wf = ((const float4 *)a.k_norm_w)[lane];
     const double one = (a.flags & VX27_GQA_NORM_W) ? 0.0 : 1.0;
     const double w[4] = {wf.x + one, wf.y + one, wf.z + one, wf.w + one};
-    const int chunk = half ? min(Q4_CS / half & ~3, VB) : VB;   // (4 rows at least: half is 128 at most)
-    for (int j0 = 0; j0 < n; j0 += chunk) {
-        const int j1 = min(j0 + chunk, n);
-        for (int e = tid; e < (j1 - j0) * half; e += 256) {
-            const int j = j0 + e / half, i = e % half;
-            double sn, c;
-            sincos((double)vx_rope_angle(a.rope.freq[i], a.pos ? a.pos[tok0 + j] : lo + j, a.yarn), &sn, &c);
-            cs[e] = make_double2(c, sn);
-        }
-        __syncthreads();
-        // (a chunk is a multiple of 4 rows, or all: a wave's rows go on from one to the next)
-#pragma unroll 1
-        for (int j = j0 + wave; j < j1; j += 4) {
-            double y[4] = {x.x, x.y, x.z, x.w};
-            x = load_row(j + 4);
-            double ss = y[0] * y[0];
-#pragma unroll
-            for (int e = 1; e < 4; e++) ss = __builtin_fma(y[e], y[e], ss);
-            const double sc = inv_sqrt(vx_wave_sum_f64_dpp(ss) * (1.0 / HDG) + 1e-6);
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = y[e] * sc * w[e];
-            if (half) {
-                *(double2 *)(row + 4 * lane) = make_double2(y[0], y[1]);
-                *(double2 *)(row + 4 * lane + 2) = make_double2(y[2], y[3]);
-                __builtin_amdgcn_wave_barrier();   // (one wave's LDS operations complete in order)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = 4 * lane + e;
-                    if (i >= 2 * half) continue;
-                    const bool second = i >= half;
-                    const double2 c = cs[(j - j0) * half + (second ? i - half : i)];
-                    const double z = row[second ? i - half : i + half] * c.y;
-                    y[e] = y[e] * c.x + (second ? z : -z);
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-            store(j, y);
-        }
-        __syncthreads();
+    for (int e = tid; e < n * half; e += 256) {
+        const int j = e / half, i = e % half;
+        double sn, c;
+        sincos((double)vx_rope_angle(a.rope.freq[i], a.pos ? a.pos[tok0 + j] : lo + j, a.yarn), &sn, &c);
+        cs[e] = make_double2(c, sn);
     }
-    const int r = vx_q4_k_row(tid), dim = 128 * ((tid >> 6) & 1) + 8 * ((tid >> 4) & 3);   // unit tid: dims dim + 32 i .. + 7 of row r
-    if (p0 + r >= lo && p0 + r < hi) {
+    __syncthreads();
+#pragma unroll 1
+    for (int j = wave; j < n; j += 4) {
+        double y[4] = {x.x, x.y, x.z, x.w};
+        x = load_row(j + 4);
+        double ss = y[0] * y[0];
+#pragma unroll
+        for (int e = 1; e < 4; e++) ss = __builtin_fma(y[e], y[e], ss);
+        const double sc = inv_sqrt(vx_wave_sum_f64_dpp(ss) * (1.0 / HDG) + 1e-6);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = y[e] * sc * w[e];
+        if (half) {
+            *(double2 *)(row + 4 * lane) = make_double2(y[0], y[1]);
+            *(double2 *)(row + 4 * lane + 2) = make_double2(y[2], y[3]);
+            __builtin_amdgcn_wave_barrier();   // (one wave's LDS operations complete in order)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = 4 * lane + e;
+                if (i >= 2 * half) continue;
+                const bool second = i >= half;
+                const double2 c = cs[j * half + (second ? i - half : i)];
+                const double z = row[second ? i - half : i + half] * c.y;
+                y[e] = y[e] * c.x + (second ? z : -z);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        store(j, y);
+    }
+    __syncthreads();
+    // unit (row, k, g): dims 128 k + 8 g + 32 i .. + 7
+    const int r = tid >> 3, dim = 128 * ((tid >> 2) & 1) + 8 * (tid & 3);
+    if (tid < 8 * Q4_ROWS && q0 + r >= lo && q0 + r < hi) {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t *c = (const uint32_t *)(codes + r * CODE_ROW + dim + 32 * i);
             u[i] = c[0] | (c[1] << 4);
         }
-        *(uint4 *)(blk + tid * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+        *(uint4 *)(blk + vx_q4_k_unit(q0 - p0 + r, dim) * 16) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
-// grid (5, or Q4 6, a 32-row block that a sequence's tokens can touch, n_kv, B),
+// grid (5, or Q4 12, a 32-row block that a sequence's tokens can touch, n_kv, B),
 // block 256.  Of a block's workgroups the first takes one KV head's keys and V
-// block (Q4: two, the keys and the V block), the others the group's query heads
-// of 8 tokens each: a prompt's
+// block (Q4: eight, of eight rows' keys or values each), the others the group's
+// query heads of 8 tokens each: a prompt's
 // workgroups are then short and many (one workgroup a block took 88 us for
 // 4364 tokens of 24 + 4 heads, its waves waiting for one another's loads).
 // V first, then the tokens' cos and sin in its place in LDS (side by side they
@@ -322,13 +321,13 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     constexpr int NR = 4;
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    constexpr int KV = Q4 ? 2 : 1;                        // workgroups of a block's keys and values
+    constexpr int KV = KV_GROUPS<Q4>;                     // workgroups of a block's keys and values
     const int blk = blockIdx.x / (KV + VB / QTOK), part = blockIdx.x % (KV + VB / QTOK);
     const bool is_k = part < KV;
     if (!is_k && !a.q) return;
     // v's rows; then the tokens' cos and sin, and a row a wave
     constexpr int CS = VB * HALFS * 4;
-    constexpr int ROTATE = 2 * CS + 4 * HDG * 4, OTHER = Q4 ? Q4_LDS : VB * HDG * 2;
+    constexpr int ROTATE = 2 * CS + 4 * HDG * 4, OTHER = Q4 ? Q4_LDS<HALFS> : VB * HDG * 2;
     __shared__ __attribute__((aligned(16))) char lds[ROTATE > OTHER ? ROTATE : OTHER];
     float (*cs)[HALFS] = (float (*)[HALFS])lds, (*sn)[HALFS] = (float (*)[HALFS])(lds + CS);
     uint16_t (*vt)[HDG] = (uint16_t (*)[HDG])lds;
@@ -336,13 +335,16 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     if (s.row0 < 0 && tid == 0 && hk == 0 && blockIdx.x == 0) *a.p.err_flag = 1;
     const int first = max(s.row0, 0);
     const int p0 = (first / VB + blk) * VB;               // first row of the block
-    const int q0 = is_k ? p0 : p0 + QTOK * (part - KV);    // this workgroup's rows [lo, hi)
-    const int lo = max(q0, first), hi = min(q0 + (is_k ? VB : QTOK), s.len);
+    const int q0 = !is_k ? p0 + QTOK * (part - KV) : Q4 ? p0 + Q4_ROWS * (part >> 1) : p0;    // this workgroup's rows [lo, hi)
+    const int lo = max(q0, first), hi = min(q0 + (is_k ? Q4 ? Q4_ROWS : VB : QTOK), s.len);
     if (lo >= hi) return;
     const int n = hi - lo, tok0 = s.start + (lo - s.row0), half = a.rope_dim / 2;
     if constexpr (Q4) {
-        if (part == 0) return append_q4_block<false>(a, hk, b, p0, lo, hi, tok0, lds);
-        if (part == 1) return append_q4_block<true>(a, hk, b, p0, lo, hi, tok0, lds);
+        if (is_k) {
+            if (part & 1) append_q4_rows<true, HALFS>(a, hk, b, p0, q0, lo, hi, tok0, lds);
+            else append_q4_rows<false, HALFS>(a, hk, b, p0, q0, lo, hi, tok0, lds);
+            return;
+        }
     }
     const int per = is_k ? 1 : a.qg, rows = n * per;      // heads of a token
     const uint32_t magic = is_k ? 0 : a.qg_magic;
@@ -466,8 +468,8 @@ int append(const char *who, vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) 
     // (a row's token by a high product: exact where 8 tokens' rows times the group stay below 2^32)
     VX_REQUIRE(!d->q || (d->n_q >= d->n_kv && d->n_q % d->n_kv == 0 && d->n_q / d->n_kv <= 4096),
                "%s: need n_q = k*n_kv with k <= 4096 (n_q=%d n_kv=%d)", who, d->n_q, d->n_kv);
-    // (five or six workgroups of 256 a 32-row block: a launch holds 2^32 threads a dimension)
-    VX_REQUIRE(d->max_T <= (1 << 26), "%s: max_T is past 2^26 (got %d)", who, d->max_T);
+    // (5 workgroups of 256 a 32-row block, or Q4 12: a launch holds 2^32 threads a dimension)
+    VX_REQUIRE(d->max_T <= (1 << (Q4 ? 25 : 26)), "%s: max_T is past 2^%d (got %d)", who, Q4 ? 25 : 26, d->max_T);
     VX_REQUIRE(d->k_new && d->v_new && d->k_norm_w && d->k_pages && d->v_pages && (!d->q || (d->q_norm_w && d->q_out)),
                "%s: null pointer in descriptor", who);
     if (d->rope_dim != 0) {
@@ -493,7 +495,7 @@ int append(const char *who, vx27_hip_ctx *ctx, const vx27_paged_append_desc *d) 
     a.pos = d->pos; a.q = d->q; a.k = d->k_new; a.v = d->v_new;
     a.q_norm_w = d->q_norm_w; a.k_norm_w = d->k_norm_w;
     a.q_out = d->q_out; a.k_pages = d->k_pages; a.v_pages = d->v_pages;
-    const dim3 grid(((d->max_T + VB - 2) / VB + 1) * ((Q4 ? 2 : 1) + VB / QTOK), d->n_kv, d->B);
+    const dim3 grid(((d->max_T + VB - 2) / VB + 1) * (KV_GROUPS<Q4> + VB / QTOK), d->n_kv, d->B);
     // (32 angles a token take 16 KiB of LDS, 128 take 36: the 143 MB prompt takes 49 us with the first, 62 with the second)
     if (d->rope_dim <= 64) VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<32, Q4>), grid, dim3(256), a);
     else VX_LAUNCH_NAMED(ctx, Q4 ? "paged_append_q4" : "paged_append", (paged_append<MAXR, Q4>), grid, dim3(256), a);

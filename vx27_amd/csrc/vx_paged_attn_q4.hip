@@ -47,10 +47,10 @@ __device__ __forceinline__ void load_block(const uint16_t *pool, uint32_t block,
             "global_load_lds_dwordx4 %1, %2 nt\n\t"
             "global_load_lds_dwordx4 %1, %2 offset:1024 nt\n\t"
             "global_load_lds_dwordx4 %1, %2 offset:2048 nt\n\t"
-            "global_load_lds_dwordx4 %1, %2 offset:3072 nt\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:%4 nt\n\t"
             "s_mov_b32 m0, %0"
             : "=&s"(saved)
-            : "v"(lane * 16), "s"(base), "s"(lds)
+            : "v"(lane * 16), "s"(base), "s"(lds), "n"(3 * 1024)
             : "memory");
     } else {
         __asm__ volatile(
@@ -60,10 +60,10 @@ __device__ __forceinline__ void load_block(const uint16_t *pool, uint32_t block,
             "global_load_lds_dwordx4 %1, %2\n\t"
             "global_load_lds_dwordx4 %1, %2 offset:1024\n\t"
             "global_load_lds_dwordx4 %1, %2 offset:2048\n\t"
-            "global_load_lds_dwordx4 %1, %2 offset:3072\n\t"
+            "global_load_lds_dwordx4 %1, %2 offset:%4\n\t"
             "s_mov_b32 m0, %0"
             : "=&s"(saved)
-            : "v"(lane * 16), "s"(base), "s"(lds)
+            : "v"(lane * 16), "s"(base), "s"(lds), "n"(3 * 1024)
             : "memory");
     }
     if (lane < 32) vx_dma16(base + VX_Q4_S, lane * 16, lds + VX_Q4_S);
