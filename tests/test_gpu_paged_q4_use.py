@@ -658,3 +658,25 @@ def test_faulty_slots_are_reported(ctx, bad):  # noqa: F811
         assert np.array_equal(got[ok], want[ok]) and np.all(got[~ok] == -7.5)
     for x in buf.values():
         x.free()
+
+
+@pytest.mark.parametrize("B,few,ended", [(1500, 0.97, True), (4096, 0.99, True), (5000, 0.5, False), (65535, 0.9, True), (1025, 0.0, True)])
+def test_plans_of_many_sequences(ctx, B, few, ended):  # noqa: F811
+    """Long runs of sequences without tokens or pages between those that have some; more tokens than one launch takes."""
+    from test_gpu_paged_plan import Plan
+    say(f"plan of {B} sequences, {few} of them idle")
+    r = np.random.default_rng([1960, B])
+    page = 32
+    idle = r.random(B) < few
+    lens = np.where(r.random(B) < 0.3, 0, r.integers(0, 100, B))
+    new = np.where(idle, 0, r.integers(0, 90, B))
+    e = (r.random(B) < 0.3).astype(int) if ended else None
+    need = int((-(-(lens + new) // page) - -(-lens // page)).sum())
+    table, free, n_free = pool(r, lens, page, need // 2, 7)
+    n_tok = int(new.sum()) + 5000
+    want = plan(lens, new, table, free, n_free, page, n_tok, e, lens + 3)
+    p = Plan(ctx, lens, new, table, free, n_free, page, n_tok, e, lens + 3)
+    p.call()
+    ctx.sync()
+    p.check(want)
+    p.free()

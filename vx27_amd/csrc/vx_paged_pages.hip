@@ -8,7 +8,9 @@
 // k-th page taken is entry total - 1 - k of the free pages with the released
 // ones on top.  Latencies bound it: 13 sequences 4.5 us, a launch and two
 // dependent loads (8.7 with a scan each by shuffles, and lengths read again in
-// each pass); 2000 sequences with 330000 tokens 20.7, 11 of them the sums.
+// each pass); 2000 sequences with 330000 tokens 18.4 (20.8 with a search a lane).
+#include <limits.h>
+
 #include <algorithm>
 
 #include "vx_paged_q4.h"
@@ -49,45 +51,88 @@ __device__ __forceinline__ int checked_page(const PlanArgs &a, int pg) {
     if (c != pg) *a.err_flag = 1;
     return c;
 }
-// Entry i of the free pages with the released ones on top.
-__device__ __forceinline__ int stack_page(const PlanArgs &a, const PlanSums &p, int i) {
-    if (i < p.was_free) return checked_page(a, a.free_pages[i]);
-    const int j = i - p.was_free, b = last_le(p.back, a.B, j);
-    return checked_page(a, a.table[(size_t)b * a.max_pages + (j - p.back[b])]);
-}
-// Item i of a plan's second half: a token's slot, position and sequence, a
-// page taken, or a released page that stays free.
-template <typename FROM>   // from(b, row0, pos0): row and position of the first token that sequence b got
-__device__ __forceinline__ void plan_item(const PlanArgs &a, const PlanSums &p, int64_t i, int tokens, int total, FROM from) {
-    const int top = p.was_free + p.released - 1;
-    if (i < a.n_tok) {
-        const int t = (int)i;
-        int slot = -1, pos = -1, b = -1;
-        if (t < tokens) {
-            b = last_le(p.start, a.B, t);
-            int row0, pos0;
-            from(b, row0, pos0);
-            const int start = p.start[b], row = row0 + t - start;
-            const int pg = a.log2_page >= 0 ? row >> a.log2_page : row / a.page_size, held = plan_ceil(a, row0);
-            const int page = pg < held ? checked_page(a, a.table[(size_t)b * a.max_pages + pg]) : stack_page(a, p, top - (p.grown[b] + pg - held));
-            slot = page * a.page_size + (row - pg * a.page_size);
-            pos = (int)((uint32_t)pos0 + (uint32_t)(t - start));
+// last_le for every lane of a wave (n entries), whose x do not fall (DOWN: do not
+// rise) from lane to lane.
+struct LaneFind {            // each by itself: arrays in LDS
+    int n;
+    template <bool DOWN>
+    __device__ __forceinline__ int find(const int *at, int x, bool need) const { return need ? last_le(at, n, x) : 0; }
+};
+struct WaveFind {            // the least x by all lanes, then on from there
+    int n;
+    template <bool DOWN>
+    __device__ __forceinline__ int find(const int *at, int x, bool need) const {
+        const uint64_t who = __ballot(need);
+        if (!who) return 0;
+        const int lane = threadIdx.x & 63, head = __builtin_ctzll(who), tail = 63 - __builtin_clzll(who);
+        const int least = __builtin_amdgcn_readlane(x, DOWN ? tail : head), most = __builtin_amdgcn_readlane(x, DOWN ? head : tail);
+        int lo = 0;
+        for (int m = n; m > 1;) {
+            const int step = (m + 63) / 64, k = 63 - __builtin_clzll(__ballot(lane == 0 || (lane * step < m && at[lo + min(lane * step, m - 1)] <= least)));
+            lo += k * step;
+            m = min(step, m - k * step);
         }
-        if (a.slot) a.slot[t] = slot;
-        if (a.pos) a.pos[t] = pos;
-        if (a.seq) a.seq[t] = b;
-        return;
+        const int next = lo + 1 + lane < n ? at[lo + 1 + lane] : INT_MAX;
+        int b = lo;
+        for (int k = 0; k < 64; k++) {
+            const int v = __builtin_amdgcn_readlane(next, k);
+            if (v > most) return b;
+            b += x >= v;
+        }
+        return need ? lo + last_le(at + lo, n - lo, x) : 0;   // (more than 64 of them among the lanes' x)
     }
-    i -= a.n_tok;
-    if (i < p.taken) {
-        const int k = (int)i, b = last_le(p.grown, a.B, k);
+};
+// Entry i of the free pages with the released ones on top.
+template <bool DOWN, typename FIND>
+__device__ __forceinline__ int stack_page(const PlanArgs &a, const PlanSums &p, const FIND &f, int i, bool need) {
+    const bool back = need && i >= p.was_free;
+    const int j = i - p.was_free, b = f.template find<DOWN>(p.back, j, back);
+    if (!need) return 0;
+    return checked_page(a, back ? a.table[(size_t)b * a.max_pages + (j - p.back[b])] : a.free_pages[i]);
+}
+// A plan's second half, for all lanes of a wave: token t's slot, position and
+// sequence.  from(b, row0, pos0): row and position of the first token that
+// sequence b got.
+template <typename FIND, typename FROM>
+__device__ __forceinline__ void plan_token(const PlanArgs &a, const PlanSums &p, const FIND &f, FROM from, int t, int tokens) {
+    const bool live = t < tokens;
+    const int b = f.template find<false>(p.start, t, live);
+    int row = 0, pg = 0, pos = -1, taken = 0;
+    bool fresh = false;
+    if (live) {
         int row0, pos0;
         from(b, row0, pos0);
-        a.table[(size_t)b * a.max_pages + plan_ceil(a, row0) + k - p.grown[b]] = stack_page(a, p, top - k);
-        return;
+        const int k = t - p.start[b];
+        row = row0 + k;
+        pos = (int)((uint32_t)pos0 + (uint32_t)k);
+        pg = a.log2_page >= 0 ? row >> a.log2_page : row / a.page_size;
+        const int held = plan_ceil(a, row0);
+        fresh = pg >= held;
+        taken = p.grown[b] + pg - held;
     }
-    const int at = p.was_free + (int)(i - p.taken);   // released and not taken
-    if (at < total - p.taken) a.free_pages[at] = stack_page(a, p, at);
+    const int mine = stack_page<true>(a, p, f, p.was_free + p.released - 1 - taken, fresh);
+    const int page = fresh ? mine : live ? checked_page(a, a.table[(size_t)b * a.max_pages + pg]) : 0;
+    if (t >= a.n_tok) return;
+    if (a.slot) a.slot[t] = live ? page * a.page_size + (row - pg * a.page_size) : -1;
+    if (a.pos) a.pos[t] = pos;
+    if (a.seq) a.seq[t] = live ? b : -1;
+}
+// Page k of those taken into its table.
+template <typename FIND, typename FROM>
+__device__ __forceinline__ void plan_taken(const PlanArgs &a, const PlanSums &p, const FIND &f, FROM from, int k) {
+    const bool live = k < p.taken;
+    const int b = f.template find<false>(p.grown, k, live), page = stack_page<true>(a, p, f, p.was_free + p.released - 1 - k, live);
+    if (!live) return;
+    int row0, pos0;
+    from(b, row0, pos0);
+    a.table[(size_t)b * a.max_pages + plan_ceil(a, row0) + k - p.grown[b]] = page;
+}
+// Released page k, counted from the lowest, onto the free ones: it was not taken.
+template <typename FIND>
+__device__ __forceinline__ void plan_freed(const PlanArgs &a, const PlanSums &p, const FIND &f, int k) {
+    const bool live = k < p.released - p.taken;
+    const int page = stack_page<false>(a, p, f, p.was_free + k, live);
+    if (live) a.free_pages[p.was_free + k] = page;
 }
 
 constexpr int PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
@@ -160,15 +205,28 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
         s.need = plan_ceil(a, s.rows + s.want) - plan_ceil(a, s.rows);
         return s;
     };
-    Seq one = {};
-    if (per == 1 && b0 < b1) one = read(b0);
-    auto look = [&](int b) { return per == 1 ? one : read(b); };   // (a thread's only sequence is read once)
+    // f(b, sequence b) for a thread's sequences: up to KEPT of them are read once
+    constexpr int KEPT = ALL ? 1 : 4;
+    Seq kept[KEPT];
+    if (per <= KEPT) {
+#pragma unroll
+        for (int k = 0; k < KEPT; k++)
+            if (b0 + k < b1) kept[k] = read(b0 + k);
+    }
+    auto each = [&](auto f) {
+        if (per <= KEPT) {
+#pragma unroll
+            for (int k = 0; k < KEPT; k++)
+                if (b0 + k < b1) f(b0 + k, kept[k]);
+        } else {
+            for (int b = b0; b < b1; b++) f(b, read(b));
+        }
+    };
     int64_t first[2] = {0, 0}, all2[2], tok[1] = {0}, all1[1], last[2] = {0, 0}, given[2];
-    for (int b = b0; b < b1; b++) {
-        const Seq s = look(b);
+    each([&](int, const Seq &s) {
         first[0] += s.back;
         first[1] += s.need;
-    }
+    });
     block_scan<2>(first, all2, sums, waves);
     int64_t released = all2[0];
     if (was_free + released > a.n_pages) {   // (pages given back twice, or not of this pool)
@@ -181,7 +239,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
         return s.need == 0 || needs <= total ? s.want : 0;
     };
     int64_t x = first[1];
-    for (int b = b0; b < b1; b++) tok[0] += served(x, look(b));
+    each([&](int, const Seq &s) { tok[0] += served(x, s); });
     block_scan<1>(tok, all1, sums + 2 * PLAN_WAVES, waves);
     auto took_of = [&](int64_t &needs, int64_t &toks, const Seq &s) {
         const int t = served(needs, s);
@@ -190,18 +248,16 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
     };
     int64_t y = tok[0];
     x = first[1];
-    for (int b = b0; b < b1; b++) {
-        const Seq s = look(b);
+    each([&](int, const Seq &s) {
         const int t = took_of(x, y, s);
         last[0] += t;
         last[1] += t ? s.need : 0;
-    }
+    });
     block_scan<2>(last, given, sums + 3 * PLAN_WAVES, waves);
     const int64_t tokens = given[0], taken = given[1];
     y = tok[0];
     x = first[1];
-    for (int b = b0; b < b1; b++) {
-        const Seq s = look(b);
+    each([&](int b, const Seq &s) {
         const int t = took_of(x, y, s);
         const int at = (int)last[0], gr = (int)last[1], bk = (int)min(first[0], released);
         const int pos = a.next_pos && !s.over ? a.next_pos[b] : 0;
@@ -214,7 +270,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
         last[0] += t;
         last[1] += t ? s.need : 0;
         first[0] += s.back;
-    }
+    });
     if (tid == 0) {
         a.q_start[a.B] = (int)tokens;
         if (!ALL) a.was_free[0] = was_free, a.was_free[1] = (int)released, a.was_free[2] = (int)taken;
@@ -224,23 +280,31 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_plan(PlanArgs a) {
     if (tid == 0) *a.n_free_out = (int)(total - taken);
     if constexpr (ALL) {
         const PlanSums p = {l_start, l_back, l_grown, was_free, (int)released, (int)taken};
-        const int64_t items = (int64_t)a.n_tok + max(released, taken);
-        for (int64_t i = tid; i < items; i += PLAN_THREADS)
-            plan_item(a, p, i, (int)tokens, (int)total, [&](int b, int &row0, int &pos0) { row0 = l_row0[b], pos0 = l_pos0[b]; });
+        const LaneFind f = {a.B};
+        auto from = [&](int b, int &row0, int &pos0) { row0 = l_row0[b], pos0 = l_pos0[b]; };
+        for (int t = tid; t < a.n_tok; t += PLAN_THREADS) plan_token(a, p, f, from, t, (int)tokens);
+        for (int k = tid; k < p.taken; k += PLAN_THREADS) plan_taken(a, p, f, from, k);
+        for (int k = tid; k < p.released - p.taken; k += PLAN_THREADS) plan_freed(a, p, f, k);
     }
 }
 
-// grid any, block 256: the second half from the sums in memory.
+// grid any, block 256: the second half from the sums in memory, 64 items a wave
+// at a time.
 __global__ __launch_bounds__(256) void pages_fill(PlanArgs a) {
     const PlanSums p = {a.q_start, a.back, a.grown, a.was_free[0], a.was_free[1], a.was_free[2]};
-    const int tokens = a.q_start[a.B], total = p.was_free + p.released;
-    const int64_t items = (int64_t)a.n_tok + max(p.released, p.taken);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        plan_item(a, p, i, tokens, total, [&](int b, int &row0, int &pos0) {
-            const int took = a.q_start[b + 1] - a.q_start[b];
-            row0 = a.len_out[b] - took;
-            pos0 = a.next_pos ? (int)((uint32_t)a.next_pos_out[b] - (uint32_t)took) : row0;
-        });
+    const WaveFind f = {a.B};
+    auto from = [&](int b, int &row0, int &pos0) {
+        const int took = a.q_start[b + 1] - a.q_start[b];
+        row0 = a.len_out[b] - took;
+        pos0 = a.next_pos ? (int)((uint32_t)a.next_pos_out[b] - (uint32_t)took) : row0;
+    };
+    const int tokens = a.q_start[a.B], lane = threadIdx.x & 63;
+    auto groups = [](int n) { return n > 0 ? (n - 1) / 64 + 1 : 0; };
+    const int g1 = groups(a.n_tok), g2 = g1 + groups(p.taken), g3 = g2 + groups(p.released - p.taken);
+    for (int g = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); g < g3; g += gridDim.x * 4) {
+        if (g < g1) plan_token(a, p, f, from, 64 * g + lane, tokens);
+        else if (g < g2) plan_taken(a, p, f, from, 64 * (g - g1) + lane);
+        else plan_freed(a, p, f, 64 * (g - g2) + lane);
     }
 }
 
