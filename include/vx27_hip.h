@@ -482,15 +482,18 @@ int vx27_hip_paged_evict(vx27_hip_ctx *ctx, const vx27_paged_evict_desc *d);
 #define VX27_Q4_BLOCK_BYTES 4608
 #define VX27_Q4_SPLIT_ROWS 96
 #define VX27_Q4_SPLIT_ROWS_F32 512
+#define VX27_Q4_SPLIT_TILES 2048
 /* vx27_hip_paged_append into 4-bit pages.  k is normed and rotated in fp64
  * (the angle is the fp32 product of the other calls), so that rounding it to
  * codes does not depend on the order of sums; q as there.  max_T at most 2^25. */
 int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d);
 /* vx27_hip_paged_attn over 4-bit pages; acc must be NULL.  Up to
  * VX27_Q4_SPLIT_ROWS query rows a KV head (max_T * n_q/n_kv; fp32 outputs:
- * VX27_Q4_SPLIT_ROWS_F32) run the decode kernels: codes and q are exact
+ * VX27_Q4_SPLIT_ROWS_F32), and more of small calls (n_kv * (n_tok * n_q/n_kv/16 + B)
+ * times the 32-row blocks that a sequence can see, at most VX27_Q4_SPLIT_TILES)
+ * run the decode kernels: codes and q are exact
  * operands of bf16 MFMAs, s and m are applied in fp32, and the softmax weights
- * are two bf16 parts (at most 2^-16 off).  More rows run the tile kernel: the
+ * are two bf16 parts (at most 2^-16 off).  The others run the tile kernel: the
  * rows' values, and the weights, are rounded to bf16 once.  A group held as NaN
  * reaches only the tokens that see its row, whose outputs are then NaN (of a
  * value row: the group's dims).

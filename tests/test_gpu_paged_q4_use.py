@@ -11,7 +11,7 @@ from gpu_common import say
 from paged_common import HD, f64
 from plan_common import plan, pool
 from q4_common import BLOCK, K_AT, V_AT, Batch4, get, norm_rope, out_tol, put, put_rows, quantise, values
-from test_gpu_paged_q4 import Attn4, append_v, ctx  # noqa: F401
+from test_gpu_paged_q4 import SHAPES, Attn4, append_v, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -680,3 +680,109 @@ def test_plans_of_many_sequences(ctx, B, few, ended):  # noqa: F811
     ctx.sync()
     p.check(want)
     p.free()
+
+
+def widen(bt, pages=2100):
+    """The batch with a page table of many more entries, behind the rows: the same rows, and a call that may see more."""
+    bt.table = np.concatenate([bt.table, np.full((bt.B, pages), -7, np.int32)], axis=1)
+    bt.max_pages += pages
+    return bt
+
+
+@pytest.mark.parametrize("out_bf16", [False, True])
+@pytest.mark.parametrize("i", [i for i, s in enumerate(SHAPES) if max(s[1]) * s[2] // s[3] > 96])
+def test_prompts_under_wide_tables(ctx, i, out_bf16):  # noqa: F811
+    """Prompts of few rows whose tables have room for many: the tile kernel (small calls run the decode kernels)."""
+    lens, new, n_q, n_kv, page, window, sink = SHAPES[i]
+    say(f"wide tables {i} {lens} {new} bf16 {out_bf16}")
+    at = Attn4(ctx, widen(Batch4(lens, new, n_q, n_kv, page, window, sink, seed=900 + i, lead=2, tail=3)), out_bf16, gate=("f32", "bf16", "none")[i % 3])
+    at.call()
+    at.check(f"{i}")
+    at.free()
+
+
+@pytest.mark.parametrize("lens,new,window,sink", [([90, 33], [60, 33], 0, 0), ([400, 90], [130, 90], 50, 4), ([1500, 10], [40, 3], 0, 0)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_nan_groups_under_wide_tables(ctx, lens, new, window, sink, what):  # noqa: F811
+    """A group held as NaN in the tile kernel: NaN where a token sees it, and nowhere else."""
+    say(f"nan groups, wide tables {what} {lens} {new}")
+    bt = widen(Batch4(lens, new, 24, 4, 64, window, sink, seed=650 + new[0]))
+    seen, j = bt.seen(0), None
+    part = np.nonzero(seen.any(0) & ~seen.all(0))[0]
+    q, where = (bt.kq, K_AT) if what == "k" else (bt.vq, V_AT)
+    clean, hit = q.copy(), np.zeros((bt.N, 24, HD), bool)
+    for i, j in enumerate((part[0], part[len(part) // 2], part[-1])):
+        p, at, g = bt.table[0, j // 64], j % 64, i % 4
+        c, s, m = (x.copy() for x in get(q[p, 1, at // 32], where, at % 32))
+        c[64 * g:64 * g + 64], s[g], m[g] = 0, 0, 0x7FC0
+        put(q[p, 1, at // 32], where, at % 32, c, s, m)
+        m[g] = 0
+        put(clean[p, 1, at // 32], where, at % 32, c, s, m)
+        hit[np.ix_(bt.start[0] + np.nonzero(seen[:, j])[0], range(6, 12), range(HD) if what == "k" else range(64 * g, 64 * g + 64))] = True
+    at = Attn4(ctx, bt, True, gate="none")
+    assert at.tiled()
+    at.call()
+    ctx.sync()
+    out = at.out()
+    if what == "k":
+        bt.kq = clean
+    else:
+        bt.vq = clean
+    ref = bt.result(False)
+    assert np.isnan(out[hit]).all()
+    assert np.all(np.abs(out[~hit] - ref["out"][~hit]) <= at.tol(ref, max(lens))[~hit])
+    at.free()
+
+
+@pytest.mark.parametrize("what", ["page", "negative page", "length", "start", "long"])
+def test_bad_indices_under_wide_tables(ctx, what):  # noqa: F811
+    """The tile kernel's faulty tables, as test_bad_indices_are_reported."""
+    from vx27_amd import lib as L
+    say(f"faulty {what}, wide tables")
+    bt = widen(Batch4([200, 100], [150, 2], seed=26))
+    if what == "page":
+        bt.table[1, 0] = bt.n_pages
+    if what == "negative page":
+        bt.table[1, 0] = -1
+    if what == "length":
+        bt.lens[0] = bt.max_pages * bt.page + 1
+    if what == "start":
+        bt.start[2] = bt.N + 1
+    if what == "long":
+        bt.start[:] = [0, bt.N, bt.N]
+    a = Attn4(ctx, bt, True, gate="none")
+    a.call()
+    with pytest.raises(L.HipError, match="paged cache"):
+        ctx.sync()
+    a.free()
+
+
+def test_graphs_under_wide_tables():
+    """Tiles, and tiles over values laid out in scratch, captured with a decode call on one workspace."""
+    from vx27_amd import lib as L
+    say("graphs, wide tables")
+    with L.Ctx(0) as c:
+        ats = [Attn4(c, widen(Batch4([800, 64], [30, 64], seed=22), 100), True), Attn4(c, widen(Batch4([800, 64], [300, 64], seed=23), 100), True),
+               Attn4(c, Batch4([1500, 90, 700], [1, 1, 1], seed=21))]
+        want, graphs = [], []
+        for x in ats:
+            x.call()
+            c.sync()
+            want.append(x.raw())
+        for x in ats:
+            c.graph_begin()
+            x.call()
+            graphs.append(c.graph_end())
+        try:
+            for rep in range(4):
+                for x, g, w in zip(ats, graphs, want):
+                    c.graph_launch(g)
+                    c.sync()
+                    assert all(np.array_equal(p, q) for p, q in zip(x.raw(), w)), rep
+                for x, w in zip(ats, want):
+                    x.call()
+                    c.sync()
+                    assert all(np.array_equal(p, q) for p, q in zip(x.raw(), w)), rep
+        finally:
+            for g in graphs:
+                L.check(L.lib().vx27_hip_graph_destroy(g), "graph_destroy")

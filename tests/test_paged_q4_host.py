@@ -80,8 +80,8 @@ def test_layouts(tmp_path):
     from vx27_amd import lib as L
     names = {"vx27_paged_read_desc": L.PagedReadDesc, "vx27_paged_plan_desc": L.PagedPlanDesc}
     src = ["#include <stdio.h>", "#include <stddef.h>", '#include "vx27_hip.h"', "int main(void) {",
-           '    printf("%d\\n%d\\n%d\\n", VX27_Q4_BLOCK_BYTES, VX27_Q4_SPLIT_ROWS, VX27_Q4_SPLIT_ROWS_F32);']
-    want = [L.Q4_BLOCK_BYTES, L.Q4_SPLIT_ROWS, L.Q4_SPLIT_ROWS_F32]
+           '    printf("%d\\n%d\\n%d\\n%d\\n", VX27_Q4_BLOCK_BYTES, VX27_Q4_SPLIT_ROWS, VX27_Q4_SPLIT_ROWS_F32, VX27_Q4_SPLIT_TILES);']
+    want = [L.Q4_BLOCK_BYTES, L.Q4_SPLIT_ROWS, L.Q4_SPLIT_ROWS_F32, L.Q4_SPLIT_TILES]
     for c, py in names.items():
         src.append(f'    printf("%zu\\n", sizeof({c}));')
         want.append(C.sizeof(py))

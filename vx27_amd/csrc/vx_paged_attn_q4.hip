@@ -479,7 +479,10 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     // 16 tokens 55, 56 | 59, 99 | 349, 323; 24 tokens 73, 66 | 78, 93 | 524, 331.
     // fp32 outputs stay with the split kernel, which rounds neither keys nor
     // values and has two parts of the weights, to where a call is a prompt.
-    if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32)) return rows_launch<true>(who, ctx, d, a, rows, 0);
+    // Short prompts too: up to 2048 tiles and blocks of 16 rows in all (prompts of 50
+    // tokens 15 us against 26, of 100 22, 28; of 200, 2432 of them, 39, 31).
+    const int64_t pairs = ((int64_t)d->n_tok * a.qg / 16 + d->B) * d->n_kv * a.tile_cap;
+    if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32) && pairs > VX27_Q4_SPLIT_TILES) return rows_launch<true>(who, ctx, d, a, rows, 0);
     // (decoding tokens of 6 heads: 8 rows a block)
     a.block_rows = rows <= 8 ? 8 : 16;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;

@@ -132,6 +132,7 @@ class PagedPlanDesc(C.Structure):
 Q4_BLOCK_BYTES = 4608           # 32 rows of K or of V of one KV head in 4-bit pages
 Q4_SPLIT_ROWS = 96              # most query rows a KV head (tokens x its group) of the 4-bit split kernel: bf16 outputs
 Q4_SPLIT_ROWS_F32 = 512         # ... and fp32 outputs
+Q4_SPLIT_TILES = 2048           # calls of more rows, but at most this many (block of 16 rows, tile) pairs, run it too
 
 
 _SIGS = {
