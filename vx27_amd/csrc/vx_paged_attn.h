@@ -136,6 +136,15 @@ __device__ __forceinline__ void add_part(float4 &O, float &L, float4 o, float l,
 // holds every (KV head, block)'s tiles; else a KV head's rows are one block.
 template <bool BL>
 __device__ __forceinline__ int seq_blocks(const Args &a, const vx_pseq &s) { return BL ? (s.T * a.qg + a.block_rows - 1) / a.block_rows : 1; }
+// A block's tiles in units of the list.  BL: rounded up to min_tiles, as a
+// workgroup's share is: in small calls, where that is the share, none takes the
+// end of one block and the start of the next, which costs it the queries, first
+// loads and merge of both (one sequence of 4000 rows 20 us, so 14; 16 of 200 rows
+// 19, 14; a prompt of 20 tokens 22, 14).  Rounded shares are the better where
+// they are a few tiles too (200 x 100 rows 39 us against 46, 24 x 700 22, 24;
+// but 64 x 300 28, 23).
+template <bool BL>
+__device__ __forceinline__ int list_tiles(const Args &a, int nt) { return BL ? (nt + a.min_tiles - 1) / a.min_tiles * a.min_tiles : nt; }
 struct Units {
     vx_pseq s;          // of sequence `lane` (B <= 64)
     vx_tiles t;
@@ -146,7 +155,7 @@ template <bool BL>
 __device__ __forceinline__ int seq_units(const Args &a, int b, vx_pseq &s, vx_tiles &t) {
     s = vx_paged_seq(a.p, b);
     t = tiles_of(a, s, 0, s.T - 1);
-    return t.nt * a.p.n_kv * seq_blocks<BL>(a, s);
+    return list_tiles<BL>(a, t.nt) * a.p.n_kv * seq_blocks<BL>(a, s);
 }
 template <bool BL>
 __device__ __forceinline__ Units units_of(const Args &a, int grid) {
@@ -159,7 +168,7 @@ __device__ __forceinline__ Units units_of(const Args &a, int grid) {
     } else {
         u.total = a.before[a.p.B];
     }
-    u.chunk = max((u.total + grid - 1) / grid, a.min_tiles);
+    u.chunk = list_tiles<BL>(a, max((u.total + grid - 1) / grid, a.min_tiles));
     return u;
 }
 // Sequence b: itself, its tiles, and the units before it.
@@ -169,7 +178,7 @@ __device__ __forceinline__ int units_before(const Args &a, const Units &u, int b
         auto get = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
         s = {get(u.s.start), get(u.s.T), get(u.s.len), get(u.s.row0)};
         t = {get(u.t.st), get(u.t.fm), get(u.t.nt)};
-        return get(u.upto) - t.nt * a.p.n_kv * seq_blocks<BL>(a, s);
+        return get(u.upto) - list_tiles<BL>(a, t.nt) * a.p.n_kv * seq_blocks<BL>(a, s);
     }
     seq_units<BL>(a, b, s, t);
     return a.before[b];
@@ -227,7 +236,7 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     const int kvh = BL ? (int)blockIdx.x % a.p.n_kv : (int)blockIdx.y, blk = BL ? (int)blockIdx.x / a.p.n_kv : 0;
     const int pr = BL ? blockIdx.y : blockIdx.x, r = BL ? blk * a.block_rows + pr : pr;   // the row, in its block and in all
     if (r >= s.T * a.qg) return;
-    const int p0 = before + (kvh * nb + blk) * tl.nt, p1 = p0 + tl.nt;
+    const int n_list = list_tiles<BL>(a, tl.nt), p0 = before + (kvh * nb + blk) * n_list, p1 = p0 + n_list;
     const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
     const int g0 = p0 / un.chunk, g1 = (p1 - 1) / un.chunk;
     if (tl.nt > 0 && g0 == g1) return;

@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
     vx_tiles tl;
     int before = units_before<true>(a, un, b, s, tl);
     for (int u = u0; u < u1;) {
-        const int nb = seq_blocks<true>(a, s), all = tl.nt * a.p.n_kv * nb;
+        const int nb = seq_blocks<true>(a, s), n_list = list_tiles<true>(a, tl.nt), all = n_list * a.p.n_kv * nb;
         if (u >= before + all) {
             before += all;
             b++;
@@ -352,11 +352,11 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
             else seq_units<true>(a, b, s, tl);
             continue;
         }
-        const int item = (u - before) / tl.nt, i0 = (u - before) - item * tl.nt;
+        const int item = (u - before) / n_list, i0 = (u - before) - item * n_list;
         const int kvh = item / nb, r0 = (item - kvh * nb) * ROWS;
-        const int cnt = min(tl.nt - i0, u1 - u);
+        const int cnt = min(n_list - i0, u1 - u), real = min(cnt, tl.nt - i0);
         const int R = min(s.T * a.qg - r0, ROWS);
-        const int mine = (cnt - wave + 3) / 4;      // this wave's tiles: i0 + wave + 4 j
+        const int mine = (real - wave + 3) / 4;     // this wave's tiles: i0 + wave + 4 j
         // lane i holds the block of this wave's tile 64 k + i
         uint32_t blocks = 0;
         auto look_up = [&](int j) {
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_split(Args a) {
         }
         vx_lds_barrier();
         // wave w merges rows w, w + 4, ..., lane L dims 4L .. 4L + 3
-        const bool whole = cnt == tl.nt;
+        const bool whole = cnt == n_list;
         const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
         for (int r = wave; r < R; r += 4) {
             const int t = row_tok(a, r0 + r), tok = s.start + t, h = row_head(a, kvh, r0 + r, t);
@@ -486,9 +486,9 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     // (decoding tokens of 6 heads: 8 rows a block)
     a.block_rows = rows <= 8 ? 8 : 16;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;
-    const int64_t units = (int64_t)d->B * d->n_kv * nb * a.tile_cap;
+    a.min_tiles = 4;                             // (a tile a wave)
+    const int64_t units = (int64_t)d->B * d->n_kv * nb * ((a.tile_cap + a.min_tiles - 1) / a.min_tiles * a.min_tiles);
     VX_REQUIRE(units < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %d tiles each)", who, d->B, d->n_kv, a.tile_cap);
-    a.min_tiles = 2;
     const int grid = (int)std::min<int64_t>((units + a.min_tiles - 1) / a.min_tiles, 2 * ctx->n_cu);
     a.part_rows = std::min(rows, a.block_rows);
     const size_t n_part = (size_t)2 * grid * a.part_rows;
