@@ -10,9 +10,9 @@
 // one for a tile's outputs).
 //
 // The split kernel on 4 x 131072 rows of 4 KV heads (604 MB): 106 us, 5.7 TB/s
-// of 7.2; a wave's 32 tiles take 2100 cycles of the VALU each (half of them the
-// codes' masks and conversions and the weights' parts), which keeps it busy for
-// about two thirds of the time at the two waves a SIMD that 235 registers allow.
+// of 7.2 (its loads alone 90).  A tile is 670 VALU instructions, half of them the
+// codes' masks and conversions and the weights' parts, which keep the VALU busy
+// for two thirds of the time at the two waves a SIMD that 235 registers allow.
 // Ragged windows of 32 sequences: 41 us for 141 MB, of which some 10 are the
 // first loads' chain (lengths, table, blocks) and the waves' merge.
 #include "vx_paged_q4.h"
@@ -479,8 +479,9 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     // 16 tokens 55, 56 | 59, 99 | 349, 323; 24 tokens 73, 66 | 78, 93 | 524, 331.
     // fp32 outputs stay with the split kernel, which rounds neither keys nor
     // values and has two parts of the weights, to where a call is a prompt.
-    // Short prompts too: up to 2048 tiles and blocks of 16 rows in all (prompts of 50
-    // tokens 15 us against 26, of 100 22, 28; of 200, 2432 of them, 39, 31).
+    // Short prompts too, up to 2048 pairs of a tile and a block of 16 rows in all
+    // (prompts of 50 tokens 15 us against 26, of 100 18, 28; of 200, 2432 pairs, 28,
+    // 31; five of 30 tokens after 270 rows, 2440, 38, 35).
     const int64_t pairs = ((int64_t)d->n_tok * a.qg / 16 + d->B) * d->n_kv * a.tile_cap;
     if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32) && pairs > VX27_Q4_SPLIT_TILES) return rows_launch<true>(who, ctx, d, a, rows, 0);
     // (decoding tokens of 6 heads: 8 rows a block)
