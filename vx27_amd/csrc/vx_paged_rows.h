@@ -99,9 +99,6 @@ __device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &
     return max(1, (tl.nt + 1) / 2);
 }
 
-// grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).  It
-// goes by B * n_rt entries, n_rt of the longest token range: 256 decoding
-// sequences beside a chunk of 8192 tokens 105 us, 4096 beside 4096 1.8 ms.
 // 4-bit pages: row tiles of the longest token range from which the values are
 // laid out in scratch, and the most tiles there (32 KiB each, K and V: 256 MiB).
 // (In us with and without, 4 x 6000 | 1 x 30000 rows, tokens of 6 heads: 86
@@ -110,6 +107,9 @@ __device__ __forceinline__ int entry_steps(const Args &a, int n_rt, int e, int &
 constexpr int FLAT_ROWS = 6;
 constexpr size_t FLAT_TILES = 8192;
 
+// grid 1, block 1024 (6 us; 9 for the 1536 items of an 8192-token prompt).  It
+// goes by B * n_rt entries, n_rt of the longest token range: 256 decoding
+// sequences beside a chunk of 8192 tokens 105 us, 4096 beside 4096 1.8 ms.
 constexpr int PLAN = 1024;
 __global__ __launch_bounds__(PLAN) void paged_plan(Args a, int n_rt, int n_cu, int max_pieces) {
     __shared__ int64_t s_steps[PLAN / 64];
