@@ -223,6 +223,14 @@ __device__ __forceinline__ floatx4_t weigh(bf16x8_t x, const Weights &w, floatx4
 // 4e-6 to 8e-6, for 1% of the time.)
 constexpr int AHEAD = 1;
 
+// The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the VALU's exchanges: a
+// swapped pair holds a lane's own value and its partner's).
+__device__ __forceinline__ float over_groups(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 // x over the 16 lanes of a lane group, by OR or AND.
 template <bool AND>
 __device__ __forceinline__ uint32_t over_rows(uint32_t x) {
@@ -252,8 +260,7 @@ __device__ __forceinline__ void attend_tile(Rows<ROWS> &w, bool whole, float (&x
     float mt = x[0];
 #pragma unroll
     for (int e = 1; e < 8; e++) mt = fmaxf(mt, x[e]);
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * SC2;
+    mt = over_groups(mt) * SC2;
     if (__any(mt > w.m)) {
         const bool up = mt > w.m;
         const float to = mt + AHEAD, alpha = up ? __builtin_amdgcn_exp2f(w.m - to) : 1.0f;
