@@ -42,6 +42,13 @@ __host__ __device__ __forceinline__ int vx_q4_k_row(int u) { return ((u >> 2) & 
 // Codes of V: unit u = lane (g,n) of quad j; its dword i holds dim
 // 64 j + 16 i + n of rows 8 g .. 8 g + 7.
 // Scales s: [4 groups][32 rows].  Minima m: K [32 rows][4 groups], V [4][32].
+// One value of a block of V.
+__device__ __forceinline__ float vx_q4_v_value(const char *blk, int row, int dim) {
+    const int group = dim / VX_Q4_GROUP;
+    const uint32_t c = (uint8_t)blk[group * 1024 + (row >> 3) * 256 + (dim & 15) * 16 + ((dim >> 4) & 3) * 4 + (row & 3)] >> (row & 4);
+    auto word = [&](int at) { return vx_bf16_to_f32(*(const uint16_t *)(blk + at + group * 64 + row * 2)); };
+    return __builtin_fmaf((float)(c & 15), word(VX_Q4_S), word(VX_Q4_M));
+}
 
 typedef __bf16 vx_bf16x8 __attribute__((ext_vector_type(8)));
 

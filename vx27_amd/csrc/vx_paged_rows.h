@@ -711,11 +711,11 @@ __global__ __launch_bounds__(256, 1) void paged_rows(Args a) {
                 const int key0 = key_of(c, h);
                 if (key0 < 0) continue;
                 const int page = vx_paged_page(a.p, b, key0), at = key0 - vx_page_slot(a.p, key0) * a.p.page_size;
-                const uint16_t *vp = Q4 ? (const uint16_t *)((const char *)a.v_pages + (size_t)vx_q4_block(a.p, page, kvh, at) * VX_Q4_BLOCK + VX_Q4_M) + tid / VX_Q4_GROUP * TILE
-                                     : PAGES == PG_FLAT ? a.flat_v + flat_at(a, s, b, kvh, key0) + tid * TILE
-                                                        : a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
-                for (int j = 0; j < TILE; j++) {   // (4-bit pages: a group that is not finite has m = NaN)
-                    const float x = vx_bf16_to_f32(vp[j]);
+                const char *blk = (const char *)a.v_pages + (size_t)vx_q4_block(a.p, page, kvh, at) * VX_Q4_BLOCK;   // (4-bit pages)
+                const uint16_t *vp = PAGES == PG_FLAT ? a.flat_v + flat_at(a, s, b, kvh, key0) + tid * TILE
+                                                      : a.v_pages + vx_v_index(a.p.n_kv, a.p.page_size, page, kvh, at, tid);
+                for (int j = 0; j < TILE; j++) {   // (of 4-bit pages as the steps rounded it: a value of 2^127 and more may be an infinity)
+                    const float x = Q4 ? __uint_as_float(pack2(vx_q4_v_value(blk, j, tid), 0.0f) << 16) : vx_bf16_to_f32(vp[j]);
                     if (is_finite(x)) continue;
                     for (int r = 0; r < TR && r0 + r < R; r++)
                         if (sight_of(a, s, r0 + r).sees(key0 + j)) so[r * HDG + ((((tid >> 2) ^ (r & 15)) << 2) | (tid & 3))] += x;
