@@ -494,7 +494,10 @@ int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d)
  * run the decode kernels: codes and q are exact
  * operands of bf16 MFMAs, s and m are applied in fp32, and the softmax weights
  * are two bf16 parts (at most 2^-16 off).  The others run the tile kernel: the
- * rows' values, and the weights, are rounded to bf16 once.  A group held as NaN
+ * rows' values, and the weights, are rounded to bf16 once.  (So do calls whose
+ * list of 32-row blocks, those that a sequence can see for each 16 query rows, or
+ * 8 where there are no more, and KV head, may be past 2^31: the blocks of max_T
+ * tokens of every sequence, or past 64 sequences of n_tok tokens in all.)  A group held as NaN
  * reaches only the tokens that see its row, whose outputs are then NaN (of a
  * value row: the group's dims).
  * Nothing overflows while the largest |s*15| + |m| of V times the number of

@@ -1,27 +1,18 @@
 """The 4-bit paged attention where values and sizes are extreme."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+import q4_bounds as Q
 from gpu_common import say
 from paged_common import HD, f64
-from q4_common import BF16_MAX, Batch4, quantise, values
+from q4_bounds import run, widen
+from q4_common import BF16_MAX, BLOCK, Batch4, quantise, values
 from test_gpu_paged_q4 import Attn4, ctx  # noqa: F401
-from test_gpu_paged_q4_use import widen
 from vx27_amd import workloads as W
 
 pytestmark = pytest.mark.gpu
-
-KERNELS = ("paged_q4_split", "paged_rows_q4", "paged_rows_flat")
-
-
-def run(at):
-    """The attention kernel that a call runs."""
-    at.ctx.prof_enable(True)
-    at.call()
-    ran = [k for k in KERNELS if at.ctx.prof_read(k)[0]]
-    at.ctx.prof_enable(False)
-    assert len(ran) == 1
-    return ran[0]
 
 
 @pytest.mark.parametrize("kernel,lens,new,window,sink,wide", [
@@ -68,3 +59,93 @@ def test_values_that_come_back_infinite(ctx, kernel, lens, new, window, sink, wi
     assert np.array_equal(out[~hit], want[~hit])
     clean.free()
     at.free()
+
+
+class Wide:
+    """B sequences that all read one page of 2^18 rows, of which 32 are there: sequence b has its first lens[b], and its
+    last new[b] are the call's tokens."""
+
+    def __init__(self, ctx, lens, new, n_q, n_kv, out_bf16, seed):
+        from vx27_amd import lib as L
+        self.ctx, self.L, self.out_bf16 = ctx, L, out_bf16
+        src = Batch4([32], [32], n_q, n_kv, 32, seed=seed)
+        pools = [np.zeros((1, n_kv, 1 << 13, BLOCK), np.uint8) for _ in range(2)]
+        for pool, q in zip(pools, (src.kq, src.vq)):
+            pool[0, :, 0] = q[src.table[0, 0], :, 0]
+        bt = self.bt = Batch4.__new__(Batch4)
+        r, bt.B, bt.lens, bt.new, bt.n_q, bt.n_kv, bt.qg, bt.window, bt.sink = src.r, len(lens), lens, new, n_q, n_kv, n_q // n_kv, 0, 0
+        bt.start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
+        bt.N = int(bt.start[-1])
+        bt.q = W.bf16_bits(W.normal(r, (bt.N, n_q, HD), 2.0))
+        held = src.held(0)
+        bt.held = lambda b: [[x[:bt.lens[b]] for x in part] for part in held]
+        up = dict(k=pools[0], v=pools[1], table=np.zeros((bt.B, 1), np.int32), len=np.asarray(lens, np.int32), start=bt.start, q=bt.q)
+        self.buf = {n: ctx.put(x) for n, x in up.items()}
+        self.buf["out"] = ctx.buf(bt.N * n_q * HD * (2 if out_bf16 else 4))
+        d = self.d = L.PagedAttnDesc(B=bt.B, n_q=n_q, n_kv=n_kv, hd=HD, page_size=1 << 18, n_pages=1, max_pages=1, n_tok=bt.N, max_T=max(new))
+        d.table, d.len, d.q_start, d.q, d.k_pages, d.v_pages, d.out = (self.buf[x].ptr for x in ("table", "len", "start", "q", "k", "v", "out"))
+        d.out_dtype = L.BF16 if out_bf16 else L.F32
+
+    def call(self):
+        self.L.check(self.L.lib().vx27_hip_paged_attn_q4(self.ctx.h, C.byref(self.d)), "paged_attn_q4")
+
+    def check(self, kernel, tokens):
+        self.ctx.sync()
+        bt = self.bt
+        res = Q.result(bt, kernel, False, tokens=tokens)
+        out = self.buf["out"].download((bt.N, bt.n_q, HD), np.uint16 if self.out_bf16 else np.float32)
+        out = f64(out) if self.out_bf16 else out.astype(np.float64)
+        most, mean = Q.check(out[tokens], {n: x[tokens] for n, x in res.items()}, kernel, 32, self.out_bf16)
+        say(f"  err {most:.3f}, mean {mean:.3f}")
+        assert most <= 1 and mean <= 1
+
+    def free(self):
+        for b in self.buf.values():
+            b.free()
+
+
+def test_many_sequences_beside_one_with_many_tokens(ctx):  # noqa: F811
+    """One sequence of 30 tokens beside 2199 of one, whose table has room for 8192 blocks: were all of 30 tokens, the list
+    would be past 2^31, but they are not."""
+    say("one of many sequences with more tokens")
+    B = 2200
+    w = Wide(ctx, [30] + [1 + b % 30 for b in range(B - 1)], [30] + [1] * (B - 1), 64, 4, False, 1800)
+    assert B * 4 * 30 * 8192 >= 2 ** 31
+    assert run(w) == "paged_q4_split"
+    w.check("paged_q4_split", np.arange(w.bt.N) % 7 < 3)
+    w.free()
+
+
+@pytest.mark.parametrize("out_bf16", [False, True])
+def test_lists_past_2_to_31_blocks(ctx, out_bf16):  # noqa: F811
+    """65535 sequences with room for 8192 blocks of 4 KV heads each: the tile kernel needs no list of them."""
+    say(f"lists past 2^31 blocks, bf16 {out_bf16}")
+    B = 65535
+    w = Wide(ctx, [1 + b % 32 for b in range(B)], [1] * B, 4, 4, out_bf16, 1810)
+    assert B * 4 * 8192 >= 2 ** 31 - 65536
+    assert run(w) == "paged_rows_q4"
+    w.check("paged_rows_q4", np.arange(B) % 97 < 4)
+    w.free()
+
+
+def test_token_ranges_that_overlap_past_2_to_31_blocks(ctx):  # noqa: F811
+    """Ranges that overlap can make a list longer than n_tok tokens do: nothing runs, and the next sync reports it."""
+    from vx27_amd import lib as L
+    say("overlapping ranges past 2^31 blocks")
+    B, T = 4200, 32
+    w = Wide(ctx, [32] * B, [T] + [0] * (B - 1), 64, 4, False, 1820)
+    assert (B // 2) * 4 * 32 * 8192 >= 2 ** 31
+    start, lens = np.zeros(B + 1, np.int32), np.full(B, 1 << 18, np.int32)
+    start[1::2] = T
+    for n, x in (("start", start), ("len", lens)):
+        w.buf[n].upload(x)
+    w.buf["out"].upload(np.full(w.buf["out"].nbytes, 0x5A, np.uint8))
+    w.call()
+    with pytest.raises(L.HipError, match="paged cache"):
+        ctx.sync()
+    assert np.all(w.buf["out"].download((w.buf["out"].nbytes,), np.uint8) == 0x5A)
+    for n, x in (("start", w.bt.start), ("len", np.asarray(w.bt.lens, np.int32))):
+        w.buf[n].upload(x)
+    assert run(w) == "paged_q4_split"
+    w.check("paged_q4_split", np.ones(w.bt.N, bool))
+    w.free()

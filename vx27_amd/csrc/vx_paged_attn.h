@@ -145,6 +145,8 @@ __device__ __forceinline__ int seq_blocks(const Args &a, const vx_pseq &s) { ret
 // but 64 x 300 28, 23).
 template <bool BL>
 __device__ __forceinline__ int list_tiles(const Args &a, int nt) { return BL ? (nt + a.min_tiles - 1) / a.min_tiles * a.min_tiles : nt; }
+// (a workgroup's share may end that much past the list)
+constexpr int64_t MOST_UNITS = (1ll << 31) - 65536;
 struct Units {
     vx_pseq s;          // of sequence `lane` (B <= 64)
     vx_tiles t;
@@ -207,8 +209,20 @@ __global__ __launch_bounds__(1024) void paged_units(Args a) {
     const int per = (a.p.B + 1023) / 1024, b0 = min(tid * per, a.p.B), b1 = min(b0 + per, a.p.B);
     vx_pseq s;
     vx_tiles t;
-    int sum = 0;
-    for (int b = b0; b < b1; b++) sum += seq_units<BL>(a, b, s, t);
+    int64_t all = 0;
+    for (int b = b0; b < b1; b++) all += seq_units<BL>(a, b, s, t);
+    int sum = (int)all;
+    bool over = false;
+    if constexpr (BL) {   // (token ranges that overlap, an error that vx_paged_seq has flagged, may list more than was checked: then nothing runs)
+        __shared__ int64_t s_all[16];
+        for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
+        if (lane == 0) s_all[wave] = all;
+        __syncthreads();
+        all = 0;
+        for (int w = 0; w < 16; w++) all += s_all[w];
+        over = all >= MOST_UNITS;
+        if (over) sum = 0, *a.p.err_flag = 1;
+    }
     int at = vx_wave_scan(sum);
     if (lane == 63) s_sum[wave] = at;
     __syncthreads();
@@ -217,7 +231,7 @@ __global__ __launch_bounds__(1024) void paged_units(Args a) {
     at -= sum;
     for (int b = b0; b < b1; b++) {
         a.before[b] = at;
-        at += seq_units<BL>(a, b, s, t);
+        at += over ? 0 : seq_units<BL>(a, b, s, t);
     }
 }
 
@@ -239,7 +253,7 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     const int n_list = list_tiles<BL>(a, tl.nt), p0 = before + (kvh * nb + blk) * n_list, p1 = p0 + n_list;
     const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
     const int g0 = p0 / un.chunk, g1 = (p1 - 1) / un.chunk;
-    if (tl.nt > 0 && g0 == g1) return;
+    if ((tl.nt > 0 && g0 == g1) || (BL && p1 > un.total)) return;   // (whole, or no list at all: paged_units)
     float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
     if (wave == 0 && a.gate) gt = gate_row(a, tok, h);
     __shared__ float4 s_o[4][64];

@@ -406,7 +406,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
     const int rows = d->max_T * a.qg;
     const size_t stat_bytes = d->acc ? ((size_t)d->n_tok * d->n_q * sizeof(float2) + 255) / 256 * 256 : 0;
     if (rows <= 16) {
-        VX_REQUIRE((int64_t)d->B * d->n_kv * tile_cap < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %lld tiles each)", who,
+        VX_REQUIRE((int64_t)d->B * d->n_kv * tile_cap < MOST_UNITS, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %lld tiles each)", who,
                    d->B, d->n_kv, (long long)tile_cap);
         // (one sequence of 1000 rows: 13.1 us with 4, 12.1 with 2, 11.9 with 1; of 3000: 16.4, 13.6, 15.8; of 8000: 18.8, 19.5, 19.5)
         a.min_tiles = 2;

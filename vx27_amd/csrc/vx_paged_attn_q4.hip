@@ -500,8 +500,11 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     a.block_rows = rows <= 8 ? 8 : 16;
     const int nb = (rows + a.block_rows - 1) / a.block_rows;
     a.min_tiles = 4;                             // (a tile a wave)
-    const int64_t units = (int64_t)d->B * d->n_kv * nb * ((a.tile_cap + a.min_tiles - 1) / a.min_tiles * a.min_tiles);
-    VX_REQUIRE(units < (1ll << 31) - 65536, "%s: more than 2^31 key tiles (B=%d n_kv=%d, %d tiles each)", who, d->B, d->n_kv, a.tile_cap);
+    // A list that may be past 2^31 units goes to the tile kernel: those of max_T tokens of every sequence, or, where
+    // paged_units adds them up, of n_tok tokens in all.
+    const int64_t tiles = ((int64_t)a.tile_cap + a.min_tiles - 1) / a.min_tiles * a.min_tiles * d->n_kv, units = tiles * d->B * nb;
+    const bool listed = units < MOST_UNITS || (d->B > 64 && ((int64_t)d->n_tok * a.qg / a.block_rows + d->B) * tiles < MOST_UNITS);
+    if (!listed) return rows_launch<true>(who, ctx, d, a, rows, 0);
     const int grid = (int)std::min<int64_t>((units + a.min_tiles - 1) / a.min_tiles, 2 * ctx->n_cu);
     a.part_rows = std::min(rows, a.block_rows);
     const size_t n_part = (size_t)2 * grid * a.part_rows;
