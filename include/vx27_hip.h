@@ -500,8 +500,10 @@ int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d)
  * tokens of every sequence, or past 64 sequences of n_tok tokens in all.)  A group held as NaN
  * reaches only the tokens that see its row, whose outputs are then NaN (of a
  * value row: the group's dims).
- * Nothing overflows while the largest |s*15| + |m| of V times the number of
- * rows seen stays below 2^127; of K, while a score's 256 products do.
+ * Nothing overflows for scores below 2^24 in magnitude (as over bf16 pages)
+ * while the largest |s*15| + |m| of V times the number of rows seen stays below
+ * 2^127, and so do, for every group of dims, 15 times the sum of a query's |q|
+ * and, of the groups together, that sum times |s*15| + |m| of a row of K.
  * Context scratch: that of vx27_hip_paged_attn, and where more than 640 query
  * rows read the same tiles, their values in bf16 (32 KiB for each 32 rows that a
  * sequence can see and KV head, 256 MB at most). */

@@ -149,3 +149,91 @@ def test_token_ranges_that_overlap_past_2_to_31_blocks(ctx):  # noqa: F811
     assert run(w) == "paged_q4_split"
     w.check("paged_q4_split", np.ones(w.bt.N, bool))
     w.free()
+
+
+SIZES = [("paged_q4_split", [300, 70], [1, 1], False), ("paged_q4_split", [300, 70], [7, 2], False), ("paged_rows_q4", [300, 70], [40, 3], True),
+         ("paged_rows_flat", [300, 170], [130, 90], False)]
+
+
+def attend(ctx, bt, kernel, out_bf16):  # noqa: F811
+    at = Attn4(ctx, bt, out_bf16, gate="none")
+    ran = run(at)
+    assert ran == kernel or (ran == "paged_q4_split" and not out_bf16)     # (fp32 outputs keep it for more tokens)
+    ctx.sync()
+    out = at.out()
+    at.free()
+    return out, ran
+
+
+@pytest.mark.parametrize("out_bf16", [False, True])
+@pytest.mark.parametrize("how", ["equal", "minus", "rising", "falling"])
+@pytest.mark.parametrize("kernel,lens,new,wide", SIZES)
+def test_scores_up_to_2_to_24(ctx, kernel, lens, new, wide, how, out_bf16):  # noqa: F811
+    """Scores of just below 2^24, of either sign: equal ones weigh the same; of rising or falling ones the largest takes
+    all the weight."""
+    say(f"scores of 2^24 {kernel} {how} bf16 {out_bf16}")
+    bt = Batch4(lens, new, 24, 4, 64, seed=1900 + new[0])
+    if wide:
+        widen(bt)
+    sign = np.where(bt.r.random(HD) < 0.5, -1.0, 1.0)
+    bt.q[:] = W.bf16_bits(np.broadcast_to(sign * 1000.0, bt.q.shape).astype(np.float32))
+    for b in range(bt.B):
+        n = bt.lens[b]
+        for j in range(n):
+            x = {"equal": 1.0, "minus": -1.0, "rising": 2 * j / n - 1, "falling": 1 - 2 * j / n}[how]
+            bt.set_row(b, j, np.broadcast_to(x * 1000.0 * sign, (4, HD)), bt.r.standard_normal((4, HD)))
+    out, ran = attend(ctx, bt, kernel, out_bf16)
+    for b in range(bt.B):
+        (kc, ks, km), v = bt.held(b)[0], values(*bt.held(b)[1])
+        s = values(kc, ks, km)[:, 0] @ f64(bt.q)[0, 0] / 16
+        assert 1.5e7 < np.abs(s).max() < 2 ** 24
+        if ran != "paged_q4_split":
+            v = Q.rounded(v)
+        for t in range(bt.new[b]):
+            i = bt.lens[b] - bt.new[b] + t
+            pick = {"rising": slice(i, i + 1), "falling": slice(0, 1)}.get(how, slice(0, i + 1))
+            want = np.repeat(v[pick].mean(0), 6, axis=0)
+            # the weights are of one size: one rounding of each (two parts), fp32 sums of terms s c + |m| (twice the largest
+            # value and what it is off by), the output's rounding
+            part = Q.PART[ran] * np.repeat(np.abs(v[pick]).mean(0), 6, axis=0) + 2.0 ** -14 * 8
+            assert np.all(np.abs(out[bt.start[b] + t] - want) <= part + (2.0 ** -8 * np.abs(want) if out_bf16 else 0.0))
+
+
+@pytest.mark.parametrize("out_bf16", [False, True])
+@pytest.mark.parametrize("kernel,lens,new,wide", SIZES)
+def test_large_queries_of_small_keys(ctx, kernel, lens, new, wide, out_bf16):  # noqa: F811
+    """Queries whose sum of 15 |q| over a group is just below 2^127, of keys as much smaller than 1."""
+    say(f"large queries {kernel} bf16 {out_bf16}")
+    bt = Batch4(lens, new, 24, 4, 64, seed=1930 + new[0], q_std=1.0)
+    if wide:
+        widen(bt)
+    q = f64(bt.q)
+    most = np.abs(q).reshape(bt.N, 24, 4, 64).sum(-1).max()
+    up = 2.0 ** np.floor(np.log2(2.0 ** 127 / (15 * most)))
+    bt.q[:] = W.bf16_bits((q * up).astype(np.float32))
+    for b in range(bt.B):
+        for j in range(bt.lens[b]):
+            bt.set_row(b, j, (bt.r.standard_normal((4, HD)) * 2 / up).astype(np.float32), bt.r.standard_normal((4, HD)))
+    out, ran = attend(ctx, bt, kernel, out_bf16)
+    most, mean = Q.check(out, Q.result(bt, ran, False), ran, max(lens), out_bf16)
+    assert most <= 1 and mean <= 1, (most, mean)
+
+
+@pytest.mark.parametrize("out_bf16", [False, True])
+@pytest.mark.parametrize("kernel,lens,new,wide", SIZES)
+def test_values_up_to_2_to_127_in_all(ctx, kernel, lens, new, wide, out_bf16):  # noqa: F811
+    """Values whose |s*15| + |m| times the rows seen is just below 2^127, under weights that are all the same."""
+    say(f"large values {kernel} bf16 {out_bf16}")
+    bt = Batch4(lens, new, 24, 4, 64, seed=1960 + new[0])
+    if wide:
+        widen(bt)
+    bt.q[:] = 0
+    r = [bt.r.standard_normal((n, 2, 4, HD)) for n in bt.lens]
+    c, s, m = quantise(r[0][:, 1])
+    up = 2.0 ** np.floor(np.log2(2.0 ** 127 / (max(lens) * (15 * f64(s) + np.abs(f64(m))).max())))
+    for b in range(bt.B):
+        for j in range(bt.lens[b]):
+            bt.set_row(b, j, r[b][j, 0], (r[b][j, 1] * up).astype(np.float32))
+    out, ran = attend(ctx, bt, kernel, out_bf16)
+    most, mean = Q.check(out, Q.result(bt, ran, False), ran, max(lens), out_bf16)
+    assert most <= 1 and mean <= 1, (most, mean)
