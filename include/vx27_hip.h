@@ -554,7 +554,8 @@ int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_desc *d);
  * Negative counts, lengths past the table, more free pages than n_pages and
  * page numbers outside the pool are clamped or dropped on the device and
  * reported by the next vx27_hip_sync; that call's outputs are undefined.
- * n_pages * page_size below 2^31.  Context scratch: 12 bytes a sequence. */
+ * n_pages * page_size below 2^31.  Context scratch: none up to 1024 sequences and
+ * 4096 tokens (n_tok), else 8 bytes a sequence and 12 more. */
 typedef struct {
     int B, page_size, n_pages, max_pages;
     int n_tok;                  /* room in slot, pos and seq */
