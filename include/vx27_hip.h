@@ -532,6 +532,9 @@ int vx27_hip_paged_read_q4(vx27_hip_ctx *ctx, const vx27_paged_read_desc *d);
  * 1. A sequence with ended[b] != 0 gives its pages back: they go on top of the
  *    free ones, in the order of the sequences and of their rows.  It has no
  *    rows then and takes no tokens in this call.
+ *    Pages are not counted: one that sequences share (a common prefix) would be
+ *    given back once for each of them and be free while others read it, so a
+ *    sequence that shares any must not end this way.
  * 2. A sequence whose rows and new tokens are past max_pages * page_size gets
  *    none of the tokens.  Of the others, one that needs no further page gets
  *    all of them, and one that needs pages does if the pages that it and the
