@@ -491,15 +491,18 @@ int vx27_hip_paged_append_q4(vx27_hip_ctx *ctx, const vx27_paged_append_desc *d)
  * VX27_Q4_SPLIT_ROWS query rows a KV head (max_T * n_q/n_kv; fp32 outputs:
  * VX27_Q4_SPLIT_ROWS_F32), and more of small calls (n_kv * (n_tok * n_q/n_kv/16 + B)
  * times the 32-row blocks that a sequence can see, at most VX27_Q4_SPLIT_TILES)
- * run the decode kernels: codes and q are exact
- * operands of bf16 MFMAs, s and m are applied in fp32, and the softmax weights
- * are two bf16 parts (at most 2^-16 off).  The others run the tile kernel: the
- * rows' values, and the weights, are rounded to bf16 once.  (So do calls whose
- * list of 32-row blocks, those that a sequence can see for each 16 query rows, or
- * 8 where there are no more, and KV head, may be past 2^31: the blocks of max_T
- * tokens of every sequence, or past 64 sequences of n_tok tokens in all.)  A group held as NaN
- * reaches only the tokens that see its row, whose outputs are then NaN (of a
- * value row: the group's dims).
+ * run the decode kernels: codes and q are exact operands of bf16 MFMAs, s and m
+ * are applied in fp32, and the softmax weights are two bf16 parts (at most 2^-16
+ * off).  The others run the tile kernel: the rows' values, and the weights, are
+ * rounded to bf16 once, for fp32 outputs too (of a value that is large beside its
+ * s this may be more than a code's step).  So do calls of more than 2^31 blocks,
+ * each counted for every KV head and 16 query rows (8 where a KV head has no
+ * more) that can see it: of max_T tokens of every sequence, or past 64 sequences
+ * of n_tok tokens in all.  What a sequence can see goes by window and max_pages,
+ * not by its rows, which are on the device: tables no wider than they need to be
+ * keep short prompts in the decode kernels.  A group held as NaN reaches only the
+ * tokens that see its row, whose outputs are then NaN (of a value row: the
+ * group's dims).
  * Nothing overflows for scores below 2^24 in magnitude (as over bf16 pages)
  * while the largest |s*15| + |m| of V times the number of rows seen stays below
  * 2^127, and so do, for every group of dims, 15 times the sum of a query's |q|

@@ -186,9 +186,10 @@ __device__ __forceinline__ double inv_sqrt(double x) {
 // One KV head's new keys or values, rows [lo, hi) of the block at row p0 of
 // sequence b: a row a wave, its codes into LDS by bytes; then thread u stores
 // 16-byte unit u of the block, or of V, where 8 rows share one, as much of it as
-// is new.  8192 tokens of 24 + 4 heads take 59 us (the copy rate's 47), keys and
-// values alone 25; with a block's 32 rows in one workgroup, whose waves' rows
-// follow one another, 65, and 4 us more for 64 tokens.
+// is new.  4362 tokens of 24 + 4 heads (130 MB, 25 us at the copy rate) take 59
+// us, keys and values alone 25; with a block's 32 rows in one workgroup, whose
+// waves' rows follow one another, 65, and 4 us more for 64 tokens.  Calls timed
+// back to back: 53 us, 8192 tokens 95, 65536 672.
 constexpr int Q4_ROWS = 8;                    // rows of a workgroup: those that share V's units
 constexpr int CODE_ROW = HDG + 4;             // (rows 8 apart then lie in different banks)
 template <bool Q4>

@@ -9,7 +9,7 @@
 // way in, and the minima's sums are MFMAs of their own (one for 16 keys' scores,
 // one for a tile's outputs).
 //
-// The split kernel on 4 x 131072 rows of 4 KV heads (604 MB): 106 us, 5.7 TB/s
+// The split kernel on 4 x 131072 rows of 4 KV heads (604 MB): 108 us, 5.6 TB/s
 // of 7.2 (its loads alone 90).  A tile is 670 VALU instructions, half of them the
 // codes' masks and conversions and the weights' parts, which keep the VALU busy
 // for two thirds of the time at the two waves a SIMD that 235 registers allow.
@@ -493,7 +493,8 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     // values and has two parts of the weights, to where a call is a prompt.
     // Short prompts too, up to 2048 pairs of a tile and a block of 16 rows in all
     // (prompts of 50 tokens 15 us against 26, of 100 18, 28; of 200, 2432 pairs, 28,
-    // 31; five of 30 tokens after 270 rows, 2440, 38, 35).
+    // 31; five of 30 tokens after 270 rows, 2440, 38, 35).  The lengths are on the
+    // device, so the pairs are those that the tables have room for.
     const int64_t pairs = ((int64_t)d->n_tok * a.qg / 16 + d->B) * d->n_kv * a.tile_cap;
     if (rows > (a.out_bf16 ? VX27_Q4_SPLIT_ROWS : VX27_Q4_SPLIT_ROWS_F32) && pairs > VX27_Q4_SPLIT_TILES) return rows_launch<true>(who, ctx, d, a, rows, 0);
     // (decoding tokens of 6 heads: 8 rows a block)
