@@ -201,20 +201,23 @@ __device__ __forceinline__ int units_find(const Args &a, const Units &u, int x) 
     return b;
 }
 
-// grid 1, block 1024: the units before each sequence, and in all.
-template <bool BL>
+// grid 1, block 1024: the units before each sequence, and in all.  CHECK: where
+// token ranges that overlap, an error that vx_paged_seq flags, could list more
+// than the host has room for: then none (a barrier and sums in 64 bits, 0.8 us).
+template <bool BL, bool CHECK>
 __global__ __launch_bounds__(1024) void paged_units(Args a) {
     __shared__ int s_sum[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (a.p.B + 1023) / 1024, b0 = min(tid * per, a.p.B), b1 = min(b0 + per, a.p.B);
     vx_pseq s;
     vx_tiles t;
-    int64_t all = 0;
-    for (int b = b0; b < b1; b++) all += seq_units<BL>(a, b, s, t);
-    int sum = (int)all;
+    int sum = 0;
     bool over = false;
-    if constexpr (BL) {   // (token ranges that overlap, an error that vx_paged_seq has flagged, may list more than was checked: then nothing runs)
+    if constexpr (CHECK) {
         __shared__ int64_t s_all[16];
+        int64_t all = 0;
+        for (int b = b0; b < b1; b++) all += seq_units<BL>(a, b, s, t);
+        sum = (int)all;
         for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
         if (lane == 0) s_all[wave] = all;
         __syncthreads();
@@ -222,6 +225,8 @@ __global__ __launch_bounds__(1024) void paged_units(Args a) {
         for (int w = 0; w < 16; w++) all += s_all[w];
         over = all >= MOST_UNITS;
         if (over) sum = 0, *a.p.err_flag = 1;
+    } else {
+        for (int b = b0; b < b1; b++) sum += seq_units<BL>(a, b, s, t);
     }
     int at = vx_wave_scan(sum);
     if (lane == 63) s_sum[wave] = at;
@@ -231,7 +236,7 @@ __global__ __launch_bounds__(1024) void paged_units(Args a) {
     at -= sum;
     for (int b = b0; b < b1; b++) {
         a.before[b] = at;
-        at += over ? 0 : seq_units<BL>(a, b, s, t);
+        if (!CHECK || !over) at += seq_units<BL>(a, b, s, t);
     }
 }
 
@@ -253,7 +258,7 @@ __global__ __launch_bounds__(256) void paged_join(Args a, int grid) {
     const int n_list = list_tiles<BL>(a, tl.nt), p0 = before + (kvh * nb + blk) * n_list, p1 = p0 + n_list;
     const int t = row_tok(a, r), tok = s.start + t, h = row_head(a, kvh, r, t);
     const int g0 = p0 / un.chunk, g1 = (p1 - 1) / un.chunk;
-    if ((tl.nt > 0 && g0 == g1) || (BL && p1 > un.total)) return;   // (whole, or no list at all: paged_units)
+    if ((tl.nt > 0 && g0 == g1) || (BL && p1 > un.total)) return;   // (whole, or no list: paged_units)
     float4 gt = make_float4(0.f, 0.f, 0.f, 0.f);
     if (wave == 0 && a.gate) gt = gate_row(a, tok, h);
     __shared__ float4 s_o[4][64];

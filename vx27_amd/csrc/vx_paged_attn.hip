@@ -424,7 +424,7 @@ extern "C" int vx27_hip_paged_attn(vx27_hip_ctx *ctx, const vx27_paged_attn_desc
         a.stat = d->acc ? (float2 *)((char *)scr + o_bytes + ml_bytes) : nullptr;
         a.stash = d->acc ? (float *)((char *)scr + o_bytes + ml_bytes + stat_bytes) : nullptr;
         a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes + stat_bytes + st_bytes) : nullptr;
-        if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<false>), dim3(1), dim3(1024), a);
+        if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<false, false>), dim3(1), dim3(1024), a);
         VX_LAUNCH(ctx, paged_split, dim3(grid), dim3(256), a);
         VX_LAUNCH_NAMED(ctx, "paged_join", (paged_join<false>), dim3(rows, d->n_kv, d->B), dim3(256), a, grid);
         if (d->acc) VX_LAUNCH(ctx, paged_weigh, dim3((a.tile_cap + 7) / 8, d->n_kv, d->B), dim3(256), a);

@@ -516,7 +516,8 @@ extern "C" int vx27_hip_paged_attn_q4(vx27_hip_ctx *ctx, const vx27_paged_attn_d
     a.part_o = (float *)scr;
     a.part_ml = (float2 *)((char *)scr + o_bytes);
     a.before = d->B > 64 ? (int *)((char *)scr + o_bytes + ml_bytes) : nullptr;
-    if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true>), dim3(1), dim3(1024), a);
+    if (a.before && units < MOST_UNITS) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true, false>), dim3(1), dim3(1024), a);
+    else if (a.before) VX_LAUNCH_NAMED(ctx, "paged_units", (paged_units<true, true>), dim3(1), dim3(1024), a);
     if (a.block_rows == 16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<16, false>), dim3(grid), dim3(256), a);
     else if (a.out_bf16) VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8, true>), dim3(grid), dim3(256), a);
     else VX_LAUNCH_NAMED(ctx, "paged_q4_split", (paged_q4_split<8, false>), dim3(grid), dim3(256), a);
